@@ -200,6 +200,35 @@ int voom_mla_pack_head_weights(const void* w, void* w_packed, int num_heads, int
                                hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Attention of drafted tokens over paged K/V: the verify step of speculative
+ * decoding.  No reference counterpart (its windows are causal,
+ * runtime/layer_runner.py:166-177).
+ *
+ * The newest draft_lens[b] (NULL: `drafts`) of the ctx_lens[b] cached tokens of
+ * sequence b are drafts.  Draft t sees every token before the drafts and those
+ * drafts j with mask[t][j] != 0 (NULL: j <= t), so that a tree's mask row holds a
+ * draft's ancestors and itself.
+ *   q          [batch, num_q_heads, drafts, head_dim] bf16, head_dim 64 or 128
+ *   k_pool, v_pool, block_table as for voom_paged_gqa_decode
+ *   mask       uint8 [mask_batch, drafts, drafts], mask_batch 1 (shared) or batch
+ *   out        [batch, drafts, num_q_heads, head_dim] bf16
+ *   lse        [batch, drafts, num_q_heads] fp32 natural log (NULL: none)
+ * Rows past draft_lens[b], and rows whose keys weigh nothing, give 0 and -inf.
+ * At most 1024 drafts, 1024 sequences and 16 q heads per kv head.  Lengths outside
+ * [0, max_pages * page_tokens] and [0, min(drafts, ctx)] are clamped.  The
+ * workspace needs no initialisation; calls that overlap need one each.
+ * ------------------------------------------------------------------------- */
+size_t voom_paged_gqa_tree_workspace_bytes(int batch, int num_q_heads, int num_kv_heads,
+                                           int head_dim, int drafts, int page_tokens,
+                                           int max_pages);
+int voom_paged_gqa_tree(const void* q, const void* k_pool, const void* v_pool,
+                        const int32_t* block_table, const int32_t* ctx_lens,
+                        const int32_t* draft_lens, const uint8_t* mask, int mask_batch, void* out,
+                        float* lse, void* workspace, size_t ws_bytes, int batch, int num_q_heads,
+                        int num_kv_heads, int head_dim, int page_tokens, int max_pages,
+                        int num_slots, int drafts, float scale, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Absorbed-MLA paged decode: the latent contraction.
  *
  * Replaces the latent part of _mla_absorbed_attention (runtime/glm.py:133-164):

@@ -317,6 +317,70 @@ def paged_gqa_prefill(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
     return out
 
 
+def _require_current(dev: torch.device) -> None:
+    """The launch goes to the current device's stream: tensors must live there."""
+    cur = _CUR_DEVICE() if _CUR_DEVICE is not None else torch.cuda.current_device()
+    _require(dev.index == cur, f"tensors are on {dev}, but cuda:{cur} is the current device")
+
+
+def _check_lens(t: torch.Tensor | None, batch: int, name: str) -> None:
+    _require(t is None or (t.dtype == torch.int32 and tuple(t.shape) == (batch,)),
+             f"{name} must be int32 [{batch}]")
+
+
+def paged_gqa_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                   block_table: torch.Tensor, ctx_lens: torch.Tensor, *,
+                   mask: torch.Tensor | None = None, draft_lens: torch.Tensor | None = None,
+                   scale: float | None = None, return_lse: bool = False):
+    """Attention of drafted tokens over paged K/V (a speculative step's verify).
+
+    q [B, NQ, T, D] bf16 holds the queries of each sequence's newest T cached
+    tokens, the drafts; ctx_lens [B] int32 counts every cached token, drafts
+    included.  Draft t sees the tokens before the drafts and those drafts j with
+    mask[t, j] set: ``mask`` bool [T, T] or [B, T, T] holds a draft's ancestors and
+    itself (None: causal).  ``draft_lens`` [B] int32: how many of a sequence's rows
+    are drafts, where not all T are.
+
+    Returns out [B, T, NQ, D] (and the fp32 natural-log LSE [B, T, NQ] when
+    ``return_lse``); rows that see nothing, and rows past draft_lens, hold 0 and -inf.
+    """
+    _require(q.dim() == 4, "q must be [B, NQ, T, D]")
+    dev = _require_device(q, k_pool, v_pool, block_table, ctx_lens, mask, draft_lens)
+    _require_current(dev)
+    B, NQ, T, D = q.shape
+    _require(k_pool.dim() == 4, "k_pool must be [slots, NKV, PT, D]")
+    slots, NKV, PT, Dk = k_pool.shape
+    _require(Dk == D, f"k_pool head_dim {Dk} != q head_dim {D}")
+    _check_v_pool(v_pool, slots, NKV, D, PT)
+    _require(q.dtype == k_pool.dtype == v_pool.dtype == torch.bfloat16,
+             "q and pools must be bfloat16")
+    _require(block_table.dtype == torch.int32 and block_table.dim() == 2
+             and block_table.shape[0] == B, "block_table must be int32 [B, max_pages]")
+    _require(ctx_lens.dtype == torch.int32 and tuple(ctx_lens.shape) == (B,),
+             "ctx_lens must be int32 [B]")
+    _check_lens(draft_lens, B, "draft_lens")
+    _require(NQ % NKV == 0, "num_q_heads must be a multiple of num_kv_heads")
+    _require(mask is None or (mask.dtype == torch.bool
+                              and tuple(mask.shape) in ((T, T), (B, T, T))),
+             f"mask must be bool [{T}, {T}] or [{B}, {T}, {T}]")
+    out = torch.empty((B, T, NQ, D), dtype=torch.bfloat16, device=dev)
+    lse = torch.empty((B, T, NQ), dtype=torch.float32, device=dev) if return_lse else None
+    if out.numel():
+        if _BOUNDS_CHECKS:
+            check_block_table(block_table, ctx_lens, slots, PT)
+        # allocated per call, so that calls on several streams or threads and captured
+        # graphs never share it
+        need = int(_lib.lib().voom_paged_gqa_tree_workspace_bytes(B, NQ, NKV, D, T, PT,
+                                                                  block_table.shape[1]))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _lib.call("voom_paged_gqa_tree", _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table),
+                  _ptr(ctx_lens), _ptr(draft_lens), _ptr(mask),
+                  mask.shape[0] if mask is not None and mask.dim() == 3 else 1, _ptr(out),
+                  _ptr(lse), _ptr(ws), need, B, NQ, NKV, D, PT, block_table.shape[1], slots, T,
+                  float(D ** -0.5 if scale is None else scale), _stream(None))
+    return (out, lse) if return_lse else out
+
+
 def merge_attn_states(o_a: torch.Tensor, lse_a: torch.Tensor, o_b: torch.Tensor,
                       lse_b: torch.Tensor, *, stream: torch.cuda.Stream | None = None):
     """Combine two attention results over disjoint key sets (LSE merge)."""
