@@ -229,6 +229,82 @@ int voom_paged_gqa_tree(const void* q, const void* k_pool, const void* v_pool,
                         int num_slots, int drafts, float scale, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Caches bounded by accumulated attention weight.  No reference counterpart (it
+ * spills pages by age, runtime/kv_paged.py:216-240, and never drops a token).
+ *
+ * voom_paged_gqa_observe adds the attention weight that each cached token
+ * receives from the newest window_lens[b] (NULL: `window`) of the ctx_lens[b]
+ * tokens, the queries of which are given:
+ *   out[b][h][p] = scores[b][h][p] + sum over window tokens t at or behind p and the
+ *                  q heads g of kv head h of exp(scale * q[g][t] . k[p] - lse[t][g])
+ * for p < ctx; the rest of out stays as it is.
+ *   q       [batch, num_q_heads, window, head_dim] bf16, head_dim 64 or 128
+ *   lse     [batch, window, num_q_heads] fp32 natural log of those queries' attention
+ *           (of -inf: the row adds nothing)
+ *   scores  [batch, num_kv_heads, score_tokens] fp32; out the same array or another one
+ * Contexts are clamped to the block table and to score_tokens.
+ *
+ * voom_evict_select chooses what a budget of tokens keeps of each head: all of a
+ * context that fits it; else the first `sink`, the newest `recent`, and of those
+ * between the ones of largest score, equal scores (and -0 as 0) lowest position first,
+ * a NaN below every number.
+ *   keep       [batch, num_kv_heads, budget] int32, ascending, -1 behind keep_lens[b]
+ *   keep_lens  [batch] int32: min(ctx, budget)
+ *
+ * voom_compact_kv moves the rows that stay: position start[b] + i (NULL: i) of every
+ * kv head takes the K and V of position keep[b][h][i], i < keep_lens[b], of its own
+ * pages.
+ *   keep       [batch, keep_heads, keep_tokens] int32 ascending, keep_heads 1 (one list
+ *              for all heads: the accepted branch of a tree of drafts) or num_kv_heads
+ *   dst_table  [batch, dst_pages]: the pages written.  block_table itself for a move in
+ *              place, which needs keep[i] >= start + i; pages of their own (for prefixes
+ *              that other sequences share); or a mix, page by page
+ *   scores     [batch, num_kv_heads, score_tokens] or NULL: moved the same way into
+ *              scores_out (the same array or another one), zero behind the last row
+ * Rows whose position or slot id lies outside the tables and the pool are left out.
+ * ------------------------------------------------------------------------- */
+int voom_paged_gqa_observe(const void* q, const float* lse, const void* k_pool,
+                           const int32_t* block_table, const int32_t* ctx_lens,
+                           const int32_t* window_lens, const float* scores, float* out, int batch,
+                           int num_q_heads, int num_kv_heads, int head_dim, int page_tokens,
+                           int max_pages, int num_slots, int window, int score_tokens, float scale,
+                           hipStream_t stream);
+int voom_evict_select(const float* scores, const int32_t* ctx_lens, int32_t* keep,
+                      int32_t* keep_lens, int batch, int num_kv_heads, int score_tokens, int budget,
+                      int sink, int recent, hipStream_t stream);
+int voom_compact_kv(void* k_pool, void* v_pool, const int32_t* block_table,
+                    const int32_t* dst_table, const int32_t* keep, const int32_t* keep_lens,
+                    const int32_t* start, const float* scores, float* scores_out, int batch,
+                    int num_kv_heads, int head_dim, int page_tokens, int max_pages, int dst_pages,
+                    int num_slots, int keep_heads, int keep_tokens, int score_tokens,
+                    hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * RMS norm of every query and key head, rotary positions, and the page write of
+ * new tokens in one launch (the RoPE and cache write of
+ * runtime/layer_runner.py:98-109,158, with per-head norms and positions that
+ * need not be the places in the cache: a draft's is its depth in the tree).
+ *   qkv        [batch, new_tokens, (nq + 2 nkv) * head_dim] bf16, head_dim a multiple of
+ *              16 up to 256
+ *   q_weight, k_weight  [head_dim] bf16 or NULL (no norm):
+ *              y = x / sqrt(mean x^2 + eps) * weight
+ *   cos, sin   fp32 [rope_rows, rotary_dim / 2]; the first rotary_dim (a multiple of 16)
+ *              dims of a head turn by the row positions[b][t] (clamped): dims (i, i +
+ *              rotary_dim / 2) as a pair, or with `interleaved` dims (2 i, 2 i + 1)
+ *   q          [batch, nq, new_tokens, head_dim]
+ *   start      [batch] int32: token t < new_lens[b] (NULL: new_tokens) is written at cache
+ *              position start[b] + t, where its page exists
+ * Everything in fp32, rounded to bf16 once.
+ * ------------------------------------------------------------------------- */
+int voom_qk_norm_rope_append(const void* qkv, const void* q_weight, const void* k_weight,
+                             float eps, const float* cos, const float* sin, int rope_rows,
+                             int rotary_dim, int interleaved, const int32_t* positions, void* q,
+                             void* k_pool, void* v_pool, const int32_t* block_table,
+                             const int32_t* start, const int32_t* new_lens, int batch,
+                             int new_tokens, int num_q_heads, int num_kv_heads, int head_dim,
+                             int page_tokens, int max_pages, int num_slots, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Absorbed-MLA paged decode: the latent contraction.
  *
  * Replaces the latent part of _mla_absorbed_attention (runtime/glm.py:133-164):

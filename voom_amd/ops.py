@@ -381,6 +381,215 @@ def paged_gqa_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     return (out, lse) if return_lse else out
 
 
+def _check_scores(t: torch.Tensor | None, batch: int, num_kv_heads: int, name: str) -> None:
+    _require(t is None or (t.dtype == torch.float32 and t.dim() == 3 and t.shape[2] > 0
+                           and tuple(t.shape[:2]) == (batch, num_kv_heads)),
+             f"{name} must be float32 [{batch}, {num_kv_heads}, tokens]")
+
+
+def paged_gqa_observe(q: torch.Tensor, lse: torch.Tensor, k_pool: torch.Tensor,
+                      block_table: torch.Tensor, ctx_lens: torch.Tensor, scores: torch.Tensor, *,
+                      window_lens: torch.Tensor | None = None, scale: float | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """Add the attention weight that each cached token receives from the newest ones.
+
+    q [B, NQ, L, D] bf16 and lse [B, L, NQ] fp32 (paged_gqa_tree's, or
+    paged_gqa_decode's [B, NQ] for one token) are the queries of each sequence's newest
+    L of ctx_lens [B] cached tokens (``window_lens`` [B] int32: of fewer) and the
+    log-sum-exp of their scaled scores.  Returns ``out`` (default: ``scores`` itself),
+    fp32 [B, NKV, tokens], which takes
+        scores[b, h, p] + sum_{t, g} exp(scale q[b, g, t] . k[p] - lse[b, t, g])
+    over the window's tokens at or behind p and the q heads of kv head h, for p < ctx;
+    what is behind the context is left as it is.
+    """
+    if q.dim() == 4 and lse.dim() == 2 and q.shape[2] == 1:
+        lse = lse[:, None]
+    _require(q.dim() == 4, "q must be [B, NQ, L, D]")
+    dev = _require_device(q, lse, k_pool, block_table, ctx_lens, scores, window_lens, out)
+    _require_current(dev)
+    B, NQ, L, D = q.shape
+    _require(k_pool.dim() == 4, "k_pool must be [slots, NKV, PT, D]")
+    slots, NKV, PT, Dk = k_pool.shape
+    _require(Dk == D, f"k_pool head_dim {Dk} != q head_dim {D}")
+    _require(q.dtype == k_pool.dtype == torch.bfloat16, "q and the pool must be bfloat16")
+    _require(lse.dtype == torch.float32 and tuple(lse.shape) == (B, L, NQ),
+             f"lse must be float32 [{B}, {L}, {NQ}]")
+    _require(block_table.dtype == torch.int32 and block_table.dim() == 2
+             and block_table.shape[0] == B, "block_table must be int32 [B, max_pages]")
+    _require(ctx_lens.dtype == torch.int32 and tuple(ctx_lens.shape) == (B,),
+             "ctx_lens must be int32 [B]")
+    _check_lens(window_lens, B, "window_lens")
+    _require(NQ % NKV == 0, "num_q_heads must be a multiple of num_kv_heads")
+    _check_scores(scores, B, NKV, "scores")
+    out = scores if out is None else out
+    _require(out.dtype == torch.float32 and out.shape == scores.shape, "out must be like scores")
+    if B == 0:
+        return out
+    if _BOUNDS_CHECKS:
+        check_block_table(block_table, ctx_lens, slots, PT)
+    if L == 0:  # nothing to add
+        q, lse, L = q.new_zeros((B, NQ, 1, D)), lse.new_full((B, 1, NQ), -float("inf")), 1
+    _lib.call("voom_paged_gqa_observe", _ptr(q), _ptr(lse), _ptr(k_pool), _ptr(block_table),
+              _ptr(ctx_lens), _ptr(window_lens), _ptr(scores), _ptr(out), B, NQ, NKV, D, PT,
+              block_table.shape[1], slots, L, scores.shape[2],
+              float(D ** -0.5 if scale is None else scale), _stream(None))
+    return out
+
+
+def evict_select(scores: torch.Tensor, ctx_lens: torch.Tensor, budget: int, *, sink: int = 0,
+                 recent: int = 0):
+    """Which tokens of each head a budget keeps: (keep [B, NKV, budget] int32 ascending
+    positions, -1 behind the last; keep_lens [B] int32 = min(ctx, budget)).
+
+    scores [B, NKV, tokens] fp32 (paged_gqa_observe's sums), ctx_lens [B] int32.  Of a
+    context longer than ``budget`` stay the first ``sink`` tokens, the newest ``recent``,
+    and of those between the ones of largest score, equal scores lowest position first
+    (a NaN counts below every number).
+    """
+    dev = _require_device(scores, ctx_lens)
+    _require_current(dev)
+    _require(scores.dim() == 3, "scores must be [B, NKV, tokens]")
+    B, NKV, cap = scores.shape
+    _check_scores(scores, B, NKV, "scores")
+    _require(ctx_lens.dtype == torch.int32 and tuple(ctx_lens.shape) == (B,),
+             "ctx_lens must be int32 [B]")
+    budget, sink, recent = int(budget), int(sink), int(recent)
+    _require(budget > 0 and sink >= 0 and recent >= 0 and sink + recent <= budget,
+             f"sink {sink} and recent {recent} must fit the budget {budget}")
+    keep = torch.empty((B, NKV, budget), dtype=torch.int32, device=dev)
+    keep_lens = torch.empty((B,), dtype=torch.int32, device=dev)
+    if B and NKV:
+        _lib.call("voom_evict_select", _ptr(scores), _ptr(ctx_lens), _ptr(keep), _ptr(keep_lens),
+                  B, NKV, cap, budget, sink, recent, _stream(None))
+    return keep, keep_lens
+
+
+def check_keep(keep: torch.Tensor, keep_lens: torch.Tensor, tokens: int,
+               start: torch.Tensor | None, in_place: bool) -> None:
+    """Raise ValueError unless every list's first keep_lens[b] positions lie in
+    [0, tokens) and ascend, and for a move in place position i is at least start[b] + i."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("bounds checks synchronise and cannot run under graph capture")
+    n = keep.shape[-1]
+    at = torch.arange(n, device=keep.device)
+    used = at < keep_lens[:, None, None]
+    if bool(((keep_lens < 0) | (keep_lens > n)).any()):
+        raise ValueError(f"keep_lens lie outside [0, {n}]")
+    if bool((used & ((keep < 0) | (keep >= tokens))).any()):
+        raise ValueError(f"keep holds positions outside [0, {tokens})")
+    if bool((used[..., 1:] & (keep[..., 1:] <= keep[..., :-1])).any()):
+        raise ValueError("keep must ascend")
+    first = 0 if start is None else start[:, None, None]
+    if in_place and bool((used & (keep < at + first)).any()):
+        raise ValueError("a move in place needs keep[i] >= start + i")
+
+
+def compact_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+               keep: torch.Tensor, keep_lens: torch.Tensor, *, start: torch.Tensor | None = None,
+               dst_table: torch.Tensor | None = None, scores: torch.Tensor | None = None,
+               scores_out: torch.Tensor | None = None) -> None:
+    """Move the cached rows that stay to the front of their sequences, bit for bit.
+
+    Position start[b] + i (``start`` [B] int32, None: 0) of every kv head takes the K and
+    V of position keep[b, h, i], i < keep_lens[b].  keep [B, NKV, n] int32 holds ascending
+    positions per head (evict_select's), or [B, 1, n] one list for all heads (the
+    accepted branch of a tree of drafts).  In place (``dst_table`` None) keep[b, h, i] must
+    be at least start[b] + i; ``dst_table`` [B, pages] int32 names other pages to write, for
+    those that sequences share: a page of it is either the sequence's own page at the same
+    index or one that block_table does not hold.
+
+    ``scores`` [B, NKV, tokens] fp32 moves along into ``scores_out`` (default: in place);
+    behind the last row kept it becomes 0.
+    """
+    dev = _require_device(k_pool, v_pool, block_table, keep, keep_lens, start, dst_table, scores,
+                          scores_out)
+    _require_current(dev)
+    _require(k_pool.dim() == 4, "k_pool must be [slots, NKV, PT, D]")
+    slots, NKV, PT, D = k_pool.shape
+    _check_v_pool(v_pool, slots, NKV, D, PT)
+    _require(k_pool.dtype == v_pool.dtype == torch.bfloat16, "pools must be bfloat16")
+    _require(block_table.dtype == torch.int32 and block_table.dim() == 2,
+             "block_table must be int32 [B, max_pages]")
+    B = block_table.shape[0]
+    _require(keep.dtype == torch.int32 and keep.dim() == 3
+             and tuple(keep.shape[:2]) in ((B, NKV), (B, 1)),
+             f"keep must be int32 [{B}, {NKV}, n] or [{B}, 1, n]")
+    _require(keep_lens.dtype == torch.int32 and tuple(keep_lens.shape) == (B,),
+             "keep_lens must be int32 [B]")
+    _check_lens(start, B, "start")
+    in_place = dst_table is None
+    dst_table = block_table if in_place else dst_table
+    _require(dst_table.dtype == torch.int32 and dst_table.dim() == 2 and dst_table.shape[0] == B,
+             "dst_table must be int32 [B, pages]")
+    _check_scores(scores, B, NKV, "scores")
+    _require(scores is not None or scores_out is None, "scores_out needs scores")
+    if scores is not None:
+        scores_out = scores if scores_out is None else scores_out
+        _require(scores_out.dtype == torch.float32 and scores_out.shape == scores.shape,
+                 "scores_out must be like scores")
+    if B == 0 or (keep.shape[2] == 0 and scores is None):
+        return
+    if _BOUNDS_CHECKS:
+        check_keep(keep, keep_lens, block_table.shape[1] * PT, start, in_place)
+    if keep.shape[2] == 0:  # only scores to clear
+        keep, keep_lens = keep.new_zeros((B, 1, 1)), torch.zeros_like(keep_lens)
+    _lib.call("voom_compact_kv", _ptr(k_pool), _ptr(v_pool), _ptr(block_table), _ptr(dst_table),
+              _ptr(keep), _ptr(keep_lens), _ptr(start), _ptr(scores), _ptr(scores_out), B, NKV, D,
+              PT, block_table.shape[1], dst_table.shape[1], slots, keep.shape[1], keep.shape[2],
+              0 if scores is None else scores.shape[2], _stream(None))
+
+
+def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                        positions: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                        block_table: torch.Tensor, start: torch.Tensor, num_q_heads: int,
+                        num_kv_heads: int, *, q_weight: torch.Tensor | None = None,
+                        k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                        interleaved: bool = False,
+                        new_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """Norm every query and key head, rotate, and write K and V into their pages.
+
+    qkv [B, L, (nq + 2 nkv) hd] bf16 holds the projections of new tokens; hd is the
+    pool's.  A head is normed x / sqrt(mean x^2 + eps) * weight where ``q_weight`` /
+    ``k_weight`` [hd] bf16 is given; its first 2 * cos.shape[1] dims turn by row
+    positions[b, t] (int32 [B, L]) of cos / sin [P, rotary / 2] fp32 (rope_cache's), dims
+    (i, i + rotary / 2) as a pair, or (2 i, 2 i + 1) with ``interleaved``.  Returns q
+    [B, nq, L, hd]; K and V of token t land at cache position start[b] + t (start [B]
+    int32) for t < new_lens[b] (None: all).  One rounding to bf16 at the end.
+    """
+    dev = _require_device(qkv, cos, sin, positions, k_pool, v_pool, block_table, start, q_weight,
+                          k_weight, new_lens)
+    _require_current(dev)
+    nq, nkv = int(num_q_heads), int(num_kv_heads)
+    _require(k_pool.dim() == 4, "k_pool must be [slots, NKV, PT, D]")
+    slots, NKVp, PT, hd = k_pool.shape
+    _require(nq > 0 and NKVp == nkv, "pool geometry does not match the heads")
+    _check_v_pool(v_pool, slots, nkv, hd, PT)
+    _require(qkv.dim() == 3 and qkv.shape[2] == (nq + 2 * nkv) * hd,
+             f"qkv must be [B, L, {(nq + 2 * nkv) * hd}]")
+    B, L, _ = qkv.shape
+    _require(qkv.dtype == k_pool.dtype == v_pool.dtype == torch.bfloat16,
+             "qkv and pools must be bfloat16")
+    _require(cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape
+             and cos.shape[0] > 0, "cos and sin must be float32 [positions, rotary / 2]")
+    _require(positions.dtype == torch.int32 and tuple(positions.shape) == (B, L),
+             f"positions must be int32 [{B}, {L}]")
+    _require(block_table.dtype == torch.int32 and block_table.dim() == 2
+             and block_table.shape[0] == B, "block_table must be int32 [B, max_pages]")
+    _require(start.dtype == torch.int32 and tuple(start.shape) == (B,), "start must be int32 [B]")
+    _check_lens(new_lens, B, "new_lens")
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        _require(w is None or (w.dtype == torch.bfloat16 and tuple(w.shape) == (hd,)),
+                 f"{name} must be bfloat16 [{hd}]")
+    q = torch.empty((B, nq, L, hd), dtype=torch.bfloat16, device=dev)
+    if q.numel():
+        _lib.call("voom_qk_norm_rope_append", _ptr(qkv), _ptr(q_weight), _ptr(k_weight),
+                  float(eps), _ptr(cos), _ptr(sin), cos.shape[0], 2 * cos.shape[1],
+                  int(bool(interleaved)), _ptr(positions), _ptr(q), _ptr(k_pool), _ptr(v_pool),
+                  _ptr(block_table), _ptr(start), _ptr(new_lens), B, L, nq, nkv, hd, PT,
+                  block_table.shape[1], slots, _stream(None))
+    return q
+
+
 def merge_attn_states(o_a: torch.Tensor, lse_a: torch.Tensor, o_b: torch.Tensor,
                       lse_b: torch.Tensor, *, stream: torch.cuda.Stream | None = None):
     """Combine two attention results over disjoint key sets (LSE merge)."""
