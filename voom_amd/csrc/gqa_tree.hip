@@ -21,11 +21,14 @@
 // written from there; of the others a workgroup holds at most two pieces (its first
 // and its last), which gqa_tree_reduce_kernel merges.
 //
-// Per 32 tokens a wavefront loads K and V^T straight into MFMA operand registers,
-// NBUF blocks ahead, with the row tiles in the N dimension:
+// A wavefront has two buffers of 32 tokens of K and V^T in LDS of its own, filled by
+// direct-to-LDS loads (1 KiB each), so that one block is under way while the other is
+// computed, without a barrier.  The row tiles are in the N dimension:
 //   scores^T[token][row] = K . Q^T,  out^T[dim][row] += V^T . P^T   16x16x32 bf16
 // Row 4g + r of score tile t holds token 8g + 4t + r, so that a lane's scores are
-// the 8 consecutive tokens that its P^T operand needs.
+// the 8 consecutive tokens that its P^T operand needs.  (Blocks in registers instead, as
+// in the decode kernel, leave too few for 64 rows: 116 spilled, 1,076 us where this takes
+// 371.)
 //
 // P is rounded to bf16 for the matrix units; its sum, and with it the LSE, is kept
 // of the unrounded fp32 weights (the roundings average out in the output, whose own
@@ -90,11 +93,14 @@ __device__ __forceinline__ long long group_of_unit(long long u, long long U, int
   return ((u + 1) * W - 1) / U;
 }
 
+typedef __attribute__((address_space(3))) void lds_void;
+
+// Chunk c (16 bytes) of K row r sits at c ^ k_swizzle(r) of its row, chunk c of V^T row
+// d at c ^ (d >> 2 & 3): the 16 rows of an operand read then spread over all banks.
 template <int D>
-struct Block {
-  u32x4 k[2][D / 32];
-  u32x4 v[D / 16];
-};
+__device__ __forceinline__ int k_swizzle(int r) {
+  return D == 128 ? (r & 3) | ((r >> 3) & 3) << 2 : ((r >> 1) & 1) | ((r >> 3) & 3) << 1;
+}
 
 // The keys of the pages that one segment's wavefront walks.
 struct Pages {
@@ -102,11 +108,14 @@ struct Pages {
   int kvh, base, tab;  // base: first of the 64 pages whose slots the lanes hold in tab
 };
 
+constexpr int kTileElems(int D) { return 2 * kBlk * D; }  // K block, V^T block
+
+// Starts the loads of block bi into a wavefront's buffer.
 template <int D, int AUX>
-__device__ __forceinline__ void load_block(Block<D>& r, const TreeArgs& a, Pages& pg, int bi,
-                                           int end, int lane, int k_lane, int v_lane) {
-  const bool live = bi < end;  // past the end: empty loads, so that the ring needs no branch
-  if (!live) bi = end - 1;
+__device__ __forceinline__ void load_tile(uint16_t* tile, const TreeArgs& a, Pages& pg, int bi,
+                                          int lane) {
+  constexpr int kPieces = kBlk * D / 512;  // 1 KiB loads per block
+  constexpr int kCpr = D / 8;              // 16-byte chunks of a K row
   const int sub_shift = a.pt_shift - 5;
   const int page = bi >> sub_shift;
   const int sub = bi & ((1 << sub_shift) - 1);
@@ -119,21 +128,38 @@ __device__ __forceinline__ void load_block(Block<D>& r, const TreeArgs& a, Pages
   int slot = __builtin_amdgcn_readlane(pg.tab, page - pg.base);
   if (static_cast<unsigned>(slot) >= static_cast<unsigned>(a.num_slots)) slot = 0;
   const size_t at = ((static_cast<size_t>(slot) * a.NKV + pg.kvh) << sub_shift) + sub;
-  const int bytes = live ? kBlk * D * 2 : 0;
   const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint16_t*>(a.k_pool + at * (kBlk * D)), static_cast<short>(0), bytes, 0x00020000);
+      const_cast<uint16_t*>(a.k_pool + at * (kBlk * D)), static_cast<short>(0), kBlk * D * 2,
+      0x00020000);
   const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint16_t*>(a.v_pool + at * (kBlk * D)), static_cast<short>(0), bytes, 0x00020000);
+      const_cast<uint16_t*>(a.v_pool + at * (kBlk * D)), static_cast<short>(0), kBlk * D * 2,
+      0x00020000);
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-#pragma unroll
-    for (int s = 0; s < D / 32; ++s)
-      r.k[t][s] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_lane + (4 * t * D + 32 * s) * 2, 0,
-                                                        AUX);
+  for (int i = 0; i < kPieces; ++i) {
+    const int r = i * (kWave / kCpr) + lane / kCpr;
+    const int src = r * (D * 2) + 16 * ((lane % kCpr) ^ k_swizzle<D>(r));
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void*)(tile + i * 512), 16, src, 0, 0, AUX);
   }
 #pragma unroll
-  for (int n = 0; n < D / 16; ++n)
-    r.v[n] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_lane + n * (16 * kBlk * 2), 0, AUX);
+  for (int i = 0; i < kPieces; ++i) {
+    const int src = (lane >> 2) * (kBlk * 2) + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void*)(tile + kBlk * D + i * 512), 16, src,
+                                             i * 1024, 0, AUX);
+  }
+}
+
+// K operand of score tile t, k-step s, and V^T operand of dims 16 n.. of a buffer.
+template <int D>
+__device__ __forceinline__ u32x4 read_k(const uint16_t* tile, int t, int s, int lane) {
+  const int i16 = lane & 15, g = lane >> 4;
+  const int r = 8 * (i16 >> 2) + (i16 & 3) + 4 * t;
+  return *reinterpret_cast<const u32x4*>(tile + r * D + 8 * ((4 * s + g) ^ k_swizzle<D>(r)));
+}
+template <int D>
+__device__ __forceinline__ u32x4 read_v(const uint16_t* tile, int n, int lane) {
+  const int i16 = lane & 15, g = lane >> 4;
+  return *reinterpret_cast<const u32x4*>(tile + kBlk * D + (16 * n + i16) * kBlk +
+                                         8 * (g ^ (i16 >> 2)));
 }
 
 template <int D, int NT>
@@ -172,8 +198,8 @@ struct View {
 };
 
 template <int D, int NT>
-__device__ __forceinline__ void scores_of(const Block<D>& r, const u32x4 (&qop)[NT][D / 32],
-                                          f32x4 (&sc)[NT][2]) {
+__device__ __forceinline__ void scores_of(const uint16_t* tile, const uint16_t* ql,
+                                          f32x4 (&sc)[NT][2], int lane) {
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     sc[i][0] = f32x4{};
@@ -181,13 +207,16 @@ __device__ __forceinline__ void scores_of(const Block<D>& r, const u32x4 (&qop)[
   }
 #pragma unroll
   for (int s = 0; s < D / 32; ++s) {
+    const u32x4 k0 = read_k<D>(tile, 0, s, lane), k1 = read_k<D>(tile, 1, s, lane);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        sc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, r.k[t][s]),
-                                                           __builtin_bit_cast(bf16x8, qop[i][s]),
-                                                           sc[i][t], 0, 0, 0);
+      const u32x4 q = *reinterpret_cast<const u32x4*>(ql + i * 16 * (D + 8) + 32 * s);
+      sc[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k0),
+                                                         __builtin_bit_cast(bf16x8, q), sc[i][0],
+                                                         0, 0, 0);
+      sc[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k1),
+                                                         __builtin_bit_cast(bf16x8, q), sc[i][1],
+                                                         0, 0, 0);
     }
   }
 }
@@ -231,17 +260,18 @@ __device__ __forceinline__ void weights_of(const f32x4 (&sc)[NT][2], float scale
 }
 
 template <int D, int NT>
-__device__ __forceinline__ void whole_block(const Block<D>& r, const u32x4 (&qop)[NT][D / 32],
-                                            float scale, State<D, NT>& st) {
+__device__ __forceinline__ void whole_block(const uint16_t* tile, const uint16_t* ql, float scale,
+                                            State<D, NT>& st, int lane) {
   f32x4 sc[NT][2];
   u32x4 p[NT];
-  scores_of<D, NT>(r, qop, sc);
+  scores_of<D, NT>(tile, ql, sc, lane);
   weights_of<D, NT>(sc, scale, st, p);
 #pragma unroll
-  for (int i = 0; i < NT; ++i) {
+  for (int n = 0; n < D / 16; ++n) {
+    const u32x4 v = read_v<D>(tile, n, lane);
 #pragma unroll
-    for (int n = 0; n < D / 16; ++n)
-      st.acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, r.v[n]),
+    for (int i = 0; i < NT; ++i)
+      st.acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v),
                                                              __builtin_bit_cast(bf16x8, p[i]),
                                                              st.acc[i][n], 0, 0, 0);
   }
@@ -250,16 +280,16 @@ __device__ __forceinline__ void whole_block(const Block<D>& r, const u32x4 (&qop
 // A block with drafts or with tokens past the end.  Keys that a row does not see
 // score -inf.  Tokens past the end are garbage and are cut out of V^T; a draft that
 // only some rows see has P = 0 in the others, but 0 times a NaN or an infinity is
-// NaN: a block whose V holds one is taken key by key, each key added only to the
-// rows that see it.
+// NaN: where V holds one it is taken out, and products of indicators (V is NaN, +inf,
+// -inf; the row sees the key) say which sums it belongs to.
 template <int D, int NT>
-__device__ __forceinline__ void edge_block(Block<D>& r, const u32x4 (&qop)[NT][D / 32],
-                                           float scale, State<D, NT>& st, const View<NT>& view,
-                                           int bi, int lane) {
+__device__ __forceinline__ void edge_block(const uint16_t* tile, const uint16_t* ql, float scale,
+                                           State<D, NT>& st, const View<NT>& view, int bi,
+                                           int lane) {
   const int g = lane >> 4;
   f32x4 sc[NT][2];
   u32x4 p[NT];
-  scores_of<D, NT>(r, qop, sc);
+  scores_of<D, NT>(tile, ql, sc, lane);
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     const uint32_t seen = view.template seen<8>(i, bi * kBlk + 8 * g);
@@ -269,46 +299,64 @@ __device__ __forceinline__ void edge_block(Block<D>& r, const u32x4 (&qop)[NT][D
   }
   weights_of<D, NT>(sc, scale, st, p);
   const int valid = view.ctx - bi * kBlk - 8 * g;
+  uint32_t keep[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    keep[e] = (2 * e < valid ? 0xffffu : 0u) | (2 * e + 1 < valid ? 0xffff0000u : 0u);
   uint32_t odd = 0;  // not 0: V holds a NaN or an infinity
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t keep =
-        (2 * e < valid ? 0xffffu : 0u) | (2 * e + 1 < valid ? 0xffff0000u : 0u);
+  for (int n = 0; n < D / 16; ++n) {
+    u32x4 v = read_v<D>(tile, n, lane);
 #pragma unroll
-    for (int n = 0; n < D / 16; ++n) {
-      r.v[n][e] &= keep;
-      odd |= nan_bf16(r.v[n][e]);
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t bad = nan_bf16(v[e] & keep[e]);
+      odd |= bad;
+      v[e] &= keep[e] & ~bad;
     }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+      st.acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v),
+                                                             __builtin_bit_cast(bf16x8, p[i]),
+                                                             st.acc[i][n], 0, 0, 0);
   }
-  if (__builtin_amdgcn_ballot_w64(odd != 0) == 0) {
+  if (__builtin_amdgcn_ballot_w64(odd != 0) == 0) return;
+  u32x4 ones[NT];  // 1 where the row sees the key
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    const uint32_t seen = view.template seen<8>(i, bi * kBlk + 8 * g);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      ones[i][e] = ((seen >> 2 * e & 1) != 0 ? 0x3f80u : 0u) |
+                   ((seen >> (2 * e + 1) & 1) != 0 ? 0x3f800000u : 0u);
+  }
+#pragma unroll
+  for (int n = 0; n < D / 16; ++n) {
+    const u32x4 v = read_v<D>(tile, n, lane);
+    u32x4 is_nan, is_pos, is_neg;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = v[e] & keep[e], lo = x & 0xffffu, hi = x >> 16;
+      is_nan[e] = ((lo & 0x7fffu) > 0x7f80u ? 0x3f80u : 0u) |
+                  ((hi & 0x7fffu) > 0x7f80u ? 0x3f800000u : 0u);
+      is_pos[e] = (lo == 0x7f80u ? 0x3f80u : 0u) | (hi == 0x7f80u ? 0x3f800000u : 0u);
+      is_neg[e] = (lo == 0xff80u ? 0x3f80u : 0u) | (hi == 0xff80u ? 0x3f800000u : 0u);
+    }
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
+      const auto count = [&](u32x4 x) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x),
+                                                       __builtin_bit_cast(bf16x8, ones[i]),
+                                                       f32x4{}, 0, 0, 0);
+      };
+      const f32x4 nan = count(is_nan), pos = count(is_pos), neg = count(is_neg);
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n)
-        st.acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            __builtin_bit_cast(bf16x8, r.v[n]), __builtin_bit_cast(bf16x8, p[i]), st.acc[i][n], 0,
-            0, 0);
-    }
-    return;
-  }
-#pragma unroll 1
-  for (int k = 0; k < kBlk; ++k) {
-    const int mine = g == (k >> 3) ? (k & 7) : -1;
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const bool sees = view.template seen<1>(i, bi * kBlk + k) != 0;
-#pragma unroll
-      for (int n = 0; n < D / 16; ++n) {
-        u32x4 one_v;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          one_v[e] = r.v[n][e] & ((mine == 2 * e ? 0xffffu : 0u) |
-                                  (mine == 2 * e + 1 ? 0xffff0000u : 0u));
-        const f32x4 one = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            __builtin_bit_cast(bf16x8, one_v), __builtin_bit_cast(bf16x8, p[i]), f32x4{}, 0, 0, 0);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) st.acc[i][n][e] += sees ? one[e] : 0.f;
+      for (int e = 0; e < 4; ++e) {
+        float add = nan[e] > 0.f ? NAN : 0.f;
+        add += pos[e] > 0.f ? INFINITY : 0.f;
+        add -= neg[e] > 0.f ? INFINITY : 0.f;
+        st.acc[i][n][e] += add;
       }
+      __builtin_amdgcn_sched_barrier(0);  // one set of products in registers at a time
     }
   }
 }
@@ -337,14 +385,17 @@ __device__ void chunk_prefix(const TreeArgs& a, int* seg, int* wave_tot) {
 }
 
 template <int D, int NT, int AUX>
-__global__ __launch_bounds__(kThreads, 1) void gqa_tree_kernel(TreeArgs a) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void gqa_tree_kernel(TreeArgs a) {
   constexpr int kRows = 16 * NT;
-  // K/V blocks in registers: two ahead of the one computed, one where two do not fit
-  constexpr int kBuffers = NT * D <= 256 ? 3 : 2;
   constexpr int kPad = D + 4;  // floats of a row in LDS: 16 rows start in 16 bank groups
   __shared__ int seg[kMaxBatch + 1];
   __shared__ int wave_tot[kWaves];
-  __shared__ __attribute__((aligned(16))) float red_o[2][kWaves][16][kPad];
+  // The wavefronts' buffers.  Two distinct objects, so that reads of one provably miss
+  // the other's pending direct-to-LDS loads; the merge uses them when the loop is done.
+  __shared__ __attribute__((aligned(1024))) uint16_t tile_a[kWaves][kTileElems(D)];
+  __shared__ __attribute__((aligned(1024))) uint16_t tile_b[kWaves][kTileElems(D)];
+  static_assert(sizeof(float) * kWaves * 16 * kPad <= sizeof(tile_a), "a merge buffer fits");
+  __shared__ __attribute__((aligned(16))) uint16_t q_rows[kRows][D + 8];
   __shared__ float red_m[kWaves][kRows];
   __shared__ float red_l[kWaves][kRows];
 
@@ -388,9 +439,6 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_tree_kernel(TreeArgs a) {
     tile = s - kvh * a.tiles;
     begin = first + static_cast<long long>(s) * chunks;
   }
-  const int k_lane = ((8 * (i16 >> 2) + (i16 & 3)) * D + 8 * g) * 2;
-  const int v_lane = (i16 * kBlk + 8 * g) * 2;
-
   for (int piece = 0;; ++piece) {
     if (a.W == 0) {
       c0 = 0;
@@ -406,26 +454,30 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_tree_kernel(TreeArgs a) {
     view.prefix = ctx - view.drafts;
     view.mask = a.mask != nullptr ? a.mask + a.mask_stride * b : nullptr;
     view.T = a.T;
-    u32x4 qop[NT][D / 32];
+    // the rows' queries, for all wavefronts
+    for (int idx = threadIdx.x; idx < kRows * (D / 8); idx += kThreads) {
+      const int row = idx / (D / 8);
+      const int c = idx - row * (D / 8);
+      const int r = tile * kRows + row;
+      const int rc = r < a.R ? r : 0;
+      const int t = rc / a.G;
+      const int head = kvh * a.G + (rc - t * a.G);
+      u32x4 x = *reinterpret_cast<const u32x4*>(
+          a.q + ((static_cast<size_t>(b) * a.NQ + head) * a.T + t) * D + 8 * c);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] ^= a.q_flip;
+        if (a.q_zero) x[e] = nan_bf16(x[e]);
+      }
+      *reinterpret_cast<u32x4*>(&q_rows[row][8 * c]) = x;
+    }
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int r = tile * kRows + 16 * i + i16;
-      const bool ok = r < a.R;
-      const int t = (ok ? r : 0) / a.G;
-      view.t[i] = ok ? t : a.T;
-      const int head = kvh * a.G + (ok ? r - t * a.G : 0);
-      const uint16_t* qr = a.q + ((static_cast<size_t>(b) * a.NQ + head) * a.T + t) * D + 8 * g;
-#pragma unroll
-      for (int s = 0; s < D / 32; ++s) {
-        u32x4 x = *reinterpret_cast<const u32x4*>(qr + 32 * s);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[e] ^= a.q_flip;
-          if (a.q_zero) x[e] = nan_bf16(x[e]);
-        }
-        qop[i][s] = x;
-      }
+      view.t[i] = r < a.R ? r / a.G : a.T;
     }
+    __syncthreads();
+    const uint16_t* ql = &q_rows[i16][8 * g];
     State<D, NT> st;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -437,42 +489,45 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_tree_kernel(TreeArgs a) {
     }
 
     // This wavefront's blocks, kWaves c + wv for chunks c of the piece: those with
-    // drafts or the end of the sequence first (their code then shares no registers
-    // with the ring's), while the first whole blocks are under way.
+    // drafts or the end of the sequence first, while the first whole one is under way.
     const int nblk = (ctx + kBlk - 1) / kBlk;
     const int end = kWaves * c1 < nblk ? kWaves * c1 : nblk;
     int bi = kWaves * c0 + wv;
-    const int last = bi < end ? bi + (end - 1 - bi) / kWaves * kWaves : -1;
+    int edge = bi < end ? bi + (end - 1 - bi) / kWaves * kWaves : -1;  // the last one
     int whole = view.prefix / kBlk;  // blocks of which every row sees all
     whole = whole < end ? whole : end;
     Pages pg{a.table + static_cast<size_t>(b) * a.max_pages, kvh, -(1 << 30), 0};
-    if (last >= whole) {
-      Block<D> blk;
-#pragma unroll 1
-      for (int e = last; e >= whole && e >= bi; e -= kWaves) {
-        pg.base = -(1 << 30);
-        load_block<D, AUX>(blk, a, pg, e, end, lane, k_lane, v_lane);
-        edge_block<D, NT>(blk, qop, a.scale, st, view, e, lane);
-      }
+    uint16_t* ta = tile_a[wv];
+    uint16_t* tb = tile_b[wv];
+    const bool any = bi < whole;
+    if (edge >= whole) {
+      load_tile<D, AUX>(tb, a, pg, edge, lane);
       pg.base = -(1 << 30);
     }
-    if (bi < whole) {
-      Block<D> ring[kBuffers];
-#pragma unroll
-      for (int j = 0; j < kBuffers - 1; ++j)
-        load_block<D, AUX>(ring[j], a, pg, bi + j * kWaves, whole, lane, k_lane, v_lane);
-      bool done = false;
-      while (!done) {
-#pragma unroll
-        for (int j = 0; j < kBuffers; ++j) {
-          if (!done) {
-            load_block<D, AUX>(ring[(j + kBuffers - 1) % kBuffers], a, pg,
-                               bi + (kBuffers - 1) * kWaves, whole, lane, k_lane, v_lane);
-            whole_block<D, NT>(ring[j], qop, a.scale, st);
-            bi += kWaves;
-            done = bi >= whole;
-          }
-        }
+    if (any) load_tile<D, AUX>(ta, a, pg, bi, lane);
+    wait_vmem_all();
+    while (edge >= whole) {
+      edge_block<D, NT>(tb, ql, a.scale, st, view, edge, lane);
+      edge -= kWaves;
+      if (edge < whole || edge < bi) break;
+      Pages back{pg.row, kvh, -(1 << 30), 0};
+      load_tile<D, AUX>(tb, a, back, edge, lane);
+      wait_vmem_all();
+    }
+    // block bi has landed in ta; the next one goes into the other buffer
+    if (any) {
+      while (true) {
+        const bool more_b = bi + kWaves < whole;
+        if (more_b) load_tile<D, AUX>(tb, a, pg, bi + kWaves, lane);
+        whole_block<D, NT>(ta, ql, a.scale, st, lane);
+        if (!more_b) break;
+        wait_vmem_all();
+        bi += 2 * kWaves;
+        const bool more_a = bi < whole;
+        if (more_a) load_tile<D, AUX>(ta, a, pg, bi, lane);
+        whole_block<D, NT>(tb, ql, a.scale, st, lane);
+        if (!more_a) break;
+        wait_vmem_all();
       }
     }
 
@@ -487,9 +542,11 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_tree_kernel(TreeArgs a) {
     }
     const bool all = c0 == 0 && c1 == chunks;
     const size_t slot = 2 * static_cast<size_t>(w) + (piece > 0 ? 1 : 0);
+    __syncthreads();  // the buffers are no longer read
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      float(&buf)[kWaves][16][kPad] = red_o[i & 1];
+      typedef float Merge[kWaves][16][kPad];
+      Merge& buf = *reinterpret_cast<Merge*>(i & 1 ? &tile_b : &tile_a);
 #pragma unroll
       for (int n = 0; n < D / 16; ++n)
         *reinterpret_cast<f32x4*>(&buf[wv][i16][16 * n + 4 * g]) = st.acc[i][n];
@@ -542,7 +599,7 @@ __global__ __launch_bounds__(kThreads, 1) void gqa_tree_kernel(TreeArgs a) {
         chunks = uniform(seg[b + 1]) - uniform(seg[b]);
       }
     }
-    __syncthreads();  // the next piece writes red_m, red_l and red_o
+    __syncthreads();  // the next piece writes q_rows, red_m, red_l and the buffers
   }
 }
 
@@ -619,13 +676,13 @@ struct TreePlan {
   int W;      // workgroups of the split; 0: one per segment, no reduce launch
 };
 
-TreePlan plan_tree(int B, int NKV, int G, int T, int max_pages, int page_tokens) {
+TreePlan plan_tree(int head_dim, int G, int T, int max_pages, int page_tokens) {
   const int R = T * G;
   TreePlan p;
   p.nt = R <= 16 ? 1 : (R <= 32 ? 2 : 4);
   p.tiles = (R + 16 * p.nt - 1) / (16 * p.nt);
   const long long cap = static_cast<long long>(max_pages) * page_tokens;
-  p.W = cap <= 1024 ? 0 : device_cu_count();
+  p.W = cap <= 1024 ? 0 : device_cu_count() * (head_dim == 64 ? 2 : 1);  // all run at once
   return p;
 }
 
@@ -666,8 +723,7 @@ extern "C" size_t voom_paged_gqa_tree_workspace_bytes(int batch, int num_q_heads
                                                       int page_tokens, int max_pages) {
   if (!tree_shape_ok(batch, num_q_heads, num_kv_heads, head_dim, drafts, page_tokens, max_pages))
     return 0;
-  const TreePlan p = plan_tree(batch, num_kv_heads, num_q_heads / num_kv_heads, drafts, max_pages,
-                               page_tokens);
+  const TreePlan p = plan_tree(head_dim, num_q_heads / num_kv_heads, drafts, max_pages, page_tokens);
   return part_o_bytes(p, head_dim) + static_cast<size_t>(2) * p.W * 16 * p.nt * 2 * sizeof(float);
 }
 
@@ -695,7 +751,7 @@ extern "C" int voom_paged_gqa_tree(const void* q, const void* k_pool, const void
                    reinterpret_cast<uintptr_t>(out) % 8 == 0,
                "%s: q and pools must be 16-byte aligned", who);
   const int G = num_q_heads / num_kv_heads;
-  const TreePlan p = plan_tree(batch, num_kv_heads, G, drafts, max_pages, page_tokens);
+  const TreePlan p = plan_tree(head_dim, G, drafts, max_pages, page_tokens);
   const size_t need = voom_paged_gqa_tree_workspace_bytes(
       batch, num_q_heads, num_kv_heads, head_dim, drafts, page_tokens, max_pages);
   VOOM_REQUIRE(need == 0 || (workspace != nullptr && ws_bytes >= need &&
