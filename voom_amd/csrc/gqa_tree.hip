@@ -12,23 +12,25 @@
 // until about 100 (draft, head of a group) rows share them, then matrix work,
 // 4 NQ D flops per (draft, visible key).
 //
-// Work decomposition.  The rows of one (sequence, kv head) go in tiles of 16 NT
-// (NT = 1, 2, 4) that share every K/V byte.  A unit is a chunk of 128 tokens of one
-// (sequence, kv head, row tile) segment, 32 per wavefront; the units of all segments
-// lie end to end and workgroup w of W takes [w U/W, (w+1) U/W), so that all stream
-// the same number of bytes whatever the context lengths.  The wavefronts of a
-// workgroup merge their states through LDS.  A segment within one workgroup is
-// written from there; of the others a workgroup holds at most two pieces (its first
-// and its last), which gqa_tree_reduce_kernel merges.
+// Work decomposition.  A workgroup takes 64 rows (128 where there are more) of a
+// (sequence, kv head), so that up to 128 share every K/V byte.  A unit is a stage of
+// 64 tokens (128 at D = 64) of one (sequence, kv head, row tile) segment; the units of
+// all segments lie end to end and workgroup w of W takes [w U/W, (w+1) U/W): all stream
+// the same number of bytes whatever the context lengths.  A segment within one
+// workgroup is written from there; of the others a workgroup holds at most two pieces
+// (its first and its last), which gqa_tree_reduce_kernel merges.
 //
-// A wavefront has two buffers of 32 tokens of K and V^T in LDS of its own, filled by
-// direct-to-LDS loads (1 KiB each), so that one block is under way while the other is
-// computed, without a barrier.  The row tiles are in the N dimension:
+// Eight wavefronts, two per SIMD, so that one's matrix work runs beside the other's
+// exponentials: four groups of 16 NT rows, two wavefronts each, which take every
+// other 32-token block.  K and V^T go straight into LDS (buffer_load ... lds, 1 KiB
+// each) through a ring of four 32 KiB stages: three are under way while one is
+// computed (a ring of two per wavefront drained it at every stage: 371 us at 16
+// sequences of 1k-32k tokens, 16 drafts, 32/8 heads, where this takes TIME_BATCH; blocks
+// in registers, as in the decode kernel, leave too few for 64 rows: 1,076).  Per block,
+// with the rows in the N dimension:
 //   scores^T[token][row] = K . Q^T,  out^T[dim][row] += V^T . P^T   16x16x32 bf16
 // Row 4g + r of score tile t holds token 8g + 4t + r, so that a lane's scores are
-// the 8 consecutive tokens that its P^T operand needs.  (Blocks in registers instead, as
-// in the decode kernel, leave too few for 64 rows: 116 spilled, 1,076 us where this takes
-// 371.)
+// the 8 consecutive tokens that its P^T operand needs.
 //
 // P is rounded to bf16 for the matrix units; its sum, and with it the LSE, is kept
 // of the unrounded fp32 weights (the roundings average out in the output, whose own
@@ -41,10 +43,15 @@
 namespace voom {
 namespace {
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kBlk = 32;               // tokens of a K/V block in the pool
-constexpr int kChunk = kWaves * kBlk;  // tokens of a unit
+constexpr int kBlk = 32;      // tokens of a K/V block in the pool
+constexpr int kKeyWaves = 2;  // wavefronts that share a group of rows
+constexpr int kRowWaves = kWaves / kKeyWaves;
+constexpr int kStages = 4;    // stages of the ring in LDS
+constexpr int kStageElems = 2 * 64 * 128;  // of K and V^T
+constexpr int stage_blocks(int D) { return kStageElems / (2 * kBlk * D); }
+constexpr int stage_tokens(int D) { return stage_blocks(D) * kBlk; }
 constexpr int kMaxBatch = 1024;
 constexpr int kMaxDrafts = 1024;
 
@@ -58,8 +65,8 @@ struct TreeArgs {
   const uint8_t* mask;    // [T, T] or [B, T, T] of 0 / 1, or null: causal
   uint16_t* out;          // [B, T, NQ, D]
   float* lse;             // [B, T, NQ], or null
-  float* part_o;          // [2 W, 16 NT, D]
-  float* part_ml;         // [2 W, 16 NT, 2]
+  float* part_o;          // [2 W, rows, D]
+  float* part_ml;         // [2 W, rows, 2]
   long long mask_stride;  // elements from one sequence's mask to the next
   int B, NQ, NKV, G, T, max_pages, pt_shift, num_slots;
   int R;         // rows of a (sequence, kv head): T * G, (draft, head), head fastest
@@ -86,7 +93,11 @@ __device__ __forceinline__ int drafts_of(const TreeArgs& a, int b, int ctx) {
   return n < ctx ? n : ctx;
 }
 
-__device__ __forceinline__ int chunks_of(int ctx) { return (ctx + kChunk - 1) / kChunk; }
+// Units of a context.
+template <int D>
+__device__ __forceinline__ int chunks_of(int ctx) {
+  return (ctx + stage_tokens(D) - 1) / stage_tokens(D);
+}
 
 // Workgroup of the split that holds unit u (the last w with w U/W <= u).
 __device__ __forceinline__ long long group_of_unit(long long u, long long U, int W) {
@@ -102,49 +113,55 @@ __device__ __forceinline__ int k_swizzle(int r) {
   return D == 128 ? (r & 3) | ((r >> 3) & 3) << 2 : ((r >> 1) & 1) | ((r >> 3) & 3) << 1;
 }
 
-// The keys of the pages that one segment's wavefront walks.
+// The keys of the pages that one segment's wavefronts walk.
 struct Pages {
   const int32_t* row;  // the sequence's table row
-  int kvh, base, tab;  // base: first of the 64 pages whose slots the lanes hold in tab
+  int kvh, last;       // last: the context's last block
+  int base, tab;       // base: first of the 64 pages whose slots the lanes hold in tab
 };
 
-constexpr int kTileElems(int D) { return 2 * kBlk * D; }  // K block, V^T block
+// A block of a stage in LDS: K [32][D], then V^T [D][32].
+constexpr int block_elems(int D) { return 2 * kBlk * D; }
 
-// Starts the loads of block bi into a wavefront's buffer.
+// Starts this wavefront's loads (of 1 KiB) of the stage whose first block is bi; blocks
+// past the context repeat its last one, and are not used.
 template <int D, int AUX>
-__device__ __forceinline__ void load_tile(uint16_t* tile, const TreeArgs& a, Pages& pg, int bi,
-                                          int lane) {
-  constexpr int kPieces = kBlk * D / 512;  // 1 KiB loads per block
+__device__ __forceinline__ void load_stage(uint16_t* stage, const TreeArgs& a, Pages& pg, int bi,
+                                           int wv, int lane) {
+  constexpr int kBlocks = stage_blocks(D);
+  constexpr int kPieces = kBlk * D / 512;  // of K, and of V^T, of a block
   constexpr int kCpr = D / 8;              // 16-byte chunks of a K row
   const int sub_shift = a.pt_shift - 5;
-  const int page = bi >> sub_shift;
-  const int sub = bi & ((1 << sub_shift) - 1);
-  if (page >= pg.base + kWave) {
-    pg.base = page;
-    const int p = page + lane;
+  const int first = bi < pg.last ? bi : pg.last;
+  if ((first + kBlocks - 1) >> sub_shift >= pg.base + kWave) {
+    pg.base = first >> sub_shift;
+    const int p = pg.base + lane;
     pg.tab = p < a.max_pages ? pg.row[p] : 0;
-    wait_vmem_all();  // here, not at the readlane below on every block
-  }
-  int slot = __builtin_amdgcn_readlane(pg.tab, page - pg.base);
-  if (static_cast<unsigned>(slot) >= static_cast<unsigned>(a.num_slots)) slot = 0;
-  const size_t at = ((static_cast<size_t>(slot) * a.NKV + pg.kvh) << sub_shift) + sub;
-  const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint16_t*>(a.k_pool + at * (kBlk * D)), static_cast<short>(0), kBlk * D * 2,
-      0x00020000);
-  const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<uint16_t*>(a.v_pool + at * (kBlk * D)), static_cast<short>(0), kBlk * D * 2,
-      0x00020000);
-#pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int r = i * (kWave / kCpr) + lane / kCpr;
-    const int src = r * (D * 2) + 16 * ((lane % kCpr) ^ k_swizzle<D>(r));
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void*)(tile + i * 512), 16, src, 0, 0, AUX);
+    wait_vmem_all();  // here, not at the readlanes below on every stage
   }
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int src = (lane >> 2) * (kBlk * 2) + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void*)(tile + kBlk * D + i * 512), 16, src,
-                                             i * 1024, 0, AUX);
+  for (int i = 0; i < 2 * kBlocks * kPieces / kWaves; ++i) {
+    // piece p = wv + 8 i: block p / (2 kPieces), first its K and then its V^T
+    const int p = wv + kWaves * i;
+    const int blk = p / (2 * kPieces);
+    const int in_blk = p % (2 * kPieces);
+    int at_blk = bi + blk;
+    at_blk = at_blk < pg.last ? at_blk : pg.last;
+    const int page = at_blk >> sub_shift;
+    int slot = __builtin_amdgcn_readlane(pg.tab, page - pg.base);
+    if (static_cast<unsigned>(slot) >= static_cast<unsigned>(a.num_slots)) slot = 0;
+    const size_t at = ((static_cast<size_t>(slot) * a.NKV + pg.kvh) << sub_shift) +
+                      (at_blk - (page << sub_shift));
+    const bool is_v = in_blk >= kPieces;
+    const int sub = in_blk % kPieces;
+    const uint16_t* from = (is_v ? a.v_pool : a.k_pool) + at * (kBlk * D);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t*>(from), static_cast<short>(0), kBlk * D * 2, 0x00020000);
+    const int krow = sub * (kWave / kCpr) + lane / kCpr;
+    const int ksrc = krow * (D * 2) + 16 * ((lane % kCpr) ^ k_swizzle<D>(krow));
+    const int vsrc = sub * 1024 + (lane >> 2) * (kBlk * 2) + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(stage + p * 512), 16,
+                                             is_v ? vsrc : ksrc, 0, 0, AUX);
   }
 }
 
@@ -176,30 +193,36 @@ struct View {
   int t[NT];            // the draft of the column's row in each tile; T: no row
   const uint8_t* mask;  // the sequence's mask, or null
   int T;
-  // Bit e: the row of tile i sees token pos + e.  Straight-line code: every mask
-  // byte is loaded from inside the mask and then chosen or not.
-  template <int N>
+  // Bit e: the row of tile i sees token pos + e, e < 8.  Bytes beside the row are read and
+  // not used; outside the sequence's mask the buffer gives 0.
   __device__ __forceinline__ uint32_t seen(int i, int pos) const {
-    const int row = t[i] < T ? t[i] : T - 1;
+    const int j = pos - prefix;
     uint32_t bits = 0;
+    if (mask != nullptr) {
+      const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(mask), static_cast<short>(0), T * T, 0x00020000);
+      uint8_t m[8];
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const int j = pos + e - prefix;
-      int ok = j <= t[i];
-      if (mask != nullptr) {
-        const int jc = j < 0 ? 0 : (j < T ? j : T - 1);
-        ok = mask[static_cast<size_t>(row) * T + jc] != 0;
-      }
-      ok = (j < 0) | ((j < drafts) & ok);
-      bits |= static_cast<uint32_t>(ok) << e;
+      for (int e = 0; e < 8; ++e)
+        m[e] = __builtin_amdgcn_raw_buffer_load_b8(r, t[i] * T + j + e, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bits |= (m[e] != 0 ? 1u : 0u) << e;
+    } else {
+      const int n = t[i] - j + 1;  // tokens up to the draft's own
+      bits = n >= 8 ? 0xffu : (n > 0 ? (1u << n) - 1 : 0u);
     }
+    const int d = drafts - j;  // tokens up to the context's end
+    bits &= d >= 8 ? 0xffu : (d > 0 ? (1u << d) - 1 : 0u);
+    const int before = -j;     // tokens before the drafts
+    bits |= before >= 8 ? 0xffu : (before > 0 ? (1u << before) - 1 : 0u);
     return t[i] < drafts ? bits : 0u;
   }
 };
 
 template <int D, int NT>
-__device__ __forceinline__ void scores_of(const uint16_t* tile, const uint16_t* ql,
-                                          f32x4 (&sc)[NT][2], int lane) {
+__device__ __forceinline__ void scores_of(const uint16_t* tile,
+                                          const u32x4 (&qop)[NT][D / 32], f32x4 (&sc)[NT][2],
+                                          int lane) {
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     sc[i][0] = f32x4{};
@@ -210,7 +233,7 @@ __device__ __forceinline__ void scores_of(const uint16_t* tile, const uint16_t* 
     const u32x4 k0 = read_k<D>(tile, 0, s, lane), k1 = read_k<D>(tile, 1, s, lane);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const u32x4 q = *reinterpret_cast<const u32x4*>(ql + i * 16 * (D + 8) + 32 * s);
+      const u32x4 q = qop[i][s];
       sc[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k0),
                                                          __builtin_bit_cast(bf16x8, q), sc[i][0],
                                                          0, 0, 0);
@@ -260,11 +283,12 @@ __device__ __forceinline__ void weights_of(const f32x4 (&sc)[NT][2], float scale
 }
 
 template <int D, int NT>
-__device__ __forceinline__ void whole_block(const uint16_t* tile, const uint16_t* ql, float scale,
+__device__ __forceinline__ void whole_block(const uint16_t* tile,
+                                            const u32x4 (&qop)[NT][D / 32], float scale,
                                             State<D, NT>& st, int lane) {
   f32x4 sc[NT][2];
   u32x4 p[NT];
-  scores_of<D, NT>(tile, ql, sc, lane);
+  scores_of<D, NT>(tile, qop, sc, lane);
   weights_of<D, NT>(sc, scale, st, p);
 #pragma unroll
   for (int n = 0; n < D / 16; ++n) {
@@ -283,19 +307,21 @@ __device__ __forceinline__ void whole_block(const uint16_t* tile, const uint16_t
 // NaN: where V holds one it is taken out, and products of indicators (V is NaN, +inf,
 // -inf; the row sees the key) say which sums it belongs to.
 template <int D, int NT>
-__device__ __forceinline__ void edge_block(const uint16_t* tile, const uint16_t* ql, float scale,
+__device__ __forceinline__ void edge_block(const uint16_t* tile,
+                                           const u32x4 (&qop)[NT][D / 32], float scale,
                                            State<D, NT>& st, const View<NT>& view, int bi,
                                            int lane) {
   const int g = lane >> 4;
   f32x4 sc[NT][2];
   u32x4 p[NT];
-  scores_of<D, NT>(tile, ql, sc, lane);
+  scores_of<D, NT>(tile, qop, sc, lane);
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    const uint32_t seen = view.template seen<8>(i, bi * kBlk + 8 * g);
+    const uint32_t seen = view.seen(i, bi * kBlk + 8 * g);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       sc[i][e >> 2][e & 3] = (seen >> e & 1) != 0 ? sc[i][e >> 2][e & 3] : -INFINITY;
+    __builtin_amdgcn_sched_barrier(0);
   }
   weights_of<D, NT>(sc, scale, st, p);
   const int valid = view.ctx - bi * kBlk - 8 * g;
@@ -323,7 +349,7 @@ __device__ __forceinline__ void edge_block(const uint16_t* tile, const uint16_t*
   u32x4 ones[NT];  // 1 where the row sees the key
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
-    const uint32_t seen = view.template seen<8>(i, bi * kBlk + 8 * g);
+    const uint32_t seen = view.seen(i, bi * kBlk + 8 * g);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       ones[i][e] = ((seen >> 2 * e & 1) != 0 ? 0x3f80u : 0u) |
@@ -363,6 +389,7 @@ __device__ __forceinline__ void edge_block(const uint16_t* tile, const uint16_t*
 
 // Exclusive prefix sum of the sequences' chunk counts into seg[0..B]; ends with a
 // barrier.
+template <int D>
 __device__ void chunk_prefix(const TreeArgs& a, int* seg, int* wave_tot) {
   const int t = threadIdx.x;
   const int lane = t & (kWave - 1);
@@ -370,7 +397,7 @@ __device__ void chunk_prefix(const TreeArgs& a, int* seg, int* wave_tot) {
   int carry = 0;
   for (int base = 0; base < a.B; base += kThreads) {
     const int i = base + t;
-    const int n = i < a.B ? chunks_of(context_of(a, i)) : 0;
+    const int n = i < a.B ? chunks_of<D>(context_of(a, i)) : 0;
     const int x = wave_inclusive_scan(n, lane);
     if (lane == kWave - 1) wave_tot[wv] = x;
     __syncthreads();
@@ -385,22 +412,26 @@ __device__ void chunk_prefix(const TreeArgs& a, int* seg, int* wave_tot) {
 }
 
 template <int D, int NT, int AUX>
-__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void gqa_tree_kernel(TreeArgs a) {
-  constexpr int kRows = 16 * NT;
+__global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
+  constexpr int kRows = 16 * NT * kRowWaves;
+  constexpr int kBlocks = stage_blocks(D);
+  constexpr int kLoads = 2 * kBlocks * (kBlk * D / 512) / kWaves;  // a wavefront's, of a stage
   constexpr int kPad = D + 4;  // floats of a row in LDS: 16 rows start in 16 bank groups
   __shared__ int seg[kMaxBatch + 1];
   __shared__ int wave_tot[kWaves];
-  // The wavefronts' buffers.  Two distinct objects, so that reads of one provably miss
-  // the other's pending direct-to-LDS loads; the merge uses them when the loop is done.
-  __shared__ __attribute__((aligned(1024))) uint16_t tile_a[kWaves][kTileElems(D)];
-  __shared__ __attribute__((aligned(1024))) uint16_t tile_b[kWaves][kTileElems(D)];
-  static_assert(sizeof(float) * kWaves * 16 * kPad <= sizeof(tile_a), "a merge buffer fits");
-  __shared__ __attribute__((aligned(16))) uint16_t q_rows[kRows][D + 8];
-  __shared__ float red_m[kWaves][kRows];
-  __shared__ float red_l[kWaves][kRows];
+  // The ring.  Distinct objects, so that reads of one provably miss the pending
+  // direct-to-LDS loads of the others; the merge uses them when the loop is done.
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_0[kStageElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_1[kStageElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_2[kStageElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_3[kStageElems];
+  static_assert(kLoads == 4, "the waits below count the loads of a stage");
+  static_assert(sizeof(float) * NT * 16 * kPad <= sizeof(stage_0), "a merge buffer fits a stage");
 
   const int lane = threadIdx.x & (kWave - 1);
   const int wv = uniform(threadIdx.x / kWave);
+  const int kw = wv % kKeyWaves;
+  const int rw = wv / kKeyWaves;
   const int i16 = lane & 15;
   const int g = lane >> 4;
   // Consecutive workgroups of one XCD take consecutive units, so that the row tiles
@@ -415,12 +446,12 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void gqa_tree_kernel(Tre
   if (a.W == 0) {
     if (w >= a.B * per_b) return;
     b = w / per_b;
-    chunks = uniform(chunks_of(context_of(a, b)));
+    chunks = uniform(chunks_of<D>(context_of(a, b)));
     const int s = w - b * per_b;
     kvh = s / a.tiles;
     tile = s - kvh * a.tiles;
   } else {
-    chunk_prefix(a, seg, wave_tot);
+    chunk_prefix<D>(a, seg, wave_tot);
     const long long U = static_cast<long long>(uniform(seg[a.B])) * per_b;
     We = static_cast<int>(U < a.W ? U : a.W);
     if (w >= We) return;
@@ -454,30 +485,32 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void gqa_tree_kernel(Tre
     view.prefix = ctx - view.drafts;
     view.mask = a.mask != nullptr ? a.mask + a.mask_stride * b : nullptr;
     view.T = a.T;
-    // the rows' queries, for all wavefronts
-    for (int idx = threadIdx.x; idx < kRows * (D / 8); idx += kThreads) {
-      const int row = idx / (D / 8);
-      const int c = idx - row * (D / 8);
-      const int r = tile * kRows + row;
-      const int rc = r < a.R ? r : 0;
-      const int t = rc / a.G;
-      const int head = kvh * a.G + (rc - t * a.G);
-      u32x4 x = *reinterpret_cast<const u32x4*>(
-          a.q + ((static_cast<size_t>(b) * a.NQ + head) * a.T + t) * D + 8 * c);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] ^= a.q_flip;
-        if (a.q_zero) x[e] = nan_bf16(x[e]);
-      }
-      *reinterpret_cast<u32x4*>(&q_rows[row][8 * c]) = x;
-    }
+    // Q^T operands of this wavefront's rows
+    u32x4 qop[NT][D / 32];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int r = tile * kRows + 16 * i + i16;
-      view.t[i] = r < a.R ? r / a.G : a.T;
+      const int r = tile * kRows + rw * (16 * NT) + 16 * i + i16;
+      const int t = (r < a.R ? r : 0) / a.G;
+      view.t[i] = r < a.R ? t : a.T;
+      const int head = kvh * a.G + (r < a.R ? r - t * a.G : 0);
+      const uint16_t* qr = a.q + ((static_cast<size_t>(b) * a.NQ + head) * a.T + t) * D + 8 * g;
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) {
+        qop[i][s] = *reinterpret_cast<const u32x4*>(qr + 32 * s);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qop[i][s][e] ^= a.q_flip;
+      }
     }
-    __syncthreads();
-    const uint16_t* ql = &q_rows[i16][8 * g];
+    if (a.q_zero) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qop[i][s][e] = nan_bf16(qop[i][s][e]);
+        }
+      }
+    }
     State<D, NT> st;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
@@ -488,100 +521,111 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void gqa_tree_kernel(Tre
       for (int n = 0; n < D / 16; ++n) st.acc[i][n] = f32x4{};
     }
 
-    // This wavefront's blocks, kWaves c + wv for chunks c of the piece: those with
-    // drafts or the end of the sequence first, while the first whole one is under way.
-    const int nblk = (ctx + kBlk - 1) / kBlk;
-    const int end = kWaves * c1 < nblk ? kWaves * c1 : nblk;
-    int bi = kWaves * c0 + wv;
-    int edge = bi < end ? bi + (end - 1 - bi) / kWaves * kWaves : -1;  // the last one
-    int whole = view.prefix / kBlk;  // blocks of which every row sees all
-    whole = whole < end ? whole : end;
-    Pages pg{a.table + static_cast<size_t>(b) * a.max_pages, kvh, -(1 << 30), 0};
-    uint16_t* ta = tile_a[wv];
-    uint16_t* tb = tile_b[wv];
-    const bool any = bi < whole;
-    if (edge >= whole) {
-      load_tile<D, AUX>(tb, a, pg, edge, lane);
-      pg.base = -(1 << 30);
-    }
-    if (any) load_tile<D, AUX>(ta, a, pg, bi, lane);
-    wait_vmem_all();
-    while (edge >= whole) {
-      edge_block<D, NT>(tb, ql, a.scale, st, view, edge, lane);
-      edge -= kWaves;
-      if (edge < whole || edge < bi) break;
-      Pages back{pg.row, kvh, -(1 << 30), 0};
-      load_tile<D, AUX>(tb, a, back, edge, lane);
+    // Stages c0 .. c1.  Those with drafts or the end of the context come first, one at a
+    // time through stage_3 while the first of the others are under way; of the others
+    // every row sees all, and stage t of them is in t % 4.
+    const int last_blk = (ctx - 1) / kBlk;
+    Pages pg{a.table + static_cast<size_t>(b) * a.max_pages, kvh, last_blk, -(1 << 30), 0};
+    int whole = view.prefix / stage_tokens(D);
+    whole = whole < c1 ? whole : c1;
+    const bool rows_here = tile * kRows + rw * (16 * NT) < a.R;  // (else this wavefront only loads)
+    int t = c0;
+    auto load = [&](int at, uint16_t* stage) {
+      load_stage<D, AUX>(stage, a, pg, at * kBlocks, wv, lane);
+    };
+    if (t < whole) load(t, stage_0);
+    if (t + 1 < whole) load(t + 1, stage_1);
+    if (t + 2 < whole) load(t + 2, stage_2);
+#pragma unroll 1
+    for (int e = whole > c0 ? whole : c0; e < c1; ++e) {
+      Pages back{pg.row, kvh, last_blk, -(1 << 30), 0};
+      load_stage<D, AUX>(stage_3, a, back, e * kBlocks, wv, lane);
       wait_vmem_all();
-    }
-    // block bi has landed in ta; the next one goes into the other buffer
-    if (any) {
-      while (true) {
-        const bool more_b = bi + kWaves < whole;
-        if (more_b) load_tile<D, AUX>(tb, a, pg, bi + kWaves, lane);
-        whole_block<D, NT>(ta, ql, a.scale, st, lane);
-        if (!more_b) break;
-        wait_vmem_all();
-        bi += 2 * kWaves;
-        const bool more_a = bi < whole;
-        if (more_a) load_tile<D, AUX>(ta, a, pg, bi, lane);
-        whole_block<D, NT>(tb, ql, a.scale, st, lane);
-        if (!more_a) break;
-        wait_vmem_all();
+      lds_barrier();
+      if (rows_here) {
+#pragma unroll 1
+        for (int j = kw; j < kBlocks && e * kBlocks + j <= last_blk; j += kKeyWaves)
+          edge_block<D, NT>(stage_3 + j * block_elems(D), qop, a.scale, st, view, e * kBlocks + j,
+                            lane);
       }
+      lds_barrier();  // stage_3 is loaded again
     }
-
-    // merge the wavefronts
+    auto step = [&](const uint16_t* cur, uint16_t* free) {
+      // Stage t has landed for every wavefront, and stage t - 1 is no longer read.  gfx9
+      // encoding: vmcnt of the loads of stages t + 1 and t + 2, expcnt 7, lgkmcnt 15.
+      if (t + 2 < whole) __builtin_amdgcn_s_waitcnt(0x0F78);
+      else if (t + 1 < whole) __builtin_amdgcn_s_waitcnt(0x0F74);
+      else __builtin_amdgcn_s_waitcnt(0x0F70);
+      lds_barrier();
+      if (t + 3 < whole) load(t + 3, free);
+      if (rows_here) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const float lt = wave_sum_across_groups(st.l[i]);
-      if (g == 0) {
-        red_m[wv][16 * i + i16] = st.m[i];
-        red_l[wv][16 * i + i16] = lt;
+        for (int j = 0; j < kBlocks / kKeyWaves; ++j)
+          whole_block<D, NT>(cur + (kKeyWaves * j + kw) * block_elems(D), qop, a.scale, st, lane);
+      }
+      return ++t < whole;
+    };
+    if (t < whole) {
+      while (step(stage_0, stage_3) && step(stage_1, stage_0) && step(stage_2, stage_1) &&
+             step(stage_3, stage_2)) {
       }
     }
+    wait_vmem_all();
+    lds_barrier();  // the ring is no longer read or written
+
+    // Merge the two wavefronts of each group of rows: one leaves its state in LDS, the
+    // other adds its own and writes.
     const bool all = c0 == 0 && c1 == chunks;
     const size_t slot = 2 * static_cast<size_t>(w) + (piece > 0 ? 1 : 0);
-    __syncthreads();  // the buffers are no longer read
+    uint16_t* const merge = rw < 2 ? (rw == 0 ? stage_0 : stage_1) : (rw == 2 ? stage_2 : stage_3);
+    float lt[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) lt[i] = wave_sum_across_groups(st.l[i]);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      typedef float Merge[kWaves][16][kPad];
-      Merge& buf = *reinterpret_cast<Merge*>(i & 1 ? &tile_b : &tile_a);
+      float* const buf = reinterpret_cast<float*>(merge) + i * 16 * kPad;
+      if (kw == 1 && rows_here) {
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n)
-        *reinterpret_cast<f32x4*>(&buf[wv][i16][16 * n + 4 * g]) = st.acc[i][n];
-      __syncthreads();
-      for (int idx = threadIdx.x; idx < 16 * (D / 4); idx += kThreads) {
-        const int row = idx / (D / 4);
-        const int d = (idx - row * (D / 4)) * 4;
-        const int r = 16 * i + row;
-        float M = red_m[0][r];
-#pragma unroll
-        for (int k = 1; k < kWaves; ++k) M = fmaxf(M, red_m[k][r]);
-        float L = 0.f;
-        f32x4 o = {};
-#pragma unroll
-        for (int k = 0; k < kWaves; ++k) {
-          const float wt = fast_exp2(red_m[k][r] - M);
-          L += red_l[k][r] * wt;
-          o += *reinterpret_cast<const f32x4*>(&buf[k][row][d]) * wt;
+        for (int n = 0; n < D / 16; ++n)
+          *reinterpret_cast<f32x4*>(buf + i16 * kPad + 16 * n + 4 * g) = st.acc[i][n];
+        if (g == 0) {
+          buf[i16 * kPad + D] = st.m[i];
+          buf[i16 * kPad + D + 1] = lt[i];
         }
-        if (!all) {
-          *reinterpret_cast<f32x4*>(a.part_o + (slot * kRows + r) * D + d) = o;
-          if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (slot * kRows + r) * 2) = {M, L};
-          continue;
-        }
+      }
+    }
+    __syncthreads();
+    if (kw == 0 && rows_here) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const float* const buf = reinterpret_cast<const float*>(merge) + (i * 16 + i16) * kPad;
+        const float m1 = buf[D];
+        const float M = fmaxf(st.m[i], m1);
+        const float f0 = fast_exp2(st.m[i] - M), f1 = fast_exp2(m1 - M);
+        const float L = lt[i] * f0 + buf[D + 1] * f1;
+        const int r = rw * (16 * NT) + 16 * i + i16;
         const int rr = tile * kRows + r;
-        if (rr >= a.R) continue;
-        const int t = rr / a.G;
-        const int head = kvh * a.G + (rr - t * a.G);
-        const size_t at = (static_cast<size_t>(b) * a.T + t) * a.NQ + head;
-        const bool empty = t >= view.drafts || L == 0.f;
-        const float inv = empty ? 0.f : 1.f / L;
-        *reinterpret_cast<u32x2*>(a.out + at * D + d) =
-            empty ? u32x2{0u, 0u}
-                  : u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
-        if (a.lse != nullptr && d == 0)
+        const int t_row = view.t[i];
+        const bool empty = t_row >= view.drafts || L == 0.f;
+        const float inv = 1.f / L;
+        const int head = kvh * a.G + (rr - t_row * a.G);
+        const size_t at = (static_cast<size_t>(b) * a.T + t_row) * a.NQ + head;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+          const f32x4 o =
+              st.acc[i][n] * f0 + *reinterpret_cast<const f32x4*>(buf + 16 * n + 4 * g) * f1;
+          if (!all) {
+            *reinterpret_cast<f32x4*>(a.part_o + (slot * kRows + r) * D + 16 * n + 4 * g) = o;
+          } else if (rr < a.R) {
+            *reinterpret_cast<u32x2*>(a.out + at * D + 16 * n + 4 * g) =
+                empty ? u32x2{0u, 0u}
+                      : u32x2{pack_bf16x2(o[0] * inv, o[1] * inv),
+                              pack_bf16x2(o[2] * inv, o[3] * inv)};
+          }
+        }
+        if (g == 0 && !all)
+          *reinterpret_cast<float2*>(a.part_ml + (slot * kRows + r) * 2) = {M, L};
+        if (g == 0 && all && rr < a.R && a.lse != nullptr)
           a.lse[at] = empty ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
       }
     }
@@ -599,17 +643,20 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 1) void gqa_tree_kernel(Tre
         chunks = uniform(seg[b + 1]) - uniform(seg[b]);
       }
     }
-    __syncthreads();  // the next piece writes q_rows, red_m, red_l and the buffers
+    __syncthreads();  // the next piece writes the ring
   }
 }
+
+constexpr int kReduceWaves = 4;
 
 // One wavefront per row: merges the pieces of its segment, where the split cut it;
 // rows of sequences without tokens are written here.
 template <int D>
-__global__ __launch_bounds__(kThreads) void gqa_tree_reduce_kernel(TreeArgs a, int rows_per_tile) {
+__global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(TreeArgs a, int rows_per_tile) {
   constexpr int DPL = D / kWave;
   const int lane = threadIdx.x & (kWave - 1);
-  const long long task = static_cast<long long>(blockIdx.x) * kWaves + uniform(threadIdx.x / kWave);
+  const long long task =
+      static_cast<long long>(blockIdx.x) * kReduceWaves + uniform(threadIdx.x / kWave);
   if (task >= static_cast<long long>(a.B) * a.NKV * a.R) return;
   const int seg = static_cast<int>(task / a.R);
   const int rr = static_cast<int>(task - static_cast<long long>(seg) * a.R);
@@ -621,7 +668,7 @@ __global__ __launch_bounds__(kThreads) void gqa_tree_reduce_kernel(TreeArgs a, i
   int before = 0, chunks = 0, total = 0;
   for (int base = 0; base < a.B; base += kWave) {
     const int i = base + lane;
-    const int n = i < a.B ? chunks_of(context_of(a, i)) : 0;
+    const int n = i < a.B ? chunks_of<D>(context_of(a, i)) : 0;
     const int x = wave_inclusive_scan(n, lane);
     if (b >= base && b < base + kWave) {
       before = total + __builtin_amdgcn_readlane(x - n, b - base);
@@ -671,18 +718,20 @@ __global__ __launch_bounds__(kThreads) void gqa_tree_reduce_kernel(TreeArgs a, i
 
 // How a call is cut.
 struct TreePlan {
-  int nt;     // 16-row column tiles of a wavefront
+  int nt;     // 16-row tiles of a wavefront
+  int rows;   // rows of a workgroup
   int tiles;  // row tiles of a (sequence, kv head)
   int W;      // workgroups of the split; 0: one per segment, no reduce launch
 };
 
-TreePlan plan_tree(int head_dim, int G, int T, int max_pages, int page_tokens) {
+TreePlan plan_tree(int G, int T, int max_pages, int page_tokens) {
   const int R = T * G;
   TreePlan p;
-  p.nt = R <= 16 ? 1 : (R <= 32 ? 2 : 4);
-  p.tiles = (R + 16 * p.nt - 1) / (16 * p.nt);
+  p.nt = R <= 64 ? 1 : 2;
+  p.rows = 16 * p.nt * kRowWaves;
+  p.tiles = (R + p.rows - 1) / p.rows;
   const long long cap = static_cast<long long>(max_pages) * page_tokens;
-  p.W = cap <= 1024 ? 0 : device_cu_count() * (head_dim == 64 ? 2 : 1);  // all run at once
+  p.W = cap <= 1024 ? 0 : device_cu_count();  // all run at once
   return p;
 }
 
@@ -697,7 +746,7 @@ bool tree_shape_ok(int batch, int num_q_heads, int num_kv_heads, int head_dim, i
 }
 
 size_t part_o_bytes(const TreePlan& p, int D) {
-  return static_cast<size_t>(2) * p.W * 16 * p.nt * D * sizeof(float);
+  return static_cast<size_t>(2) * p.W * p.rows * D * sizeof(float);
 }
 
 template <int D>
@@ -705,12 +754,10 @@ void launch_tree(const TreeArgs& a, const TreePlan& p, dim3 grid, hipStream_t st
   // (a byte of K/V that one row tile alone reads is streamed past the caches)
   if (p.nt == 1)
     hipLaunchKernelGGL((gqa_tree_kernel<D, 1, 2>), grid, dim3(kThreads), 0, stream, a);
-  else if (p.nt == 2)
-    hipLaunchKernelGGL((gqa_tree_kernel<D, 2, 2>), grid, dim3(kThreads), 0, stream, a);
   else if (p.tiles == 1)
-    hipLaunchKernelGGL((gqa_tree_kernel<D, 4, 2>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((gqa_tree_kernel<D, 2, 2>), grid, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((gqa_tree_kernel<D, 4, 0>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((gqa_tree_kernel<D, 2, 0>), grid, dim3(kThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -723,8 +770,8 @@ extern "C" size_t voom_paged_gqa_tree_workspace_bytes(int batch, int num_q_heads
                                                       int page_tokens, int max_pages) {
   if (!tree_shape_ok(batch, num_q_heads, num_kv_heads, head_dim, drafts, page_tokens, max_pages))
     return 0;
-  const TreePlan p = plan_tree(head_dim, num_q_heads / num_kv_heads, drafts, max_pages, page_tokens);
-  return part_o_bytes(p, head_dim) + static_cast<size_t>(2) * p.W * 16 * p.nt * 2 * sizeof(float);
+  const TreePlan p = plan_tree(num_q_heads / num_kv_heads, drafts, max_pages, page_tokens);
+  return part_o_bytes(p, head_dim) + static_cast<size_t>(2) * p.W * p.rows * 2 * sizeof(float);
 }
 
 extern "C" int voom_paged_gqa_tree(const void* q, const void* k_pool, const void* v_pool,
@@ -751,7 +798,7 @@ extern "C" int voom_paged_gqa_tree(const void* q, const void* k_pool, const void
                    reinterpret_cast<uintptr_t>(out) % 8 == 0,
                "%s: q and pools must be 16-byte aligned", who);
   const int G = num_q_heads / num_kv_heads;
-  const TreePlan p = plan_tree(head_dim, G, drafts, max_pages, page_tokens);
+  const TreePlan p = plan_tree(G, drafts, max_pages, page_tokens);
   const size_t need = voom_paged_gqa_tree_workspace_bytes(
       batch, num_q_heads, num_kv_heads, head_dim, drafts, page_tokens, max_pages);
   VOOM_REQUIRE(need == 0 || (workspace != nullptr && ws_bytes >= need &&
@@ -795,12 +842,12 @@ extern "C" int voom_paged_gqa_tree(const void* q, const void* k_pool, const void
   const int rc = VOOM_LAUNCH_CHECK("paged_gqa_tree: kernel launch");
   if (rc || p.W == 0) return rc;
   const long long rows = static_cast<long long>(batch) * num_kv_heads * a.R;
-  const dim3 rgrid(static_cast<unsigned>((rows + kWaves - 1) / kWaves));
+  const dim3 rgrid(static_cast<unsigned>((rows + kReduceWaves - 1) / kReduceWaves));
   if (head_dim == 128)
-    hipLaunchKernelGGL(gqa_tree_reduce_kernel<128>, rgrid, dim3(kThreads), 0, stream, a,
-                       16 * p.nt);
+    hipLaunchKernelGGL(gqa_tree_reduce_kernel<128>, rgrid, dim3(kReduceWaves * kWave), 0, stream,
+                       a, p.rows);
   else
-    hipLaunchKernelGGL(gqa_tree_reduce_kernel<64>, rgrid, dim3(kThreads), 0, stream, a,
-                       16 * p.nt);
+    hipLaunchKernelGGL(gqa_tree_reduce_kernel<64>, rgrid, dim3(kReduceWaves * kWave), 0, stream,
+                       a, p.rows);
   return VOOM_LAUNCH_CHECK("paged_gqa_tree: reduce launch");
 }
