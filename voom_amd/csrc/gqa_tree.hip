@@ -179,6 +179,30 @@ __device__ __forceinline__ u32x4 read_v(const uint16_t* tile, int n, int lane) {
                                          8 * (g ^ (i16 >> 2)));
 }
 
+// A block's K and V^T operands.
+template <int D>
+struct Operands {
+  u32x4 k[D / 32][2];
+  u32x4 v[D / 16];
+};
+
+template <int D>
+__device__ __forceinline__ void read_keys(Operands<D>& o, const uint16_t* tile, int lane) {
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) o.k[s][t] = read_k<D>(tile, t, s, lane);
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void read_block(Operands<D>& o, const uint16_t* tile, int lane) {
+  read_keys<D>(o, tile, lane);
+#pragma unroll
+  for (int n = 0; n < D / 16; ++n) o.v[n] = read_v<D>(tile, n, lane);
+  __builtin_amdgcn_sched_barrier(0);  // all of them on their way before the first is waited for
+}
+
 template <int D, int NT>
 struct State {
   f32x4 acc[NT][D / 16];
@@ -220,9 +244,8 @@ struct View {
 };
 
 template <int D, int NT>
-__device__ __forceinline__ void scores_of(const uint16_t* tile,
-                                          const u32x4 (&qop)[NT][D / 32], f32x4 (&sc)[NT][2],
-                                          int lane) {
+__device__ __forceinline__ void scores_of(const Operands<D>& o, const u32x4 (&qop)[NT][D / 32],
+                                          f32x4 (&sc)[NT][2]) {
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     sc[i][0] = f32x4{};
@@ -230,16 +253,13 @@ __device__ __forceinline__ void scores_of(const uint16_t* tile,
   }
 #pragma unroll
   for (int s = 0; s < D / 32; ++s) {
-    const u32x4 k0 = read_k<D>(tile, 0, s, lane), k1 = read_k<D>(tile, 1, s, lane);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const u32x4 q = qop[i][s];
-      sc[i][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k0),
-                                                         __builtin_bit_cast(bf16x8, q), sc[i][0],
-                                                         0, 0, 0);
-      sc[i][1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k1),
-                                                         __builtin_bit_cast(bf16x8, q), sc[i][1],
-                                                         0, 0, 0);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        sc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o.k[s][t]),
+                                                           __builtin_bit_cast(bf16x8, qop[i][s]),
+                                                           sc[i][t], 0, 0, 0);
     }
   }
 }
@@ -283,19 +303,18 @@ __device__ __forceinline__ void weights_of(const f32x4 (&sc)[NT][2], float scale
 }
 
 template <int D, int NT>
-__device__ __forceinline__ void whole_block(const uint16_t* tile,
+__device__ __forceinline__ void whole_block(const Operands<D>& o,
                                             const u32x4 (&qop)[NT][D / 32], float scale,
-                                            State<D, NT>& st, int lane) {
+                                            State<D, NT>& st) {
   f32x4 sc[NT][2];
   u32x4 p[NT];
-  scores_of<D, NT>(tile, qop, sc, lane);
+  scores_of<D, NT>(o, qop, sc);
   weights_of<D, NT>(sc, scale, st, p);
 #pragma unroll
   for (int n = 0; n < D / 16; ++n) {
-    const u32x4 v = read_v<D>(tile, n, lane);
 #pragma unroll
     for (int i = 0; i < NT; ++i)
-      st.acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, v),
+      st.acc[i][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, o.v[n]),
                                                              __builtin_bit_cast(bf16x8, p[i]),
                                                              st.acc[i][n], 0, 0, 0);
   }
@@ -314,7 +333,11 @@ __device__ __forceinline__ void edge_block(const uint16_t* tile,
   const int g = lane >> 4;
   f32x4 sc[NT][2];
   u32x4 p[NT];
-  scores_of<D, NT>(tile, qop, sc, lane);
+  {
+    Operands<D> o;
+    read_keys<D>(o, tile, lane);
+    scores_of<D, NT>(o, qop, sc);
+  }
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
     const uint32_t seen = view.seen(i, bi * kBlk + 8 * g);
@@ -429,7 +452,7 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
   static_assert(sizeof(float) * NT * 16 * kPad <= sizeof(stage_0), "a merge buffer fits a stage");
 
   const int lane = threadIdx.x & (kWave - 1);
-  const int wv = uniform(threadIdx.x / kWave);
+  const int wv = uniform(threadIdx.x / kWave) & (kWaves - 1);
   const int kw = wv % kKeyWaves;
   const int rw = wv / kKeyWaves;
   const int i16 = lane & 15;
@@ -557,11 +580,13 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
       else if (t + 1 < whole) __builtin_amdgcn_s_waitcnt(0x0F74);
       else __builtin_amdgcn_s_waitcnt(0x0F70);
       lds_barrier();
+      Operands<D> o;  // (the next loads are prepared while the first operands come)
+      read_block<D>(o, cur + kw * block_elems(D), lane);
       if (t + 3 < whole) load(t + 3, free);
-      if (rows_here) {
 #pragma unroll
-        for (int j = 0; j < kBlocks / kKeyWaves; ++j)
-          whole_block<D, NT>(cur + (kKeyWaves * j + kw) * block_elems(D), qop, a.scale, st, lane);
+      for (int j = 0; j < kBlocks / kKeyWaves && rows_here; ++j) {
+        if (j != 0) read_block<D>(o, cur + (kKeyWaves * j + kw) * block_elems(D), lane);
+        whole_block<D, NT>(o, qop, a.scale, st);
       }
       return ++t < whole;
     };
@@ -694,19 +719,45 @@ __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(T
     last = group_of_unit(S + chunks - 1, U, We);
     if (first == last) return;  // written by its workgroup
   }
+  // Up to 64 pieces at a time, one per lane for their maxima and sums.  A segment that
+  // starts inside its first workgroup's range is that one's last piece, else its first.
   float M = -FLT_MAX, L = 0.f, acc[DPL] = {};
-  for (long long w = first; w <= last; ++w) {
-    // a segment that starts inside its first workgroup's range is that one's last piece
-    const bool later = w == first && w * U / We < S;
-    const size_t p = (2 * static_cast<size_t>(w) + (later ? 1 : 0)) * rows_per_tile + r;
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
-    const float mn = fmaxf(M, ml.x);
-    const float f = fast_exp2(M - mn), wt = fast_exp2(ml.x - mn);
+  const bool later = chunks > 0 && first * U / We < S;
+  for (long long w0 = first; w0 <= last; w0 += kWave) {
+    const int n = static_cast<int>(last - w0 + 1 < kWave ? last - w0 + 1 : kWave);
+    const size_t p0 = 2 * static_cast<size_t>(w0) * rows_per_tile + r;
+    const int odd = later && w0 == first ? rows_per_tile : 0;  // of lane 0's piece
+    const int k = lane < n ? lane : 0;
+    const float2 ml = *reinterpret_cast<const float2*>(
+        a.part_ml + (p0 + 2 * static_cast<size_t>(k) * rows_per_tile + (k == 0 ? odd : 0)) * 2);
+    const float mn = fmaxf(M, wave_max_uniform(lane < n ? ml.x : -FLT_MAX));
+    const float wt = lane < n ? fast_exp2(ml.x - mn) : 0.f;
+    const float f = fast_exp2(M - mn);
     M = mn;
-    L = L * f + ml.y * wt;
-    const float* po = a.part_o + p * D + lane * DPL;
+    L = L * f + wave_sum_uniform(lane < n ? ml.y * wt : 0.f);
 #pragma unroll
-    for (int d = 0; d < DPL; ++d) acc[d] = acc[d] * f + po[d] * wt;
+    for (int d = 0; d < DPL; ++d) acc[d] *= f;
+    for (int k0 = 0; k0 < n; k0 += 8) {
+      float v[8][DPL];  // eight pieces' rows in flight
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int at_k = k0 + u < n ? k0 + u : n - 1;
+        const float* po =
+            a.part_o + (p0 + 2 * static_cast<size_t>(at_k) * rows_per_tile +
+                        (at_k == 0 ? odd : 0)) * D + lane * DPL;
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) v[u][d] = po[d];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (k0 + u >= n) break;
+        const float ws = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wt), k0 + u));
+#pragma unroll
+        for (int d = 0; d < DPL; ++d) acc[d] += v[u][d] * ws;
+      }
+    }
   }
   const bool empty = dead || L == 0.f;
   const float inv = empty ? 0.f : 1.f / L;
