@@ -118,25 +118,36 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_observe_kernel(ObserveArgs a)
     const size_t out_row = (static_cast<size_t>(b) * a.NKV + kvh) * a.cap;
 
     // a unit's keys of this wavefront: two 32-token blocks (past the context: the
-    // last one again, not stored)
+    // last one again, not stored), the slots of 64 pages from win_page on in the lanes
     const int last_blk = (ctx - 1) / kBlk;
     const int sub_shift = a.pt_shift - 5;
+    int win_page = -(1 << 30), win = 0;
     auto load_keys = [&](int c, Keys<D>& r) {
+      int first = (c * kUnit + wv * kMine) / kBlk;
+      first = first < last_blk ? first : last_blk;
+      if (first >> sub_shift < win_page || (first + 1) >> sub_shift >= win_page + kWave) {
+        win_page = first >> sub_shift;
+        win = win_page + lane < a.max_pages ? trow[win_page + lane] : 0;
+        wait_vmem_all();  // here, not at the readlanes below for every unit
+      }
 #pragma unroll
       for (int j = 0; j < kMine / kBlk; ++j) {
-        int blk = (c * kUnit + wv * kMine) / kBlk + j;
+        int blk = first + j;
         blk = blk < last_blk ? blk : last_blk;
         const int page = blk >> sub_shift;
-        int slot = uniform(trow[page]);
+        int slot = __builtin_amdgcn_readlane(win, page - win_page);
         if (static_cast<unsigned>(slot) >= static_cast<unsigned>(a.num_slots)) slot = 0;
         const size_t at = ((static_cast<size_t>(slot) * a.NKV + kvh) << sub_shift) +
                           (blk - (page << sub_shift));
-        const uint16_t* kr = a.k_pool + at * (kBlk * D) + i16 * D + 8 * g;
+        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint16_t*>(a.k_pool + at * (kBlk * D)), static_cast<short>(0),
+            kBlk * D * 2, 0x00020000);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
           for (int s = 0; s < D / 32; ++s)
-            r.k[2 * j + t][s] = *reinterpret_cast<const u32x4*>(kr + 16 * t * D + 32 * s);
+            r.k[2 * j + t][s] = __builtin_amdgcn_raw_buffer_load_b128(
+                kr, (i16 * D + 8 * g) * 2 + (16 * t * D + 32 * s) * 2, 0, 2);
         }
       }
     };

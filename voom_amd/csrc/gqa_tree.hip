@@ -25,7 +25,7 @@
 // other 32-token block.  K and V^T go straight into LDS (buffer_load ... lds, 1 KiB
 // each) through a ring of four 32 KiB stages: three are under way while one is
 // computed (a ring of two per wavefront drained it at every stage: 371 us at 16
-// sequences of 1k-32k tokens, 16 drafts, 32/8 heads, where this takes TIME_BATCH; blocks
+// sequences of 1k-32k tokens, 16 drafts, 32/8 heads, where this takes 251; blocks
 // in registers, as in the decode kernel, leave too few for 64 rows: 1,076).  Per block,
 // with the rows in the N dimension:
 //   scores^T[token][row] = K . Q^T,  out^T[dim][row] += V^T . P^T   16x16x32 bf16
@@ -70,6 +70,7 @@ struct TreeArgs {
   long long mask_stride;  // elements from one sequence's mask to the next
   int B, NQ, NKV, G, T, max_pages, pt_shift, num_slots;
   int R;         // rows of a (sequence, kv head): T * G, (draft, head), head fastest
+  int rows;      // rows of a tile
   int tiles;     // row tiles along R
   int W;         // workgroups of the split, 0: one per segment
   int per_xcd;   // workgroups per XCD
@@ -99,9 +100,41 @@ __device__ __forceinline__ int chunks_of(int ctx) {
   return (ctx + stage_tokens(D) - 1) / stage_tokens(D);
 }
 
-// Workgroup of the split that holds unit u (the last w with w U/W <= u).
-__device__ __forceinline__ long long group_of_unit(long long u, long long U, int W) {
-  return ((u + 1) * W - 1) / U;
+// Units 0 .. U - 1 over the workgroups: the first `rem` take base + 1, the others base.
+struct Split {
+  int We, base, rem;
+  __device__ __forceinline__ Split(int U, int W) {
+    We = U < 1 ? 1 : (U < W ? U : W);
+    base = U / We;
+    rem = U - base * We;
+  }
+  __device__ __forceinline__ int begin(int w) const { return w * base + (w < rem ? w : rem); }
+  // the workgroup that holds unit u
+  __device__ __forceinline__ int group(int u) const {
+    const int u_rem = rem * (base + 1);
+    return u < u_rem ? u / (base + 1) : rem + (u - u_rem) / base;
+  }
+};
+
+// Units of a sequence: its chunks for every kv head and row tile that holds a draft.
+template <int D>
+struct Units {
+  int chunks, tiles;
+  __device__ __forceinline__ Units(const TreeArgs& a, int b) {
+    const int ctx = context_of(a, b);
+    chunks = chunks_of<D>(ctx);
+    const int t = (drafts_of(a, b, ctx) * a.G + a.rows - 1) / a.rows;
+    tiles = t < 1 ? 1 : t;
+  }
+};
+
+// The units of up to 64 sequences from `base` on, one per lane, and their inclusive sum.
+template <int D>
+__device__ __forceinline__ Units<D> scan_units(const TreeArgs& a, int base, int lane, int& x) {
+  const bool in = base + lane < a.B;
+  const Units<D> u(a, in ? base + lane : 0);
+  x = wave_inclusive_scan(in ? u.chunks * u.tiles * a.NKV : 0, lane);
+  return u;
 }
 
 typedef __attribute__((address_space(3))) void lds_void;
@@ -133,7 +166,7 @@ __device__ __forceinline__ void load_stage(uint16_t* stage, const TreeArgs& a, P
   constexpr int kCpr = D / 8;              // 16-byte chunks of a K row
   const int sub_shift = a.pt_shift - 5;
   const int first = bi < pg.last ? bi : pg.last;
-  if ((first + kBlocks - 1) >> sub_shift >= pg.base + kWave) {
+  if (first >> sub_shift < pg.base || (first + kBlocks - 1) >> sub_shift >= pg.base + kWave) {
     pg.base = first >> sub_shift;
     const int p = pg.base + lane;
     pg.tab = p < a.max_pages ? pg.row[p] : 0;
@@ -264,7 +297,11 @@ __device__ __forceinline__ void scores_of(const Operands<D>& o, const u32x4 (&qo
   }
 }
 
-// Raises the reference maxima to those of the scores, and forms P.
+// Forms P.  The reference maxima are raised to those of the scores only where one is
+// more than kSlack ahead: weights up to 2^kSlack lose nothing in bf16 and fp32, and
+// after its first blocks a wavefront hardly ever rescales its sums.
+constexpr float kSlack = 8.f;
+
 template <int D, int NT>
 __device__ __forceinline__ void weights_of(const f32x4 (&sc)[NT][2], float scale,
                                            State<D, NT>& st, u32x4 (&p)[NT]) {
@@ -276,7 +313,7 @@ __device__ __forceinline__ void weights_of(const f32x4 (&sc)[NT][2], float scale
 #pragma unroll
     for (int e = 1; e < 4; ++e) x = fmaxf(fmaxf(x, sc[i][0][e]), sc[i][1][e]);
     mx[i] = x * scale;
-    up |= mx[i] > st.m[i];
+    up |= mx[i] > st.m[i] + kSlack;
   }
   if (__builtin_amdgcn_ballot_w64(up) != 0) {
 #pragma unroll
@@ -410,38 +447,12 @@ __device__ __forceinline__ void edge_block(const uint16_t* tile,
   }
 }
 
-// Exclusive prefix sum of the sequences' chunk counts into seg[0..B]; ends with a
-// barrier.
-template <int D>
-__device__ void chunk_prefix(const TreeArgs& a, int* seg, int* wave_tot) {
-  const int t = threadIdx.x;
-  const int lane = t & (kWave - 1);
-  const int wv = t / kWave;
-  int carry = 0;
-  for (int base = 0; base < a.B; base += kThreads) {
-    const int i = base + t;
-    const int n = i < a.B ? chunks_of<D>(context_of(a, i)) : 0;
-    const int x = wave_inclusive_scan(n, lane);
-    if (lane == kWave - 1) wave_tot[wv] = x;
-    __syncthreads();
-    int before = carry;
-    for (int k = 0; k < wv; ++k) before += wave_tot[k];
-    if (i < a.B) seg[i] = before + x - n;
-    for (int k = 0; k < kWaves; ++k) carry += wave_tot[k];
-    __syncthreads();
-  }
-  if (t == 0) seg[a.B] = carry;
-  __syncthreads();
-}
-
 template <int D, int NT, int AUX>
 __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
   constexpr int kRows = 16 * NT * kRowWaves;
   constexpr int kBlocks = stage_blocks(D);
   constexpr int kLoads = 2 * kBlocks * (kBlk * D / 512) / kWaves;  // a wavefront's, of a stage
   constexpr int kPad = D + 4;  // floats of a row in LDS: 16 rows start in 16 bank groups
-  __shared__ int seg[kMaxBatch + 1];
-  __shared__ int wave_tot[kWaves];
   // The ring.  Distinct objects, so that reads of one provably miss the pending
   // direct-to-LDS loads of the others; the merge uses them when the loop is done.
   __shared__ __attribute__((aligned(1024))) uint16_t stage_0[kStageElems];
@@ -462,44 +473,56 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
   const int bid = static_cast<int>(blockIdx.x);
   const int w = (bid & 7) * a.per_xcd + (bid >> 3);
 
-  int b, kvh, tile, c0, c1, chunks;
-  long long u0 = 0, u1 = 0, begin = 0;
-  int We = 0;
-  const int per_b = a.NKV * a.tiles;
+  int b = 0, kvh, tile, c0, c1, chunks = 0, tiles = a.tiles;
+  int u0 = 0, u1 = 0, begin = 0;  // the workgroup's units, and the segment's first one
   if (a.W == 0) {
-    if (w >= a.B * per_b) return;
-    b = w / per_b;
-    chunks = uniform(chunks_of<D>(context_of(a, b)));
-    const int s = w - b * per_b;
-    kvh = s / a.tiles;
-    tile = s - kvh * a.tiles;
+    if (w >= a.B * a.NKV * tiles) return;
+    b = w / (a.NKV * tiles);
+    const int s = w - b * (a.NKV * tiles);
+    kvh = s / tiles;
+    tile = s - kvh * tiles;
+    const Units<D> units(a, b);
+    chunks = tile < uniform(units.tiles) ? uniform(units.chunks) : 0;
   } else {
-    chunk_prefix<D>(a, seg, wave_tot);
-    const long long U = static_cast<long long>(uniform(seg[a.B])) * per_b;
-    We = static_cast<int>(U < a.W ? U : a.W);
-    if (w >= We) return;
-    u0 = static_cast<long long>(w) * U / We;
-    u1 = static_cast<long long>(w + 1) * U / We;
-    int lo = 0, hi = a.B - 1;  // the sequence that holds unit u0
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (static_cast<long long>(uniform(seg[mid])) * per_b <= u0) lo = mid; else hi = mid - 1;
+    int x0;  // (every wavefront for itself: no barrier)
+    const Units<D> first = scan_units<D>(a, 0, lane, x0);
+    int U = __builtin_amdgcn_readlane(x0, kWave - 1);
+    for (int base = kWave; base < a.B; base += kWave) {
+      int x;
+      scan_units<D>(a, base, lane, x);
+      U += __builtin_amdgcn_readlane(x, kWave - 1);
     }
-    b = lo;
-    chunks = uniform(seg[b + 1]) - uniform(seg[b]);
-    const long long first = static_cast<long long>(uniform(seg[b])) * per_b;
-    const int s = static_cast<int>((u0 - first) / chunks);
-    kvh = s / a.tiles;
-    tile = s - kvh * a.tiles;
-    begin = first + static_cast<long long>(s) * chunks;
+    const Split split(U, a.W);
+    if (w >= split.We || U == 0) return;
+    u0 = split.begin(w);
+    u1 = split.begin(w + 1);
+    for (int base = 0;; base += kWave) {  // the sequence that holds unit u0
+      int x = x0;
+      Units<D> units = first;
+      if (base != 0) units = scan_units<D>(a, base, lane, x);
+      const int here = __builtin_amdgcn_readlane(x, kWave - 1);
+      if (u0 < begin + here) {
+        const int k = __popcll(__builtin_amdgcn_ballot_w64(begin + x <= u0));
+        b = base + k;
+        chunks = __builtin_amdgcn_readlane(units.chunks, k);
+        tiles = __builtin_amdgcn_readlane(units.tiles, k);
+        begin += __builtin_amdgcn_readlane(x, k) - chunks * tiles * a.NKV;
+        break;
+      }
+      begin += here;
+    }
+    const int s = (u0 - begin) / chunks;
+    kvh = s / tiles;
+    tile = s - kvh * tiles;
+    begin += s * chunks;
   }
   for (int piece = 0;; ++piece) {
     if (a.W == 0) {
       c0 = 0;
       c1 = chunks;
     } else {
-      c0 = static_cast<int>(u0 - begin);
-      c1 = static_cast<int>((u1 < begin + chunks ? u1 : begin + chunks) - begin);
+      c0 = u0 - begin;
+      c1 = (u1 < begin + chunks ? u1 : begin + chunks) - begin;
     }
     const int ctx = uniform(context_of(a, b));
     View<NT> view;
@@ -551,7 +574,8 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
     Pages pg{a.table + static_cast<size_t>(b) * a.max_pages, kvh, last_blk, -(1 << 30), 0};
     int whole = view.prefix / stage_tokens(D);
     whole = whole < c1 ? whole : c1;
-    const bool rows_here = tile * kRows + rw * (16 * NT) < a.R;  // (else this wavefront only loads)
+    // (else this wavefront only loads)
+    const bool rows_here = tile * kRows + rw * (16 * NT) < view.drafts * a.G;
     int t = c0;
     auto load = [&](int at, uint16_t* stage) {
       load_stage<D, AUX>(stage, a, pg, at * kBlocks, wv, lane);
@@ -561,8 +585,7 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
     if (t + 2 < whole) load(t + 2, stage_2);
 #pragma unroll 1
     for (int e = whole > c0 ? whole : c0; e < c1; ++e) {
-      Pages back{pg.row, kvh, last_blk, -(1 << 30), 0};
-      load_stage<D, AUX>(stage_3, a, back, e * kBlocks, wv, lane);
+      load(e, stage_3);
       wait_vmem_all();
       lds_barrier();
       if (rows_here) {
@@ -609,7 +632,7 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       float* const buf = reinterpret_cast<float*>(merge) + i * 16 * kPad;
-      if (kw == 1 && rows_here) {
+      if (kw == 1) {
 #pragma unroll
         for (int n = 0; n < D / 16; ++n)
           *reinterpret_cast<f32x4*>(buf + i16 * kPad + 16 * n + 4 * g) = st.acc[i][n];
@@ -620,7 +643,7 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
       }
     }
     __syncthreads();
-    if (kw == 0 && rows_here) {
+    if (kw == 0) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const float* const buf = reinterpret_cast<const float*>(merge) + (i * 16 + i16) * kPad;
@@ -639,7 +662,7 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
         for (int n = 0; n < D / 16; ++n) {
           const f32x4 o =
               st.acc[i][n] * f0 + *reinterpret_cast<const f32x4*>(buf + 16 * n + 4 * g) * f1;
-          if (!all) {
+          if (!all) {  // (rows past R too: they are in the workspace)
             *reinterpret_cast<f32x4*>(a.part_o + (slot * kRows + r) * D + 16 * n + 4 * g) = o;
           } else if (rr < a.R) {
             *reinterpret_cast<u32x2*>(a.out + at * D + 16 * n + 4 * g) =
@@ -658,14 +681,15 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
     u0 = u1 < begin + chunks ? u1 : begin + chunks;
     if (u0 >= u1) return;
     begin += chunks;
-    if (++tile == a.tiles) {
+    if (++tile == tiles) {
       tile = 0;
       if (++kvh == a.NKV) {
         kvh = 0;
         do {
-          ++b;
-        } while (b < a.B - 1 && uniform(seg[b + 1]) == uniform(seg[b]));
-        chunks = uniform(seg[b + 1]) - uniform(seg[b]);
+          const Units<D> units(a, ++b);
+          chunks = uniform(units.chunks);
+          tiles = uniform(units.tiles);
+        } while (b < a.B - 1 && chunks == 0);
       }
     }
     __syncthreads();  // the next piece writes the ring
@@ -675,9 +699,9 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
 constexpr int kReduceWaves = 4;
 
 // One wavefront per row: merges the pieces of its segment, where the split cut it;
-// rows of sequences without tokens are written here.
+// rows of sequences without tokens and of tiles without drafts are written here.
 template <int D>
-__global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(TreeArgs a, int rows_per_tile) {
+__global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(TreeArgs a) {
   constexpr int DPL = D / kWave;
   const int lane = threadIdx.x & (kWave - 1);
   const long long task =
@@ -687,19 +711,19 @@ __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(T
   const int rr = static_cast<int>(task - static_cast<long long>(seg) * a.R);
   const int b = seg / a.NKV;
   const int kvh = seg - b * a.NKV;
-  const int tile = rr / rows_per_tile;
-  const int r = rr - tile * rows_per_tile;
-  // chunks before sequence b, of b, and of all
-  int before = 0, chunks = 0, total = 0;
+  const int tile = rr / a.rows;
+  const int r = rr - tile * a.rows;
+  // units before sequence b, and of all; chunks and row tiles of b
+  int before = 0, chunks = 0, tiles = 1, U = 0;
   for (int base = 0; base < a.B; base += kWave) {
-    const int i = base + lane;
-    const int n = i < a.B ? chunks_of<D>(context_of(a, i)) : 0;
-    const int x = wave_inclusive_scan(n, lane);
+    int x;
+    const Units<D> units = scan_units<D>(a, base, lane, x);
     if (b >= base && b < base + kWave) {
-      before = total + __builtin_amdgcn_readlane(x - n, b - base);
-      chunks = __builtin_amdgcn_readlane(n, b - base);
+      chunks = __builtin_amdgcn_readlane(units.chunks, b - base);
+      tiles = __builtin_amdgcn_readlane(units.tiles, b - base);
+      before = U + __builtin_amdgcn_readlane(x, b - base) - chunks * tiles * a.NKV;
     }
-    total += __builtin_amdgcn_readlane(x, kWave - 1);
+    U += __builtin_amdgcn_readlane(x, kWave - 1);
   }
   const int t = rr / a.G;
   const int head = kvh * a.G + (rr - t * a.G);
@@ -707,29 +731,26 @@ __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(T
   uint16_t* o = a.out + at * D + lane * DPL;
   const int ctx = uniform(context_of(a, b));
   const bool dead = t >= uniform(drafts_of(a, b, ctx));
-  const int per_b = a.NKV * a.tiles;
-  long long first = 0, last = -1, S = 0, U = 1;
-  int We = 1;
-  if (chunks > 0) {
-    U = static_cast<long long>(total) * per_b;
-    We = static_cast<int>(U < a.W ? U : a.W);
-    S = static_cast<long long>(before) * per_b +
-        static_cast<long long>(kvh * a.tiles + tile) * chunks;
-    first = group_of_unit(S, U, We);
-    last = group_of_unit(S + chunks - 1, U, We);
+  int first = 0, last = -1;
+  bool later = false;
+  if (chunks > 0 && tile < tiles) {
+    const Split split(U, a.W);
+    const int S = before + (kvh * tiles + tile) * chunks;
+    first = split.group(S);
+    last = split.group(S + chunks - 1);
     if (first == last) return;  // written by its workgroup
+    later = split.begin(first) < S;
   }
   // Up to 64 pieces at a time, one per lane for their maxima and sums.  A segment that
   // starts inside its first workgroup's range is that one's last piece, else its first.
   float M = -FLT_MAX, L = 0.f, acc[DPL] = {};
-  const bool later = chunks > 0 && first * U / We < S;
-  for (long long w0 = first; w0 <= last; w0 += kWave) {
-    const int n = static_cast<int>(last - w0 + 1 < kWave ? last - w0 + 1 : kWave);
-    const size_t p0 = 2 * static_cast<size_t>(w0) * rows_per_tile + r;
-    const int odd = later && w0 == first ? rows_per_tile : 0;  // of lane 0's piece
+  for (int w0 = first; w0 <= last; w0 += kWave) {
+    const int n = last - w0 + 1 < kWave ? last - w0 + 1 : kWave;
+    const size_t p0 = 2 * static_cast<size_t>(w0) * a.rows + r;
+    const int odd = later && w0 == first ? a.rows : 0;  // of lane 0's piece
     const int k = lane < n ? lane : 0;
     const float2 ml = *reinterpret_cast<const float2*>(
-        a.part_ml + (p0 + 2 * static_cast<size_t>(k) * rows_per_tile + (k == 0 ? odd : 0)) * 2);
+        a.part_ml + (p0 + 2 * static_cast<size_t>(k) * a.rows + (k == 0 ? odd : 0)) * 2);
     const float mn = fmaxf(M, wave_max_uniform(lane < n ? ml.x : -FLT_MAX));
     const float wt = lane < n ? fast_exp2(ml.x - mn) : 0.f;
     const float f = fast_exp2(M - mn);
@@ -743,7 +764,7 @@ __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(T
       for (int u = 0; u < 8; ++u) {
         const int at_k = k0 + u < n ? k0 + u : n - 1;
         const float* po =
-            a.part_o + (p0 + 2 * static_cast<size_t>(at_k) * rows_per_tile +
+            a.part_o + (p0 + 2 * static_cast<size_t>(at_k) * a.rows +
                         (at_k == 0 ? odd : 0)) * D + lane * DPL;
 #pragma unroll
         for (int d = 0; d < DPL; ++d) v[u][d] = po[d];
@@ -850,6 +871,10 @@ extern "C" int voom_paged_gqa_tree(const void* q, const void* k_pool, const void
                "%s: q and pools must be 16-byte aligned", who);
   const int G = num_q_heads / num_kv_heads;
   const TreePlan p = plan_tree(G, drafts, max_pages, page_tokens);
+  const long long stages = (static_cast<long long>(max_pages) * page_tokens + 63) / 64;
+  VOOM_REQUIRE(stages * batch * num_kv_heads * p.tiles < (1LL << 31),
+               "%s: %d pages of %d tokens for %d sequences are too many", who, max_pages,
+               page_tokens, batch);
   const size_t need = voom_paged_gqa_tree_workspace_bytes(
       batch, num_q_heads, num_kv_heads, head_dim, drafts, page_tokens, max_pages);
   VOOM_REQUIRE(need == 0 || (workspace != nullptr && ws_bytes >= need &&
@@ -879,6 +904,7 @@ extern "C" int voom_paged_gqa_tree(const void* q, const void* k_pool, const void
   a.pt_shift = ilog2(page_tokens);
   a.num_slots = num_slots;
   a.R = drafts * G;
+  a.rows = p.rows;
   a.tiles = p.tiles;
   a.W = p.W;
   const long long groups =
@@ -896,9 +922,9 @@ extern "C" int voom_paged_gqa_tree(const void* q, const void* k_pool, const void
   const dim3 rgrid(static_cast<unsigned>((rows + kReduceWaves - 1) / kReduceWaves));
   if (head_dim == 128)
     hipLaunchKernelGGL(gqa_tree_reduce_kernel<128>, rgrid, dim3(kReduceWaves * kWave), 0, stream,
-                       a, p.rows);
+                       a);
   else
     hipLaunchKernelGGL(gqa_tree_reduce_kernel<64>, rgrid, dim3(kReduceWaves * kWave), 0, stream,
-                       a, p.rows);
+                       a);
   return VOOM_LAUNCH_CHECK("paged_gqa_tree: reduce launch");
 }
