@@ -11,27 +11,31 @@
 // the sums) up to about 200 (token, head of the group) rows, then matrix work and an
 // exponential per (row, key).
 //
-// Keys are independent of each other, so nothing is merged: the 256-token units of
-// all (sequence, kv head) segments lie end to end and workgroup w of W takes
-// [w U/W, (w+1) U/W).  The rows' queries (256 at a time) sit in LDS, a wavefront
-// holds 64 keys in registers while the next 64 are under way, and
+// Keys are independent of each other, so nothing is merged: units of one stage (128
+// tokens, 256 at D = 64) of all (sequence, kv head) segments lie end to end and are dealt
+// out evenly.  K goes straight into LDS (1 KiB loads) through a ring of four 32 KiB
+// stages, three of them under way; loaded into operand registers instead, 64 bytes of
+// a row at a time, the same keys came 20 % slower even with no work on them.
+//
+// Eight wavefronts compute, RW of them on other rows (16 NT each, queries in registers)
+// and 8 / RW on other keys of the stage:
 //   scores[row][key] = Q . K^T   on v_mfma_f32_16x16x32_bf16, rows in the M dimension
-// leaves a lane with four rows of one key: the sum over the rows needs no exchange
-// until the end of the unit.
-#include "common.h"
+// leaves a lane with four rows of one key, so that the sum over the rows needs one
+// exchange per key tile.  A ninth wavefront adds the wavefronts' sums, one stage later,
+// to the sums before and stores them: its loads and stores do not sit between the others'
+// loads, which return in order.
+#include "paged_ring.h"
 
 #include <cmath>
 
 namespace voom {
 namespace {
 
-constexpr int kWaves = 4;
-constexpr int kThreads = kWaves * kWave;
-constexpr int kBlk = 32;              // tokens of a K block in the pool
-constexpr int kMine = 64;             // keys of a wavefront in a unit
-constexpr int kUnit = kWaves * kMine;
-constexpr int kRows = 256;            // rows in LDS at a time
+constexpr int kWaves = 8;                         // that compute
+constexpr int kThreads = (kWaves + 1) * kWave;    // and the one that stores
 constexpr int kMaxBatch = 1024;
+constexpr int kStageElems = 128 * 128;
+constexpr int stage_tokens(int D) { return kStageElems / D; }
 
 struct ObserveArgs {
   const uint16_t* q;     // [B, NQ, L, D]
@@ -54,175 +58,213 @@ __device__ __forceinline__ int context_of(const ObserveArgs& a, int b) {
   return c < 0 ? 0 : (c > most ? most : c);
 }
 
+// Chunk c (16 bytes) of K row r of a stage sits at c ^ k_swizzle(r) of its row: 16
+// consecutive rows read one chunk each from 16 different 16-byte columns.
 template <int D>
-struct Keys {
-  u32x4 k[kMine / 16][D / 32];  // 16-key tiles x k-steps
-};
+__device__ __forceinline__ int k_swizzle(int r) {
+  return D == 128 ? (r & 15) : ((r >> 1) & 7);
+}
 
+// Starts this wavefront's loads of stage t (past the piece: empty ones, so that what is
+// waited for does not depend on a branch).
 template <int D>
-__global__ __launch_bounds__(kThreads, 2) void gqa_observe_kernel(ObserveArgs a) {
-  constexpr int kStride = D + 8;  // elements of a row in LDS: 16 rows start in 16 bank groups
-  __shared__ int seg[kMaxBatch + 1];
-  __shared__ int wave_tot[kWaves];
-  __shared__ __attribute__((aligned(16))) uint16_t rows[kRows][kStride];
-  __shared__ __attribute__((aligned(16))) float neg_lse[kRows];  // -lse in log2 units; -inf: no row
+__device__ __forceinline__ void load_stage(uint16_t* stage, const ObserveArgs& a, Pages& pg, int t,
+                                           bool live, int wv, int lane) {
+  constexpr int kBlocks = stage_tokens(D) / kBlk;
+  constexpr int kPieces = kBlk * D / 512;  // of a block
+  constexpr int kCpr = D / 8;              // 16-byte chunks of a row
+  pg.hold(t * kBlocks, kBlocks, lane);
+#pragma unroll
+  for (int i = 0; i < kBlocks * kPieces / kWaves; ++i) {
+    const int p = wv + kWaves * i;
+    const int r = (p % kPieces) * (kWave / kCpr) + lane / kCpr;
+    load_piece<2>(a.k_pool + pg.block(t * kBlocks + p / kPieces) * (kBlk * D),
+                  live ? kBlk * D * 2 : 0,
+                  r * (D * 2) + 16 * ((lane % kCpr) ^ k_swizzle<D>(r)), stage + p * 512);
+  }
+}
+
+template <int D, int NT, int RW>
+__global__ __launch_bounds__(kThreads) void gqa_observe_kernel(ObserveArgs a) {
+  constexpr int kST = stage_tokens(D);
+  constexpr int kRows = 16 * NT * RW;         // rows at a time
+  constexpr int kKeys = kST / (kWaves / RW);  // a wavefront's keys of a stage
+  // The ring: distinct objects, so that reads of one provably miss the pending loads of
+  // the others.
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_0[kStageElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_1[kStageElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_2[kStageElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_3[kStageElems];
+  __shared__ float part[2][RW][kST];  // a stage's sums of each group of rows
+  static_assert(kStageElems * 2 / 1024 == 4 * kWaves, "the waits below count four loads a stage");
 
   const int lane = threadIdx.x & (kWave - 1);
-  const int wv = uniform(threadIdx.x / kWave);
+  const int wv = uniform(threadIdx.x / kWave) & 15;
   const int i16 = lane & 15;
   const int g = lane >> 4;
-
-  {  // exclusive prefix sum of the sequences' units
-    int carry = 0;
-    for (int base = 0; base < a.B; base += kThreads) {
-      const int i = base + static_cast<int>(threadIdx.x);
-      const int n = i < a.B ? (context_of(a, i) + kUnit - 1) / kUnit : 0;
-      const int x = wave_inclusive_scan(n, lane);
-      if (lane == kWave - 1) wave_tot[wv] = x;
-      __syncthreads();
-      int before = carry;
-      for (int k = 0; k < wv; ++k) before += wave_tot[k];
-      if (i < a.B) seg[i] = before + x - n;
-      for (int k = 0; k < kWaves; ++k) carry += wave_tot[k];
-      __syncthreads();
-    }
-    if (threadIdx.x == 0) seg[a.B] = carry;
-    __syncthreads();
-  }
-  const long long U = static_cast<long long>(uniform(seg[a.B])) * a.NKV;
-  const int We = static_cast<int>(U < a.W ? U : a.W);
   const int w = static_cast<int>(blockIdx.x);
-  if (w >= We) return;
-  long long u0 = static_cast<long long>(w) * U / We;
-  const long long u1 = static_cast<long long>(w + 1) * U / We;
-  int lo = 0, hi = a.B - 1;  // the sequence that holds unit u0
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (static_cast<long long>(uniform(seg[mid])) * a.NKV <= u0) lo = mid; else hi = mid - 1;
+
+  // This workgroup's units, found by every wavefront for itself.
+  auto units_of = [&](int b) { return (context_of(a, b) + kST - 1) / kST; };
+  int U = 0;
+  for (int base = 0; base < a.B; base += kWave) {
+    const int n = base + lane < a.B ? units_of(base + lane) * a.NKV : 0;
+    U += __builtin_amdgcn_readlane(wave_inclusive_scan(n, lane), kWave - 1);
   }
-  int b = lo;
-  int units = uniform(seg[b + 1]) - uniform(seg[b]);
-  long long begin = static_cast<long long>(uniform(seg[b])) * a.NKV;
-  int kvh = static_cast<int>((u0 - begin) / units);
-  begin += static_cast<long long>(kvh) * units;
+  const Split split(U, a.W);
+  if (w >= split.We || U == 0) return;
+  int u0 = split.begin(w);
+  const int u1 = split.begin(w + 1);
+  int b = 0, units = 0, begin = 0;
+  for (int base = 0;; base += kWave) {  // the sequence that holds unit u0
+    const int n = base + lane < a.B ? units_of(base + lane) * a.NKV : 0;
+    const int x = wave_inclusive_scan(n, lane);
+    const int here = __builtin_amdgcn_readlane(x, kWave - 1);
+    if (u0 < begin + here) {
+      const int k = __popcll(__builtin_amdgcn_ballot_w64(begin + x <= u0));
+      b = base + k;
+      const int mine = __builtin_amdgcn_readlane(n, k);
+      begin += __builtin_amdgcn_readlane(x, k) - mine;
+      units = mine / a.NKV;
+      break;
+    }
+    begin += here;
+  }
+  int kvh = (u0 - begin) / units;
+  begin += kvh * units;
 
   while (true) {
-    const int c0 = static_cast<int>(u0 - begin);
-    const int c1 = static_cast<int>((u1 < begin + units ? u1 : begin + units) - begin);
+    const int c0 = u0 - begin;
+    const int c1 = (u1 < begin + units ? u1 : begin + units) - begin;
     const int ctx = uniform(context_of(a, b));
     int n = a.lens != nullptr ? uniform(a.lens[b]) : a.L;
     n = n < 0 ? 0 : (n > a.L ? a.L : n);
     n = n < ctx ? n : ctx;
     const int live = n * a.G;  // rows of the window, (token, head) with the head fastest
-    const int32_t* trow = a.table + static_cast<size_t>(b) * a.max_pages;
     const size_t out_row = (static_cast<size_t>(b) * a.NKV + kvh) * a.cap;
 
-    // a unit's keys of this wavefront: two 32-token blocks (past the context: the
-    // last one again, not stored), the slots of 64 pages from win_page on in the lanes
-    const int last_blk = (ctx - 1) / kBlk;
-    const int sub_shift = a.pt_shift - 5;
-    int win_page = -(1 << 30), win = 0;
-    auto load_keys = [&](int c, Keys<D>& r) {
-      int first = (c * kUnit + wv * kMine) / kBlk;
-      first = first < last_blk ? first : last_blk;
-      if (first >> sub_shift < win_page || (first + 1) >> sub_shift >= win_page + kWave) {
-        win_page = first >> sub_shift;
-        win = win_page + lane < a.max_pages ? trow[win_page + lane] : 0;
-        wait_vmem_all();  // here, not at the readlanes below for every unit
-      }
-#pragma unroll
-      for (int j = 0; j < kMine / kBlk; ++j) {
-        int blk = first + j;
-        blk = blk < last_blk ? blk : last_blk;
-        const int page = blk >> sub_shift;
-        int slot = __builtin_amdgcn_readlane(win, page - win_page);
-        if (static_cast<unsigned>(slot) >= static_cast<unsigned>(a.num_slots)) slot = 0;
-        const size_t at = ((static_cast<size_t>(slot) * a.NKV + kvh) << sub_shift) +
-                          (blk - (page << sub_shift));
-        const __amdgpu_buffer_rsrc_t kr = __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint16_t*>(a.k_pool + at * (kBlk * D)), static_cast<short>(0),
-            kBlk * D * 2, 0x00020000);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-          for (int s = 0; s < D / 32; ++s)
-            r.k[2 * j + t][s] = __builtin_amdgcn_raw_buffer_load_b128(
-                kr, (i16 * D + 8 * g) * 2 + (16 * t * D + 32 * s) * 2, 0, 2);
-        }
-      }
-    };
-
     for (int r0 = 0; r0 == 0 || r0 < live; r0 += kRows) {
-      const int here = live - r0 < kRows ? live - r0 : kRows;
-      __syncthreads();  // the rows before are no longer read
-      for (int idx = threadIdx.x; idx < ((here + 15) & ~15) * (D / 8); idx += kThreads) {
-        const int r = idx / (D / 8);
-        const int c = idx - r * (D / 8);
-        u32x4 x = {0u, 0u, 0u, 0u};
-        const int rr = r0 + r;
-        const int t = rr / a.G;
-        const int head = kvh * a.G + (rr - t * a.G);
-        if (r < here)
-          x = *reinterpret_cast<const u32x4*>(
-              a.q + ((static_cast<size_t>(b) * a.NQ + head) * a.L + t) * D + 8 * c);
-        *reinterpret_cast<u32x4*>(&rows[r][8 * c]) = x;
-        if (c == 0) {
-          const float v = r < here ? a.lse[(static_cast<size_t>(b) * a.L + t) * a.NQ + head]
-                                   : -INFINITY;
-          neg_lse[r] = v == -INFINITY ? -INFINITY : v * -1.4426950408889634f;
+      if (wv == kWaves) {
+        // the wavefront that stores: stage t - 1 while the others compute stage t
+        const float* from = (r0 == 0 ? a.scores : a.out) + out_row;
+        float old[kST / kWave];
+        auto load_old = [&](int t) {
+#pragma unroll
+          for (int j = 0; j < kST / kWave; ++j) {
+            const int p = t * kST + j * kWave + lane;
+            old[j] = from[p < ctx ? p : ctx - 1];
+          }
+        };
+        load_old(c0);
+        lds_barrier();
+        for (int t = c0; t < c1; ++t) {
+          lds_barrier();  // stage t is computed
+#pragma unroll
+          for (int j = 0; j < kST / kWave; ++j) {
+            float v = 0.f;
+#pragma unroll
+            for (int r = 0; r < RW; ++r) v += part[(t - c0) & 1][r][j * kWave + lane];
+            const int p = t * kST + j * kWave + lane;
+            if (p < ctx) a.out[out_row + p] = old[j] + v;
+          }
+          if (t + 1 < c1) load_old(t + 1);
+        }
+        continue;
+      }
+      const int rw = wv % RW;
+      const int kw = wv / RW;
+      // A operands of this wavefront's rows, their -lse in log2 units, and the last token
+      // that each sees (-1: no row)
+      u32x4 qa[NT][D / 32];
+      f32x4 nl[NT];
+      int vis[NT][4];
+      bool some_dead = false;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int first = r0 + (rw * NT + i) * 16;
+        const int r = first + i16 < live ? first + i16 : 0;
+        const int tok = r / a.G;
+        const int head = kvh * a.G + (r - tok * a.G);
+        const uint16_t* qr =
+            a.q + ((static_cast<size_t>(b) * a.NQ + head) * a.L + tok) * D + 8 * g;
+#pragma unroll
+        for (int s = 0; s < D / 32; ++s) qa[i][s] = *reinterpret_cast<const u32x4*>(qr + 32 * s);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int re = first + 4 * g + e < live ? first + 4 * g + e : 0;
+          const int te = re / a.G;
+          const float v = a.lse[(static_cast<size_t>(b) * a.L + te) * a.NQ + kvh * a.G +
+                                (re - te * a.G)];
+          const bool none = v == -INFINITY || first + 4 * g + e >= live;
+          nl[i][e] = none ? 0.f : v * -1.4426950408889634f;
+          vis[i][e] = none ? -1 : ctx - n + te;
+          some_dead |= none;
         }
       }
-      __syncthreads();
+      const bool dead_rows = __builtin_amdgcn_ballot_w64(some_dead) != 0;
+      const bool rows_here = r0 + rw * NT * 16 < live;
 
-      Keys<D> cur, nxt;
-      load_keys(c0, cur);
-      for (int c = c0; c < c1; ++c) {
-        if (c + 1 < c1) load_keys(c + 1, nxt);
-        const int first = c * kUnit + wv * kMine;
-        const bool edge = first + kMine > ctx - n;  // some row may not see some key
-        float sum[kMine / 16] = {};
-        for (int i = 0; i < here; i += 16) {
-          u32x4 qa[D / 32];
-#pragma unroll
-          for (int s = 0; s < D / 32; ++s)
-            qa[s] = *reinterpret_cast<const u32x4*>(&rows[i + i16][32 * s + 8 * g]);
-          const f32x4 nl = *reinterpret_cast<const f32x4*>(&neg_lse[i + 4 * g]);
-          f32x4 sc[kMine / 16];
-#pragma unroll
-          for (int j = 0; j < kMine / 16; ++j) {
-            sc[j] = f32x4{};
+      Pages pg(a.table + static_cast<size_t>(b) * a.max_pages, a.max_pages, a.num_slots, a.NKV,
+               kvh, a.pt_shift - 5, (ctx - 1) / kBlk);
+      load_stage<D>(stage_0, a, pg, c0, true, wv, lane);
+      load_stage<D>(stage_1, a, pg, c0 + 1, c0 + 1 < c1, wv, lane);
+      load_stage<D>(stage_2, a, pg, c0 + 2, c0 + 2 < c1, wv, lane);
+      int t = c0;
+      // One stage: it has landed for every wavefront, and the one before is no longer read.
+      auto step = [&](const uint16_t* cur, uint16_t* free) {
+        __builtin_amdgcn_s_waitcnt(0x0F78);  // gfx9 encoding: vmcnt 8 (two stages), expcnt 7, lgkmcnt 15
+        lds_barrier();
+        load_stage<D>(free, a, pg, t + 3, t + 3 < c1, wv, lane);
+        const bool masked = dead_rows || (t + 1) * kST > ctx - n;
+#pragma unroll 2
+        for (int j = 0; j < kKeys / 16; ++j) {
+          const int key = kw * kKeys + 16 * j + i16;  // of the stage
+          float sum = 0.f;
+          if (rows_here) {
+            f32x4 sc[NT];
+            u32x4 kb[D / 32];
 #pragma unroll
             for (int s = 0; s < D / 32; ++s)
-              sc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  __builtin_bit_cast(bf16x8, qa[s]), __builtin_bit_cast(bf16x8, cur.k[j][s]),
-                  sc[j], 0, 0, 0);
-          }
+              kb[s] = *reinterpret_cast<const u32x4*>(cur + key * D +
+                                                      8 * ((4 * s + g) ^ k_swizzle<D>(key)));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const bool dead = nl[e] == -INFINITY;
-            // the last token that the row sees
-            const int vis = ctx - n + (edge ? (r0 + i + 4 * g + e) / a.G : n);
+            for (int i = 0; i < NT; ++i) sc[i] = f32x4{};
 #pragma unroll
-            for (int j = 0; j < kMine / 16; ++j) {
-              const float x = fast_exp2(__builtin_fmaf(sc[j][e], a.scale, nl[e]));
-              sum[j] += dead || first + 16 * j + i16 > vis ? 0.f : x;
+            for (int s = 0; s < D / 32; ++s) {
+#pragma unroll
+              for (int i = 0; i < NT; ++i)
+                sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                    __builtin_bit_cast(bf16x8, qa[i][s]), __builtin_bit_cast(bf16x8, kb[s]), sc[i],
+                    0, 0, 0);
             }
-          }
-        }
-        // over the lane groups; group g then stores key tile g
-        float mine = 0.f;
+            if (!masked) {
 #pragma unroll
-        for (int j = 0; j < kMine / 16; ++j) {
-          const float v = wave_sum_across_groups(sum[j]);
-          mine = g == j ? v : mine;
+              for (int i = 0; i < NT; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  sum += fast_exp2(__builtin_fmaf(sc[i][e], a.scale, nl[i][e]));
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < NT; ++i) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float x = fast_exp2(__builtin_fmaf(sc[i][e], a.scale, nl[i][e]));
+                  sum += t * kST + key > vis[i][e] ? 0.f : x;
+                }
+              }
+            }
+            sum = wave_sum_across_groups(sum);
+          }
+          if (g == 0) part[(t - c0) & 1][rw][key] = sum;
         }
-        const int p = first + lane;
-        if (p < ctx) {
-          const float* from = r0 == 0 ? a.scores : a.out;
-          a.out[out_row + p] = from[out_row + p] + mine;
-        }
-        cur = nxt;
+        return ++t < c1;
+      };
+      while (step(stage_0, stage_3) && step(stage_1, stage_0) && step(stage_2, stage_1) &&
+             step(stage_3, stage_2)) {
       }
+      wait_vmem_all();
+      lds_barrier();  // the last stage is computed, the ring no longer read or written
     }
     u0 = u1 < begin + units ? u1 : begin + units;
     if (u0 >= u1) return;
@@ -230,11 +272,30 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_observe_kernel(ObserveArgs a)
     if (++kvh == a.NKV) {
       kvh = 0;
       do {
-        ++b;
-      } while (b < a.B - 1 && uniform(seg[b + 1]) == uniform(seg[b]));
-      units = uniform(seg[b + 1]) - uniform(seg[b]);
+        units = uniform(units_of(++b));
+      } while (b < a.B - 1 && units == 0);
     }
   }
+}
+
+template <int D, int NT, int RW>
+void launch_shape(const ObserveArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((gqa_observe_kernel<D, NT, RW>), dim3(static_cast<unsigned>(a.W)),
+                     dim3(kThreads), 0, stream, a);
+}
+
+// As few wavefronts on other rows as hold them: the others then read other keys, and a
+// key is read from LDS by fewer (131,072 tokens, 132 rows, 32/8 heads: NT = 2 on eight
+// wavefronts 129 us, NT = 3 on four 90).
+template <int D>
+void launch_observe(const ObserveArgs& a, hipStream_t stream) {
+  const int rows = a.L * a.G;
+  if (rows <= 16) launch_shape<D, 1, 1>(a, stream);
+  else if (rows <= 32) launch_shape<D, 2, 1>(a, stream);
+  else if (rows <= 64) launch_shape<D, 2, 2>(a, stream);
+  else if (rows <= 128) launch_shape<D, 4, 2>(a, stream);
+  else if (rows <= 192) launch_shape<D, 3, 4>(a, stream);
+  else launch_shape<D, 4, 4>(a, stream);
 }
 
 }  // namespace
@@ -286,13 +347,13 @@ extern "C" int voom_paged_gqa_observe(const void* q, const float* lse, const voi
   a.pt_shift = ilog2(page_tokens);
   a.num_slots = num_slots;
   a.scale = scale * 1.4426950408889634f;
-  const long long most = static_cast<long long>(batch) * num_kv_heads *
-                         ((static_cast<long long>(max_pages) * page_tokens + kUnit - 1) / kUnit);
-  a.W = static_cast<int>(most < 2LL * device_cu_count() ? most : 2LL * device_cu_count());
-  const dim3 grid(static_cast<unsigned>(a.W));
-  if (head_dim == 128)
-    hipLaunchKernelGGL(gqa_observe_kernel<128>, grid, dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL(gqa_observe_kernel<64>, grid, dim3(kThreads), 0, stream, a);
+  const int st = stage_tokens(head_dim);
+  const long long most = ((static_cast<long long>(max_pages) * page_tokens + st - 1) / st) * batch *
+                         num_kv_heads;
+  VOOM_REQUIRE(most < (1LL << 31), "%s: %d pages of %d tokens for %d sequences are too many", who,
+               max_pages, page_tokens, batch);
+  a.W = static_cast<int>(most < device_cu_count() ? most : device_cu_count());  // all run at once
+  if (head_dim == 128) launch_observe<128>(a, stream);
+  else launch_observe<64>(a, stream);
   return VOOM_LAUNCH_CHECK("paged_gqa_observe: launch");
 }

@@ -35,7 +35,7 @@
 // P is rounded to bf16 for the matrix units; its sum, and with it the LSE, is kept
 // of the unrounded fp32 weights (the roundings average out in the output, whose own
 // rounding is as large as one of them).
-#include "common.h"
+#include "paged_ring.h"
 
 #include <cfloat>
 #include <cmath>
@@ -45,7 +45,6 @@ namespace {
 
 constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kBlk = 32;      // tokens of a K/V block in the pool
 constexpr int kKeyWaves = 2;  // wavefronts that share a group of rows
 constexpr int kRowWaves = kWaves / kKeyWaves;
 constexpr int kStages = 4;    // stages of the ring in LDS
@@ -100,22 +99,6 @@ __device__ __forceinline__ int chunks_of(int ctx) {
   return (ctx + stage_tokens(D) - 1) / stage_tokens(D);
 }
 
-// Units 0 .. U - 1 over the workgroups: the first `rem` take base + 1, the others base.
-struct Split {
-  int We, base, rem;
-  __device__ __forceinline__ Split(int U, int W) {
-    We = U < 1 ? 1 : (U < W ? U : W);
-    base = U / We;
-    rem = U - base * We;
-  }
-  __device__ __forceinline__ int begin(int w) const { return w * base + (w < rem ? w : rem); }
-  // the workgroup that holds unit u
-  __device__ __forceinline__ int group(int u) const {
-    const int u_rem = rem * (base + 1);
-    return u < u_rem ? u / (base + 1) : rem + (u - u_rem) / base;
-  }
-};
-
 // Units of a sequence: its chunks for every kv head and row tile that holds a draft.
 template <int D>
 struct Units {
@@ -137,21 +120,12 @@ __device__ __forceinline__ Units<D> scan_units(const TreeArgs& a, int base, int 
   return u;
 }
 
-typedef __attribute__((address_space(3))) void lds_void;
-
 // Chunk c (16 bytes) of K row r sits at c ^ k_swizzle(r) of its row, chunk c of V^T row
 // d at c ^ (d >> 2 & 3): the 16 rows of an operand read then spread over all banks.
 template <int D>
 __device__ __forceinline__ int k_swizzle(int r) {
   return D == 128 ? (r & 3) | ((r >> 3) & 3) << 2 : ((r >> 1) & 1) | ((r >> 3) & 3) << 1;
 }
-
-// The keys of the pages that one segment's wavefronts walk.
-struct Pages {
-  const int32_t* row;  // the sequence's table row
-  int kvh, last;       // last: the context's last block
-  int base, tab;       // base: first of the 64 pages whose slots the lanes hold in tab
-};
 
 // A block of a stage in LDS: K [32][D], then V^T [D][32].
 constexpr int block_elems(int D) { return 2 * kBlk * D; }
@@ -164,37 +138,20 @@ __device__ __forceinline__ void load_stage(uint16_t* stage, const TreeArgs& a, P
   constexpr int kBlocks = stage_blocks(D);
   constexpr int kPieces = kBlk * D / 512;  // of K, and of V^T, of a block
   constexpr int kCpr = D / 8;              // 16-byte chunks of a K row
-  const int sub_shift = a.pt_shift - 5;
-  const int first = bi < pg.last ? bi : pg.last;
-  if (first >> sub_shift < pg.base || (first + kBlocks - 1) >> sub_shift >= pg.base + kWave) {
-    pg.base = first >> sub_shift;
-    const int p = pg.base + lane;
-    pg.tab = p < a.max_pages ? pg.row[p] : 0;
-    wait_vmem_all();  // here, not at the readlanes below on every stage
-  }
+  pg.hold(bi, kBlocks, lane);
 #pragma unroll
   for (int i = 0; i < 2 * kBlocks * kPieces / kWaves; ++i) {
     // piece p = wv + 8 i: block p / (2 kPieces), first its K and then its V^T
     const int p = wv + kWaves * i;
-    const int blk = p / (2 * kPieces);
     const int in_blk = p % (2 * kPieces);
-    int at_blk = bi + blk;
-    at_blk = at_blk < pg.last ? at_blk : pg.last;
-    const int page = at_blk >> sub_shift;
-    int slot = __builtin_amdgcn_readlane(pg.tab, page - pg.base);
-    if (static_cast<unsigned>(slot) >= static_cast<unsigned>(a.num_slots)) slot = 0;
-    const size_t at = ((static_cast<size_t>(slot) * a.NKV + pg.kvh) << sub_shift) +
-                      (at_blk - (page << sub_shift));
+    const size_t at = pg.block(bi + p / (2 * kPieces));
     const bool is_v = in_blk >= kPieces;
     const int sub = in_blk % kPieces;
-    const uint16_t* from = (is_v ? a.v_pool : a.k_pool) + at * (kBlk * D);
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-        const_cast<uint16_t*>(from), static_cast<short>(0), kBlk * D * 2, 0x00020000);
     const int krow = sub * (kWave / kCpr) + lane / kCpr;
     const int ksrc = krow * (D * 2) + 16 * ((lane % kCpr) ^ k_swizzle<D>(krow));
     const int vsrc = sub * 1024 + (lane >> 2) * (kBlk * 2) + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(stage + p * 512), 16,
-                                             is_v ? vsrc : ksrc, 0, 0, AUX);
+    load_piece<AUX>((is_v ? a.v_pool : a.k_pool) + at * (kBlk * D), kBlk * D * 2,
+                    is_v ? vsrc : ksrc, stage + p * 512);
   }
 }
 
@@ -571,7 +528,8 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
     // time through stage_3 while the first of the others are under way; of the others
     // every row sees all, and stage t of them is in t % 4.
     const int last_blk = (ctx - 1) / kBlk;
-    Pages pg{a.table + static_cast<size_t>(b) * a.max_pages, kvh, last_blk, -(1 << 30), 0};
+    Pages pg(a.table + static_cast<size_t>(b) * a.max_pages, a.max_pages, a.num_slots, a.NKV, kvh,
+             a.pt_shift - 5, last_blk);
     int whole = view.prefix / stage_tokens(D);
     whole = whole < c1 ? whole : c1;
     // (else this wavefront only loads)
