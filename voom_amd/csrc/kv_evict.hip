@@ -15,25 +15,33 @@ namespace {
 // -0 as 0); three histogram passes over 11, 11 and 10 bits find the n-th largest one,
 // and a last pass writes the positions in ascending order.
 //
-// What bounds it: the scores once, 4 bytes per token and head, and the latency of the
-// four passes of one workgroup per (sequence, head).
+// What bounds it: the scores once, 4 bytes per token and head, and the latency of one
+// workgroup per (sequence, head).  Up to 65,536 candidates stay in registers, all loads
+// in flight at once (a loop that loaded them for every pass: 43 us for 16 x 8 heads of
+// up to 32,768 tokens, where this takes TIME_SELECT); of longer ones every pass loads
+// 65,536 at a time.  A histogram has eight copies, by lane: scores share few leading bits,
+// and atomics of one wavefront on one address take turns.
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kBins = 2048;
+constexpr int kCopies = 8;
 
 // Larger score, larger key; NaN 0.
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);  // -0 + 0 is 0
-  if (x != x) return 0u;
-  return (b & 0x80000000u) != 0 ? ~b : b | 0x80000000u;
+  const uint32_t k = (b & 0x80000000u) != 0 ? ~b : b | 0x80000000u;
+  return x != x ? 0u : k;
 }
 
+// E: candidates per thread and round.  Round c, wavefront w, element e, lane l hold
+// candidate ((c * 16 + w) * E + e) * 64 + l.
+template <int E>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     const float* __restrict__ scores, const int32_t* __restrict__ ctx_lens,
     int32_t* __restrict__ keep, int32_t* __restrict__ keep_lens, int NKV, int cap, int budget,
     int sink, int recent) {
-  __shared__ int hist[kBins];
+  __shared__ __attribute__((aligned(16))) int hist[kBins][kCopies];
   __shared__ int part[kSelWaves];
   __shared__ int found[2];  // digit that holds the n-th largest, keys above it in this pass
   __shared__ int above_tot[kSelWaves], equal_tot[kSelWaves];
@@ -44,7 +52,6 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
   const int b = row / NKV;
   int ctx = uniform(ctx_lens[b]);
   ctx = ctx < 0 ? 0 : (ctx > cap ? cap : ctx);
-  const float* s = scores + static_cast<size_t>(row) * cap;
   int32_t* out = keep + static_cast<size_t>(row) * budget;
   if (row == b * NKV && tid == 0) keep_lens[b] = ctx < budget ? ctx : budget;
   if (ctx <= budget) {
@@ -55,24 +62,54 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
   for (int i = tid; i < recent; i += kSelThreads) out[budget - recent + i] = ctx - recent + i;
   const int n = budget - sink - recent;
   if (n == 0) return;
-  const int lo = sink, hi = ctx - recent;  // more than n candidates
+  const float* s = scores + static_cast<size_t>(row) * cap + sink;
+  const int count = ctx - recent - sink;  // candidates, more than n
+  const int rounds = (count + kSelThreads * E - 1) / (kSelThreads * E);
+
+  uint32_t key[E];
+  const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<float*>(s), static_cast<short>(0), count * 4, 0x00020000);  // past it: 0
+  auto load = [&](int c) {
+    const int first = (c * kSelWaves + wv) * (E * kWave) + lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      key[e] = __builtin_amdgcn_raw_buffer_load_b32(from, first * 4, e * (kWave * 4), 0);
+#pragma unroll
+    for (int e = 0; e < E; ++e) key[e] = order_key(__builtin_bit_cast(float, key[e]));
+  };
+  // the candidates of this wavefront's element e, round c
+  auto inside = [&](int c, int e) {
+    return ((c * kSelWaves + wv) * E + e) * kWave + lane < count;
+  };
+  load(0);
 
   uint32_t prefix = 0, mask = 0;  // the bits of the n-th largest key found so far
   int need = n;                   // its rank among the keys with that prefix
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     const int bins = pass == 2 ? 1024 : 2048;
-    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    for (int i = tid; i < kBins * kCopies / 4; i += kSelThreads)
+      *reinterpret_cast<u32x4*>(&hist[0][0] + 4 * i) = zero;
     __syncthreads();
-    for (int i = lo + tid; i < hi; i += kSelThreads) {
-      const uint32_t k = order_key(s[i]);
-      if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+    for (int c = 0; c < rounds; ++c) {
+      if (rounds > 1 && (pass > 0 || c > 0)) load(c);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (inside(c, e) && (key[e] & mask) == prefix)
+          atomicAdd(&hist[(key[e] >> shift) & (bins - 1)][lane % kCopies], 1);
+      }
     }
     __syncthreads();
     // thread t owns bins t * per .. of the descending order
     const int per = bins / kSelThreads;
     int mine[2] = {0, 0};
-    for (int j = 0; j < per; ++j) mine[j] = hist[bins - 1 - (tid * per + j)];
+    for (int j = 0; j < per; ++j) {
+      const int* h = hist[bins - 1 - (tid * per + j)];
+      const u32x4 lo = *reinterpret_cast<const u32x4*>(h), hi = *reinterpret_cast<const u32x4*>(h + 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mine[j] += static_cast<int>(lo[k] + hi[k]);
+    }
     const int x = wave_inclusive_scan(mine[0] + mine[1], lane);
     if (lane == kWave - 1) part[wv] = x;
     __syncthreads();
@@ -89,45 +126,55 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     prefix |= static_cast<uint32_t>(found[0]) << shift;
     mask |= static_cast<uint32_t>(bins - 1) << shift;
     need -= found[1];
-    __syncthreads();
   }
 
   // `prefix` is the n-th largest key; `need` of those equal to it stay.  Each
-  // wavefront takes a run of the candidates, counts, and writes behind the runs
-  // before its own.
-  const int run = ((hi - lo + kSelWaves - 1) / kSelWaves + kWave - 1) & ~(kWave - 1);
-  const int r0 = lo + wv * run;
-  const int r1 = r0 + run < hi ? r0 + run : hi;
-  int above = 0, equal = 0;
-  for (int i = r0; i < r1; i += kWave) {
-    const uint32_t k = i + lane < r1 ? order_key(s[i + lane]) : 0u;
-    above += __popcll(__builtin_amdgcn_ballot_w64(i + lane < r1 && k > prefix));
-    equal += __popcll(__builtin_amdgcn_ballot_w64(i + lane < r1 && k == prefix));
-  }
-  if (lane == 0) {
-    above_tot[wv] = above;
-    equal_tot[wv] = equal;
-  }
-  __syncthreads();
-  int at = 0, same = 0;  // kept above the key, and equal to it, in the runs before
-  for (int k = 0; k < wv; ++k) {
-    at += above_tot[k];
-    same += equal_tot[k];
-  }
-  for (int i = r0; i < r1; i += kWave) {
-    const bool in = i + lane < r1;
-    const uint32_t k = in ? order_key(s[i + lane]) : 0u;
-    const uint64_t up = __builtin_amdgcn_ballot_w64(in && k > prefix);
-    const uint64_t eq = __builtin_amdgcn_ballot_w64(in && k == prefix);
-    const uint64_t low = (1ull << lane) - 1;
-    const int eq_before = same + __popcll(eq & low);
-    const bool take = in && (k > prefix || (k == prefix && eq_before < need));
-    if (take) {
-      const int eq_kept = eq_before < need ? eq_before : need;
-      out[sink + at + __popcll(up & low) + eq_kept] = i + lane;
+  // wavefront counts its run of the candidates and writes behind the runs before it.
+  int at = 0, same = 0;  // kept above the key, and equal to it, before the run
+  for (int c = 0; c < rounds; ++c) {
+    if (rounds > 1) load(c);
+    int above = 0, equal = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      above += __popcll(__builtin_amdgcn_ballot_w64(inside(c, e) && key[e] > prefix));
+      equal += __popcll(__builtin_amdgcn_ballot_w64(inside(c, e) && key[e] == prefix));
     }
-    at += __popcll(up);
-    same += __popcll(eq);
+    // (keeps the compiler from holding two lane masks per element until below)
+#pragma unroll
+    for (int e = 0; e < E; ++e) asm volatile("" : "+v"(key[e]));
+    __syncthreads();  // the totals of the round before are read
+    if (lane == 0) {
+      above_tot[wv] = above;
+      equal_tot[wv] = equal;
+    }
+    __syncthreads();
+    int up_all = 0, eq_all = 0;
+    for (int k = 0; k < kSelWaves; ++k) {
+      if (k == wv) {
+        above = up_all;
+        equal = eq_all;
+      }
+      up_all += above_tot[k];
+      eq_all += equal_tot[k];
+    }
+    int up_at = at + above, eq_at = same + equal;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const bool in = inside(c, e);
+      const uint64_t up = __builtin_amdgcn_ballot_w64(in && key[e] > prefix);
+      const uint64_t eq = __builtin_amdgcn_ballot_w64(in && key[e] == prefix);
+      const uint64_t low = (1ull << lane) - 1;
+      const int eq_before = eq_at + __popcll(eq & low);
+      if (in && (key[e] > prefix || (key[e] == prefix && eq_before < need))) {
+        const int eq_kept = eq_before < need ? eq_before : need;
+        out[sink + up_at + __popcll(up & low) + eq_kept] =
+            sink + ((c * kSelWaves + wv) * E + e) * kWave + lane;
+      }
+      up_at += __popcll(up);
+      eq_at += __popcll(eq);
+    }
+    at += up_all;
+    same += eq_all;
   }
 }
 
@@ -139,13 +186,14 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
 // One workgroup moves some dims of a head's rows: 32 dims (64 bytes) of K, or 16 dims
 // of V, whose 32-token blocks are transposed.  It reads a step's rows into registers,
 // waits until all of it is read, and writes: a later step's sources lie behind every
-// row written so far, so the move may be in place.
+// row written so far, so the move may be in place.  The next step's places are looked
+// up while its rows come.
 //
 // What bounds it: the kept rows read and written once; a V block is read in lines of
 // 32 tokens of a dim, whichever of them stay.
 
 constexpr int kMoveThreads = 512;
-constexpr int kStep = 1024;  // rows of a step
+constexpr int kStep = 512;  // rows of a step
 constexpr int kKDims = 32, kVDims = 16;
 constexpr uint32_t kNoRow = 0xffffffffu;
 
@@ -180,8 +228,61 @@ __device__ __forceinline__ void all_read() {
   __syncthreads();
 }
 
+// Where position `from` is read and position `to` written; kNoRow: nothing to move.
+__device__ __forceinline__ void places(const CompactArgs& a, const int32_t* trow,
+                                       const int32_t* drow, int from, long long to, int kvh,
+                                       uint32_t& src, uint32_t& dst) {
+  const uint32_t s = row_of(trow, a.max_pages, from, kvh, a);
+  const uint32_t d =
+      to < (1LL << 30) ? row_of(drow, a.dst_pages, static_cast<int>(to), kvh, a) : kNoRow;
+  src = d == kNoRow || d == s ? kNoRow : s;
+  dst = d;
+}
+
+// Element of V(row, d) = block row / VB of [D, VB], VB = 1 << vb = min(page, 32).
+__device__ __forceinline__ size_t v_element(uint32_t row, int d, int vb, int D) {
+  return ((static_cast<size_t>(row >> vb) * D + d) << vb) + (row & ((1u << vb) - 1));
+}
+
+// One workgroup: the scores of one (sequence, kv head), and zeros behind them.
+__device__ __forceinline__ void move_scores(const CompactArgs& a, const int32_t* keep, int b,
+                                            int kvh, int n, int start) {
+  const int tid = static_cast<int>(threadIdx.x);
+  const size_t row = (static_cast<size_t>(b) * a.NKV + kvh) * a.cap;
+  const float* s = a.scores + row;
+  float* o = a.scores_out + row;
+  const int first = start < a.cap ? start : a.cap;
+  if (s != o)
+    for (int i = tid; i < first; i += kMoveThreads) o[i] = s[i];
+  constexpr int kLoads = 8;
+  for (int i0 = 0; i0 < n; i0 += kLoads * kMoveThreads) {
+    int from[kLoads];
+    float v[kLoads];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int i = i0 + j * kMoveThreads + tid;
+      from[j] = i < n ? keep[i] : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) v[j] = from[j] >= 0 && from[j] < a.cap ? s[from[j]] : 0.f;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) asm volatile("" : "+v"(v[j]));
+    all_read();
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int i = i0 + j * kMoveThreads + tid;
+      if (i < n && start + static_cast<long long>(i) < a.cap) o[start + i] = v[j];
+    }
+  }
+  for (long long i = static_cast<long long>(first) + n + tid; i < a.cap; i += kMoveThreads)
+    o[i] = 0.f;
+}
+
 __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactArgs a) {
-  __shared__ uint32_t src[kStep], dst[kStep];
+  static_assert(kStep == kMoveThreads, "a thread looks one row up");
+  // Places of three steps: while the next step's are looked up, a wavefront may still
+  // store the rows of the step before.
+  __shared__ uint32_t src[3][kStep], dst[3][kStep];
   const int tid = static_cast<int>(threadIdx.x);
   const int kvh = static_cast<int>(blockIdx.y);
   const int b = static_cast<int>(blockIdx.z);
@@ -194,43 +295,24 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactArgs a) {
   int start = a.start != nullptr ? uniform(a.start[b]) : 0;
   start = start < 0 ? 0 : start;
 
-  if (part == k_parts + v_parts) {  // the scores
-    const size_t row = (static_cast<size_t>(b) * a.NKV + kvh) * a.cap;
-    const float* s = a.scores + row;
-    float* o = a.scores_out + row;
-    const int first = start < a.cap ? start : a.cap;
-    if (s != o)
-      for (int i = tid; i < first; i += kMoveThreads) o[i] = s[i];
-    for (int i0 = 0; i0 < n; i0 += kMoveThreads) {
-      float v = 0.f;
-      const int i = i0 + tid;
-      if (i < n) {
-        const int from = keep[i];
-        if (from >= 0 && from < a.cap) v = s[from];
-      }
-      asm volatile("" : "+v"(v));
-      all_read();
-      if (i < n && start + static_cast<long long>(i) < a.cap) o[start + i] = v;
-    }
-    for (long long i = static_cast<long long>(first) + n + tid; i < a.cap; i += kMoveThreads)
-      o[i] = 0.f;
+  if (part == k_parts + v_parts) {
+    move_scores(a, keep, b, kvh, n, start);
     return;
   }
 
   const int32_t* trow = a.table + static_cast<size_t>(b) * a.max_pages;
   const int32_t* drow = a.dst_table + static_cast<size_t>(b) * a.dst_pages;
+  auto look_up = [&](int i0, int buf) {
+    const int i = i0 + tid;
+    if (i >= n) return;
+    places(a, trow, drow, keep[i], start + static_cast<long long>(i), kvh, src[buf][tid],
+           dst[buf][tid]);
+  };
+  look_up(0, 0);
+  __syncthreads();
+  int buf = 0, next = 1;
   for (int i0 = 0; i0 < n; i0 += kStep) {
     const int m = n - i0 < kStep ? n - i0 : kStep;
-    for (int i = tid; i < m; i += kMoveThreads) {
-      const long long to = static_cast<long long>(start) + i0 + i;
-      uint32_t from = row_of(trow, a.max_pages, keep[i0 + i], kvh, a);
-      const uint32_t at =
-          to < (1LL << 30) ? row_of(drow, a.dst_pages, static_cast<int>(to), kvh, a) : kNoRow;
-      if (at == kNoRow || at == from) from = kNoRow;  // nothing to move
-      src[i] = from;
-      dst[i] = at;
-    }
-    __syncthreads();
     if (part < k_parts) {
       constexpr int kChunks = kKDims / 8;
       constexpr int kPass = kMoveThreads / kChunks;
@@ -240,46 +322,113 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactArgs a) {
       u32x4 v[kLoads];
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
-        const int i = r + j * kPass;
-        const uint32_t from = i < m ? src[i] : kNoRow;
+        const uint32_t from = r + j * kPass < m ? src[buf][r + j * kPass] : kNoRow;
         if (from != kNoRow)
           v[j] = *reinterpret_cast<const u32x4*>(a.k_pool + static_cast<size_t>(from) * a.D + c);
       }
+      look_up(i0 + kStep, next);
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) asm volatile("" : "+v"(v[j]));
       all_read();
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int i = r + j * kPass;
-        if (i < m && src[i] != kNoRow)
-          *reinterpret_cast<u32x4*>(a.k_pool + static_cast<size_t>(dst[i]) * a.D + c) = v[j];
+        if (i < m && src[buf][i] != kNoRow)
+          *reinterpret_cast<u32x4*>(a.k_pool + static_cast<size_t>(dst[buf][i]) * a.D + c) = v[j];
       }
     } else {
-      // V(row, d) = block row / VB of [D, VB], VB = min(page, 32)
       constexpr int kLoads = kStep / 32;
       const int vb = a.pt_shift < 5 ? a.pt_shift : 5;
       const int d = (part - k_parts) * kVDims + tid / 32;
-      auto at = [&](uint32_t row) {
-        return a.v_pool + (((static_cast<size_t>(row >> vb) * a.D) + d) << vb) +
-               (row & ((1u << vb) - 1));
-      };
       uint32_t v[kLoads];
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int i = (tid & 31) + 32 * j;
-        const uint32_t from = i < m ? src[i] : kNoRow;
-        if (from != kNoRow) v[j] = *at(from);
+        const uint32_t from = i < m ? src[buf][i] : kNoRow;
+        if (from != kNoRow) v[j] = a.v_pool[v_element(from, d, vb, a.D)];
       }
+      look_up(i0 + kStep, next);
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) asm volatile("" : "+v"(v[j]));
       all_read();
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) {
         const int i = (tid & 31) + 32 * j;
-        if (i < m && src[i] != kNoRow) *at(dst[i]) = static_cast<uint16_t>(v[j]);
+        if (i < m && src[buf][i] != kNoRow)
+          a.v_pool[v_element(dst[buf][i], d, vb, a.D)] = static_cast<uint16_t>(v[j]);
       }
     }
-    __syncthreads();  // src and dst are written again
+    buf = next;
+    next = next == 2 ? 0 : next + 1;
+  }
+}
+
+// Few rows (the accepted branch of a tree of drafts): one workgroup per (sequence, kv
+// head) moves all of them, every row of 128 dims read before the first is written.
+constexpr int kFewRows = 64;
+constexpr int kFewDims = 128;
+
+__global__ __launch_bounds__(kMoveThreads) void compact_few_kernel(CompactArgs a) {
+  __shared__ uint32_t src[kFewRows], dst[kFewRows];
+  const int tid = static_cast<int>(threadIdx.x);
+  const int kvh = static_cast<int>(blockIdx.y);
+  const int b = static_cast<int>(blockIdx.z);
+  const int32_t* keep = a.keep + (static_cast<size_t>(b) * a.keep_heads +
+                                  (a.keep_heads == 1 ? 0 : kvh)) * a.n;
+  int n = uniform(a.keep_lens[b]);
+  n = n < 0 ? 0 : (n > a.n ? a.n : n);
+  int start = a.start != nullptr ? uniform(a.start[b]) : 0;
+  start = start < 0 ? 0 : start;
+  if (blockIdx.x == 1) {
+    move_scores(a, keep, b, kvh, n, start);
+    return;
+  }
+  if (tid < n)
+    places(a, a.table + static_cast<size_t>(b) * a.max_pages,
+           a.dst_table + static_cast<size_t>(b) * a.dst_pages, keep[tid],
+           start + static_cast<long long>(tid), kvh, src[tid], dst[tid]);
+  __syncthreads();
+  const int vb = a.pt_shift < 5 ? a.pt_shift : 5;
+  for (int d0 = 0; d0 < a.D; d0 += kFewDims) {
+    const int dims = a.D - d0 < kFewDims ? a.D - d0 : kFewDims;
+    constexpr int kLoads = kFewRows * kFewDims / 8 / kMoveThreads;  // K, 16 bytes each
+    constexpr int kColumns = kFewRows * kFewDims / kMoveThreads;    // V, elements
+    const int chunk = tid % (kFewDims / 8), r0 = tid / (kFewDims / 8);
+    u32x4 k[kLoads];
+    uint32_t v[kColumns];
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int i = r0 + j * (kMoveThreads / (kFewDims / 8));
+      if (i < n && 8 * chunk < dims && src[i] != kNoRow)
+        k[j] = *reinterpret_cast<const u32x4*>(a.k_pool + static_cast<size_t>(src[i]) * a.D + d0 +
+                                               8 * chunk);
+    }
+#pragma unroll
+    for (int j = 0; j < kColumns; ++j) {  // 16 rows side by side, 32 dims, rows slowest
+      const int i = (tid & 15) + 16 * (j / (kFewDims / 32));
+      const int d = tid / 16 + 32 * (j % (kFewDims / 32));
+      if (i < n && d < dims && src[i] != kNoRow)
+        v[j] = a.v_pool[v_element(src[i], d0 + d, vb, a.D)];
+    }
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) asm volatile("" : "+v"(k[j]));
+#pragma unroll
+    for (int j = 0; j < kColumns; ++j) asm volatile("" : "+v"(v[j]));
+    all_read();
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int i = r0 + j * (kMoveThreads / (kFewDims / 8));
+      if (i < n && 8 * chunk < dims && src[i] != kNoRow)
+        *reinterpret_cast<u32x4*>(a.k_pool + static_cast<size_t>(dst[i]) * a.D + d0 + 8 * chunk) =
+            k[j];
+    }
+#pragma unroll
+    for (int j = 0; j < kColumns; ++j) {
+      const int i = (tid & 15) + 16 * (j / (kFewDims / 32));
+      const int d = tid / 16 + 32 * (j % (kFewDims / 32));
+      if (i < n && d < dims && src[i] != kNoRow)
+        a.v_pool[v_element(dst[i], d0 + d, vb, a.D)] = static_cast<uint16_t>(v[j]);
+    }
   }
 }
 
@@ -301,9 +450,16 @@ extern "C" int voom_evict_select(const float* scores, const int32_t* ctx_lens, i
                num_kv_heads, score_tokens);
   VOOM_REQUIRE(budget > 0 && sink >= 0 && recent >= 0 && sink <= budget && recent <= budget - sink,
                "%s: sink %d and recent %d must fit the budget %d", who, sink, recent, budget);
-  hipLaunchKernelGGL(evict_select_kernel, dim3(static_cast<unsigned>(batch * num_kv_heads)),
-                     dim3(kSelThreads), 0, stream, scores, ctx_lens, keep, keep_lens, num_kv_heads,
-                     score_tokens, budget, sink, recent);
+  const dim3 grid(static_cast<unsigned>(batch * num_kv_heads)), block(kSelThreads);
+  if (score_tokens <= 8 * kSelThreads)
+    hipLaunchKernelGGL(evict_select_kernel<8>, grid, block, 0, stream, scores, ctx_lens, keep,
+                       keep_lens, num_kv_heads, score_tokens, budget, sink, recent);
+  else if (score_tokens <= 32 * kSelThreads)
+    hipLaunchKernelGGL(evict_select_kernel<32>, grid, block, 0, stream, scores, ctx_lens, keep,
+                       keep_lens, num_kv_heads, score_tokens, budget, sink, recent);
+  else
+    hipLaunchKernelGGL(evict_select_kernel<64>, grid, block, 0, stream, scores, ctx_lens, keep,
+                       keep_lens, num_kv_heads, score_tokens, budget, sink, recent);
   return VOOM_LAUNCH_CHECK("evict_select: launch");
 }
 
@@ -355,9 +511,13 @@ extern "C" int voom_compact_kv(void* k_pool, void* v_pool, const int32_t* block_
   a.dst_pages = dst_pages;
   a.pt_shift = ilog2(page_tokens);
   a.num_slots = num_slots;
-  const unsigned parts = head_dim / kKDims + head_dim / kVDims + (scores != nullptr ? 1 : 0);
-  hipLaunchKernelGGL(compact_kernel,
-                     dim3(parts, static_cast<unsigned>(num_kv_heads), static_cast<unsigned>(batch)),
-                     dim3(kMoveThreads), 0, stream, a);
+  const unsigned moves_scores = scores != nullptr ? 1 : 0;
+  dim3 grid(1 + moves_scores, static_cast<unsigned>(num_kv_heads), static_cast<unsigned>(batch));
+  if (keep_tokens <= kFewRows) {
+    hipLaunchKernelGGL(compact_few_kernel, grid, dim3(kMoveThreads), 0, stream, a);
+  } else {
+    grid.x = head_dim / kKDims + head_dim / kVDims + moves_scores;
+    hipLaunchKernelGGL(compact_kernel, grid, dim3(kMoveThreads), 0, stream, a);
+  }
   return VOOM_LAUNCH_CHECK("compact_kv: launch");
 }

@@ -10,13 +10,17 @@
 // All of it in fp32, rounded to bf16 once.
 //
 // What bounds it: the projections read and q, k, v written once; one launch for a
-// token's few heads.
+// token's few heads.  Some workgroups take the query and key heads, 8 dims per lane; the
+// others the value heads, a 32-token cache block each, which they transpose in LDS: V
+// pages hold 64-byte rows of 32 tokens, and written element by element a prompt of
+// 2,011 tokens (32/8 heads of 128) took 23 us where this takes TIME_PROMPT.
 #include "common.h"
 
 namespace voom {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMaxDim = 256;
 
 struct QkArgs {
   const uint16_t* qkv;
@@ -32,7 +36,9 @@ struct QkArgs {
   const int32_t* start;      // [B]
   const int32_t* lens;       // [B], or null: L each
   float eps;
-  int P, rd, interleaved, B, L, nq, nkv, hd, group, pt_shift, max_pages, num_slots;
+  int P, rd, interleaved, B, L, nq, nkv, hd, group_shift, pt_shift, max_pages, num_slots;
+  int blocks;     // V blocks that the new tokens of a sequence can touch
+  int qk_groups;  // workgroups of query and key heads, before those of V
 };
 
 __device__ __forceinline__ void unpack8(u32x4 x, float (&f)[8]) {
@@ -52,72 +58,70 @@ __device__ __forceinline__ void load8(const float* p, float (&f)[8]) {
   }
 }
 
-// `group` lanes (a power of two, 8 dims each) per head of a token.
-__global__ __launch_bounds__(kThreads) void qk_norm_rope_append_kernel(QkArgs a) {
-  const int heads = a.nq + 2 * a.nkv;
-  const long long idx = static_cast<long long>(blockIdx.x) * kThreads + threadIdx.x;
-  const long long rh = idx / a.group;
-  const int lane = static_cast<int>(idx - rh * a.group);
-  const long long row = rh / heads;
-  const int h = static_cast<int>(rh - row * heads);
-  const bool in = row < static_cast<long long>(a.B) * a.L && 8 * lane < a.hd;
-  const int b = in ? static_cast<int>(row / a.L) : 0;
-  const int t = in ? static_cast<int>(row - static_cast<long long>(b) * a.L) : 0;
+// Query and key heads: `group` lanes (a power of two, 8 dims each) per head of a token.
+__device__ __forceinline__ void query_and_key_heads(const QkArgs& a) {
+  const int heads = a.nq + a.nkv;
+  const unsigned idx = blockIdx.x * kThreads + threadIdx.x;
+  const int rh = static_cast<int>(idx >> a.group_shift);
+  const int lane = static_cast<int>(idx & ((1u << a.group_shift) - 1));
+  const int row = rh / heads;
+  const int h = rh - row * heads;
+  const bool in = row < a.B * a.L && 8 * lane < a.hd;
+  const int b = in ? row / a.L : 0;
+  const int t = in ? row - b * a.L : 0;
   const int d0 = in ? 8 * lane : 0;
-  const uint16_t* src = a.qkv + (in ? rh : 0) * a.hd;
+  const uint16_t* src = a.qkv + (in ? static_cast<size_t>(row) * (heads + a.nkv) + h : 0) * a.hd;
   const u32x4 raw = *reinterpret_cast<const u32x4*>(src + d0);
   u32x4 o = raw;
-  if (h < a.nq + a.nkv) {
-    float x[8];
-    unpack8(raw, x);
-    const uint16_t* w = h < a.nq ? a.q_weight : a.k_weight;
-    const int half = a.rd / 2;
-    const bool turn = d0 < a.rd;
-    // the dims that these turn with, half layout
-    const int p0 = a.interleaved || !turn ? d0 : (d0 < half ? d0 + half : d0 - half);
-    float y[8];
-    unpack8(*reinterpret_cast<const u32x4*>(src + p0), y);
-    if (w != nullptr) {
-      float ss = 0.f;
+  float x[8];
+  unpack8(raw, x);
+  const uint16_t* w = h < a.nq ? a.q_weight : a.k_weight;
+  const int half = a.rd / 2;
+  const bool turn = d0 < a.rd;
+  // the dims that these turn with, half layout
+  const int p0 = a.interleaved || !turn ? d0 : (d0 < half ? d0 + half : d0 - half);
+  float y[8];
+  unpack8(*reinterpret_cast<const u32x4*>(src + p0), y);
+  if (w != nullptr) {
+    float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = in ? __builtin_fmaf(x[e], x[e], ss) : 0.f;
-      for (int k = 1; k < a.group; k <<= 1) ss += __shfl_xor(ss, k);
-      const float r = 1.f / sqrtf(ss / static_cast<float>(a.hd) + a.eps);
-      float wx[8], wy[8];
-      unpack8(*reinterpret_cast<const u32x4*>(w + d0), wx);
-      unpack8(*reinterpret_cast<const u32x4*>(w + p0), wy);
+    for (int e = 0; e < 8; ++e) ss = in ? __builtin_fmaf(x[e], x[e], ss) : 0.f;
+    for (int k = 1; k < 1 << a.group_shift; k <<= 1) ss += __shfl_xor(ss, k);
+    const float r = 1.f / sqrtf(ss / static_cast<float>(a.hd) + a.eps);
+    float wx[8], wy[8];
+    unpack8(*reinterpret_cast<const u32x4*>(w + d0), wx);
+    unpack8(*reinterpret_cast<const u32x4*>(w + p0), wy);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = x[e] * r * wx[e];
-        y[e] = y[e] * r * wy[e];
+    for (int e = 0; e < 8; ++e) {
+      x[e] = x[e] * r * wx[e];
+      y[e] = y[e] * r * wy[e];
+    }
+  }
+  if (turn) {
+    int pos = a.positions[in ? row : 0];
+    pos = pos < 0 ? 0 : (pos < a.P ? pos : a.P - 1);
+    const size_t at = static_cast<size_t>(pos) * half;
+    if (a.interleaved) {
+      const f32x4 c = *reinterpret_cast<const f32x4*>(a.cos_t + at + d0 / 2);
+      const f32x4 s = *reinterpret_cast<const f32x4*>(a.sin_t + at + d0 / 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float u = x[2 * e], v = x[2 * e + 1];
+        x[2 * e] = u * c[e] - v * s[e];
+        x[2 * e + 1] = v * c[e] + u * s[e];
       }
-    }
-    if (turn) {
-      int pos = a.positions[in ? row : 0];
-      pos = pos < 0 ? 0 : (pos < a.P ? pos : a.P - 1);
-      const size_t at = static_cast<size_t>(pos) * half;
-      if (a.interleaved) {
-        const f32x4 c = *reinterpret_cast<const f32x4*>(a.cos_t + at + d0 / 2);
-        const f32x4 s = *reinterpret_cast<const f32x4*>(a.sin_t + at + d0 / 2);
+    } else {
+      const float sign = d0 < half ? -1.f : 1.f;
+      float c[8], s[8];
+      load8(a.cos_t + at + (d0 < half ? d0 : d0 - half), c);
+      load8(a.sin_t + at + (d0 < half ? d0 : d0 - half), s);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float u = x[2 * e], v = x[2 * e + 1];
-          x[2 * e] = u * c[e] - v * s[e];
-          x[2 * e + 1] = v * c[e] + u * s[e];
-        }
-      } else {
-        const float sign = d0 < half ? -1.f : 1.f;
-        float c[8], s[8];
-        load8(a.cos_t + at + (d0 < half ? d0 : d0 - half), c);
-        load8(a.sin_t + at + (d0 < half ? d0 : d0 - half), s);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * c[e] + sign * y[e] * s[e];
-      }
+      for (int e = 0; e < 8; ++e) x[e] = x[e] * c[e] + sign * y[e] * s[e];
     }
-    if (w != nullptr || turn) {
+  }
+  if (w != nullptr || turn) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
-    }
+    for (int e = 0; e < 4; ++e) o[e] = pack_bf16x2(x[2 * e], x[2 * e + 1]);
   }
   if (!in) return;
   if (h < a.nq) {
@@ -129,20 +133,70 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_append_kernel(QkArgs a)
   const long long pos = static_cast<long long>(a.start[b]) + t;
   if (a.start[b] < 0 || pos >= static_cast<long long>(a.max_pages) << a.pt_shift) return;
   const int off = static_cast<int>(pos) & ((1 << a.pt_shift) - 1);
-  const int slot = a.table[static_cast<size_t>(b) * a.max_pages + (static_cast<int>(pos) >> a.pt_shift)];
+  const int slot =
+      a.table[static_cast<size_t>(b) * a.max_pages + (static_cast<int>(pos) >> a.pt_shift)];
   if (static_cast<unsigned>(slot) >= static_cast<unsigned>(a.num_slots)) return;
-  const bool is_k = h < a.nq + a.nkv;
-  const int kvh = h - a.nq - (is_k ? 0 : a.nkv);
-  const size_t at = ((static_cast<size_t>(slot) * a.nkv + kvh) << a.pt_shift) + off;
-  if (is_k) {
-    *reinterpret_cast<u32x4*>(a.k_pool + at * a.hd + d0) = o;
+  const size_t at = ((static_cast<size_t>(slot) * a.nkv + (h - a.nq)) << a.pt_shift) + off;
+  *reinterpret_cast<u32x4*>(a.k_pool + at * a.hd + d0) = o;
+}
+
+// One block of up to 32 consecutive cache positions of one (sequence, value head).
+__device__ __forceinline__ void value_block(const QkArgs& a, int task) {
+  __shared__ __attribute__((aligned(16))) uint16_t tile[32][kMaxDim + 8];
+  const int vb = a.pt_shift < 5 ? a.pt_shift : 5;
+  const int VB = 1 << vb;
+  const int bh = task / a.blocks;
+  const int j = task - bh * a.blocks;  // of the blocks that the sequence's tokens can touch
+  const int b = bh / a.nkv;
+  const int h = bh - b * a.nkv;
+  int n = a.lens != nullptr ? uniform(a.lens[b]) : a.L;
+  n = n < a.L ? n : a.L;
+  const int start = uniform(a.start[b]);
+  const int cap = a.max_pages << a.pt_shift;
+  if (start < 0 || start >= cap) return;
+  // tokens t0 .. t1 land in this block, at its columns c0 ..
+  const int first = ((start >> vb) + j) << vb;  // cache position of the block
+  const int t0 = first > start ? first - start : 0;
+  int t1 = first + VB - start;
+  t1 = t1 < n ? t1 : n;
+  if (t0 >= t1 || first >= cap) return;
+  const int c0 = start + t0 - first;
+  const int slot = uniform(a.table[static_cast<size_t>(b) * a.max_pages + (first >> a.pt_shift)]);
+  if (static_cast<unsigned>(slot) >= static_cast<unsigned>(a.num_slots)) return;
+  const int chunks = a.hd / 8;
+  const int heads = a.nq + 2 * a.nkv;
+  for (int i = threadIdx.x; i < (t1 - t0) * chunks; i += kThreads) {
+    const int t = i / chunks;
+    const int c = i - t * chunks;
+    *reinterpret_cast<u32x4*>(&tile[c0 + t][8 * c]) = *reinterpret_cast<const u32x4*>(
+        a.qkv + ((static_cast<size_t>(b) * a.L + t0 + t) * heads + a.nq + a.nkv + h) * a.hd +
+        8 * c);
+  }
+  __syncthreads();
+  const size_t head_page = static_cast<size_t>(slot) * a.nkv + h;
+  uint16_t* v = a.v_pool + (((head_page << (a.pt_shift - vb)) +
+                             ((first & ((1 << a.pt_shift) - 1)) >> vb)) * a.hd << vb);
+  if (t1 - t0 == 32) {  // whole rows of 32 tokens, 16 bytes per lane
+    for (int i = threadIdx.x; i < a.hd * 4; i += kThreads) {
+      const int d = i >> 2, g = i & 3;
+      u32x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        o[e] = tile[8 * g + 2 * e][d] | static_cast<uint32_t>(tile[8 * g + 2 * e + 1][d]) << 16;
+      *reinterpret_cast<u32x4*>(v + d * 32 + 8 * g) = o;
+    }
     return;
   }
-  const int vb = a.pt_shift < 5 ? a.pt_shift : 5;
-  uint16_t* v = a.v_pool + (((at >> vb) * a.hd + d0) << vb) + (off & ((1 << vb) - 1));
-#pragma unroll
-  for (int e = 0; e < 8; ++e)
-    v[e << vb] = static_cast<uint16_t>(e & 1 ? o[e >> 1] >> 16 : o[e >> 1] & 0xffffu);
+  for (int i = threadIdx.x; i < a.hd << vb; i += kThreads) {
+    const int d = i >> vb, c = i & (VB - 1);
+    if (c >= c0 && c < c0 + t1 - t0) v[i] = tile[c][d];
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void qk_norm_rope_append_kernel(QkArgs a) {
+  const int task = static_cast<int>(blockIdx.x) - a.qk_groups;
+  if (task < 0) query_and_key_heads(a);
+  else value_block(a, task);
 }
 
 }  // namespace
@@ -166,7 +220,7 @@ extern "C" int voom_qk_norm_rope_append(const void* qkv, const void* q_weight,
                    max_pages > 0 && num_slots > 0 && rope_rows > 0,
                "%s: bad geometry (batch %d, %d new tokens, heads %d/%d, %d rope rows)", who, batch,
                new_tokens, num_q_heads, num_kv_heads, rope_rows);
-  VOOM_REQUIRE(head_dim > 0 && head_dim % 16 == 0 && head_dim <= 256,
+  VOOM_REQUIRE(head_dim > 0 && head_dim % 16 == 0 && head_dim <= kMaxDim,
                "%s: head_dim %d must be a multiple of 16 up to 256", who, head_dim);
   VOOM_REQUIRE(rotary_dim > 0 && rotary_dim % 16 == 0 && rotary_dim <= head_dim,
                "%s: rotary_dim %d must be a multiple of 16 up to head_dim %d", who, rotary_dim,
@@ -203,16 +257,21 @@ extern "C" int voom_qk_norm_rope_append(const void* qkv, const void* q_weight,
   a.nq = num_q_heads;
   a.nkv = num_kv_heads;
   a.hd = head_dim;
-  a.group = 1;
-  while (8 * a.group < head_dim) a.group <<= 1;
+  a.group_shift = 0;
+  while (8 << a.group_shift < head_dim) ++a.group_shift;
   a.pt_shift = ilog2(page_tokens);
   a.max_pages = max_pages;
   a.num_slots = num_slots;
-  const long long total = static_cast<long long>(batch) * new_tokens *
-                          (num_q_heads + 2LL * num_kv_heads) * a.group;
-  VOOM_REQUIRE(total < (1LL << 38), "%s: too many heads in one call", who);
-  hipLaunchKernelGGL(qk_norm_rope_append_kernel,
-                     dim3(static_cast<unsigned>((total + kThreads - 1) / kThreads)), dim3(kThreads),
-                     0, stream, a);
+  const int block_tokens = page_tokens < 32 ? page_tokens : 32;
+  a.blocks = (new_tokens + block_tokens - 2) / block_tokens + 1;
+  const long long lanes = static_cast<long long>(batch) * new_tokens *
+                          (num_q_heads + static_cast<long long>(num_kv_heads)) << a.group_shift;
+  const long long v_groups = static_cast<long long>(batch) * num_kv_heads * a.blocks;
+  VOOM_REQUIRE(lanes < (1LL << 31) - kThreads && v_groups < (1LL << 30),
+               "%s: too many heads of too many tokens in one call", who);
+  a.qk_groups = static_cast<int>((lanes + kThreads - 1) / kThreads);
+  const long long groups = a.qk_groups + v_groups;
+  hipLaunchKernelGGL(qk_norm_rope_append_kernel, dim3(static_cast<unsigned>(groups)),
+                     dim3(kThreads), 0, stream, a);
   return VOOM_LAUNCH_CHECK("qk_norm_rope_append: launch");
 }
