@@ -16,16 +16,16 @@ namespace {
 // and a last pass writes the positions in ascending order.
 //
 // What bounds it: the scores once, 4 bytes per token and head, and the latency of one
-// workgroup per (sequence, head).  Up to 65,536 candidates stay in registers, all loads
+// workgroup per (sequence, head).  Up to 49,152 candidates stay in registers, all loads
 // in flight at once (a loop that loaded them for every pass: 43 us for 16 x 8 heads of
 // up to 32,768 tokens, where this takes TIME_SELECT); of longer ones every pass loads
-// 65,536 at a time.  A histogram has eight copies, by lane: scores share few leading bits,
-// and atomics of one wavefront on one address take turns.
+// 49,152 at a time.  Its histogram has eight copies, by lane: scores share few leading bits,
+// and atomics of one wavefront on one address take turns.  The second and third
+// pass look only at the keys that share the first digit, from a list in LDS where it
+// holds them.
 
-constexpr int kSelThreads = 1024;
-constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kBins = 2048;
-constexpr int kCopies = 8;
+constexpr int kList = 16384;  // candidates that share their first digit with the n-th largest
 
 // Larger score, larger key; NaN 0.
 __device__ __forceinline__ uint32_t order_key(float x) {
@@ -34,17 +34,30 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   return x != x ? 0u : k;
 }
 
+// Exclusive prefix sum of the wavefronts' totals (at most 16) for wavefront wv, and
+// their sum.
+template <int WAVES>
+__device__ __forceinline__ int before_wave(const int* tot, int wv, int lane, int& all) {
+  const int x = wave_inclusive_scan(lane < WAVES ? tot[lane] : 0, lane);
+  all = __builtin_amdgcn_readlane(x, kWave - 1);
+  return wv == 0 ? 0 : __builtin_amdgcn_readlane(x, wv - 1);
+}
+
 // E: candidates per thread and round.  Round c, wavefront w, element e, lane l hold
-// candidate ((c * 16 + w) * E + e) * 64 + l.
-template <int E>
+// candidate ((c * waves + w) * E + e) * 64 + l; past the last one the key is 0.
+// COPIES: of the histogram, by lane.
+template <int kSelThreads, int E, int COPIES>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     const float* __restrict__ scores, const int32_t* __restrict__ ctx_lens,
     int32_t* __restrict__ keep, int32_t* __restrict__ keep_lens, int NKV, int cap, int budget,
     int sink, int recent) {
-  __shared__ __attribute__((aligned(16))) int hist[kBins][kCopies];
+  constexpr int kSelWaves = kSelThreads / kWave;
+  __shared__ __attribute__((aligned(16))) int hist[kBins][COPIES];
+  __shared__ uint32_t list[E > 8 ? kList : 1];
+  __shared__ int listed;
   __shared__ int part[kSelWaves];
-  __shared__ int found[2];  // digit that holds the n-th largest, keys above it in this pass
-  __shared__ int above_tot[kSelWaves], equal_tot[kSelWaves];
+  __shared__ int found[3];  // digit that holds the n-th largest; keys above it, keys in it
+  __shared__ int kept_tot[kSelWaves], equal_tot[kSelWaves];
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & (kWave - 1);
   const int wv = uniform(tid / kWave);
@@ -58,67 +71,79 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     for (int i = tid; i < budget; i += kSelThreads) out[i] = i < ctx ? i : -1;
     return;
   }
-  for (int i = tid; i < sink; i += kSelThreads) out[i] = i;
-  for (int i = tid; i < recent; i += kSelThreads) out[budget - recent + i] = ctx - recent + i;
   const int n = budget - sink - recent;
-  if (n == 0) return;
   const float* s = scores + static_cast<size_t>(row) * cap + sink;
   const int count = ctx - recent - sink;  // candidates, more than n
   const int rounds = (count + kSelThreads * E - 1) / (kSelThreads * E);
 
   uint32_t key[E];
   const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<float*>(s), static_cast<short>(0), count * 4, 0x00020000);  // past it: 0
+      const_cast<float*>(s), static_cast<short>(0), count * 4, 0x00020000);
+  auto first_of = [&](int c) { return (c * kSelWaves + wv) * (E * kWave) + lane; };
   auto load = [&](int c) {
-    const int first = (c * kSelWaves + wv) * (E * kWave) + lane;
+    const int first = first_of(c);
 #pragma unroll
     for (int e = 0; e < E; ++e)
       key[e] = __builtin_amdgcn_raw_buffer_load_b32(from, first * 4, e * (kWave * 4), 0);
 #pragma unroll
-    for (int e = 0; e < E; ++e) key[e] = order_key(__builtin_bit_cast(float, key[e]));
+    for (int e = 0; e < E; ++e) {
+      const uint32_t k = order_key(__builtin_bit_cast(float, key[e]));
+      key[e] = first + e * kWave < count ? k : 0u;
+    }
   };
-  // the candidates of this wavefront's element e, round c
-  auto inside = [&](int c, int e) {
-    return ((c * kSelWaves + wv) * E + e) * kWave + lane < count;
-  };
-  load(0);
+  if (n != 0) load(0);
+  for (int i = tid; i < sink; i += kSelThreads) out[i] = i;
+  for (int i = tid; i < recent; i += kSelThreads) out[budget - recent + i] = ctx - recent + i;
+  if (n == 0) return;
 
   uint32_t prefix = 0, mask = 0;  // the bits of the n-th largest key found so far
   int need = n;                   // its rank among the keys with that prefix
+  bool short_list = false;        // those keys are in `list`
+  if (tid == 0) listed = 0;
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     const int bins = pass == 2 ? 1024 : 2048;
-    const u32x4 zero = {0u, 0u, 0u, 0u};
-    for (int i = tid; i < kBins * kCopies / 4; i += kSelThreads)
-      *reinterpret_cast<u32x4*>(&hist[0][0] + 4 * i) = zero;
+    for (int i = tid; i < kBins * COPIES; i += kSelThreads) (&hist[0][0])[i] = 0;
     __syncthreads();
-    for (int c = 0; c < rounds; ++c) {
-      if (rounds > 1 && (pass > 0 || c > 0)) load(c);
+    if (short_list) {
+      for (int i = tid; i < listed; i += kSelThreads)
+        if ((list[i] & mask) == prefix)
+          atomicAdd(&hist[(list[i] >> shift) & (bins - 1)][lane % COPIES], 1);
+    } else {
+      for (int c = 0; c < rounds; ++c) {
+        if (rounds > 1 && (pass > 0 || c > 0)) load(c);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (inside(c, e) && (key[e] & mask) == prefix)
-          atomicAdd(&hist[(key[e] >> shift) & (bins - 1)][lane % kCopies], 1);
+        for (int e = 0; e < E; ++e) {
+          if (first_of(c) + e * kWave < count && (key[e] & mask) == prefix)
+            atomicAdd(&hist[(key[e] >> shift) & (bins - 1)][lane % COPIES], 1);
+        }
       }
     }
     __syncthreads();
     // thread t owns bins t * per .. of the descending order
+    constexpr int kPer = kBins / kSelThreads;
     const int per = bins / kSelThreads;
-    int mine[2] = {0, 0};
-    for (int j = 0; j < per; ++j) {
-      const int* h = hist[bins - 1 - (tid * per + j)];
-      const u32x4 lo = *reinterpret_cast<const u32x4*>(h), hi = *reinterpret_cast<const u32x4*>(h + 4);
+    int mine[kPer] = {}, sum = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mine[j] += static_cast<int>(lo[k] + hi[k]);
+    for (int j = 0; j < kPer; ++j) {
+      if (j < per) {
+        const int* h = hist[bins - 1 - (tid * per + j)];
+#pragma unroll
+        for (int k = 0; k < COPIES; ++k) mine[j] += h[k];
+      }
+      sum += mine[j];
     }
-    const int x = wave_inclusive_scan(mine[0] + mine[1], lane);
+    const int x = wave_inclusive_scan(sum, lane);
     if (lane == kWave - 1) part[wv] = x;
     __syncthreads();
-    int before = x - (mine[0] + mine[1]);
-    for (int k = 0; k < wv; ++k) before += part[k];
-    for (int j = 0; j < per; ++j) {
-      if (before < need && before + mine[j] >= need) {
+    int all;
+    int before = before_wave<kSelWaves>(part, wv, lane, all) + x - sum;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      if (j < per && before < need && before + mine[j] >= need) {
         found[0] = bins - 1 - (tid * per + j);
         found[1] = before;
+        found[2] = mine[j];
       }
       before += mine[j];
     }
@@ -126,55 +151,79 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     prefix |= static_cast<uint32_t>(found[0]) << shift;
     mask |= static_cast<uint32_t>(bins - 1) << shift;
     need -= found[1];
+    if (E > 8 && pass == 0 && found[2] <= kList) {
+      short_list = true;
+      for (int c = 0; c < rounds; ++c) {
+        if (rounds > 1) load(c);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (first_of(c) + e * kWave < count && (key[e] & mask) == prefix)
+            list[atomicAdd(&listed, 1)] = key[e];
+      }
+    }
   }
 
-  // `prefix` is the n-th largest key; `need` of those equal to it stay.  Each
-  // wavefront counts its run of the candidates and writes behind the runs before it.
-  int at = 0, same = 0;  // kept above the key, and equal to it, before the run
+  // `prefix` is the n-th largest key; `need` of those equal to it stay, mostly all of
+  // them.  Each wavefront counts what its run of the candidates keeps, and writes behind
+  // the runs before it.
+  const bool all_equal = prefix != 0 && need == found[2];
+  int at = 0, same = 0;  // kept, and (where not all stay) equal to the key, before the run
   for (int c = 0; c < rounds; ++c) {
     if (rounds > 1) load(c);
-    int above = 0, equal = 0;
+    const int first = first_of(c);
+    int kept = 0, equal = 0;
+    if (all_equal) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      above += __popcll(__builtin_amdgcn_ballot_w64(inside(c, e) && key[e] > prefix));
-      equal += __popcll(__builtin_amdgcn_ballot_w64(inside(c, e) && key[e] == prefix));
+      for (int e = 0; e < E; ++e) kept += __popcll(__builtin_amdgcn_ballot_w64(key[e] >= prefix));
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        kept += __popcll(__builtin_amdgcn_ballot_w64(key[e] > prefix));
+        equal += __popcll(
+            __builtin_amdgcn_ballot_w64(key[e] == prefix && first + e * kWave < count));
+      }
     }
     // (keeps the compiler from holding two lane masks per element until below)
 #pragma unroll
     for (int e = 0; e < E; ++e) asm volatile("" : "+v"(key[e]));
     __syncthreads();  // the totals of the round before are read
     if (lane == 0) {
-      above_tot[wv] = above;
+      kept_tot[wv] = kept;
       equal_tot[wv] = equal;
     }
     __syncthreads();
-    int up_all = 0, eq_all = 0;
-    for (int k = 0; k < kSelWaves; ++k) {
-      if (k == wv) {
-        above = up_all;
-        equal = eq_all;
-      }
-      up_all += above_tot[k];
-      eq_all += equal_tot[k];
-    }
-    int up_at = at + above, eq_at = same + equal;
+    int kept_all, equal_all;
+    int run_at = at + before_wave<kSelWaves>(kept_tot, wv, lane, kept_all);
+    int run_same = same + before_wave<kSelWaves>(equal_tot, wv, lane, equal_all);
+    at += kept_all;
+    same += equal_all;
+    if (all_equal) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const bool in = inside(c, e);
-      const uint64_t up = __builtin_amdgcn_ballot_w64(in && key[e] > prefix);
-      const uint64_t eq = __builtin_amdgcn_ballot_w64(in && key[e] == prefix);
-      const uint64_t low = (1ull << lane) - 1;
-      const int eq_before = eq_at + __popcll(eq & low);
-      if (in && (key[e] > prefix || (key[e] == prefix && eq_before < need))) {
-        const int eq_kept = eq_before < need ? eq_before : need;
-        out[sink + up_at + __popcll(up & low) + eq_kept] =
-            sink + ((c * kSelWaves + wv) * E + e) * kWave + lane;
+      for (int e = 0; e < E; ++e) {
+        const uint64_t up = __builtin_amdgcn_ballot_w64(key[e] >= prefix);
+        if (key[e] >= prefix)
+          out[sink + run_at + __builtin_amdgcn_mbcnt_hi(
+                                  static_cast<uint32_t>(up >> 32),
+                                  __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(up), 0))] =
+              sink + first + e * kWave;
+        run_at += __popcll(up);
       }
-      up_at += __popcll(up);
-      eq_at += __popcll(eq);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const bool same_key = key[e] == prefix && first + e * kWave < count;
+        const uint64_t up = __builtin_amdgcn_ballot_w64(key[e] > prefix);
+        const uint64_t eq = __builtin_amdgcn_ballot_w64(same_key);
+        const uint64_t low = (1ull << lane) - 1;
+        const int eq_before = run_same + __popcll(eq & low);
+        if (key[e] > prefix || (same_key && eq_before < need)) {
+          const int eq_kept = eq_before < need ? eq_before : need;
+          out[sink + run_at + __popcll(up & low) + eq_kept] = sink + first + e * kWave;
+        }
+        run_at += __popcll(up);
+        run_same += __popcll(eq);
+      }
     }
-    at += up_all;
-    same += eq_all;
   }
 }
 
@@ -183,18 +232,24 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
 // Row start + i of a (sequence, kv head) takes row keep[i], K and V (and the score),
 // ascending keep, keep[i] >= start + i where the pages are the same ones.
 //
-// One workgroup moves some dims of a head's rows: 32 dims (64 bytes) of K, or 16 dims
-// of V, whose 32-token blocks are transposed.  It reads a step's rows into registers,
-// waits until all of it is read, and writes: a later step's sources lie behind every
-// row written so far, so the move may be in place.  The next step's places are looked
-// up while its rows come.
+// One workgroup moves some dims of a head's rows: of K, or of V, whose 32-token blocks
+// are transposed.  It reads a step of 512 rows into registers, waits until all of it is
+// read, and writes: a later step's sources lie behind every row written so far, so the
+// move may be in place, and the next step's rows, and the places of the one after it,
+// are asked for before a step is written.  (Two steps ahead, and places looked up by a
+// wavefront of their own, leave one workgroup per CU for four: 95 against 63 us for
+// 16 x 8 heads, half of 4,096 tokens.)
 //
 // What bounds it: the kept rows read and written once; a V block is read in lines of
-// 32 tokens of a dim, whichever of them stay.
+// 32 tokens of a dim, whichever of them stay.  64 dims of K and 16 of V per workgroup,
+// since smaller pieces read lines of K more than once (the same: 63 against 75 us with
+// 32 dims of K); half of both where fewer than 64 segments leave CUs idle (8 heads,
+// 8,192 of 32,768 tokens: 41 against 69 us).
 
 constexpr int kMoveThreads = 512;
 constexpr int kStep = 512;  // rows of a step
-constexpr int kKDims = 32, kVDims = 16;
+static_assert(kStep == kMoveThreads, "a thread looks one row up");
+
 constexpr uint32_t kNoRow = 0xffffffffu;
 
 struct CompactArgs {
@@ -210,16 +265,42 @@ struct CompactArgs {
   int NKV, D, keep_heads, n, cap, max_pages, dst_pages, pt_shift, num_slots;
 };
 
+// Page of a position within a table of so many (clamped: what lies outside is not used).
+__device__ __forceinline__ int page_of(long long pos, int pages, const CompactArgs& a) {
+  const long long page = pos >> a.pt_shift;
+  return page < 0 ? 0 : (page < pages ? static_cast<int>(page) : pages - 1);
+}
+
 // Row of the pool (slot, kv head, token) of a position, in units of D elements.
-__device__ __forceinline__ uint32_t row_of(const int32_t* table, int pages, int pos, int kvh,
+__device__ __forceinline__ uint32_t row_of(int slot, long long pos, int pages, int kvh,
                                            const CompactArgs& a) {
-  if (pos < 0) return kNoRow;
-  const int page = pos >> a.pt_shift;
-  if (page >= pages) return kNoRow;
-  const int slot = table[page];
-  if (static_cast<unsigned>(slot) >= static_cast<unsigned>(a.num_slots)) return kNoRow;
-  return ((static_cast<uint32_t>(slot) * a.NKV + kvh) << a.pt_shift) +
-         (pos & ((1 << a.pt_shift) - 1));
+  const bool ok = pos >= 0 && pos >> a.pt_shift < pages &&
+                  static_cast<unsigned>(slot) < static_cast<unsigned>(a.num_slots);
+  const uint32_t row = ((static_cast<uint32_t>(slot) * a.NKV + kvh) << a.pt_shift) +
+                       (static_cast<uint32_t>(pos) & ((1u << a.pt_shift) - 1));
+  return ok ? row : kNoRow;
+}
+
+// Where row i of the list is read and written; kNoRow: nothing to move.
+__device__ __forceinline__ void look_up(const CompactArgs& a, const int32_t* keep, int n, int start,
+                                        int b, int kvh, int i, uint32_t& src, uint32_t& dst) {
+  const int32_t* trow = a.table + static_cast<size_t>(b) * a.max_pages;
+  const int32_t* drow = a.dst_table + static_cast<size_t>(b) * a.dst_pages;
+  const long long to = start + static_cast<long long>(i);
+  const int d_slot = drow[page_of(to, a.dst_pages, a)];
+  const int from = keep[i < n ? i : n - 1];
+  const int s_slot = trow[page_of(from, a.max_pages, a)];
+  const uint32_t s = row_of(s_slot, from, a.max_pages, kvh, a);
+  const uint32_t d = row_of(d_slot, to, a.dst_pages, kvh, a);
+  src = i >= n || d == kNoRow || d == s ? kNoRow : s;
+  dst = d;
+}
+
+// The values are loaded here, not later.
+template <typename T, int N>
+__device__ __forceinline__ void pin(T (&v)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) asm volatile("" : "+v"(v[j]));
 }
 
 // Every load of this wavefront has landed, and nothing moves across.
@@ -228,23 +309,13 @@ __device__ __forceinline__ void all_read() {
   __syncthreads();
 }
 
-// Where position `from` is read and position `to` written; kNoRow: nothing to move.
-__device__ __forceinline__ void places(const CompactArgs& a, const int32_t* trow,
-                                       const int32_t* drow, int from, long long to, int kvh,
-                                       uint32_t& src, uint32_t& dst) {
-  const uint32_t s = row_of(trow, a.max_pages, from, kvh, a);
-  const uint32_t d =
-      to < (1LL << 30) ? row_of(drow, a.dst_pages, static_cast<int>(to), kvh, a) : kNoRow;
-  src = d == kNoRow || d == s ? kNoRow : s;
-  dst = d;
-}
-
 // Element of V(row, d) = block row / VB of [D, VB], VB = 1 << vb = min(page, 32).
 __device__ __forceinline__ size_t v_element(uint32_t row, int d, int vb, int D) {
   return ((static_cast<size_t>(row >> vb) * D + d) << vb) + (row & ((1u << vb) - 1));
 }
 
 // One workgroup: the scores of one (sequence, kv head), and zeros behind them.
+template <int THREADS>
 __device__ __forceinline__ void move_scores(const CompactArgs& a, const int32_t* keep, int b,
                                             int kvh, int n, int start) {
   const int tid = static_cast<int>(threadIdx.x);
@@ -253,14 +324,14 @@ __device__ __forceinline__ void move_scores(const CompactArgs& a, const int32_t*
   float* o = a.scores_out + row;
   const int first = start < a.cap ? start : a.cap;
   if (s != o)
-    for (int i = tid; i < first; i += kMoveThreads) o[i] = s[i];
+    for (int i = tid; i < first; i += THREADS) o[i] = s[i];
   constexpr int kLoads = 8;
-  for (int i0 = 0; i0 < n; i0 += kLoads * kMoveThreads) {
+  for (int i0 = 0; i0 < n; i0 += kLoads * THREADS) {
     int from[kLoads];
     float v[kLoads];
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-      const int i = i0 + j * kMoveThreads + tid;
+      const int i = i0 + j * THREADS + tid;
       from[j] = i < n ? keep[i] : -1;
     }
 #pragma unroll
@@ -270,23 +341,22 @@ __device__ __forceinline__ void move_scores(const CompactArgs& a, const int32_t*
     all_read();
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
-      const int i = i0 + j * kMoveThreads + tid;
+      const int i = i0 + j * THREADS + tid;
       if (i < n && start + static_cast<long long>(i) < a.cap) o[start + i] = v[j];
     }
   }
-  for (long long i = static_cast<long long>(first) + n + tid; i < a.cap; i += kMoveThreads)
+  for (long long i = static_cast<long long>(first) + n + tid; i < a.cap; i += THREADS)
     o[i] = 0.f;
 }
 
+template <int kKDims, int kVDims>
 __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactArgs a) {
-  static_assert(kStep == kMoveThreads, "a thread looks one row up");
-  // Places of three steps: while the next step's are looked up, a wavefront may still
-  // store the rows of the step before.
-  __shared__ uint32_t src[3][kStep], dst[3][kStep];
+  // Places of four steps: being written, being read, and looked up.
+  __shared__ uint32_t src[4][kStep], dst[4][kStep];
   const int tid = static_cast<int>(threadIdx.x);
   const int kvh = static_cast<int>(blockIdx.y);
   const int b = static_cast<int>(blockIdx.z);
-  const int k_parts = a.D / kKDims, v_parts = a.D / kVDims;
+  const int k_parts = (a.D + kKDims - 1) / kKDims, v_parts = a.D / kVDims;
   const int part = static_cast<int>(blockIdx.x);
   const int32_t* keep = a.keep + (static_cast<size_t>(b) * a.keep_heads +
                                   (a.keep_heads == 1 ? 0 : kvh)) * a.n;
@@ -294,72 +364,76 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactArgs a) {
   n = n < 0 ? 0 : (n > a.n ? a.n : n);
   int start = a.start != nullptr ? uniform(a.start[b]) : 0;
   start = start < 0 ? 0 : start;
-
   if (part == k_parts + v_parts) {
-    move_scores(a, keep, b, kvh, n, start);
+    move_scores<kMoveThreads>(a, keep, b, kvh, n, start);
     return;
   }
+  if (n == 0) return;
+  const int steps = (n + kStep - 1) / kStep;
 
-  const int32_t* trow = a.table + static_cast<size_t>(b) * a.max_pages;
-  const int32_t* drow = a.dst_table + static_cast<size_t>(b) * a.dst_pages;
-  auto look_up = [&](int i0, int buf) {
-    const int i = i0 + tid;
-    if (i >= n) return;
-    places(a, trow, drow, keep[i], start + static_cast<long long>(i), kvh, src[buf][tid],
-           dst[buf][tid]);
+  constexpr int kKPass = kMoveThreads / (kKDims / 8), kVPass = kMoveThreads / kVDims;
+  constexpr int kKLoads = kStep / kKPass, kVLoads = kStep / kVPass;
+  const int kr = tid / (kKDims / 8);
+  const int kc = part * kKDims + 8 * (tid % (kKDims / 8));
+  const int vb = a.pt_shift < 5 ? a.pt_shift : 5;
+  const int vd = (part - k_parts) * kVDims + tid / kVPass;
+  auto step_places = [&](int s) {
+    look_up(a, keep, n, start, b, kvh, s * kStep + tid, src[s & 3][tid], dst[s & 3][tid]);
   };
-  look_up(0, 0);
-  __syncthreads();
-  int buf = 0, next = 1;
-  for (int i0 = 0; i0 < n; i0 += kStep) {
-    const int m = n - i0 < kStep ? n - i0 : kStep;
-    if (part < k_parts) {
-      constexpr int kChunks = kKDims / 8;
-      constexpr int kPass = kMoveThreads / kChunks;
-      constexpr int kLoads = kStep / kPass;
-      const int c = part * kKDims + 8 * (tid % kChunks);
-      const int r = tid / kChunks;
-      u32x4 v[kLoads];
+  auto read_k = [&](int s, u32x4 (&v)[kKLoads]) {
 #pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const uint32_t from = r + j * kPass < m ? src[buf][r + j * kPass] : kNoRow;
-        if (from != kNoRow)
-          v[j] = *reinterpret_cast<const u32x4*>(a.k_pool + static_cast<size_t>(from) * a.D + c);
-      }
-      look_up(i0 + kStep, next);
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) asm volatile("" : "+v"(v[j]));
-      all_read();
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const int i = r + j * kPass;
-        if (i < m && src[buf][i] != kNoRow)
-          *reinterpret_cast<u32x4*>(a.k_pool + static_cast<size_t>(dst[buf][i]) * a.D + c) = v[j];
-      }
-    } else {
-      constexpr int kLoads = kStep / 32;
-      const int vb = a.pt_shift < 5 ? a.pt_shift : 5;
-      const int d = (part - k_parts) * kVDims + tid / 32;
-      uint32_t v[kLoads];
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const int i = (tid & 31) + 32 * j;
-        const uint32_t from = i < m ? src[buf][i] : kNoRow;
-        if (from != kNoRow) v[j] = a.v_pool[v_element(from, d, vb, a.D)];
-      }
-      look_up(i0 + kStep, next);
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) asm volatile("" : "+v"(v[j]));
-      all_read();
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) {
-        const int i = (tid & 31) + 32 * j;
-        if (i < m && src[buf][i] != kNoRow)
-          a.v_pool[v_element(dst[buf][i], d, vb, a.D)] = static_cast<uint16_t>(v[j]);
-      }
+    for (int j = 0; j < kKLoads; ++j) {
+      const uint32_t from = src[s & 3][kr + j * kKPass];
+      if (from != kNoRow && kc < a.D)
+        v[j] = *reinterpret_cast<const u32x4*>(a.k_pool + static_cast<size_t>(from) * a.D + kc);
     }
-    buf = next;
-    next = next == 2 ? 0 : next + 1;
+  };
+  auto write_k = [&](int s, const u32x4 (&v)[kKLoads]) {
+#pragma unroll
+    for (int j = 0; j < kKLoads; ++j) {
+      const int at = kr + j * kKPass;
+      if (src[s & 3][at] != kNoRow && kc < a.D)
+        *reinterpret_cast<u32x4*>(a.k_pool + static_cast<size_t>(dst[s & 3][at]) * a.D + kc) = v[j];
+    }
+  };
+  auto read_v = [&](int s, uint32_t (&v)[kVLoads]) {
+#pragma unroll
+    for (int j = 0; j < kVLoads; ++j) {
+      const uint32_t from = src[s & 3][tid % kVPass + j * kVPass];
+      if (from != kNoRow) v[j] = a.v_pool[v_element(from, vd, vb, a.D)];
+    }
+  };
+  auto write_v = [&](int s, const uint32_t (&v)[kVLoads]) {
+#pragma unroll
+    for (int j = 0; j < kVLoads; ++j) {
+      const int at = tid % kVPass + j * kVPass;
+      if (src[s & 3][at] != kNoRow)
+        a.v_pool[v_element(dst[s & 3][at], vd, vb, a.D)] = static_cast<uint16_t>(v[j]);
+    }
+  };
+  auto run = [&](auto& even, auto& odd, auto read, auto write) {
+    step_places(0);
+    step_places(1);
+    __syncthreads();
+    read(0, even);
+    int s = 0;
+    auto step = [&](auto& cur, auto& next) {
+      pin(cur);
+      all_read();  // every wavefront has read step s, and step s + 1 is looked up
+      read(s + 1, next);
+      step_places(s + 2);
+      write(s, cur);
+      return ++s < steps;
+    };
+    while (step(even, odd) && step(odd, even)) {
+    }
+  };
+  if (part < k_parts) {
+    u32x4 even[kKLoads], odd[kKLoads];
+    run(even, odd, read_k, write_k);
+  } else {
+    uint32_t even[kVLoads], odd[kVLoads];
+    run(even, odd, read_v, write_v);
   }
 }
 
@@ -380,13 +454,11 @@ __global__ __launch_bounds__(kMoveThreads) void compact_few_kernel(CompactArgs a
   int start = a.start != nullptr ? uniform(a.start[b]) : 0;
   start = start < 0 ? 0 : start;
   if (blockIdx.x == 1) {
-    move_scores(a, keep, b, kvh, n, start);
+    move_scores<kMoveThreads>(a, keep, b, kvh, n, start);
     return;
   }
-  if (tid < n)
-    places(a, a.table + static_cast<size_t>(b) * a.max_pages,
-           a.dst_table + static_cast<size_t>(b) * a.dst_pages, keep[tid],
-           start + static_cast<long long>(tid), kvh, src[tid], dst[tid]);
+  if (n == 0) return;
+  if (tid < n) look_up(a, keep, n, start, b, kvh, tid, src[tid], dst[tid]);
   __syncthreads();
   const int vb = a.pt_shift < 5 ? a.pt_shift : 5;
   for (int d0 = 0; d0 < a.D; d0 += kFewDims) {
@@ -450,16 +522,15 @@ extern "C" int voom_evict_select(const float* scores, const int32_t* ctx_lens, i
                num_kv_heads, score_tokens);
   VOOM_REQUIRE(budget > 0 && sink >= 0 && recent >= 0 && sink <= budget && recent <= budget - sink,
                "%s: sink %d and recent %d must fit the budget %d", who, sink, recent, budget);
-  const dim3 grid(static_cast<unsigned>(batch * num_kv_heads)), block(kSelThreads);
-  if (score_tokens <= 8 * kSelThreads)
-    hipLaunchKernelGGL(evict_select_kernel<8>, grid, block, 0, stream, scores, ctx_lens, keep,
-                       keep_lens, num_kv_heads, score_tokens, budget, sink, recent);
-  else if (score_tokens <= 32 * kSelThreads)
-    hipLaunchKernelGGL(evict_select_kernel<32>, grid, block, 0, stream, scores, ctx_lens, keep,
-                       keep_lens, num_kv_heads, score_tokens, budget, sink, recent);
-  else
-    hipLaunchKernelGGL(evict_select_kernel<64>, grid, block, 0, stream, scores, ctx_lens, keep,
-                       keep_lens, num_kv_heads, score_tokens, budget, sink, recent);
+  const auto launch = [&](auto kernel, int threads) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(batch * num_kv_heads)), dim3(threads), 0,
+                       stream, scores, ctx_lens, keep, keep_lens, num_kv_heads, score_tokens,
+                       budget, sink, recent);
+  };
+  if (score_tokens <= 8 * 256) launch(evict_select_kernel<256, 8, 1>, 256);
+  else if (score_tokens <= 8 * 1024) launch(evict_select_kernel<1024, 8, 2>, 1024);
+  else if (score_tokens <= 32 * 1024) launch(evict_select_kernel<1024, 32, 8>, 1024);
+  else launch(evict_select_kernel<1024, 48, 8>, 1024);
   return VOOM_LAUNCH_CHECK("evict_select: launch");
 }
 
@@ -516,8 +587,13 @@ extern "C" int voom_compact_kv(void* k_pool, void* v_pool, const int32_t* block_
   if (keep_tokens <= kFewRows) {
     hipLaunchKernelGGL(compact_few_kernel, grid, dim3(kMoveThreads), 0, stream, a);
   } else {
-    grid.x = head_dim / kKDims + head_dim / kVDims + moves_scores;
-    hipLaunchKernelGGL(compact_kernel, grid, dim3(kMoveThreads), 0, stream, a);
+    const long long segs = static_cast<long long>(batch) * num_kv_heads;
+    const auto launch = [&](auto kernel, int k_dims, int v_dims) {
+      grid.x = (head_dim + k_dims - 1) / k_dims + head_dim / v_dims + moves_scores;
+      hipLaunchKernelGGL(kernel, grid, dim3(kMoveThreads), 0, stream, a);
+    };
+    if (segs >= 64) launch(compact_kernel<64, 16>, 64, 16);
+    else launch(compact_kernel<32, 8>, 32, 8);
   }
   return VOOM_LAUNCH_CHECK("compact_kv: launch");
 }
