@@ -317,15 +317,51 @@ def paged_gqa_prefill(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
     return out
 
 
-def _require_current(dev: torch.device) -> None:
-    """The launch goes to the current device's stream: tensors must live there."""
-    cur = _CUR_DEVICE() if _CUR_DEVICE is not None else torch.cuda.current_device()
-    _require(dev.index == cur, f"tensors are on {dev}, but cuda:{cur} is the current device")
+def _require_here(*tensors: torch.Tensor | None) -> None:
+    """Contiguous tensors on the current device, to whose stream the launch goes."""
+    here = _CUR_DEVICE() if _CUR_DEVICE is not None else torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (t.get_device() != here or not t.is_contiguous()):
+            dev = _require_device(*tensors)
+            raise ValueError(f"tensors are on {dev}, but cuda:{here} is the current device")
 
 
-def _check_lens(t: torch.Tensor | None, batch: int, name: str) -> None:
-    _require(t is None or (t.dtype == torch.int32 and tuple(t.shape) == (batch,)),
-             f"{name} must be int32 [{batch}]")
+def _is_i32(t: torch.Tensor, *shape: int) -> bool:
+    return t.dtype is torch.int32 and t.shape == shape
+
+
+def _is_scores(t: torch.Tensor, batch: int, num_kv_heads: int) -> bool:
+    return (t.dtype is torch.float32 and t.dim() == 3 and t.shape[2] > 0
+            and t.shape[0] == batch and t.shape[1] == num_kv_heads)
+
+
+def _new_tokens_geometry(q, k_pool, v_pool, block_table, ctx_lens):
+    """Checks what the calls over a window of new tokens share; their sizes (v_pool None:
+    keys alone).  (The messages are put together only where a check fails: calls of a
+    decode step count microseconds.)"""
+    if q.dim() != 4:
+        raise ValueError("q must be [B, NQ, T, D]")
+    if k_pool.dim() != 4:
+        raise ValueError("k_pool must be [slots, NKV, PT, D]")
+    B, NQ, T, D = q.shape
+    slots, NKV, PT, Dk = k_pool.shape
+    if Dk != D:
+        raise ValueError(f"k_pool head_dim {Dk} != q head_dim {D}")
+    if v_pool is not None:
+        if v_pool.shape != (slots,) + v_slot_shape(NKV, D, PT):
+            _check_v_pool(v_pool, slots, NKV, D, PT)
+        if v_pool.dtype is not torch.bfloat16:
+            raise ValueError("q and pools must be bfloat16")
+    if q.dtype is not torch.bfloat16 or k_pool.dtype is not torch.bfloat16:
+        raise ValueError("q and pools must be bfloat16")
+    if (block_table.dtype is not torch.int32 or block_table.dim() != 2
+            or block_table.shape[0] != B):
+        raise ValueError(f"block_table must be int32 [{B}, max_pages]")
+    if not _is_i32(ctx_lens, B):
+        raise ValueError(f"ctx_lens must be int32 [{B}]")
+    if NKV == 0 or NQ % NKV:
+        raise ValueError("num_q_heads must be a multiple of num_kv_heads")
+    return B, NQ, T, D, slots, NKV, PT, block_table.shape[1]
 
 
 def paged_gqa_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -344,47 +380,34 @@ def paged_gqa_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     Returns out [B, T, NQ, D] (and the fp32 natural-log LSE [B, T, NQ] when
     ``return_lse``); rows that see nothing, and rows past draft_lens, hold 0 and -inf.
     """
-    _require(q.dim() == 4, "q must be [B, NQ, T, D]")
-    dev = _require_device(q, k_pool, v_pool, block_table, ctx_lens, mask, draft_lens)
-    _require_current(dev)
-    B, NQ, T, D = q.shape
-    _require(k_pool.dim() == 4, "k_pool must be [slots, NKV, PT, D]")
-    slots, NKV, PT, Dk = k_pool.shape
-    _require(Dk == D, f"k_pool head_dim {Dk} != q head_dim {D}")
-    _check_v_pool(v_pool, slots, NKV, D, PT)
-    _require(q.dtype == k_pool.dtype == v_pool.dtype == torch.bfloat16,
-             "q and pools must be bfloat16")
-    _require(block_table.dtype == torch.int32 and block_table.dim() == 2
-             and block_table.shape[0] == B, "block_table must be int32 [B, max_pages]")
-    _require(ctx_lens.dtype == torch.int32 and tuple(ctx_lens.shape) == (B,),
-             "ctx_lens must be int32 [B]")
-    _check_lens(draft_lens, B, "draft_lens")
-    _require(NQ % NKV == 0, "num_q_heads must be a multiple of num_kv_heads")
-    _require(mask is None or (mask.dtype == torch.bool
-                              and tuple(mask.shape) in ((T, T), (B, T, T))),
-             f"mask must be bool [{T}, {T}] or [{B}, {T}, {T}]")
-    out = torch.empty((B, T, NQ, D), dtype=torch.bfloat16, device=dev)
-    lse = torch.empty((B, T, NQ), dtype=torch.float32, device=dev) if return_lse else None
-    if out.numel():
+    _require_here(q, k_pool, v_pool, block_table, ctx_lens, mask, draft_lens)
+    B, NQ, T, D, slots, NKV, PT, pages = _new_tokens_geometry(q, k_pool, v_pool, block_table,
+                                                              ctx_lens)
+    if draft_lens is not None and not _is_i32(draft_lens, B):
+        raise ValueError(f"draft_lens must be int32 [{B}]")
+    masks = 1
+    if mask is not None:
+        if mask.dtype is not torch.bool or mask.shape not in ((T, T), (B, T, T)):
+            raise ValueError(f"mask must be bool [{T}, {T}] or [{B}, {T}, {T}]")
+        masks = B if mask.dim() == 3 else 1
+    out = q.new_empty((B, T, NQ, D))
+    lse = q.new_empty((B, T, NQ), dtype=torch.float32) if return_lse else None
+    if B and T and NQ:
         if _BOUNDS_CHECKS:
             check_block_table(block_table, ctx_lens, slots, PT)
+        lib = _lib.lib()
         # allocated per call, so that calls on several streams or threads and captured
         # graphs never share it
-        need = int(_lib.lib().voom_paged_gqa_tree_workspace_bytes(B, NQ, NKV, D, T, PT,
-                                                                  block_table.shape[1]))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _lib.call("voom_paged_gqa_tree", _ptr(q), _ptr(k_pool), _ptr(v_pool), _ptr(block_table),
-                  _ptr(ctx_lens), _ptr(draft_lens), _ptr(mask),
-                  mask.shape[0] if mask is not None and mask.dim() == 3 else 1, _ptr(out),
-                  _ptr(lse), _ptr(ws), need, B, NQ, NKV, D, PT, block_table.shape[1], slots, T,
-                  float(D ** -0.5 if scale is None else scale), _stream(None))
+        need = lib.voom_paged_gqa_tree_workspace_bytes(B, NQ, NKV, D, T, PT, pages)
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        rc = lib.voom_paged_gqa_tree(
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
+            ctx_lens.data_ptr(), _ptr(draft_lens), _ptr(mask), masks, out.data_ptr(), _ptr(lse),
+            _ptr(ws), need, B, NQ, NKV, D, PT, pages, slots, T,
+            D ** -0.5 if scale is None else float(scale), _stream(None))
+        if rc:
+            _lib.check(rc, "voom_paged_gqa_tree")
     return (out, lse) if return_lse else out
-
-
-def _check_scores(t: torch.Tensor | None, batch: int, num_kv_heads: int, name: str) -> None:
-    _require(t is None or (t.dtype == torch.float32 and t.dim() == 3 and t.shape[2] > 0
-                           and tuple(t.shape[:2]) == (batch, num_kv_heads)),
-             f"{name} must be float32 [{batch}, {num_kv_heads}, tokens]")
 
 
 def paged_gqa_observe(q: torch.Tensor, lse: torch.Tensor, k_pool: torch.Tensor,
@@ -404,35 +427,32 @@ def paged_gqa_observe(q: torch.Tensor, lse: torch.Tensor, k_pool: torch.Tensor,
     """
     if q.dim() == 4 and lse.dim() == 2 and q.shape[2] == 1:
         lse = lse[:, None]
-    _require(q.dim() == 4, "q must be [B, NQ, L, D]")
-    dev = _require_device(q, lse, k_pool, block_table, ctx_lens, scores, window_lens, out)
-    _require_current(dev)
-    B, NQ, L, D = q.shape
-    _require(k_pool.dim() == 4, "k_pool must be [slots, NKV, PT, D]")
-    slots, NKV, PT, Dk = k_pool.shape
-    _require(Dk == D, f"k_pool head_dim {Dk} != q head_dim {D}")
-    _require(q.dtype == k_pool.dtype == torch.bfloat16, "q and the pool must be bfloat16")
-    _require(lse.dtype == torch.float32 and tuple(lse.shape) == (B, L, NQ),
-             f"lse must be float32 [{B}, {L}, {NQ}]")
-    _require(block_table.dtype == torch.int32 and block_table.dim() == 2
-             and block_table.shape[0] == B, "block_table must be int32 [B, max_pages]")
-    _require(ctx_lens.dtype == torch.int32 and tuple(ctx_lens.shape) == (B,),
-             "ctx_lens must be int32 [B]")
-    _check_lens(window_lens, B, "window_lens")
-    _require(NQ % NKV == 0, "num_q_heads must be a multiple of num_kv_heads")
-    _check_scores(scores, B, NKV, "scores")
-    out = scores if out is None else out
-    _require(out.dtype == torch.float32 and out.shape == scores.shape, "out must be like scores")
+    _require_here(q, lse, k_pool, block_table, ctx_lens, scores, window_lens, out)
+    B, NQ, L, D, slots, NKV, PT, pages = _new_tokens_geometry(q, k_pool, None, block_table,
+                                                              ctx_lens)
+    if lse.dtype is not torch.float32 or lse.shape != (B, L, NQ):
+        raise ValueError(f"lse must be float32 [{B}, {L}, {NQ}]")
+    if window_lens is not None and not _is_i32(window_lens, B):
+        raise ValueError(f"window_lens must be int32 [{B}]")
+    if not _is_scores(scores, B, NKV):
+        raise ValueError(f"scores must be float32 [{B}, {NKV}, tokens]")
+    if out is None:
+        out = scores
+    elif out.dtype is not torch.float32 or out.shape != scores.shape:
+        raise ValueError("out must be like scores")
     if B == 0:
         return out
     if _BOUNDS_CHECKS:
         check_block_table(block_table, ctx_lens, slots, PT)
     if L == 0:  # nothing to add
         q, lse, L = q.new_zeros((B, NQ, 1, D)), lse.new_full((B, 1, NQ), -float("inf")), 1
-    _lib.call("voom_paged_gqa_observe", _ptr(q), _ptr(lse), _ptr(k_pool), _ptr(block_table),
-              _ptr(ctx_lens), _ptr(window_lens), _ptr(scores), _ptr(out), B, NQ, NKV, D, PT,
-              block_table.shape[1], slots, L, scores.shape[2],
-              float(D ** -0.5 if scale is None else scale), _stream(None))
+    rc = _lib.lib().voom_paged_gqa_observe(
+        q.data_ptr(), lse.data_ptr(), k_pool.data_ptr(), block_table.data_ptr(),
+        ctx_lens.data_ptr(), _ptr(window_lens), scores.data_ptr(), out.data_ptr(), B, NQ, NKV, D,
+        PT, pages, slots, L, scores.shape[2], D ** -0.5 if scale is None else float(scale),
+        _stream(None))
+    if rc:
+        _lib.check(rc, "voom_paged_gqa_observe")
     return out
 
 
@@ -446,21 +466,24 @@ def evict_select(scores: torch.Tensor, ctx_lens: torch.Tensor, budget: int, *, s
     and of those between the ones of largest score, equal scores lowest position first
     (a NaN counts below every number).
     """
-    dev = _require_device(scores, ctx_lens)
-    _require_current(dev)
-    _require(scores.dim() == 3, "scores must be [B, NKV, tokens]")
-    B, NKV, cap = scores.shape
-    _check_scores(scores, B, NKV, "scores")
-    _require(ctx_lens.dtype == torch.int32 and tuple(ctx_lens.shape) == (B,),
-             "ctx_lens must be int32 [B]")
+    _require_here(scores, ctx_lens)
+    B = scores.shape[0] if scores.dim() == 3 else 0
+    if scores.dim() != 3 or not _is_scores(scores, B, scores.shape[1]):
+        raise ValueError("scores must be float32 [B, NKV, tokens]")
+    NKV, cap = scores.shape[1:]
+    if not _is_i32(ctx_lens, B):
+        raise ValueError(f"ctx_lens must be int32 [{B}]")
     budget, sink, recent = int(budget), int(sink), int(recent)
-    _require(budget > 0 and sink >= 0 and recent >= 0 and sink + recent <= budget,
-             f"sink {sink} and recent {recent} must fit the budget {budget}")
-    keep = torch.empty((B, NKV, budget), dtype=torch.int32, device=dev)
-    keep_lens = torch.empty((B,), dtype=torch.int32, device=dev)
+    if budget <= 0 or sink < 0 or recent < 0 or sink + recent > budget:
+        raise ValueError(f"sink {sink} and recent {recent} must fit the budget {budget}")
+    keep = ctx_lens.new_empty((B, NKV, budget))
+    keep_lens = ctx_lens.new_empty((B,))
     if B and NKV:
-        _lib.call("voom_evict_select", _ptr(scores), _ptr(ctx_lens), _ptr(keep), _ptr(keep_lens),
-                  B, NKV, cap, budget, sink, recent, _stream(None))
+        rc = _lib.lib().voom_evict_select(
+            scores.data_ptr(), ctx_lens.data_ptr(), keep.data_ptr(), keep_lens.data_ptr(), B, NKV,
+            cap, budget, sink, recent, _stream(None))
+        if rc:
+            _lib.check(rc, "voom_evict_select")
     return keep, keep_lens
 
 
@@ -501,42 +524,54 @@ def compact_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Te
     ``scores`` [B, NKV, tokens] fp32 moves along into ``scores_out`` (default: in place);
     behind the last row kept it becomes 0.
     """
-    dev = _require_device(k_pool, v_pool, block_table, keep, keep_lens, start, dst_table, scores,
-                          scores_out)
-    _require_current(dev)
-    _require(k_pool.dim() == 4, "k_pool must be [slots, NKV, PT, D]")
+    _require_here(k_pool, v_pool, block_table, keep, keep_lens, start, dst_table, scores,
+                  scores_out)
+    if k_pool.dim() != 4:
+        raise ValueError("k_pool must be [slots, NKV, PT, D]")
     slots, NKV, PT, D = k_pool.shape
-    _check_v_pool(v_pool, slots, NKV, D, PT)
-    _require(k_pool.dtype == v_pool.dtype == torch.bfloat16, "pools must be bfloat16")
-    _require(block_table.dtype == torch.int32 and block_table.dim() == 2,
-             "block_table must be int32 [B, max_pages]")
+    if v_pool.shape != (slots,) + v_slot_shape(NKV, D, PT):
+        _check_v_pool(v_pool, slots, NKV, D, PT)
+    if k_pool.dtype is not torch.bfloat16 or v_pool.dtype is not torch.bfloat16:
+        raise ValueError("pools must be bfloat16")
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
+        raise ValueError("block_table must be int32 [B, max_pages]")
     B = block_table.shape[0]
-    _require(keep.dtype == torch.int32 and keep.dim() == 3
-             and tuple(keep.shape[:2]) in ((B, NKV), (B, 1)),
-             f"keep must be int32 [{B}, {NKV}, n] or [{B}, 1, n]")
-    _require(keep_lens.dtype == torch.int32 and tuple(keep_lens.shape) == (B,),
-             "keep_lens must be int32 [B]")
-    _check_lens(start, B, "start")
+    if (keep.dtype is not torch.int32 or keep.dim() != 3 or keep.shape[0] != B
+            or keep.shape[1] not in (1, NKV)):
+        raise ValueError(f"keep must be int32 [{B}, {NKV}, n] or [{B}, 1, n]")
+    if not _is_i32(keep_lens, B):
+        raise ValueError(f"keep_lens must be int32 [{B}]")
+    if start is not None and not _is_i32(start, B):
+        raise ValueError(f"start must be int32 [{B}]")
     in_place = dst_table is None
-    dst_table = block_table if in_place else dst_table
-    _require(dst_table.dtype == torch.int32 and dst_table.dim() == 2 and dst_table.shape[0] == B,
-             "dst_table must be int32 [B, pages]")
-    _check_scores(scores, B, NKV, "scores")
-    _require(scores is not None or scores_out is None, "scores_out needs scores")
-    if scores is not None:
-        scores_out = scores if scores_out is None else scores_out
-        _require(scores_out.dtype == torch.float32 and scores_out.shape == scores.shape,
-                 "scores_out must be like scores")
-    if B == 0 or (keep.shape[2] == 0 and scores is None):
+    if in_place:
+        dst_table = block_table
+    elif (dst_table.dtype is not torch.int32 or dst_table.dim() != 2
+          or dst_table.shape[0] != B):
+        raise ValueError(f"dst_table must be int32 [{B}, pages]")
+    if scores is None:
+        if scores_out is not None:
+            raise ValueError("scores_out needs scores")
+    elif not _is_scores(scores, B, NKV):
+        raise ValueError(f"scores must be float32 [{B}, {NKV}, tokens]")
+    elif scores_out is None:
+        scores_out = scores
+    elif scores_out.dtype is not torch.float32 or scores_out.shape != scores.shape:
+        raise ValueError("scores_out must be like scores")
+    n = keep.shape[2]
+    if B == 0 or (n == 0 and scores is None):
         return
     if _BOUNDS_CHECKS:
         check_keep(keep, keep_lens, block_table.shape[1] * PT, start, in_place)
-    if keep.shape[2] == 0:  # only scores to clear
-        keep, keep_lens = keep.new_zeros((B, 1, 1)), torch.zeros_like(keep_lens)
-    _lib.call("voom_compact_kv", _ptr(k_pool), _ptr(v_pool), _ptr(block_table), _ptr(dst_table),
-              _ptr(keep), _ptr(keep_lens), _ptr(start), _ptr(scores), _ptr(scores_out), B, NKV, D,
-              PT, block_table.shape[1], dst_table.shape[1], slots, keep.shape[1], keep.shape[2],
-              0 if scores is None else scores.shape[2], _stream(None))
+    if n == 0:  # only scores to clear
+        keep, keep_lens, n = keep.new_zeros((B, 1, 1)), torch.zeros_like(keep_lens), 1
+    rc = _lib.lib().voom_compact_kv(
+        k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), dst_table.data_ptr(),
+        keep.data_ptr(), keep_lens.data_ptr(), _ptr(start), _ptr(scores), _ptr(scores_out), B, NKV,
+        D, PT, block_table.shape[1], dst_table.shape[1], slots, keep.shape[1], n,
+        0 if scores is None else scores.shape[2], _stream(None))
+    if rc:
+        _lib.check(rc, "voom_compact_kv")
 
 
 def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
@@ -556,37 +591,48 @@ def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
     [B, nq, L, hd]; K and V of token t land at cache position start[b] + t (start [B]
     int32) for t < new_lens[b] (None: all).  One rounding to bf16 at the end.
     """
-    dev = _require_device(qkv, cos, sin, positions, k_pool, v_pool, block_table, start, q_weight,
-                          k_weight, new_lens)
-    _require_current(dev)
+    _require_here(qkv, cos, sin, positions, k_pool, v_pool, block_table, start, q_weight, k_weight,
+                  new_lens)
     nq, nkv = int(num_q_heads), int(num_kv_heads)
-    _require(k_pool.dim() == 4, "k_pool must be [slots, NKV, PT, D]")
+    if k_pool.dim() != 4:
+        raise ValueError("k_pool must be [slots, NKV, PT, D]")
     slots, NKVp, PT, hd = k_pool.shape
-    _require(nq > 0 and NKVp == nkv, "pool geometry does not match the heads")
-    _check_v_pool(v_pool, slots, nkv, hd, PT)
-    _require(qkv.dim() == 3 and qkv.shape[2] == (nq + 2 * nkv) * hd,
-             f"qkv must be [B, L, {(nq + 2 * nkv) * hd}]")
+    if nq <= 0 or NKVp != nkv:
+        raise ValueError("pool geometry does not match the heads")
+    if v_pool.shape != (slots,) + v_slot_shape(nkv, hd, PT):
+        _check_v_pool(v_pool, slots, nkv, hd, PT)
+    if qkv.dim() != 3 or qkv.shape[2] != (nq + 2 * nkv) * hd:
+        raise ValueError(f"qkv must be [B, L, {(nq + 2 * nkv) * hd}]")
     B, L, _ = qkv.shape
-    _require(qkv.dtype == k_pool.dtype == v_pool.dtype == torch.bfloat16,
-             "qkv and pools must be bfloat16")
-    _require(cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape
-             and cos.shape[0] > 0, "cos and sin must be float32 [positions, rotary / 2]")
-    _require(positions.dtype == torch.int32 and tuple(positions.shape) == (B, L),
-             f"positions must be int32 [{B}, {L}]")
-    _require(block_table.dtype == torch.int32 and block_table.dim() == 2
-             and block_table.shape[0] == B, "block_table must be int32 [B, max_pages]")
-    _require(start.dtype == torch.int32 and tuple(start.shape) == (B,), "start must be int32 [B]")
-    _check_lens(new_lens, B, "new_lens")
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        _require(w is None or (w.dtype == torch.bfloat16 and tuple(w.shape) == (hd,)),
-                 f"{name} must be bfloat16 [{hd}]")
-    q = torch.empty((B, nq, L, hd), dtype=torch.bfloat16, device=dev)
-    if q.numel():
-        _lib.call("voom_qk_norm_rope_append", _ptr(qkv), _ptr(q_weight), _ptr(k_weight),
-                  float(eps), _ptr(cos), _ptr(sin), cos.shape[0], 2 * cos.shape[1],
-                  int(bool(interleaved)), _ptr(positions), _ptr(q), _ptr(k_pool), _ptr(v_pool),
-                  _ptr(block_table), _ptr(start), _ptr(new_lens), B, L, nq, nkv, hd, PT,
-                  block_table.shape[1], slots, _stream(None))
+    if (qkv.dtype is not torch.bfloat16 or k_pool.dtype is not torch.bfloat16
+            or v_pool.dtype is not torch.bfloat16):
+        raise ValueError("qkv and pools must be bfloat16")
+    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.dim() != 2
+            or cos.shape != sin.shape or cos.shape[0] == 0):
+        raise ValueError("cos and sin must be float32 [positions, rotary / 2]")
+    if not _is_i32(positions, B, L):
+        raise ValueError(f"positions must be int32 [{B}, {L}]")
+    if (block_table.dtype is not torch.int32 or block_table.dim() != 2
+            or block_table.shape[0] != B):
+        raise ValueError(f"block_table must be int32 [{B}, max_pages]")
+    if not _is_i32(start, B):
+        raise ValueError(f"start must be int32 [{B}]")
+    if new_lens is not None and not _is_i32(new_lens, B):
+        raise ValueError(f"new_lens must be int32 [{B}]")
+    if q_weight is not None and (q_weight.dtype is not torch.bfloat16 or q_weight.shape != (hd,)):
+        raise ValueError(f"q_weight must be bfloat16 [{hd}]")
+    if k_weight is not None and (k_weight.dtype is not torch.bfloat16 or k_weight.shape != (hd,)):
+        raise ValueError(f"k_weight must be bfloat16 [{hd}]")
+    q = qkv.new_empty((B, nq, L, hd))
+    if B and L:
+        rc = _lib.lib().voom_qk_norm_rope_append(
+            qkv.data_ptr(), _ptr(q_weight), _ptr(k_weight), float(eps), cos.data_ptr(),
+            sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], 1 if interleaved else 0,
+            positions.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
+            block_table.data_ptr(), start.data_ptr(), _ptr(new_lens), B, L, nq, nkv, hd, PT,
+            block_table.shape[1], slots, _stream(None))
+        if rc:
+            _lib.check(rc, "voom_qk_norm_rope_append")
     return q
 
 
