@@ -1,0 +1,193 @@
+"""GPU test of PagedKVCache's verbs for drafted tokens and bounded caches, run together as a
+serving step runs them: projections appended with head norms and rotation, a tree of drafts
+attended, the accepted branch kept, its weights observed, the cache cut to a budget, and a
+token decoded over what is left.  Every attention is compared with fp64 over the rows that
+the reference says are there; K and V rows exactly.
+
+Bars: outputs as of the tree and decode kernels (relative L2 4e-3); weights relative 4e-4
+(the log-sum-exp and the scores are off by 2e-4 each, see the tests of the operators).
+"""
+import pytest
+import torch
+
+from paged_inputs import trees
+from voom_amd import ops
+from voom_amd.decoder import DecoderConfig, PagedDecoder, random_weights
+from voom_amd.kv_paged import PagedKVCache
+
+pytestmark = pytest.mark.gpu
+
+REL, WEIGHT = 4e-3, 4e-4
+B, NQ, NKV, D, LAYERS = 2, 8, 2, 64, 2
+G = NQ // NKV
+
+
+def rel(a, b):
+    return ((a.double() - b).norm() / b.norm()).item()
+
+
+def attend64(q, k, v, sees):
+    """fp64 (out [B, NQ, T, D], weights [B, NQ, T, S]); sees bool [B, T, S]."""
+    k, v = (x.double().repeat_interleave(G, 1) for x in (k, v))
+    s = torch.matmul(q.double(), k.transpose(2, 3).contiguous()) * D ** -0.5
+    w = torch.softmax(s.masked_fill(~sees[:, None], -float("inf")), -1)
+    return torch.matmul(w, v), w
+
+
+@pytest.mark.parametrize("page,spilled", [(32, False), (64, True), (256, False)])
+def test_a_speculative_step_on_a_bounded_cache(page, spilled):
+    print(f"[speculative] page={page} spilled={spilled}", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(page)
+
+    def rnd(*shape, std=1.0):
+        return (torch.randn(shape, generator=g, device="cuda") * std).to(torch.bfloat16)
+
+    S, T, path, budget, sink, recent = 300, 9, [0, 2, 5, 8], 120, 4, 16
+    kv = PagedKVCache(LAYERS, 1 << 40, page_positions=page, resident_pages=1)
+    cos, sin = ops.rope_cache(600, D, 1e4)
+    wq, wk = (1 + rnd(2, D, std=0.2)).unbind()
+    norm = dict(q_weight=wq.contiguous(), k_weight=wk.contiguous())
+    for layer in range(LAYERS):
+        q = kv.append_qkv(layer, rnd(B, S, (NQ + 2 * NKV) * D), cos, sin, NQ, NKV, **norm)
+        assert q.shape == (B, NQ, S, D)
+    assert kv.offset == S == kv.next_position
+    if spilled:
+        kv.spill([(layer, i) for layer in range(LAYERS) for i in (0, 2)])
+
+    mask = trees(1, T, 3)[0].cuda()
+    depth = mask.sum(-1).int() - 1
+    rows = {}
+    for layer in range(LAYERS):
+        qkv = rnd(B, T, (NQ + 2 * NKV) * D)
+        q = kv.append_qkv(layer, qkv, cos, sin, NQ, NKV, positions=(S + depth).repeat(B, 1), **norm)
+        out, lse = kv.attend_tree(layer, q, mask, return_lse=True)
+        k, v = kv.gather(layer)
+        sees = torch.ones((B, T, S + T), dtype=torch.bool, device="cuda")
+        sees[:, :, S:] = mask
+        want, _ = attend64(q, k, v, sees)
+        torch.cuda.synchronize()
+        assert rel(out, want) <= REL
+        rows[layer] = (q, lse, k, v)
+    assert kv.offset == S + T
+
+    kv.keep_drafts(T, path)
+    n = len(path)
+    stay = list(range(S)) + [S + i for i in path]
+    assert kv.offset == S + n and kv.layer_lengths() == (S + n,) * LAYERS
+    for layer in range(LAYERS):
+        k, v = kv.gather(layer)
+        assert torch.equal(k, rows[layer][2][:, :, stay])
+        assert torch.equal(v, rows[layer][3][:, :, stay])
+
+    # the accepted branch is a chain here or not: its rows saw what a chain sees only if
+    # every draft of the path is the next one's parent
+    chain = all(bool(mask[b, a]) for a, b in zip(path, path[1:]))
+    for layer in range(LAYERS):
+        q, lse, k, v = rows[layer]
+        q = q[:, :, path].contiguous()
+        k, v = k[:, :, stay], v[:, :, stay]
+        sees = torch.ones((n, S + n), dtype=torch.bool, device="cuda").tril(S).repeat(B, 1, 1)
+        _, w = attend64(q, k, v, sees)
+        if chain:
+            lse = lse[:, path].contiguous()
+        else:
+            _, lse = kv.attend_tree(layer, q, return_lse=True)
+        kv.observe(layer, q, lse)
+        got = kv._weights[layer]
+        added = w.reshape(B, NKV, G * n, -1).sum(2)
+        torch.cuda.synchronize()
+        assert (got[:, :, S + n:] == 0).all()
+        off = (got[:, :, :S + n].double() - added).abs()
+        assert (off <= WEIGHT * added + 1e-6).all()
+
+    sums = [kv._weights[layer][:, :, :S + n].cpu() for layer in range(LAYERS)]
+    before = [kv.gather(layer) for layer in range(LAYERS)]
+    assert kv.evict(budget, sink=sink, recent=recent) == S + n - budget
+    assert kv.offset == budget and kv.next_position == S + n
+    assert kv.evict(budget, sink=sink, recent=recent) == 0
+    for layer in range(LAYERS):
+        k, v = kv.gather(layer)
+        kept = torch.zeros((B, NKV, budget), dtype=torch.long)
+        for b in range(B):
+            for h in range(NKV):
+                s = sums[layer][b, h].clone()
+                s[:sink] = s[S + n - recent:] = float("inf")
+                kept[b, h] = torch.sort(s, descending=True, stable=True).indices[:budget].sort()[0]
+        at = kept.cuda()[..., None].expand(-1, -1, -1, D)
+        assert torch.equal(k, before[layer][0].gather(2, at))
+        assert torch.equal(v, before[layer][1].gather(2, at))
+        want = sums[layer].gather(2, kept)
+        got = kv._weights[layer].cpu()
+        assert torch.equal(got[:, :, :budget], want) and (got[:, :, budget:] == 0).all()
+
+    # a token decoded over what is left, its key rotated at its true position
+    for layer in range(LAYERS):
+        q = kv.append_qkv(layer, rnd(B, 1, (NQ + 2 * NKV) * D), cos, sin, NQ, NKV, **norm)
+        k, v = kv.gather(layer)
+        out = kv.attend(layer, q)
+        want, _ = attend64(q, k, v, torch.ones((B, 1, budget + 1), dtype=torch.bool, device="cuda"))
+        torch.cuda.synchronize()
+        assert rel(out, want) <= REL
+    assert kv.offset == budget + 1 and kv.next_position == S + n + 1
+    with pytest.raises(ValueError, match="after evict"):
+        kv.reserve(400)
+    kv.trim(0)
+    assert kv.next_position == 0
+
+
+def test_refusals_and_small_calls():
+    kv = PagedKVCache(1, 1 << 40, page_positions=32)
+    with pytest.raises(ValueError, match="kv cache"):
+        kv.evict(5)
+    k = torch.randn((1, 2, 40, 64), device="cuda").to(torch.bfloat16)
+    kv.append(0, k, k)
+    q = torch.randn((1, 4, 41, 64), device="cuda").to(torch.bfloat16)
+    with pytest.raises(ValueError, match="41 drafts"):
+        kv.attend_tree(0, q)
+    with pytest.raises(ValueError, match="41 queries"):
+        kv.observe(0, q, torch.zeros((1, 41, 4), device="cuda"))
+    assert kv.attend_tree(0, q[:, :, :0]).shape == (1, 4, 0, 64)
+    with pytest.raises(ValueError, match="observe"):
+        kv.evict(30)
+    assert kv.evict(40) == 0
+    for budget, sink, recent in ((0, 0, 0), (10, 6, 5), (10, -1, 0)):
+        with pytest.raises(ValueError, match="budget"):
+            kv.evict(budget, sink=sink, recent=recent)
+    for path in ([1, 1], [2, 0], [-1], [5], [[0], [1]], [0, 1, 2, 3, 4, 5]):
+        with pytest.raises(ValueError, match="path"):
+            kv.keep_drafts(5, path)
+    with pytest.raises(ValueError, match="drafts"):
+        kv.keep_drafts(41, [0])
+    kv.keep_drafts(5, [])
+    assert kv.offset == 35
+    kv.keep_drafts(3, [0, 1, 2])
+    assert kv.offset == 35
+    kv.keep_drafts(3, torch.tensor([2], device="cuda"))
+    got, _ = kv.gather(0)
+    assert kv.offset == 33 and torch.equal(got[:, :, 32], k[:, :, 34])
+    with pytest.raises(ValueError, match="geometry"):
+        kv.append_qkv(0, torch.zeros((1, 2, 100), dtype=torch.bfloat16, device="cuda"), None, None, 3,
+                      1)
+    kv.reserve(64)
+    _, lse = kv.attend_tree(0, q[:, :, :1].contiguous(), return_lse=True)
+    kv.observe(0, q[:, :, :1], lse)
+    with pytest.raises(ValueError, match="captured"):
+        kv.evict(10)
+
+
+def test_a_decoder_goes_on_after_an_eviction_at_the_next_position():
+    cfg = DecoderConfig(num_hidden_layers=2, hidden_size=128, num_attention_heads=2,
+                        num_key_value_heads=1, head_dim=64, intermediate_size=128, vocab_size=256)
+    model = PagedDecoder(cfg, random_weights(cfg, 3))
+    kv = model.new_cache(page_positions=32)
+    prompt = torch.randint(0, 256, (1, 90), device="cuda")
+    model.forward(prompt, kv, last_only=True)
+    for layer in range(2):
+        q = torch.randn((1, 2, 8, 64), device="cuda").to(torch.bfloat16)
+        kv.observe(layer, q, kv.attend_tree(layer, q, return_lse=True)[1])
+    kv.evict(50, sink=2, recent=10)
+    seen = []
+    tables = model._rope_tables
+    model._rope_tables = lambda positions: seen.append(positions.tolist()) or tables(positions)
+    logits = model.forward(prompt[:, :1], kv)
+    assert torch.isfinite(logits).all() and seen == [[90]] and kv.offset == 51

@@ -250,7 +250,7 @@ class PagedDecoder:
     def forward(self, tokens: torch.Tensor, kv: PagedKVCache,
                 last_only: bool = False) -> torch.Tensor:
         """Logits [B, L, vocab] (fp32) for tokens [B, L] appended at kv.offset."""
-        offset = kv.offset
+        offset = kv.next_position
         L = tokens.shape[1]
         cos, sin = self._rope_tables(torch.arange(offset, offset + L, device=self.device))
         x = self.embed[tokens]

@@ -12,6 +12,11 @@ introspection its tests use, and adds the explicit verbs of the paged path:
                            pages are reloaded on a side stream while the
                            resident pages are attended, then LSE-merged
   attend_prefill(layer, q) causal attention of a prompt through the paged prefill kernel
+  append_qkv(layer, qkv)   append of projections: head norms, rotation and page write
+  attend_tree(layer, q)    attention of a tree of drafted tokens (the newest ones)
+  keep_drafts(n, path)     of the newest n tokens only the accepted branch stays
+  observe(layer, q, lse)   the attention weight that cached tokens receive is summed up
+  evict(budget)            tokens of least weight leave, head by head
   append_latent / update_latent / attend_mla
                            the absorbed-MLA latent cache (runtime/glm.py:265-330)
   spill(pages)             byte-plane split on the GPU -> D2H into the arena
@@ -605,6 +610,11 @@ class PagedKVCache:
         self._tables_host: list[np.ndarray | None] = [None] * L
         # ("kv", B, NKV, D) or ("latent", B, latent_dim), fixed by the first write
         self._geom: tuple | None = None
+        # attention weight that each cached token has received, [B, NKV, tokens] fp32,
+        # 0 behind the layer's length; and the tokens that evict() has dropped
+        self._weights: list[torch.Tensor | None] = [None] * L
+        self._dropped = 0
+        self._has_reserved = False  # since the cache was last empty
 
     @property
     def stats(self) -> KVStats:
@@ -760,6 +770,11 @@ class PagedKVCache:
     def layer_length(self, layer: int) -> int:
         return self._len[layer]
 
+    @property
+    def next_position(self) -> int:
+        """Rotary position of the next token: the offset, and what evict() dropped."""
+        return self._offset + self._dropped
+
     def nbytes(self) -> int:
         """Resident bytes: resident closed pages plus open-page tokens (kv_paged.py:187-194)."""
         if self._geom is None:
@@ -803,6 +818,33 @@ class PagedKVCache:
                                          **norm)
 
         self._append(layer, h.shape[1], write)
+        return q
+
+    def append_qkv(self, layer: int, qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                   num_q_heads: int, num_kv_heads: int, *, positions: torch.Tensor | None = None,
+                   **norm) -> torch.Tensor:
+        """``append`` of projected tokens qkv [B, L, (nq + 2 nkv) hd], their query and key
+        heads normed and rotated on the way (``ops.qk_norm_rope_append``, whose ``norm``
+        arguments these are); returns q [B, nq, L, hd].  ``positions`` [B, L] int32: rows of
+        cos / sin, where they are not the next ones (a draft's is its depth in the tree)."""
+        B, L, W = qkv.shape
+        heads = num_q_heads + 2 * num_kv_heads
+        if heads <= 0 or W % heads:
+            raise ValueError(f"qkv width {W} is not a multiple of {heads} heads")
+        self._set_geometry(("kv", B, num_kv_heads, W // heads), qkv.dtype)
+        if positions is None:
+            first = self._len[layer] + self._dropped
+            positions = torch.arange(first, first + L, dtype=torch.int32,
+                                     device=self.device).repeat(B, 1)
+        q = qkv.new_empty((B, num_q_heads, 0, W // heads))
+
+        def write(pool, start):
+            nonlocal q
+            q = ops.qk_norm_rope_append(qkv.contiguous(), cos, sin, positions, pool.k, pool.v,
+                                        self._tables[layer], self._positions(start), num_q_heads,
+                                        num_kv_heads, **norm)
+
+        self._append(layer, L, write)
         return q
 
     def append_latent(self, layer: int, lat: torch.Tensor) -> None:
@@ -862,6 +904,9 @@ class PagedKVCache:
         """
         if self._geom is None:
             raise ValueError("reserve() needs the page geometry: append once first")
+        if self._dropped:
+            raise ValueError("reserve(): after evict() a token's place in the cache is not its "
+                             "position, which captured steps take it for")
         PT = self.page_positions
         B = self._batch
         total_pages = -(-int(total_len) // PT)
@@ -885,6 +930,7 @@ class PagedKVCache:
                 self._open_slots[layer][page] = cols[page]
             self._set_table_cols(layer, cols)
         self._reserved = int(total_len)
+        self._has_reserved = True
         # one [2, B] tensor, so a step advances both counters in one launch
         self._counters_dev = torch.tensor([[self._offset] * B, [self._offset + 1] * B],
                                           dtype=torch.int32, device=self.device)
@@ -997,7 +1043,11 @@ class PagedKVCache:
                 else:
                     self._drop_host(p)
             self._len[layer] = n
+            if self._weights[layer] is not None:
+                self._weights[layer][:, :, n:] = 0
         self._offset = targets[0] if targets else 0
+        if not any(self._len):
+            self._dropped = 0
         if getattr(self, "_counters_dev", None) is not None:
             B = self._batch
             self._counters_dev.copy_(torch.tensor(
@@ -2024,6 +2074,126 @@ class PagedKVCache:
         else:
             out = ops.paged_gqa_prefill(q, pool.k, pool.v, table, S, scale=scale)
         return out.permute(0, 2, 1, 3)
+
+    def attend_tree(self, layer: int, q: torch.Tensor, mask: torch.Tensor | None = None,
+                    scale: float | None = None, return_lse: bool = False):
+        """Attention of the layer's newest T tokens as a tree of drafts: q [B, NQ, T, D]
+        holds the queries of drafts whose K/V were just appended.  Draft t sees every
+        token before the drafts and those drafts j with mask[t, j] set (bool [T, T] or
+        [B, T, T]; None: causal).  Returns out [B, NQ, T, D] (and the LSE [B, T, NQ] that
+        ``observe`` takes).  Spilled pages of the layer are made resident first.
+        """
+        self._require_kind(layer, "kv")
+        B, NQ, T, D = q.shape
+        S = self._len[layer]
+        if T > S:
+            raise ValueError(f"{T} drafts but the layer holds {S} tokens")
+        if T == 0:
+            out = torch.empty_like(q)
+            return (out, q.new_empty((B, 0, NQ), dtype=torch.float32)) if return_lse else out
+        pool, table = self._resident(layer)
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()  # the kernel loads 16 bytes per lane
+        got = ops.paged_gqa_tree(q, pool.k, pool.v, table, self._positions(S), mask=mask,
+                                 scale=scale, return_lse=return_lse)
+        out, lse = got if return_lse else (got, None)
+        out = out.permute(0, 2, 1, 3)
+        return (out, lse) if return_lse else out
+
+    def _resident(self, layer: int):
+        """(pool, block table) of a layer with every page resident."""
+        spilled = [p for p in self._pages[layer] if not p.resident]
+        if spilled:
+            self.reload(spilled)
+        return self._pool(layer), self._tables[layer]
+
+    def keep_drafts(self, drafts: int, path) -> None:
+        """Of every layer's newest ``drafts`` tokens keep those of ``path`` (ascending draft
+        indices, [n] for all sequences or [B, n]) and drop the others: the accepted branch
+        of a tree.  The cache is then ``drafts - n`` tokens shorter."""
+        self._require_kind(0, "kv")
+        drafts = int(drafts)
+        B = self._batch
+        if not (isinstance(path, torch.Tensor) and path.is_cuda):  # known here: checked here
+            host = np.asarray(path, dtype=np.int64)
+            if host.size and (host.min() < 0 or host.max() >= drafts
+                              or (np.diff(host, axis=-1) <= 0).any()):
+                raise ValueError(f"path must ascend within [0, {drafts})")
+            path = host
+        path = torch.as_tensor(path, dtype=torch.int32, device=self.device)
+        if path.dim() == 1:
+            path = path.expand(B, -1)
+        if path.dim() != 2 or path.shape[0] != B or path.shape[1] > drafts:
+            raise ValueError(f"path must hold at most {drafts} drafts of each of {B} sequences")
+        n = path.shape[1]
+        if drafts < 0 or drafts > min(self._len):
+            raise ValueError(f"{drafts} drafts but a layer holds {min(self._len)} tokens")
+        if n and n < drafts:
+            counts = torch.full((B,), n, dtype=torch.int32, device=self.device)
+            for layer in range(self.num_layers):
+                first = self._len[layer] - drafts
+                pool, table = self._resident(layer)
+                ops.compact_kv(pool.k, pool.v, table, (path + first)[:, None].contiguous(), counts,
+                               start=self._positions(first), scores=self._weights[layer])
+        self._trim_to([length - drafts + n for length in self._len])
+
+    def observe(self, layer: int, q: torch.Tensor, lse: torch.Tensor,
+                scale: float | None = None) -> None:
+        """Add the attention weight that the layer's tokens receive from its newest L tokens,
+        whose queries q [B, NQ, L, D] and LSE [B, L, NQ] are given (``attend_tree``'s), to
+        the sums that ``evict`` chooses by."""
+        self._require_kind(layer, "kv")
+        S = self._len[layer]
+        if q.shape[2] > S:
+            raise ValueError(f"{q.shape[2]} queries but the layer holds {S} tokens")
+        _, B, NKV, _ = self._geom
+        sums = self._weights[layer]
+        if sums is None or sums.shape[2] < S:
+            PT = self.page_positions
+            grown = torch.zeros((B, NKV, -(-max(2 * S, PT) // PT) * PT), dtype=torch.float32,
+                                device=self.device)
+            if sums is not None:
+                grown[:, :, :sums.shape[2]] = sums
+            self._weights[layer] = sums = grown
+        pool, table = self._resident(layer)
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()
+        ops.paged_gqa_observe(q, lse.contiguous(), pool.k, table, self._positions(S), sums,
+                              scale=scale)
+
+    def evict(self, budget: int, *, sink: int = 0, recent: int = 0) -> int:
+        """Cut every layer to ``budget`` tokens: of each head stay the first ``sink``, the
+        newest ``recent``, and of the others those that received most attention weight
+        (``observe``).  Keys keep the rotation of their position; the next token's is
+        ``next_position``.  Returns how many tokens were dropped."""
+        self._require_kind(0, "kv")
+        budget = int(budget)
+        if len(set(self._len)) != 1:
+            raise ValueError("evict() needs layers of one length")
+        if self._has_reserved:
+            raise ValueError("evict(): the steps captured after reserve() take a token's place "
+                             "in the cache for its position")
+        S = self._len[0]
+        if budget <= 0 or sink < 0 or recent < 0 or sink + recent > budget:
+            raise ValueError(f"sink {sink} and recent {recent} must fit the budget {budget}")
+        if S <= budget:
+            return 0
+        if any(w is None for w in self._weights):
+            raise ValueError("evict() needs the weights that observe() sums up in every layer")
+        ctx = self._positions(S)
+        for layer in range(self.num_layers):
+            sums = self._weights[layer]
+            if sums.shape[2] < S:  # tokens behind them were not observed yet
+                sums = torch.nn.functional.pad(sums, (0, S - sums.shape[2]))
+                self._weights[layer] = sums
+            pool, table = self._resident(layer)
+            keep, counts = ops.evict_select(sums, ctx, budget, sink=sink, recent=recent)
+            ops.compact_kv(pool.k, pool.v, table, keep, counts, scores=sums)
+        self._trim_to([budget] * self.num_layers)
+        self._dropped += S - budget
+        return S - budget
 
     def attend_mla(self, layer: int, q_nope: torch.Tensor, q_rope: torch.Tensor,
                    w_uk, w_uv_t, scale: float,
