@@ -121,10 +121,17 @@ __device__ __forceinline__ Units<D> scan_units(const TreeArgs& a, int base, int 
 }
 
 // Chunk c (16 bytes) of K row r sits at c ^ k_swizzle(r) of its row, chunk c of V^T row
-// d at c ^ (d >> 2 & 3): the 16 rows of an operand read then spread over all banks.
+// d at c ^ v_swizzle(d >> 2): the rows of an operand read then spread over all banks,
+// whether 16 consecutive lanes are served together or lanes 0-3, 12-15, 20-27 (as d >> 2
+// itself does not: two cycles of conflicts per read).
 template <int D>
 __device__ __forceinline__ int k_swizzle(int r) {
   return D == 128 ? (r & 3) | ((r >> 3) & 3) << 2 : ((r >> 1) & 1) | ((r >> 3) & 3) << 1;
+}
+
+__device__ __forceinline__ int v_swizzle(int h) {  // 0, 2, 3, 1
+  h &= 3;
+  return ((h ^ h >> 1) & 1) << 1 | h >> 1;
 }
 
 // A block of a stage in LDS: K [32][D], then V^T [D][32].
@@ -149,7 +156,7 @@ __device__ __forceinline__ void load_stage(uint16_t* stage, const TreeArgs& a, P
     const int sub = in_blk % kPieces;
     const int krow = sub * (kWave / kCpr) + lane / kCpr;
     const int ksrc = krow * (D * 2) + 16 * ((lane % kCpr) ^ k_swizzle<D>(krow));
-    const int vsrc = sub * 1024 + (lane >> 2) * (kBlk * 2) + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
+    const int vsrc = sub * 1024 + (lane >> 2) * (kBlk * 2) + 16 * ((lane & 3) ^ v_swizzle(lane >> 4));
     load_piece<AUX>((is_v ? a.v_pool : a.k_pool) + at * (kBlk * D), kBlk * D * 2,
                     is_v ? vsrc : ksrc, stage + p * 512);
   }
@@ -166,7 +173,7 @@ template <int D>
 __device__ __forceinline__ u32x4 read_v(const uint16_t* tile, int n, int lane) {
   const int i16 = lane & 15, g = lane >> 4;
   return *reinterpret_cast<const u32x4*>(tile + kBlk * D + (16 * n + i16) * kBlk +
-                                         8 * (g ^ (i16 >> 2)));
+                                         8 * (g ^ v_swizzle(i16 >> 2)));
 }
 
 // A block's K and V^T operands.
