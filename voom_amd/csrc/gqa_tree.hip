@@ -667,7 +667,10 @@ constexpr int kReduceWaves = 4;
 // rows of sequences without tokens and of tiles without drafts are written here.
 template <int D>
 __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(TreeArgs a) {
-  constexpr int DPL = D / kWave;
+  // A wavefront holds the row of kTogether pieces at a time, 4 dims per lane.
+  constexpr int kLanes = D / 4;
+  constexpr int kTogether = kWave / kLanes;
+  constexpr int kAhead = 8;  // loads in flight
   const int lane = threadIdx.x & (kWave - 1);
   const long long task =
       static_cast<long long>(blockIdx.x) * kReduceWaves + uniform(threadIdx.x / kWave);
@@ -693,7 +696,8 @@ __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(T
   const int t = rr / a.G;
   const int head = kvh * a.G + (rr - t * a.G);
   const size_t at = (static_cast<size_t>(b) * a.T + t) * a.NQ + head;
-  uint16_t* o = a.out + at * D + lane * DPL;
+  const int sub = lane / kLanes;
+  const int dim = lane % kLanes * 4;
   const int ctx = uniform(context_of(a, b));
   const bool dead = t >= uniform(drafts_of(a, b, ctx));
   int first = 0, last = -1;
@@ -708,47 +712,53 @@ __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(T
   }
   // Up to 64 pieces at a time, one per lane for their maxima and sums.  A segment that
   // starts inside its first workgroup's range is that one's last piece, else its first.
-  float M = -FLT_MAX, L = 0.f, acc[DPL] = {};
+  float M = -FLT_MAX, L = 0.f;
+  f32x4 acc = {};
   for (int w0 = first; w0 <= last; w0 += kWave) {
     const int n = last - w0 + 1 < kWave ? last - w0 + 1 : kWave;
     const size_t p0 = 2 * static_cast<size_t>(w0) * a.rows + r;
-    const int odd = later && w0 == first ? a.rows : 0;  // of lane 0's piece
-    const int k = lane < n ? lane : 0;
-    const float2 ml = *reinterpret_cast<const float2*>(
-        a.part_ml + (p0 + 2 * static_cast<size_t>(k) * a.rows + (k == 0 ? odd : 0)) * 2);
+    const int odd = later && w0 == first ? a.rows : 0;  // of the first one
+    auto row_at = [&](int k) {
+      k = k < n ? k : n - 1;
+      return p0 + 2 * static_cast<size_t>(k) * a.rows + (k == 0 ? odd : 0);
+    };
+    f32x4 v[kAhead];
+    auto read = [&](int k0) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        v[u] = *reinterpret_cast<const f32x4*>(a.part_o + row_at(k0 + u * kTogether + sub) * D +
+                                               dim);
+    };
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + row_at(lane) * 2);
+    read(0);  // (under way while the weights are formed)
     const float mn = fmaxf(M, wave_max_uniform(lane < n ? ml.x : -FLT_MAX));
     const float wt = lane < n ? fast_exp2(ml.x - mn) : 0.f;
     const float f = fast_exp2(M - mn);
     M = mn;
     L = L * f + wave_sum_uniform(lane < n ? ml.y * wt : 0.f);
+    acc *= f;
+    for (int k0 = 0; k0 < n; k0 += kAhead * kTogether) {
+      if (k0 != 0) read(k0);
 #pragma unroll
-    for (int d = 0; d < DPL; ++d) acc[d] *= f;
-    for (int k0 = 0; k0 < n; k0 += 8) {
-      float v[8][DPL];  // eight pieces' rows in flight
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int at_k = k0 + u < n ? k0 + u : n - 1;
-        const float* po =
-            a.part_o + (p0 + 2 * static_cast<size_t>(at_k) * a.rows +
-                        (at_k == 0 ? odd : 0)) * D + lane * DPL;
-#pragma unroll
-        for (int d = 0; d < DPL; ++d) v[u][d] = po[d];
-      }
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        if (k0 + u >= n) break;
-        const float ws = __builtin_bit_cast(
-            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wt), k0 + u));
-#pragma unroll
-        for (int d = 0; d < DPL; ++d) acc[d] += v[u][d] * ws;
+      for (int u = 0; u < kAhead; ++u) {
+        const int k = k0 + u * kTogether + sub;
+        const float ws = __shfl(wt, k & (kWave - 1));
+        acc += v[u] * (k < n ? ws : 0.f);
       }
     }
   }
-  const bool empty = dead || L == 0.f;
-  const float inv = empty ? 0.f : 1.f / L;
 #pragma unroll
-  for (int d = 0; d < DPL; ++d) o[d] = empty ? static_cast<uint16_t>(0) : f2bf(acc[d] * inv);
+  for (int k = kLanes; k < kWave; k <<= 1) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], k);
+  }
+  const bool empty = dead || L == 0.f;
+  const float inv = 1.f / L;
+  if (sub == 0)
+    *reinterpret_cast<u32x2*>(a.out + at * D + dim) =
+        empty ? u32x2{0u, 0u}
+              : u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv),
+                      pack_bf16x2(acc[2] * inv, acc[3] * inv)};
   if (a.lse != nullptr && lane == 0)
     a.lse[at] = empty ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
 }
@@ -761,14 +771,23 @@ struct TreePlan {
   int W;      // workgroups of the split; 0: one per segment, no reduce launch
 };
 
-TreePlan plan_tree(int G, int T, int max_pages, int page_tokens) {
+constexpr int kShort = 8;
+
+TreePlan plan_tree(int B, int NKV, int D, int G, int T, int max_pages, int page_tokens) {
   const int R = T * G;
   TreePlan p;
   p.nt = R <= 64 ? 1 : 2;
   p.rows = 16 * p.nt * kRowWaves;
   p.tiles = (R + p.rows - 1) / p.rows;
-  const long long cap = static_cast<long long>(max_pages) * page_tokens;
-  p.W = cap <= 1024 ? 0 : device_cu_count();  // all run at once
+  const long long stages = (static_cast<long long>(max_pages) * page_tokens + 64 * 128 / D - 1) /
+                           (64 * 128 / D);
+  const long long segs = static_cast<long long>(B) * NKV * p.tiles;
+  // A segment of few stages is walked by one workgroup, which saves the reduce launch (8
+  // heads, 8 stages: 12.0 us so, 12.7 split; 12 stages: 13.4 and 12.4; 16: 20 and 14), and
+  // so are twice as many where there are enough of them; all workgroups of a split run
+  // at once.
+  const int cus = device_cu_count();
+  p.W = stages <= kShort || (stages <= 16 && segs >= cus) ? 0 : cus;
   return p;
 }
 
@@ -807,7 +826,8 @@ extern "C" size_t voom_paged_gqa_tree_workspace_bytes(int batch, int num_q_heads
                                                       int page_tokens, int max_pages) {
   if (!tree_shape_ok(batch, num_q_heads, num_kv_heads, head_dim, drafts, page_tokens, max_pages))
     return 0;
-  const TreePlan p = plan_tree(num_q_heads / num_kv_heads, drafts, max_pages, page_tokens);
+  const TreePlan p = plan_tree(batch, num_kv_heads, head_dim, num_q_heads / num_kv_heads, drafts,
+                               max_pages, page_tokens);
   return part_o_bytes(p, head_dim) + static_cast<size_t>(2) * p.W * p.rows * 2 * sizeof(float);
 }
 
@@ -835,7 +855,7 @@ extern "C" int voom_paged_gqa_tree(const void* q, const void* k_pool, const void
                    reinterpret_cast<uintptr_t>(out) % 8 == 0,
                "%s: q and pools must be 16-byte aligned", who);
   const int G = num_q_heads / num_kv_heads;
-  const TreePlan p = plan_tree(G, drafts, max_pages, page_tokens);
+  const TreePlan p = plan_tree(batch, num_kv_heads, head_dim, G, drafts, max_pages, page_tokens);
   const long long stages = (static_cast<long long>(max_pages) * page_tokens + 63) / 64;
   VOOM_REQUIRE(stages * batch * num_kv_heads * p.tiles < (1LL << 31),
                "%s: %d pages of %d tokens for %d sequences are too many", who, max_pages,
