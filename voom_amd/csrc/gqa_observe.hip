@@ -15,7 +15,8 @@
 // tokens, 256 at D = 64) of all (sequence, kv head) segments lie end to end and are dealt
 // out evenly.  K goes straight into LDS (1 KiB loads) through a ring of four 32 KiB
 // stages, three of them under way; loaded into operand registers instead, 64 bytes of
-// a row at a time, the same keys came 20 % slower even with no work on them.
+// a row at a time, the same keys took 147 us with no work on them, where 16 sequences of
+// 1k-32k tokens, 32/8 heads, take 136 with all of it.
 //
 // Eight wavefronts compute, RW of them on other rows (16 NT each, queries in registers)
 // and 8 / RW on other keys of the stage:

@@ -25,7 +25,7 @@
 // other 32-token block.  K and V^T go straight into LDS (buffer_load ... lds, 1 KiB
 // each) through a ring of four 32 KiB stages: three are under way while one is
 // computed (a ring of two per wavefront drained it at every stage: 371 us at 16
-// sequences of 1k-32k tokens, 16 drafts, 32/8 heads, where this takes 251; blocks
+// sequences of 1k-32k tokens, 16 drafts, 32/8 heads, where this takes 249; blocks
 // in registers, as in the decode kernel, leave too few for 64 rows: 1,076).  Per block,
 // with the rows in the N dimension:
 //   scores^T[token][row] = K . Q^T,  out^T[dim][row] += V^T . P^T   16x16x32 bf16

@@ -16,13 +16,14 @@ namespace {
 // and a last pass writes the positions in ascending order.
 //
 // What bounds it: the scores once, 4 bytes per token and head, and the latency of one
-// workgroup per (sequence, head).  Up to 49,152 candidates stay in registers, all loads
+// workgroup per (sequence, head).  Up to 32,768 candidates stay in registers, all loads
 // in flight at once (a loop that loaded them for every pass: 43 us for 16 x 8 heads of
-// up to 32,768 tokens, where this takes TIME_SELECT); of longer ones every pass loads
-// 49,152 at a time.  Its histogram has eight copies, by lane: scores share few leading bits,
-// and atomics of one wavefront on one address take turns.  The second and third
-// pass look only at the keys that share the first digit, from a list in LDS where it
-// holds them.
+// up to 32,768 tokens, where this takes 20); of longer ones every pass loads 32,768 at a
+// time (8 heads of 131,072: 66 us; with 49,152 at a time, some of them spilled, 76, and
+// 50 against 36 at 65,536, though 29 against 34 at 49,000).  Each histogram of a long row
+// has eight copies, by lane: scores share their leading bits, and atomics of one wavefront
+// on one address take turns.  The second and third pass look only at the keys that share
+// the first digit, from a list in LDS where it holds them.
 
 constexpr int kBins = 2048;
 constexpr int kList = 16384;  // candidates that share their first digit with the n-th largest
@@ -77,14 +78,16 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
   const int rounds = (count + kSelThreads * E - 1) / (kSelThreads * E);
 
   uint32_t key[E];
+  // (candidates past the last one load 0: the whole offset is in the part of the address
+  // that is checked)
   const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<float*>(s), static_cast<short>(0), count * 4, 0x00020000);
+      const_cast<float*>(s), static_cast<short>(0), count * 4u, 0x00020000);
   auto first_of = [&](int c) { return (c * kSelWaves + wv) * (E * kWave) + lane; };
   auto load = [&](int c) {
     const int first = first_of(c);
 #pragma unroll
     for (int e = 0; e < E; ++e)
-      key[e] = __builtin_amdgcn_raw_buffer_load_b32(from, first * 4, e * (kWave * 4), 0);
+      key[e] = __builtin_amdgcn_raw_buffer_load_b32(from, (first + e * kWave) * 4u, 0, 0);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const uint32_t k = order_key(__builtin_bit_cast(float, key[e]));
@@ -529,8 +532,7 @@ extern "C" int voom_evict_select(const float* scores, const int32_t* ctx_lens, i
   };
   if (score_tokens <= 8 * 256) launch(evict_select_kernel<256, 8, 1>, 256);
   else if (score_tokens <= 8 * 1024) launch(evict_select_kernel<1024, 8, 2>, 1024);
-  else if (score_tokens <= 32 * 1024) launch(evict_select_kernel<1024, 32, 8>, 1024);
-  else launch(evict_select_kernel<1024, 48, 8>, 1024);
+  else launch(evict_select_kernel<1024, 32, 8>, 1024);
   return VOOM_LAUNCH_CHECK("evict_select: launch");
 }
 
