@@ -12,7 +12,7 @@ drive the cache:
     RMSNorm, attention, residual, RMSNorm, SwiGLU, residual;
   * the greedy decode loop of StreamingEngine.generate
     (runtime/engine.py:8459-8503): embed the pending token, sweep the
-    layers at ``kv.offset``, final norm + tied lm_head, argmax.
+    layers at ``kv.next_position``, final norm + tied lm_head, argmax.
 
 A prompt's projections carry the residual add + RMSNorm, RoPE with the page
 write, and SwiGLU in their own launches (voom_qkv_rope_append_rows,
@@ -249,7 +249,7 @@ class PagedDecoder:
     @torch.no_grad()
     def forward(self, tokens: torch.Tensor, kv: PagedKVCache,
                 last_only: bool = False) -> torch.Tensor:
-        """Logits [B, L, vocab] (fp32) for tokens [B, L] appended at kv.offset."""
+        """Logits [B, L, vocab] (fp32) for tokens [B, L] appended at kv.next_position."""
         offset = kv.next_position
         L = tokens.shape[1]
         cos, sin = self._rope_tables(torch.arange(offset, offset + L, device=self.device))

@@ -614,7 +614,7 @@ class PagedKVCache:
         # 0 behind the layer's length; and the tokens that evict() has dropped
         self._weights: list[torch.Tensor | None] = [None] * L
         self._dropped = 0
-        self._has_reserved = False  # since the cache was last empty
+        self._has_reserved = False  # captured steps may exist (until release())
 
     @property
     def stats(self) -> KVStats:
