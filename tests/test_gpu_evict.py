@@ -290,6 +290,39 @@ def test_rows_outside_the_tables_are_left_out():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("bad_page", [0, 12, 30])
+@pytest.mark.parametrize("B,D", [(1, 96), (33, 64)])
+def test_a_page_outside_the_pool_in_a_long_list(B, D, bad_page):
+    """Lists of several steps, a page of one sequence -1: what would come from it or go to
+    it stays, all else is moved."""
+    print(f"[compact] bad page {bad_page} B={B} D={D}", flush=True)
+    NKV, PT, ctx, n = 2, 64, 2500, 1400
+    rng = np.random.default_rng(bad_page)
+    _, k, v = inputs(B, NKV, NKV, D, ctx, 1)
+    k_pool, v_pool, table = cache(k, v, PT)
+    k_pool[torch.isnan(k_pool)] = 0
+    v_pool[torch.isnan(v_pool)] = 0
+    keep, lens = kept_lists(rng, B, NKV, n, np.zeros(B, np.int64), ctx)
+    src_k, src_v = ops.gather_kv(k_pool, v_pool, table, ctx)
+    want_k, want_v = src_k.clone(), src_v.clone()
+    for b in range(B):
+        for h in range(NKV):
+            for_b = keep[b, h, :lens[b]]
+            to = np.arange(lens[b])
+            if b == 0:
+                moved = (for_b // PT != bad_page) & (to // PT != bad_page)
+                for_b, to = for_b[moved], to[moved]
+            want_k[b, h, torch.from_numpy(to)] = src_k[b, h, torch.from_numpy(for_b).long()]
+            want_v[b, h, torch.from_numpy(to)] = src_v[b, h, torch.from_numpy(for_b).long()]
+    broken = table.clone()
+    broken[0, bad_page] = -1
+    ops.compact_kv(k_pool, v_pool, broken, torch.from_numpy(keep).cuda(), lens_tensor(lens))
+    torch.cuda.synchronize()
+    got_k, got_v = ops.gather_kv(k_pool, v_pool, table, ctx)
+    assert torch.equal(got_k, want_k) and torch.equal(got_v, want_v)
+
+
+@pytest.mark.gpu
 def test_checked_lists_raise():
     _, k, v = inputs(1, 1, 1, 64, 64, 1)
     k_pool, v_pool, table = cache(k, v, 32)

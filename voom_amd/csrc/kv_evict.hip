@@ -238,16 +238,16 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
 // One workgroup moves some dims of a head's rows: of K, or of V, whose 32-token blocks
 // are transposed.  It reads a step of 512 rows into registers, waits until all of it is
 // read, and writes: a later step's sources lie behind every row written so far, so the
-// move may be in place, and the next step's rows, and the places of the one after it,
-// are asked for before a step is written.  (Two steps ahead, and places looked up by a
-// wavefront of their own, leave one workgroup per CU for four: 95 against 63 us for
-// 16 x 8 heads, half of 4,096 tokens.)
+// move may be in place, and the next step's rows, and the places of the two after it,
+// are asked for before a step is written.  A step waits for its rows alone, not for the
+// stores behind them (16 x 8 heads, half of 4,096 tokens, from memory: 68 us, with stores
+// in the wait 79).
 //
 // What bounds it: the kept rows read and written once; a V block is read in lines of
 // 32 tokens of a dim, whichever of them stay.  64 dims of K and 16 of V per workgroup,
-// since smaller pieces read lines of K more than once (the same: 63 against 75 us with
-// 32 dims of K); half of both where fewer than 64 segments leave CUs idle (8 heads,
-// 8,192 of 32,768 tokens: 41 against 69 us).
+// since smaller pieces read lines of K more than once (the same: 68 against 75 us with
+// half of both); half of both where fewer than 64 segments leave CUs idle (8 heads, 7,000
+// of 8,192 tokens: 39 against 47 us; 4 x 8 heads, 4,096 of up to 16,384: 53 against 55).
 
 constexpr int kMoveThreads = 512;
 constexpr int kStep = 512;  // rows of a step
@@ -354,8 +354,11 @@ __device__ __forceinline__ void move_scores(const CompactArgs& a, const int32_t*
 
 template <int kKDims, int kVDims>
 __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactArgs a) {
-  // Places of four steps: being written, being read, and looked up.
-  __shared__ uint32_t src[4][kStep], dst[4][kStep];
+  // Places of the step being written, the one being read, and the one looked up.
+  // As offsets in bytes of a row's first element: of K, or of V.
+  __shared__ uint64_t src[4][kStep], dst[4][kStep];
+  __shared__ bool ok[kStep];
+  __shared__ int bad[4];  // the step has rows outside the tables or the pool
   const int tid = static_cast<int>(threadIdx.x);
   const int kvh = static_cast<int>(blockIdx.y);
   const int b = static_cast<int>(blockIdx.z);
@@ -376,67 +379,111 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactArgs a) {
 
   constexpr int kKPass = kMoveThreads / (kKDims / 8), kVPass = kMoveThreads / kVDims;
   constexpr int kKLoads = kStep / kKPass, kVLoads = kStep / kVPass;
-  const int kr = tid / (kKDims / 8);
-  const int kc = part * kKDims + 8 * (tid % (kKDims / 8));
+  int kc = part * kKDims + 8 * (tid % (kKDims / 8));
+  kc = kc < a.D ? kc : a.D - 8;  // (moved twice, the same values)
   const int vb = a.pt_shift < 5 ? a.pt_shift : 5;
   const int vd = (part - k_parts) * kVDims + tid / kVPass;
-  auto step_places = [&](int s) {
-    look_up(a, keep, n, start, b, kvh, s * kStep + tid, src[s & 3][tid], dst[s & 3][tid]);
+  const int32_t* trow = a.table + static_cast<size_t>(b) * a.max_pages;
+  const int32_t* drow = a.dst_table + static_cast<size_t>(b) * a.dst_pages;
+  // Row tid of step s (past the last one: that one again, the same values).
+  auto index_of = [&](int s) {
+    const int i = s * kStep + tid;
+    return i < n ? i : n - 1;
   };
-  auto read_k = [&](int s, u32x4 (&v)[kKLoads]) {
-#pragma unroll
-    for (int j = 0; j < kKLoads; ++j) {
-      const uint32_t from = src[s & 3][kr + j * kKPass];
-      if (from != kNoRow && kc < a.D)
-        v[j] = *reinterpret_cast<const u32x4*>(a.k_pool + static_cast<size_t>(from) * a.D + kc);
-    }
+  struct Slots {
+    int from, src, dst;
   };
-  auto write_k = [&](int s, const u32x4 (&v)[kKLoads]) {
-#pragma unroll
-    for (int j = 0; j < kKLoads; ++j) {
-      const int at = kr + j * kKPass;
-      if (src[s & 3][at] != kNoRow && kc < a.D)
-        *reinterpret_cast<u32x4*>(a.k_pool + static_cast<size_t>(dst[s & 3][at]) * a.D + kc) = v[j];
-    }
+  auto slots_of = [&](int s, int from) {
+    const long long to = start + static_cast<long long>(index_of(s));
+    return Slots{from, trow[page_of(from, a.max_pages, a)], drow[page_of(to, a.dst_pages, a)]};
   };
-  auto read_v = [&](int s, uint32_t (&v)[kVLoads]) {
-#pragma unroll
-    for (int j = 0; j < kVLoads; ++j) {
-      const uint32_t from = src[s & 3][tid % kVPass + j * kVPass];
-      if (from != kNoRow) v[j] = a.v_pool[v_element(from, vd, vb, a.D)];
-    }
+  const bool keys = part < k_parts;
+  auto set_places = [&](int s, const Slots& x) {
+    const long long at = start + static_cast<long long>(index_of(s));
+    const uint32_t from = row_of(x.src, x.from, a.max_pages, kvh, a);
+    const uint32_t to = row_of(x.dst, at, a.dst_pages, kvh, a);
+    const int shift = keys ? 0 : vb;
+    src[s & 3][tid] = v_element(from, 0, shift, a.D) * 2;
+    dst[s & 3][tid] = v_element(to, 0, shift, a.D) * 2;
+    const bool in_pool = from != kNoRow && to != kNoRow;
+    ok[tid] = in_pool;
+    if (!in_pool) bad[s & 3] = 1;
+    return from != to;
   };
-  auto write_v = [&](int s, const uint32_t (&v)[kVLoads]) {
-#pragma unroll
-    for (int j = 0; j < kVLoads; ++j) {
-      const int at = tid % kVPass + j * kVPass;
-      if (src[s & 3][at] != kNoRow)
-        a.v_pool[v_element(dst[s & 3][at], vd, vb, a.D)] = static_cast<uint16_t>(v[j]);
-    }
+  // (the address is one addition: with the products here a step was bound by them)
+  char* const k_base = reinterpret_cast<char*>(a.k_pool + kc);
+  char* const v_base = reinterpret_cast<char*>(a.v_pool + (static_cast<size_t>(vd) << vb));
+  auto read_k = [&](uint64_t from, u32x4& v) {
+    v = *reinterpret_cast<const u32x4*>(k_base + from);
   };
-  auto run = [&](auto& even, auto& odd, auto read, auto write) {
-    step_places(0);
-    step_places(1);
+  auto write_k = [&](uint64_t to, const u32x4& v) { *reinterpret_cast<u32x4*>(k_base + to) = v; };
+  auto read_v = [&](uint64_t from, uint32_t& v) {
+    v = *reinterpret_cast<const uint16_t*>(v_base + from);
+  };
+  auto write_v = [&](uint64_t to, uint32_t v) {
+    *reinterpret_cast<uint16_t*>(v_base + to) = static_cast<uint16_t>(v);
+  };
+  // A thread's rows of a step are first, first + stride ...
+  auto run = [&](auto& even, auto& odd, int first, int stride, auto read, auto write) {
+    constexpr int kLoads = sizeof(even) / sizeof(even[0]);
+    if (tid < 4) bad[tid] = 0;
     __syncthreads();
-    read(0, even);
     int s = 0;
-    auto step = [&](auto& cur, auto& next) {
-      pin(cur);
-      all_read();  // every wavefront has read step s, and step s + 1 is looked up
-      read(s + 1, next);
-      step_places(s + 2);
-      write(s, cur);
-      return ++s < steps;
-    };
-    while (step(even, odd) && step(odd, even)) {
+    // steps whose rows stay where they are (of a sequence within its budget: all)
+    while (__syncthreads_or(set_places(s, slots_of(s, keep[index_of(s)]))) == 0)
+      if (++s == steps) return;
+    if (bad[s & 3] == 0) {
+      auto load = [&](int t, auto& v) {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) read(src[t & 3][first + j * stride], v[j]);
+      };
+      Slots ahead = slots_of(s + 1, keep[index_of(s + 1)]);
+      int from = keep[index_of(s + 2)];
+      load(s, even);
+      pin(even);
+      // (no load or store here depends on a branch, and a step ends where its rows are
+      // waited for: that wait then does not include the stores behind them)
+      auto step = [&](auto& cur, auto& next) {
+        set_places(s + 1, ahead);
+        lds_barrier();  // every wavefront has read step s
+        const bool go_on = bad[(s + 1) & 3] == 0;
+        if (go_on) {
+          ahead = slots_of(s + 2, from);
+          from = keep[index_of(s + 3)];
+          load(s + 1, next);
+        }
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) write(dst[s & 3][first + j * stride], cur[j]);
+        pin(next);
+        return ++s < steps && go_on;
+      };
+      while (step(even, odd) && step(odd, even)) {
+      }
+    }
+    for (; s < steps; ++s) {  // (tables that name places outside the pool)
+      __syncthreads();
+      set_places(s, slots_of(s, keep[index_of(s)]));
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int at = first + j * stride;
+        if (ok[at]) read(src[s & 3][at], even[j]);
+      }
+      pin(even);
+      all_read();
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        const int at = first + j * stride;
+        if (ok[at]) write(dst[s & 3][at], even[j]);
+      }
     }
   };
   if (part < k_parts) {
     u32x4 even[kKLoads], odd[kKLoads];
-    run(even, odd, read_k, write_k);
+    run(even, odd, tid / (kKDims / 8), kKPass, read_k, write_k);
   } else {
     uint32_t even[kVLoads], odd[kVLoads];
-    run(even, odd, read_v, write_v);
+    run(even, odd, tid % kVPass, kVPass, read_v, write_v);
   }
 }
 
