@@ -257,8 +257,10 @@ int voom_paged_gqa_tree(const void* q, const void* k_pool, const void* v_pool,
  *   keep       [batch, keep_heads, keep_tokens] int32 ascending, keep_heads 1 (one list
  *              for all heads: the accepted branch of a tree of drafts) or num_kv_heads
  *   dst_table  [batch, dst_pages]: the pages written.  block_table itself for a move in
- *              place, which needs keep[i] >= start + i; pages of their own (for prefixes
- *              that other sequences share); or a mix, page by page
+ *              place, which needs keep[i] >= start + i; pages that no list reads (for
+ *              prefixes that other sequences share); or a mix, page by page: the
+ *              sequence's own page at the same index, in a list that may move in place, or
+ *              one that no list reads.  No page for two sequences
  *   scores     [batch, num_kv_heads, score_tokens] or NULL: moved the same way into
  *              scores_out (the same array or another one), zero behind the last row
  * Rows whose position or slot id lies outside the tables and the pool are left out.

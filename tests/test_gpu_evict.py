@@ -339,7 +339,16 @@ def test_checked_lists_raise():
                             ("keep_lens", ([1, 2], 3)), ("in place", ([1, 2], 2, 2))):
             with pytest.raises(ValueError, match=match):
                 move(*args)
-        move([1, 2], 2, 2, table.clone())
+        other = torch.tensor([[1, 0]], dtype=torch.int32).cuda() if table[0, 0] == 0 else (
+            torch.tensor([[0, 1]], dtype=torch.int32).cuda())
+        assert (other != table).all()
+        for match, args in (("own pages", ([1, 2], 2, 2, table.clone())),
+                            ("read elsewhere", ([1, 40], 2, 0, other)),
+                            ("twice", ([1, 2, 3], 3, 31, other * 0 + 1 - table[0, 0]))):
+            with pytest.raises(ValueError, match=match):
+                move(*args)
+        move([1, 2], 2, 2, other)  # page 1 of the pool is not read
+        move([5, 6], 2, 2, table.clone())
     finally:
         ops.set_bounds_checks(False)
 

@@ -243,14 +243,19 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
 // stores behind them (16 x 8 heads, half of 4,096 tokens, from memory: 68 us, with stores
 // in the wait 79).
 //
+// A list that writes none of its own pages is moved in pieces by workgroups of their own,
+// as many as make kFull segments (8 heads, 8,192 of 32,768 tokens: 34 us, in one piece 52;
+// 4 x 8 heads, 4,096 of up to 16,384: 42 and 52, in four pieces 45).
+//
 // What bounds it: the kept rows read and written once; a V block is read in lines of
 // 32 tokens of a dim, whichever of them stay.  64 dims of K and 16 of V per workgroup,
-// since smaller pieces read lines of K more than once (the same: 68 against 75 us with
-// half of both); half of both where fewer than 64 segments leave CUs idle (8 heads, 7,000
-// of 8,192 tokens: 39 against 47 us; 4 x 8 heads, 4,096 of up to 16,384: 53 against 55).
+// since smaller pieces read lines of K more than once (16 x 8 heads, half of 4,096 tokens:
+// 68 against 75 us with half of both); half of both where fewer than kFull segments leave
+// CUs idle (in place; 8 heads, 7,000 of 8,192 tokens: 39 against 47 us).
 
 constexpr int kMoveThreads = 512;
 constexpr int kStep = 512;  // rows of a step
+constexpr int kFull = 64;   // segments that fill the card
 static_assert(kStep == kMoveThreads, "a thread looks one row up");
 
 constexpr uint32_t kNoRow = 0xffffffffu;
@@ -266,6 +271,7 @@ struct CompactArgs {
   const float* scores;       // [B, NKV, cap], or null
   float* scores_out;
   int NKV, D, keep_heads, n, cap, max_pages, dst_pages, pt_shift, num_slots;
+  int chunks, chunk_steps;  // pieces of a list that goes to other pages, and their steps
 };
 
 // Page of a position within a table of so many (clamped: what lies outside is not used).
@@ -363,19 +369,36 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactArgs a) {
   const int kvh = static_cast<int>(blockIdx.y);
   const int b = static_cast<int>(blockIdx.z);
   const int k_parts = (a.D + kKDims - 1) / kKDims, v_parts = a.D / kVDims;
-  const int part = static_cast<int>(blockIdx.x);
+  const int chunk = static_cast<int>(blockIdx.x) / (k_parts + v_parts);
+  const int part = static_cast<int>(blockIdx.x) - chunk * (k_parts + v_parts);
   const int32_t* keep = a.keep + (static_cast<size_t>(b) * a.keep_heads +
                                   (a.keep_heads == 1 ? 0 : kvh)) * a.n;
   int n = uniform(a.keep_lens[b]);
   n = n < 0 ? 0 : (n > a.n ? a.n : n);
   int start = a.start != nullptr ? uniform(a.start[b]) : 0;
   start = start < 0 ? 0 : start;
-  if (part == k_parts + v_parts) {
+  if (chunk == a.chunks) {
     move_scores<kMoveThreads>(a, keep, b, kvh, n, start);
     return;
   }
-  if (n == 0) return;
-  const int steps = (n + kStep - 1) / kStep;
+  const int32_t* trow = a.table + static_cast<size_t>(b) * a.max_pages;
+  const int32_t* drow = a.dst_table + static_cast<size_t>(b) * a.dst_pages;
+  int s = 0, steps = (n + kStep - 1) / kStep;  // the steps s .. steps are this workgroup's
+  if (a.chunks > 1) {
+    // a list that writes none of its own pages is moved in pieces, at the same time
+    bool own = false;
+    const long long to = start + static_cast<long long>(n) - 1;
+    for (long long p = (start >> a.pt_shift) + tid; p <= to >> a.pt_shift; p += kMoveThreads)
+      own |= p < a.max_pages && p < a.dst_pages && trow[p] == drow[p];
+    if (__syncthreads_or(own) == 0) {
+      s = chunk * a.chunk_steps;
+      steps = min(steps, s + a.chunk_steps);
+      n = min(n, steps * kStep);
+    } else if (chunk != 0) {
+      return;
+    }
+  }
+  if (s >= steps) return;
 
   constexpr int kKPass = kMoveThreads / (kKDims / 8), kVPass = kMoveThreads / kVDims;
   constexpr int kKLoads = kStep / kKPass, kVLoads = kStep / kVPass;
@@ -383,8 +406,6 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactArgs a) {
   kc = kc < a.D ? kc : a.D - 8;  // (moved twice, the same values)
   const int vb = a.pt_shift < 5 ? a.pt_shift : 5;
   const int vd = (part - k_parts) * kVDims + tid / kVPass;
-  const int32_t* trow = a.table + static_cast<size_t>(b) * a.max_pages;
-  const int32_t* drow = a.dst_table + static_cast<size_t>(b) * a.dst_pages;
   // Row tid of step s (past the last one: that one again, the same values).
   auto index_of = [&](int s) {
     const int i = s * kStep + tid;
@@ -428,7 +449,6 @@ __global__ __launch_bounds__(kMoveThreads) void compact_kernel(CompactArgs a) {
     constexpr int kLoads = sizeof(even) / sizeof(even[0]);
     if (tid < 4) bad[tid] = 0;
     __syncthreads();
-    int s = 0;
     // steps whose rows stay where they are (of a sequence within its budget: all)
     while (__syncthreads_or(set_places(s, slots_of(s, keep[index_of(s)]))) == 0)
       if (++s == steps) return;
@@ -637,11 +657,16 @@ extern "C" int voom_compact_kv(void* k_pool, void* v_pool, const int32_t* block_
     hipLaunchKernelGGL(compact_few_kernel, grid, dim3(kMoveThreads), 0, stream, a);
   } else {
     const long long segs = static_cast<long long>(batch) * num_kv_heads;
+    const int steps = (keep_tokens + kStep - 1) / kStep;
+    const int pieces = dst_table == block_table || segs >= kFull
+                           ? 1 : static_cast<int>((kFull + segs - 1) / segs);
+    a.chunk_steps = (steps + pieces - 1) / pieces;
+    a.chunks = (steps + a.chunk_steps - 1) / a.chunk_steps;
     const auto launch = [&](auto kernel, int k_dims, int v_dims) {
-      grid.x = (head_dim + k_dims - 1) / k_dims + head_dim / v_dims + moves_scores;
+      grid.x = ((head_dim + k_dims - 1) / k_dims + head_dim / v_dims) * a.chunks + moves_scores;
       hipLaunchKernelGGL(kernel, grid, dim3(kMoveThreads), 0, stream, a);
     };
-    if (segs >= 64) launch(compact_kernel<64, 16>, 64, 16);
+    if (segs * a.chunks >= kFull) launch(compact_kernel<64, 16>, 64, 16);
     else launch(compact_kernel<32, 8>, 32, 8);
   }
   return VOOM_LAUNCH_CHECK("compact_kv: launch");

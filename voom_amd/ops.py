@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes
 import os
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -507,6 +508,33 @@ def check_keep(keep: torch.Tensor, keep_lens: torch.Tensor, tokens: int,
         raise ValueError("a move in place needs keep[i] >= start + i")
 
 
+def check_destination(block_table: torch.Tensor, dst_table: torch.Tensor, keep: torch.Tensor,
+                      keep_lens: torch.Tensor, start: torch.Tensor | None, page: int) -> None:
+    """Raise ValueError where a move to ``dst_table`` writes a page that it also reads, or one
+    page for two sequences.  A sequence's own page at the same index may be written, as in
+    place: with keep[i] >= start + i throughout the list."""
+    table, dst = block_table.cpu().numpy(), dst_table.cpu().numpy()
+    lists, lens = keep.cpu().numpy(), keep_lens.cpu().numpy()
+    first = np.zeros(len(lens), np.int64) if start is None else start.cpu().numpy()
+    reads, writes = {}, {}  # slot -> the (sequence, index) that read it; the one that writes it
+    for b, n in enumerate(lens):
+        for p in np.unique(lists[b, :, :n] // page):
+            reads.setdefault(int(table[b, p]), set()).add((b, int(p)))
+    for b, n in enumerate(lens):
+        if n <= 0:
+            continue
+        for p in range(int(first[b]) // page, min((int(first[b]) + int(n) - 1) // page + 1,
+                                                  dst.shape[1])):
+            slot = int(dst[b, p])
+            if writes.setdefault(slot, (b, p)) != (b, p):
+                raise ValueError(f"dst_table names page {slot} twice")
+            if reads.get(slot, set()) - {(b, p)}:
+                raise ValueError(f"dst_table names page {slot}, which is read elsewhere")
+            if p < table.shape[1] and slot == table[b, p]:
+                if (lists[b, :, :n] < first[b] + np.arange(n)).any():
+                    raise ValueError("a move to own pages needs keep[i] >= start + i")
+
+
 def compact_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
                keep: torch.Tensor, keep_lens: torch.Tensor, *, start: torch.Tensor | None = None,
                dst_table: torch.Tensor | None = None, scores: torch.Tensor | None = None,
@@ -518,8 +546,9 @@ def compact_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Te
     positions per head (evict_select's), or [B, 1, n] one list for all heads (the
     accepted branch of a tree of drafts).  In place (``dst_table`` None) keep[b, h, i] must
     be at least start[b] + i; ``dst_table`` [B, pages] int32 names other pages to write, for
-    those that sequences share: a page of it is either the sequence's own page at the same
-    index or one that block_table does not hold.
+    those that sequences share: a page of it is either one that block_table does not hold,
+    or the sequence's own page at the same index (a list with such pages needs keep[b, h, i]
+    >= start[b] + i as well).
 
     ``scores`` [B, NKV, tokens] fp32 moves along into ``scores_out`` (default: in place);
     behind the last row kept it becomes 0.
@@ -563,6 +592,8 @@ def compact_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Te
         return
     if _BOUNDS_CHECKS:
         check_keep(keep, keep_lens, block_table.shape[1] * PT, start, in_place)
+        if not in_place:
+            check_destination(block_table, dst_table, keep, keep_lens, start, PT)
     if n == 0:  # only scores to clear
         keep, keep_lens, n = keep.new_zeros((B, 1, 1)), torch.zeros_like(keep_lens), 1
     rc = _lib.lib().voom_compact_kv(
