@@ -250,6 +250,11 @@ int voom_paged_gqa_tree(const void* q, const void* k_pool, const void* v_pool,
  * a NaN below every number.
  *   keep       [batch, num_kv_heads, budget] int32, ascending, -1 behind keep_lens[b]
  *   keep_lens  [batch] int32: min(ctx, budget)
+ * voom_evict_select_split is the same with a workspace of
+ * voom_evict_select_workspace_bytes (16-byte aligned, contents of no matter; calls that
+ * overlap need one each): up to 64 rows of more than 32,768 scores then go over several
+ * workgroups each and four launches.  NULL, and where 0 bytes are asked for: one
+ * workgroup per row.
  *
  * voom_compact_kv moves the rows that stay: position start[b] + i (NULL: i) of every
  * kv head takes the K and V of position keep[b][h][i], i < keep_lens[b], of its own
@@ -274,6 +279,11 @@ int voom_paged_gqa_observe(const void* q, const float* lse, const void* k_pool,
 int voom_evict_select(const float* scores, const int32_t* ctx_lens, int32_t* keep,
                       int32_t* keep_lens, int batch, int num_kv_heads, int score_tokens, int budget,
                       int sink, int recent, hipStream_t stream);
+size_t voom_evict_select_workspace_bytes(int batch, int num_kv_heads, int score_tokens);
+int voom_evict_select_split(const float* scores, const int32_t* ctx_lens, int32_t* keep,
+                            int32_t* keep_lens, void* workspace, size_t ws_bytes, int batch,
+                            int num_kv_heads, int score_tokens, int budget, int sink, int recent,
+                            hipStream_t stream);
 int voom_compact_kv(void* k_pool, void* v_pool, const int32_t* block_table,
                     const int32_t* dst_table, const int32_t* keep, const int32_t* keep_lens,
                     const int32_t* start, const float* scores, float* scores_out, int batch,

@@ -198,6 +198,69 @@ def test_selection_is_exact(name, cap, ctx, budget, sink, recent):
     assert np.array_equal(keep.cpu().numpy(), want)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["ties", "odd", "equal"])
+@pytest.mark.parametrize("B,NKV,cap,budget,sink,recent", [
+    (33, 2, 40000, 5000, 4, 100),      # more long rows than are cut into pieces
+    (1, 2, 1048576, 65536, 4, 1000),   # as many pieces as a row is cut into
+    (1, 1, 1048577, 3, 1, 1),          # one token more
+    (1, 3, 32769, 32000, 16000, 16000),  # nothing to choose
+    (2, 1, 50000, 49999, 0, 0),        # all but one
+])
+def test_long_rows(name, B, NKV, cap, budget, sink, recent):
+    print(f"[select] {name} B={B} cap={cap} budget={budget}", flush=True)
+    rng = np.random.default_rng(cap)
+    s = select_case(name, rng, B, NKV, cap)
+    ctx = [cap - (17 * b) % cap for b in range(B)]
+    scores, lens = torch.from_numpy(s).cuda(), lens_tensor(ctx)
+    keep, counts = ops.evict_select(scores, lens, budget, sink=sink, recent=recent)
+    one = torch.empty_like(keep)  # the same by one workgroup per row
+    assert _lib.lib().voom_evict_select(scores.data_ptr(), lens.data_ptr(), one.data_ptr(),
+                                        counts.data_ptr(), B, NKV, cap, budget, sink, recent,
+                                        0) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(keep, one)
+    for b in range(B):
+        assert int(counts[b]) == min(ctx[b], budget)
+        for h in range(NKV):
+            x = s[b, h, sink:ctx[b] - recent].astype(np.float64)
+            lowest = np.isnan(x)
+            x[lowest] = -np.inf
+            order = np.lexsort((np.arange(len(x)), -x, lowest))[:budget - sink - recent]
+            want = np.sort(np.concatenate([np.arange(sink), order + sink,
+                                           np.arange(ctx[b] - recent, ctx[b])]))
+            want = want if ctx[b] > budget else np.arange(ctx[b])
+            got = keep[b, h].cpu().numpy()
+            assert np.array_equal(got[:len(want)], want) and (got[len(want):] == -1).all()
+
+
+@pytest.mark.gpu
+def test_long_rows_in_a_graph_and_on_two_streams():
+    """Each call has a workspace of its own."""
+    print("[select] long rows replayed and on two streams", flush=True)
+    scores = [torch.rand((1, 4, 70000), device="cuda") ** 3 for _ in range(2)]
+    ctx = lens_tensor([70000])
+    want = [ops.evict_select(s, ctx, 4000, sink=4, recent=64)[0] for s in scores]
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for s, stream in zip(scores, side):
+            with torch.cuda.stream(stream):
+                got.append(ops.evict_select(s, ctx, 4000, sink=4, recent=64)[0])
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    live = scores[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        keep, _ = ops.evict_select(live, ctx, 4000, sink=4, recent=64)
+    for i in (0, 1, 0, 1):
+        live.copy_(scores[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(keep, want[i])
+
+
 # ---- the move -----------------------------------------------------------------------
 
 
@@ -491,3 +554,17 @@ def test_abi_refusals():
     refused("lists", compact(heads=3))
     refused("scores", compact(scores=p))
     refused("scores", compact(scores=p, out=p, cap=0))
+
+
+def test_abi_refusals_of_workspaces_of_long_rows():
+    lib, p = _lib.lib(), 1 << 20
+    need = lib.voom_evict_select_workspace_bytes(2, 8, 100000)
+    assert need > 0 and lib.voom_evict_select_workspace_bytes(2, 8, 200000) > need
+    for args in ((2, 8, 32768), (9, 8, 100000), (1, 1, (1 << 20) + 1), (0, 8, 100000)):
+        assert lib.voom_evict_select_workspace_bytes(*args) == 0
+    for ws, size in ((p, need - 1), (p + 4, need)):
+        assert lib.voom_evict_select_split(p, p, p, p, ws, size, 2, 8, 100000, 100, 4, 4,
+                                           None) == _lib.VOOM_EINVAL
+        assert "workspace" in _lib.last_error()
+    assert lib.voom_evict_select_split(p, p, p, p, p, need, 2, 8, 100000, 4, 4, 4,
+                                       None) == _lib.VOOM_EINVAL

@@ -47,6 +47,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                     c_float, _P]),
     "voom_paged_gqa_observe": (c_int, [_P] * 8 + [c_int] * 9 + [c_float, _P]),
     "voom_evict_select": (c_int, [_P] * 4 + [c_int] * 6 + [_P]),
+    "voom_evict_select_workspace_bytes": (c_size_t, [c_int] * 3),
+    "voom_evict_select_split": (c_int, [_P] * 5 + [c_size_t] + [c_int] * 6 + [_P]),
     "voom_compact_kv": (c_int, [_P] * 9 + [c_int] * 10 + [_P]),
     "voom_qk_norm_rope_append": (c_int, [_P, _P, _P, c_float, _P, _P, c_int, c_int, c_int]
                                  + [_P] * 7 + [c_int] * 8 + [_P]),

@@ -19,8 +19,7 @@ namespace {
 // workgroup per (sequence, head).  Up to 32,768 candidates stay in registers, all loads
 // in flight at once (a loop that loaded them for every pass: 43 us for 16 x 8 heads of
 // up to 32,768 tokens, where this takes 20); of longer ones every pass loads 32,768 at a
-// time (8 heads of 131,072: 66 us; with 49,152 at a time, some of them spilled, 76, and
-// 50 against 36 at 65,536, though 29 against 34 at 49,000).  Each histogram of a long row
+// time (64 heads of 131,072: 65 us; with 49,152 at a time, some of them spilled, 76).  Each histogram of a long row
 // has eight copies, by lane: scores share their leading bits, and atomics of one wavefront
 // on one address take turns.  The second and third pass look only at the keys that share
 // the first digit, from a list in LDS where it holds them.
@@ -43,6 +42,127 @@ __device__ __forceinline__ int before_wave(const int* tot, int wv, int lane, int
   all = __builtin_amdgcn_readlane(x, kWave - 1);
   return wv == 0 ? 0 : __builtin_amdgcn_readlane(x, wv - 1);
 }
+
+// Which bin of a histogram holds the need-th largest key.  Thread t holds, in `mine`, bins
+// t per .. of the descending order, per = bins / THREADS.
+template <int THREADS>
+__device__ __forceinline__ void find_digit(const int (&mine)[kBins / THREADS], int bins, int need,
+                                           int* part, int* found) {
+  const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & (kWave - 1);
+  const int wv = uniform(tid / kWave);
+  constexpr int kPer = kBins / THREADS;
+  const int per = bins / THREADS;
+  int sum = 0;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) sum += mine[j];
+  const int x = wave_inclusive_scan(sum, lane);
+  if (lane == kWave - 1) part[wv] = x;
+  __syncthreads();
+  int all;
+  int before = before_wave<THREADS / kWave>(part, wv, lane, all) + x - sum;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (j < per && before < need && before + mine[j] >= need) {
+      found[0] = bins - 1 - (tid * per + j);
+      found[1] = before;
+      found[2] = mine[j];
+    }
+    before += mine[j];
+  }
+  __syncthreads();
+}
+
+// Writes the positions of the candidates in registers that stay: of those equal to
+// `prefix`, the n-th largest key, the first `need`, mostly all of them (all_equal).  Each
+// wavefront counts what its run of the candidates keeps, and writes behind the runs before
+// it; at, same: how many were kept, and (where not all stay) equal to the key, before.
+template <int THREADS, int E>
+__device__ __forceinline__ void write_kept(uint32_t (&key)[E], int first, int count,
+                                           uint32_t prefix, int need, bool all_equal, int sink,
+                                           int32_t* out, int* kept_tot, int* equal_tot, int& at,
+                                           int& same) {
+  constexpr int kWaves = THREADS / kWave;
+  const int lane = static_cast<int>(threadIdx.x) & (kWave - 1);
+  const int wv = uniform(static_cast<int>(threadIdx.x) / kWave);
+  int kept = 0, equal = 0;
+  if (all_equal) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) kept += __popcll(__builtin_amdgcn_ballot_w64(key[e] >= prefix));
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      kept += __popcll(__builtin_amdgcn_ballot_w64(key[e] > prefix));
+      equal +=
+          __popcll(__builtin_amdgcn_ballot_w64(key[e] == prefix && first + e * kWave < count));
+    }
+  }
+  // (keeps the compiler from holding two lane masks per element until below)
+#pragma unroll
+  for (int e = 0; e < E; ++e) asm volatile("" : "+v"(key[e]));
+  __syncthreads();  // the totals of the call before are read
+  if (lane == 0) {
+    kept_tot[wv] = kept;
+    equal_tot[wv] = equal;
+  }
+  __syncthreads();
+  int kept_all, equal_all;
+  int run_at = at + before_wave<kWaves>(kept_tot, wv, lane, kept_all);
+  int run_same = same + before_wave<kWaves>(equal_tot, wv, lane, equal_all);
+  at += kept_all;
+  same += equal_all;
+  if (all_equal) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const uint64_t up = __builtin_amdgcn_ballot_w64(key[e] >= prefix);
+      if (key[e] >= prefix)
+        out[sink + run_at +
+            __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(up >> 32),
+                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(up), 0))] =
+            sink + first + e * kWave;
+      run_at += __popcll(up);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const bool same_key = key[e] == prefix && first + e * kWave < count;
+      const uint64_t up = __builtin_amdgcn_ballot_w64(key[e] > prefix);
+      const uint64_t eq = __builtin_amdgcn_ballot_w64(same_key);
+      const uint64_t low = (1ull << lane) - 1;
+      const int eq_before = run_same + __popcll(eq & low);
+      if (key[e] > prefix || (same_key && eq_before < need)) {
+        const int eq_kept = eq_before < need ? eq_before : need;
+        out[sink + run_at + __popcll(up & low) + eq_kept] = sink + first + e * kWave;
+      }
+      run_at += __popcll(up);
+      run_same += __popcll(eq);
+    }
+  }
+}
+
+// This thread's keys of the candidates from `first` on, 64 apart, 0 past the last one.
+template <int E>
+__device__ __forceinline__ void load_keys(const float* s, int first, int count,
+                                          uint32_t (&key)[E]) {
+  // (candidates past the last one load 0: the whole offset is in the part of the address
+  // that is checked)
+  const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<float*>(s), static_cast<short>(0), count * 4u, 0x00020000);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    key[e] = __builtin_amdgcn_raw_buffer_load_b32(from, (first + e * kWave) * 4u, 0, 0);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const uint32_t k = order_key(__builtin_bit_cast(float, key[e]));
+    key[e] = first + e * kWave < count ? k : 0u;
+  }
+}
+
+// The digits of a key from the highest on, 11, 11 and 10 bits.
+__device__ __forceinline__ int digit_shift(int pass) {
+  return pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+}
+__device__ __forceinline__ int digit_bins(int pass) { return pass == 2 ? 1024 : 2048; }
 
 // E: candidates per thread and round.  Round c, wavefront w, element e, lane l hold
 // candidate ((c * waves + w) * E + e) * 64 + l; past the last one the key is 0.
@@ -78,22 +198,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
   const int rounds = (count + kSelThreads * E - 1) / (kSelThreads * E);
 
   uint32_t key[E];
-  // (candidates past the last one load 0: the whole offset is in the part of the address
-  // that is checked)
-  const __amdgpu_buffer_rsrc_t from = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<float*>(s), static_cast<short>(0), count * 4u, 0x00020000);
   auto first_of = [&](int c) { return (c * kSelWaves + wv) * (E * kWave) + lane; };
-  auto load = [&](int c) {
-    const int first = first_of(c);
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      key[e] = __builtin_amdgcn_raw_buffer_load_b32(from, (first + e * kWave) * 4u, 0, 0);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint32_t k = order_key(__builtin_bit_cast(float, key[e]));
-      key[e] = first + e * kWave < count ? k : 0u;
-    }
-  };
+  auto load = [&](int c) { load_keys<E>(s, first_of(c), count, key); };
   if (n != 0) load(0);
   for (int i = tid; i < sink; i += kSelThreads) out[i] = i;
   for (int i = tid; i < recent; i += kSelThreads) out[budget - recent + i] = ctx - recent + i;
@@ -104,8 +210,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
   bool short_list = false;        // those keys are in `list`
   if (tid == 0) listed = 0;
   for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
-    const int bins = pass == 2 ? 1024 : 2048;
+    const int shift = digit_shift(pass), bins = digit_bins(pass);
     for (int i = tid; i < kBins * COPIES; i += kSelThreads) (&hist[0][0])[i] = 0;
     __syncthreads();
     if (short_list) {
@@ -126,7 +231,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     // thread t owns bins t * per .. of the descending order
     constexpr int kPer = kBins / kSelThreads;
     const int per = bins / kSelThreads;
-    int mine[kPer] = {}, sum = 0;
+    int mine[kPer] = {};
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       if (j < per) {
@@ -134,23 +239,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
 #pragma unroll
         for (int k = 0; k < COPIES; ++k) mine[j] += h[k];
       }
-      sum += mine[j];
     }
-    const int x = wave_inclusive_scan(sum, lane);
-    if (lane == kWave - 1) part[wv] = x;
-    __syncthreads();
-    int all;
-    int before = before_wave<kSelWaves>(part, wv, lane, all) + x - sum;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      if (j < per && before < need && before + mine[j] >= need) {
-        found[0] = bins - 1 - (tid * per + j);
-        found[1] = before;
-        found[2] = mine[j];
-      }
-      before += mine[j];
-    }
-    __syncthreads();
+    find_digit<kSelThreads>(mine, bins, need, part, found);
     prefix |= static_cast<uint32_t>(found[0]) << shift;
     mask |= static_cast<uint32_t>(bins - 1) << shift;
     need -= found[1];
@@ -166,66 +256,173 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     }
   }
 
-  // `prefix` is the n-th largest key; `need` of those equal to it stay, mostly all of
-  // them.  Each wavefront counts what its run of the candidates keeps, and writes behind
-  // the runs before it.
   const bool all_equal = prefix != 0 && need == found[2];
-  int at = 0, same = 0;  // kept, and (where not all stay) equal to the key, before the run
+  int at = 0, same = 0;
   for (int c = 0; c < rounds; ++c) {
     if (rounds > 1) load(c);
-    const int first = first_of(c);
-    int kept = 0, equal = 0;
-    if (all_equal) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) kept += __popcll(__builtin_amdgcn_ballot_w64(key[e] >= prefix));
+    write_kept<kSelThreads, E>(key, first_of(c), count, prefix, need, all_equal, sink, out,
+                               kept_tot, equal_tot, at, same);
+  }
+}
+
+// Few rows of more than kRowMost scores: a workgroup takes a piece of kPiece candidates,
+// and the row goes through four launches.  Pass 0, 1 and 2 count a digit of the piece's
+// keys, and pass 1, 2 and 3 find the one before from all pieces' counts; pass 3 writes,
+// behind what the pieces before it keep.  8 rows of 131,072: 28 us, 64 for one workgroup per
+// row; 64 rows: 54 and 65; 128 rows of 65,536, which fill the card by themselves, 46 and 38;
+// 8 rows of 36,000: 22 and 34.
+constexpr int kSplitThreads = 1024;
+constexpr int kSplitE = 16;
+constexpr int kPiece = kSplitThreads * kSplitE;
+constexpr int kRowMost = 32 * 1024;
+constexpr int kMostPieces = 64;  // (each workgroup adds up the counts of all)
+constexpr int kFewSplit = 64;    // rows
+
+// A row's part of the workspace.
+struct SplitRow {
+  int* hist;   // [3][pieces][kBins]
+  int* above;  // [2][pieces]: a piece's keys above the digit, of those that share the digits before
+  int* found;  // [2][2]: the digit, and how many keys of the row lie above it
+  __device__ __forceinline__ SplitRow(int* ws, int row, int pieces) {
+    hist = ws + static_cast<size_t>(row) * ints(pieces);
+    above = hist + 3 * pieces * kBins;
+    found = above + 2 * pieces;
+  }
+  __host__ __device__ static constexpr size_t ints(int pieces) {
+    return static_cast<size_t>(3) * pieces * kBins + 2 * pieces + 4;
+  }
+};
+
+template <int PASS>
+__global__ __launch_bounds__(kSplitThreads) void evict_split_kernel(
+    const float* __restrict__ scores, const int32_t* __restrict__ ctx_lens,
+    int32_t* __restrict__ keep, int32_t* __restrict__ keep_lens, int* __restrict__ ws, int NKV,
+    int cap, int budget, int sink, int recent, int pieces) {
+  constexpr int kWaves = kSplitThreads / kWave, kCopies = 8;
+  __shared__ __attribute__((aligned(16))) int hist[PASS < 3 ? kBins : 1][kCopies];
+  __shared__ int part[kWaves], kept_tot[kWaves], equal_tot[kWaves];
+  __shared__ int found[3];
+  const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & (kWave - 1);
+  const int wv = uniform(tid / kWave);
+  const int piece = static_cast<int>(blockIdx.x);
+  const int row = static_cast<int>(blockIdx.y);
+  const int b = row / NKV;
+  int ctx = uniform(ctx_lens[b]);
+  ctx = ctx < 0 ? 0 : (ctx > cap ? cap : ctx);
+  int32_t* out = keep + static_cast<size_t>(row) * budget;
+  const int n = budget - sink - recent;
+  if (PASS == 0) {  // what needs no choice
+    const int at = piece * kSplitThreads + tid, step = pieces * kSplitThreads;
+    if (row == b * NKV && at == 0) keep_lens[b] = ctx < budget ? ctx : budget;
+    if (ctx <= budget) {
+      for (int i = at; i < budget; i += step) out[i] = i < ctx ? i : -1;
     } else {
+      for (int i = at; i < sink; i += step) out[i] = i;
+      for (int i = at; i < recent; i += step) out[budget - recent + i] = ctx - recent + i;
+    }
+  }
+  if (ctx <= budget || n == 0) return;
+  const float* s = scores + static_cast<size_t>(row) * cap + sink;
+  const int count = ctx - recent - sink;  // candidates, more than n
+  const int used = (count + kPiece - 1) / kPiece;
+  if (piece >= used) return;
+  uint32_t key[kSplitE];
+  const int first = (piece * kWaves + wv) * (kSplitE * kWave) + lane;
+  load_keys<kSplitE>(s, first, count, key);
+  const SplitRow w(ws, row, pieces);
+
+  uint32_t prefix = 0, mask = 0;
+  int need = n;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        kept += __popcll(__builtin_amdgcn_ballot_w64(key[e] > prefix));
-        equal += __popcll(
-            __builtin_amdgcn_ballot_w64(key[e] == prefix && first + e * kWave < count));
+  for (int p = 0; p + 1 < PASS; ++p) {
+    prefix |= static_cast<uint32_t>(uniform(w.found[2 * p])) << digit_shift(p);
+    mask |= static_cast<uint32_t>(digit_bins(p) - 1) << digit_shift(p);
+    need -= uniform(w.found[2 * p + 1]);
+  }
+  int at = 0, same = 0;  // in the pieces before this one: kept, and equal to the key
+  bool all_equal = false;
+  if constexpr (PASS > 0) {
+    constexpr int kPer = kBins / kSplitThreads;
+    constexpr int p = PASS - 1;
+    const int bins = digit_bins(p), per = bins / kSplitThreads;
+    const int* counts = w.hist + static_cast<size_t>(p) * pieces * kBins;
+    int mine[kPer] = {}, before[kPer] = {}, here[kPer] = {};
+    const int low = bins - per * (tid + 1);  // this thread's bins, ascending
+    for (int c = 0; c < used; ++c) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        if (j < per) {
+          const int v = counts[c * kBins + low + per - 1 - j];
+          mine[j] += v;
+          before[j] += c < piece ? v : 0;
+          here[j] = c == piece ? v : here[j];
+        }
       }
     }
-    // (keeps the compiler from holding two lane masks per element until below)
+    find_digit<kSplitThreads>(mine, bins, need, part, found);
+    const int digit = found[0];
+    prefix |= static_cast<uint32_t>(digit) << digit_shift(p);
+    mask |= static_cast<uint32_t>(bins - 1) << digit_shift(p);
+    need -= found[1];
+    // sums over the bins above the digit: of this piece, for pass 3; there, of those before
+    int up = 0, eq = 0;
 #pragma unroll
-    for (int e = 0; e < E; ++e) asm volatile("" : "+v"(key[e]));
-    __syncthreads();  // the totals of the round before are read
-    if (lane == 0) {
-      kept_tot[wv] = kept;
-      equal_tot[wv] = equal;
+    for (int j = 0; j < kPer; ++j) {
+      const int bin = low + per - 1 - j;
+      if (j < per) {
+        up += bin > digit ? (PASS == 3 ? before[j] : here[j]) : 0;
+        eq += bin == digit ? before[j] : 0;
+      }
+    }
+    up = wave_inclusive_scan(up, lane);
+    eq = wave_inclusive_scan(eq, lane);
+    if (lane == kWave - 1) {
+      kept_tot[wv] = up;
+      equal_tot[wv] = eq;
     }
     __syncthreads();
-    int kept_all, equal_all;
-    int run_at = at + before_wave<kSelWaves>(kept_tot, wv, lane, kept_all);
-    int run_same = same + before_wave<kSelWaves>(equal_tot, wv, lane, equal_all);
-    at += kept_all;
-    same += equal_all;
-    if (all_equal) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const uint64_t up = __builtin_amdgcn_ballot_w64(key[e] >= prefix);
-        if (key[e] >= prefix)
-          out[sink + run_at + __builtin_amdgcn_mbcnt_hi(
-                                  static_cast<uint32_t>(up >> 32),
-                                  __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(up), 0))] =
-              sink + first + e * kWave;
-        run_at += __popcll(up);
+    int up_all, eq_all;
+    before_wave<kWaves>(kept_tot, wv, lane, up_all);
+    before_wave<kWaves>(equal_tot, wv, lane, eq_all);
+    if constexpr (PASS < 3) {
+      if (tid == 0) {
+        w.above[p * pieces + piece] = up_all;
+        if (piece == 0) {
+          w.found[2 * p] = digit;
+          w.found[2 * p + 1] = found[1];
+        }
       }
     } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const bool same_key = key[e] == prefix && first + e * kWave < count;
-        const uint64_t up = __builtin_amdgcn_ballot_w64(key[e] > prefix);
-        const uint64_t eq = __builtin_amdgcn_ballot_w64(same_key);
-        const uint64_t low = (1ull << lane) - 1;
-        const int eq_before = run_same + __popcll(eq & low);
-        if (key[e] > prefix || (same_key && eq_before < need)) {
-          const int eq_kept = eq_before < need ? eq_before : need;
-          out[sink + run_at + __popcll(up & low) + eq_kept] = sink + first + e * kWave;
-        }
-        run_at += __popcll(up);
-        run_same += __popcll(eq);
+      all_equal = prefix != 0 && need == found[2];
+      at = up_all;
+      same = eq_all;
+      for (int c = 0; c < piece; ++c) at += w.above[c] + w.above[pieces + c];
+      if (all_equal) {  // (then they count as kept)
+        at += same;
+        same = 0;
       }
+    }
+  }
+  if constexpr (PASS == 3) {
+    write_kept<kSplitThreads, kSplitE>(key, first, count, prefix, need, all_equal, sink, out,
+                                       kept_tot, equal_tot, at, same);
+  } else {
+    const int shift = digit_shift(PASS), bins = digit_bins(PASS);
+    for (int i = tid; i < bins * kCopies; i += kSplitThreads) (&hist[0][0])[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kSplitE; ++e) {
+      if (first + e * kWave < count && (key[e] & mask) == prefix)
+        atomicAdd(&hist[(key[e] >> shift) & (bins - 1)][lane % kCopies], 1);
+    }
+    __syncthreads();
+    int* counts = w.hist + (static_cast<size_t>(PASS) * pieces + piece) * kBins;
+    for (int i = tid; i < bins; i += kSplitThreads) {
+      int sum = 0;
+#pragma unroll
+      for (int k = 0; k < kCopies; ++k) sum += hist[i][k];
+      counts[i] = sum;
     }
   }
 }
@@ -579,19 +776,68 @@ __global__ __launch_bounds__(kMoveThreads) void compact_few_kernel(CompactArgs a
 
 using namespace voom;
 
+namespace {
+
+// Pieces of a row in a call, 0: one workgroup takes the row.
+int split_pieces(long long rows, int score_tokens) {
+  const int pieces = (score_tokens + kPiece - 1) / kPiece;
+  return score_tokens > kRowMost && pieces <= kMostPieces && rows <= kFewSplit ? pieces : 0;
+}
+
+bool select_shape_ok(int batch, int num_kv_heads, int score_tokens) {
+  return batch > 0 && num_kv_heads > 0 && score_tokens > 0 && score_tokens < (1 << 30) &&
+         static_cast<long long>(batch) * num_kv_heads < (1LL << 30);
+}
+
+}  // namespace
+
+extern "C" size_t voom_evict_select_workspace_bytes(int batch, int num_kv_heads,
+                                                    int score_tokens) {
+  if (!select_shape_ok(batch, num_kv_heads, score_tokens)) return 0;
+  const long long rows = static_cast<long long>(batch) * num_kv_heads;
+  const int pieces = split_pieces(rows, score_tokens);
+  return pieces == 0 ? 0 : rows * SplitRow::ints(pieces) * sizeof(int);
+}
+
 extern "C" int voom_evict_select(const float* scores, const int32_t* ctx_lens, int32_t* keep,
                                  int32_t* keep_lens, int batch, int num_kv_heads,
                                  int score_tokens, int budget, int sink, int recent,
                                  hipStream_t stream) {
+  return voom_evict_select_split(scores, ctx_lens, keep, keep_lens, nullptr, 0, batch,
+                                 num_kv_heads, score_tokens, budget, sink, recent, stream);
+}
+
+extern "C" int voom_evict_select_split(const float* scores, const int32_t* ctx_lens,
+                                       int32_t* keep, int32_t* keep_lens, void* workspace,
+                                       size_t ws_bytes, int batch, int num_kv_heads,
+                                       int score_tokens, int budget, int sink, int recent,
+                                       hipStream_t stream) {
   const char* who = "evict_select";
   VOOM_REQUIRE(scores && ctx_lens && keep && keep_lens, "%s: null pointer argument", who);
-  VOOM_REQUIRE(batch > 0 && num_kv_heads > 0 && score_tokens > 0 &&
-                   score_tokens < (1 << 30) &&
-                   static_cast<long long>(batch) * num_kv_heads < (1LL << 30),
+  VOOM_REQUIRE(select_shape_ok(batch, num_kv_heads, score_tokens),
                "%s: unsupported geometry (batch %d, %d kv heads, %d tokens)", who, batch,
                num_kv_heads, score_tokens);
   VOOM_REQUIRE(budget > 0 && sink >= 0 && recent >= 0 && sink <= budget && recent <= budget - sink,
                "%s: sink %d and recent %d must fit the budget %d", who, sink, recent, budget);
+  const size_t need = voom_evict_select_workspace_bytes(batch, num_kv_heads, score_tokens);
+  if (workspace != nullptr && need != 0) {
+    VOOM_REQUIRE(ws_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+                 "%s: workspace %zu bytes < required %zu (16-byte aligned)", who, ws_bytes, need);
+    const int pieces = split_pieces(static_cast<long long>(batch) * num_kv_heads, score_tokens);
+    const auto pass = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel,
+                         dim3(static_cast<unsigned>(pieces),
+                              static_cast<unsigned>(batch * num_kv_heads)),
+                         dim3(kSplitThreads), 0, stream, scores, ctx_lens, keep, keep_lens,
+                         static_cast<int*>(workspace), num_kv_heads, score_tokens, budget, sink,
+                         recent, pieces);
+    };
+    pass(evict_split_kernel<0>);
+    pass(evict_split_kernel<1>);
+    pass(evict_split_kernel<2>);
+    pass(evict_split_kernel<3>);
+    return VOOM_LAUNCH_CHECK("evict_select: launch");
+  }
   const auto launch = [&](auto kernel, int threads) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(batch * num_kv_heads)), dim3(threads), 0,
                        stream, scores, ctx_lens, keep, keep_lens, num_kv_heads, score_tokens,

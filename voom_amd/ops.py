@@ -480,9 +480,12 @@ def evict_select(scores: torch.Tensor, ctx_lens: torch.Tensor, budget: int, *, s
     keep = ctx_lens.new_empty((B, NKV, budget))
     keep_lens = ctx_lens.new_empty((B,))
     if B and NKV:
-        rc = _lib.lib().voom_evict_select(
-            scores.data_ptr(), ctx_lens.data_ptr(), keep.data_ptr(), keep_lens.data_ptr(), B, NKV,
-            cap, budget, sink, recent, _stream(None))
+        lib = _lib.lib()
+        need = lib.voom_evict_select_workspace_bytes(B, NKV, cap) if cap > 32768 else 0
+        ws = scores.new_empty(need, dtype=torch.uint8) if need else None
+        rc = lib.voom_evict_select_split(
+            scores.data_ptr(), ctx_lens.data_ptr(), keep.data_ptr(), keep_lens.data_ptr(), _ptr(ws),
+            need, B, NKV, cap, budget, sink, recent, _stream(None))
         if rc:
             _lib.check(rc, "voom_evict_select")
     return keep, keep_lens
