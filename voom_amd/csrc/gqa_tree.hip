@@ -15,17 +15,19 @@
 // Work decomposition.  A workgroup takes 64 rows (128 where there are more) of a
 // (sequence, kv head), so that up to 128 share every K/V byte.  A unit is a stage of
 // 64 tokens (128 at D = 64) of one (sequence, kv head, row tile) segment; the units of
-// all segments lie end to end and workgroup w of W takes [w U/W, (w+1) U/W): all stream
-// the same number of bytes whatever the context lengths.  A segment within one
-// workgroup is written from there; of the others a workgroup holds at most two pieces
-// (its first and its last), which gqa_tree_reduce_kernel merges.
+// all segments lie end to end, each after kLead that stand for what a segment costs
+// besides, and workgroup w of W takes [w U/W, (w+1) U/W): all work as long whatever the
+// context lengths (without kLead those with many short segments were the last: 32
+// sequences of up to 4,000 tokens, 8 drafts, 32/8 heads, 139 us instead of 72).  A
+// segment within one workgroup is written from there; of the others a workgroup holds at
+// most two pieces, an end and a start, which gqa_tree_reduce_kernel merges.
 //
 // Eight wavefronts, two per SIMD, so that one's matrix work runs beside the other's
 // exponentials: four groups of 16 NT rows, two wavefronts each, which take every
 // other 32-token block.  K and V^T go straight into LDS (buffer_load ... lds, 1 KiB
 // each) through a ring of four 32 KiB stages: three are under way while one is
 // computed (a ring of two per wavefront drained it at every stage: 371 us at 16
-// sequences of 1k-32k tokens, 16 drafts, 32/8 heads, where this takes 249; blocks
+// sequences of 1k-32k tokens, 16 drafts, 32/8 heads, where this takes 231; blocks
 // in registers, as in the decode kernel, leave too few for 64 rows: 1,076).  Per block,
 // with the rows in the N dimension:
 //   scores^T[token][row] = K . Q^T,  out^T[dim][row] += V^T . P^T   16x16x32 bf16
@@ -51,6 +53,7 @@ constexpr int kStages = 4;    // stages of the ring in LDS
 constexpr int kStageElems = 2 * 64 * 128;  // of K and V^T
 constexpr int stage_blocks(int D) { return kStageElems / (2 * kBlk * D); }
 constexpr int stage_tokens(int D) { return stage_blocks(D) * kBlk; }
+constexpr int kLead = 8;      // units that a segment costs besides its chunks
 constexpr int kMaxBatch = 1024;
 constexpr int kMaxDrafts = 1024;
 
@@ -99,10 +102,15 @@ __device__ __forceinline__ int chunks_of(int ctx) {
   return (ctx + stage_tokens(D) - 1) / stage_tokens(D);
 }
 
-// Units of a sequence: its chunks for every kv head and row tile that holds a draft.
+// Units of a sequence: for every kv head and row tile that holds a draft its chunks, after
+// kLead units that stand for what a segment costs besides (queries, the first loads of an
+// empty ring, drafts and masks, the merge).
 template <int D>
 struct Units {
   int chunks, tiles;
+  __device__ __forceinline__ int all(const TreeArgs& a) const {
+    return chunks == 0 ? 0 : (chunks + kLead) * tiles * a.NKV;
+  }
   __device__ __forceinline__ Units(const TreeArgs& a, int b) {
     const int ctx = context_of(a, b);
     chunks = chunks_of<D>(ctx);
@@ -116,7 +124,7 @@ template <int D>
 __device__ __forceinline__ Units<D> scan_units(const TreeArgs& a, int base, int lane, int& x) {
   const bool in = base + lane < a.B;
   const Units<D> u(a, in ? base + lane : 0);
-  x = wave_inclusive_scan(in ? u.chunks * u.tiles * a.NKV : 0, lane);
+  x = wave_inclusive_scan(in ? u.all(a) : 0, lane);
   return u;
 }
 
@@ -156,7 +164,8 @@ __device__ __forceinline__ void load_stage(uint16_t* stage, const TreeArgs& a, P
     const int sub = in_blk % kPieces;
     const int krow = sub * (kWave / kCpr) + lane / kCpr;
     const int ksrc = krow * (D * 2) + 16 * ((lane % kCpr) ^ k_swizzle<D>(krow));
-    const int vsrc = sub * 1024 + (lane >> 2) * (kBlk * 2) + 16 * ((lane & 3) ^ v_swizzle(lane >> 4));
+    const int vsrc =
+        sub * 1024 + (lane >> 2) * (kBlk * 2) + 16 * ((lane & 3) ^ v_swizzle(lane >> 4));
     load_piece<AUX>((is_v ? a.v_pool : a.k_pool) + at * (kBlk * D), kBlk * D * 2,
                     is_v ? vsrc : ksrc, stage + p * 512);
   }
@@ -470,23 +479,25 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
         b = base + k;
         chunks = __builtin_amdgcn_readlane(units.chunks, k);
         tiles = __builtin_amdgcn_readlane(units.tiles, k);
-        begin += __builtin_amdgcn_readlane(x, k) - chunks * tiles * a.NKV;
+        begin += __builtin_amdgcn_readlane(x, k) - (chunks + kLead) * tiles * a.NKV;
         break;
       }
       begin += here;
     }
-    const int s = (u0 - begin) / chunks;
+    const int s = (u0 - begin) / (chunks + kLead);
     kvh = s / tiles;
     tile = s - kvh * tiles;
-    begin += s * chunks;
+    begin += s * (chunks + kLead);
   }
-  for (int piece = 0;; ++piece) {
+  while (true) {
     if (a.W == 0) {
       c0 = 0;
       c1 = chunks;
     } else {
-      c0 = u0 - begin;
-      c1 = (u1 < begin + chunks ? u1 : begin + chunks) - begin;
+      const int first = begin + kLead;  // the segment's first chunk
+      if (u1 <= first) return;
+      c0 = u0 > first ? u0 - first : 0;
+      c1 = (u1 < first + chunks ? u1 : first + chunks) - first;
     }
     const int ctx = uniform(context_of(a, b));
     View<NT> view;
@@ -589,7 +600,7 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
     // Merge the two wavefronts of each group of rows: one leaves its state in LDS, the
     // other adds its own and writes.
     const bool all = c0 == 0 && c1 == chunks;
-    const size_t slot = 2 * static_cast<size_t>(w) + (piece > 0 ? 1 : 0);
+    const size_t slot = 2 * static_cast<size_t>(w) + (c0 == 0 ? 1 : 0);
     uint16_t* const merge = rw < 2 ? (rw == 0 ? stage_0 : stage_1) : (rw == 2 ? stage_2 : stage_3);
     float lt[NT];
 #pragma unroll
@@ -643,9 +654,9 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_tree_kernel(TreeArgs a) {
       }
     }
     if (a.W == 0) return;
-    u0 = u1 < begin + chunks ? u1 : begin + chunks;
+    begin += kLead + chunks;
+    u0 = u1 < begin ? u1 : begin;
     if (u0 >= u1) return;
-    begin += chunks;
     if (++tile == tiles) {
       tile = 0;
       if (++kvh == a.NKV) {
@@ -689,7 +700,8 @@ __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(T
     if (b >= base && b < base + kWave) {
       chunks = __builtin_amdgcn_readlane(units.chunks, b - base);
       tiles = __builtin_amdgcn_readlane(units.tiles, b - base);
-      before = U + __builtin_amdgcn_readlane(x, b - base) - chunks * tiles * a.NKV;
+      before = U + __builtin_amdgcn_readlane(x, b - base) -
+               (chunks == 0 ? 0 : (chunks + kLead) * tiles * a.NKV);
     }
     U += __builtin_amdgcn_readlane(x, kWave - 1);
   }
@@ -699,25 +711,24 @@ __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(T
   const int sub = lane / kLanes;
   const int dim = lane % kLanes * 4;
   const int ctx = uniform(context_of(a, b));
-  const bool dead = t >= uniform(drafts_of(a, b, ctx));
+  const bool dead = uniform(t >= drafts_of(a, b, ctx) ? 1 : 0) != 0;
   int first = 0, last = -1;
-  bool later = false;
   if (chunks > 0 && tile < tiles) {
     const Split split(U, a.W);
-    const int S = before + (kvh * tiles + tile) * chunks;
+    const int S = before + (kvh * tiles + tile) * (chunks + kLead) + kLead;
     first = split.group(S);
     last = split.group(S + chunks - 1);
     if (first == last) return;  // written by its workgroup
-    later = split.begin(first) < S;
+    if (dead) last = first - 1;
   }
-  // Up to 64 pieces at a time, one per lane for their maxima and sums.  A segment that
-  // starts inside its first workgroup's range is that one's last piece, else its first.
+  // Up to 64 pieces at a time, one per lane for their maxima and sums.  A workgroup leaves
+  // the piece that starts a segment, its last one, in its second slot.
   float M = -FLT_MAX, L = 0.f;
   f32x4 acc = {};
   for (int w0 = first; w0 <= last; w0 += kWave) {
     const int n = last - w0 + 1 < kWave ? last - w0 + 1 : kWave;
     const size_t p0 = 2 * static_cast<size_t>(w0) * a.rows + r;
-    const int odd = later && w0 == first ? a.rows : 0;  // of the first one
+    const int odd = w0 == first ? a.rows : 0;  // of the first one
     auto row_at = [&](int k) {
       k = k < n ? k : n - 1;
       return p0 + 2 * static_cast<size_t>(k) * a.rows + (k == 0 ? odd : 0);
@@ -771,7 +782,7 @@ struct TreePlan {
   int W;      // workgroups of the split; 0: one per segment, no reduce launch
 };
 
-constexpr int kShort = 8;
+constexpr int kShort = 8, kLong = 64;  // stages of a segment that is not cut
 
 TreePlan plan_tree(int B, int NKV, int D, int G, int T, int max_pages, int page_tokens) {
   const int R = T * G;
@@ -782,12 +793,15 @@ TreePlan plan_tree(int B, int NKV, int D, int G, int T, int max_pages, int page_
   const long long stages = (static_cast<long long>(max_pages) * page_tokens + 64 * 128 / D - 1) /
                            (64 * 128 / D);
   const long long segs = static_cast<long long>(B) * NKV * p.tiles;
-  // A segment of few stages is walked by one workgroup, which saves the reduce launch (8
-  // heads, 8 stages: 12.0 us so, 12.7 split; 12 stages: 13.4 and 12.4; 16: 20 and 14), and
-  // so are twice as many where there are enough of them; all workgroups of a split run
-  // at once.
+  // All workgroups of a split run at once.  Without one a workgroup walks a segment, which
+  // saves the merges and the reduce launch: where the segments are short (8 heads, 8 stages:
+  // 12.0 us so, 12.7 split; 12 stages: 13.4 and 12.4; 16: 20 and 14), the longer the better
+  // they fill the card (192 of up to 9 stages: 14 and 21; 256 of up to 63: 61 and 72; 184
+  // of up to 64: 76 and 51).
   const int cus = device_cu_count();
-  p.W = stages <= kShort || (stages <= 16 && segs >= cus) ? 0 : cus;
+  const long long full = (segs + cus - 1) / cus * cus;
+  const int most = 16 * segs >= 15 * full ? kLong : (2 * segs >= full ? 2 * kShort : kShort);
+  p.W = stages <= most ? 0 : cus;
   return p;
 }
 
@@ -857,7 +871,7 @@ extern "C" int voom_paged_gqa_tree(const void* q, const void* k_pool, const void
   const int G = num_q_heads / num_kv_heads;
   const TreePlan p = plan_tree(batch, num_kv_heads, head_dim, G, drafts, max_pages, page_tokens);
   const long long stages = (static_cast<long long>(max_pages) * page_tokens + 63) / 64;
-  VOOM_REQUIRE(stages * batch * num_kv_heads * p.tiles < (1LL << 31),
+  VOOM_REQUIRE((stages + kLead) * batch * num_kv_heads * p.tiles < (1LL << 31),
                "%s: %d pages of %d tokens for %d sequences are too many", who, max_pages,
                page_tokens, batch);
   const size_t need = voom_paged_gqa_tree_workspace_bytes(
