@@ -94,6 +94,39 @@ def test_batches_of_many_sequences(B, spare):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_ragged_windows_of_several_loads_in_a_large_batch(D):
+    """Windows whose rows go through the keys once, twice or three times, in one call."""
+    print(f"[limits] windows of several loads, D={D}", flush=True)
+    B, NQ, NKV, L = 70, 8, 2, 150
+    rng = np.random.default_rng(D)
+    ctx = rng.integers(0, 900, B)
+    ctx[[3, 69]] = 0
+    ctx[40] = 900
+    lens = np.minimum(rng.integers(0, L + 1, B), ctx)
+    lens[40] = L
+    q, k, v = inputs(B, NQ, NKV, D, 900, L)
+    k_pool, v_pool, table = cache(k, v, 64)
+    ctx_t, lens_t = lens_tensor(ctx.tolist()), lens_tensor(lens.tolist())
+    _, lse = ops.paged_gqa_tree(q, k_pool, v_pool, table, ctx_t, draft_lens=lens_t,
+                                return_lse=True)
+    sums = torch.full((B, NKV, 901), 0.25, device="cuda")
+    ops.paged_gqa_observe(q, lse, k_pool, table, ctx_t, sums, window_lens=lens_t)
+    tril = torch.ones((L, L), dtype=torch.bool, device="cuda").tril()
+    for b in range(B):
+        n, c = int(lens[b]), int(ctx[b])
+        assert (sums[b, :, c:] == 0.25).all()
+        if n == 0:
+            assert (sums[b] == 0.25).all()
+            continue
+        _, want_lse, weight = reference(q[b], k[b], v[b], c, n, tril)
+        assert ((lse[b, :n].double() - want_lse).abs() <= LSE_ABS).all()
+        # three loads: three more roundings of the sum than where a window is one
+        assert ((sums[b, :, :c].double() - weight - 0.25).abs()
+                <= (WEIGHT + 2 * LSE_ABS) * weight + 4 * SUM * (weight + 0.25)).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("NQ,NKV,D,ctx", [(2, 1, 64, 1500), (2, 2, 128, 1024)])
 def test_as_many_drafts_as_a_call_takes(NQ, NKV, D, ctx):
     T = 1024

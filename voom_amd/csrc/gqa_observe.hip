@@ -12,11 +12,13 @@
 // exponential per (row, key).
 //
 // Keys are independent of each other, so nothing is merged: units of one stage (128
-// tokens, 256 at D = 64) of all (sequence, kv head) segments lie end to end and are dealt
-// out evenly.  K goes straight into LDS (1 KiB loads) through a ring of four 32 KiB
+// tokens, 256 at D = 64) of all (sequence, kv head) segments lie end to end, as often as
+// the window's rows go through the keys and after kLead that stand for what a segment costs
+// besides, and are dealt out evenly (32 sequences of up to 4,000 tokens, 32/8 heads: 32 us,
+// without kLead 62).  K goes straight into LDS (1 KiB loads) through a ring of four 32 KiB
 // stages, three of them under way; loaded into operand registers instead, 64 bytes of
 // a row at a time, the same keys took 147 us with no work on them, where 16 sequences of
-// 1k-32k tokens, 32/8 heads, take 136 with all of it.
+// 1k-32k tokens, 32/8 heads, took 136 with all of it (128 since kLead).
 //
 // Eight wavefronts compute, RW of them on other rows (16 NT each, queries in registers)
 // and 8 / RW on other keys of the stage:
@@ -37,6 +39,7 @@ namespace {
 
 constexpr int kWaves = 8;                         // that compute
 constexpr int kThreads = (kWaves + 1) * kWave;    // and the one that stores
+constexpr int kLead = 3;                          // units that a segment costs besides its stages
 constexpr int kMaxBatch = 1024;
 constexpr int kStageElems = 128 * 128;
 constexpr int stage_tokens(int D) { return kStageElems / D; }
@@ -60,6 +63,12 @@ __device__ __forceinline__ int context_of(const ObserveArgs& a, int b) {
   most = most < a.cap ? most : a.cap;
   const int c = a.ctx[b];
   return c < 0 ? 0 : (c > most ? most : c);
+}
+
+__device__ __forceinline__ int window_of(const ObserveArgs& a, int b, int ctx) {
+  int n = a.lens != nullptr ? a.lens[b] : a.L;
+  n = n < 0 ? 0 : (n > a.L ? a.L : n);
+  return n < ctx ? n : ctx;
 }
 
 // Chunk c (16 bytes) of K row r of a stage sits at c ^ k_swizzle(r) of its row: 16
@@ -109,7 +118,15 @@ __global__ __launch_bounds__(kThreads) void gqa_observe_kernel(ObserveArgs a) {
   const int w = static_cast<int>(blockIdx.x);
 
   // This workgroup's units, found by every wavefront for itself.
-  auto units_of = [&](int b) { return (context_of(a, b) + kST - 1) / kST; };
+  auto loads_of = [&](int b) {  // how often a sequence's keys are gone through
+    if (a.L * a.G <= kRows) return 1;
+    const int loads = (window_of(a, b, context_of(a, b)) * a.G + kRows - 1) / kRows;
+    return loads < 1 ? 1 : loads;
+  };
+  auto units_of = [&](int b) {
+    const int chunks = (context_of(a, b) + kST - 1) / kST;
+    return chunks == 0 ? 0 : chunks * loads_of(b) + kLead;
+  };
   int U = 0;
   for (int base = 0; base < a.B; base += kWave) {
     const int n = base + lane < a.B ? units_of(base + lane) * a.NKV : 0;
@@ -138,16 +155,21 @@ __global__ __launch_bounds__(kThreads) void gqa_observe_kernel(ObserveArgs a) {
   begin += kvh * units;
 
   while (true) {
-    const int c0 = u0 - begin;
-    const int c1 = (u1 < begin + units ? u1 : begin + units) - begin;
+    const int first = begin + kLead;  // the segment's first stage
+    if (u1 <= first) return;
+    const int loads = uniform(loads_of(b));
+    int c0 = u0 > first ? u0 - first : 0;
+    int c1 = (u1 < begin + units ? u1 : begin + units) - first;
+    if (loads > 1) {
+      c0 = (c0 + loads - 1) / loads;
+      c1 = (c1 + loads - 1) / loads;
+    }
     const int ctx = uniform(context_of(a, b));
-    int n = a.lens != nullptr ? uniform(a.lens[b]) : a.L;
-    n = n < 0 ? 0 : (n > a.L ? a.L : n);
-    n = n < ctx ? n : ctx;
+    const int n = uniform(window_of(a, b, ctx));
     const int live = n * a.G;  // rows of the window, (token, head) with the head fastest
     const size_t out_row = (static_cast<size_t>(b) * a.NKV + kvh) * a.cap;
 
-    for (int r0 = 0; r0 == 0 || r0 < live; r0 += kRows) {
+    for (int r0 = 0; c0 < c1 && (r0 == 0 || r0 < live); r0 += kRows) {
       if (wv == kWaves) {
         // the wavefront that stores: stage t - 1 while the others compute stage t
         const float* from = (r0 == 0 ? a.scores : a.out) + out_row;
@@ -216,7 +238,8 @@ __global__ __launch_bounds__(kThreads) void gqa_observe_kernel(ObserveArgs a) {
       int t = c0;
       // One stage: it has landed for every wavefront, and the one before is no longer read.
       auto step = [&](const uint16_t* cur, uint16_t* free) {
-        __builtin_amdgcn_s_waitcnt(0x0F78);  // gfx9 encoding: vmcnt 8 (two stages), expcnt 7, lgkmcnt 15
+        // gfx9 encoding: vmcnt 8 (two stages), expcnt 7, lgkmcnt 15
+        __builtin_amdgcn_s_waitcnt(0x0F78);
         lds_barrier();
         load_stage<D>(free, a, pg, t + 3, t + 3 < c1, wv, lane);
         const bool masked = dead_rows || (t + 1) * kST > ctx - n;
@@ -352,8 +375,10 @@ extern "C" int voom_paged_gqa_observe(const void* q, const float* lse, const voi
   a.num_slots = num_slots;
   a.scale = scale * 1.4426950408889634f;
   const int st = stage_tokens(head_dim);
-  const long long most = ((static_cast<long long>(max_pages) * page_tokens + st - 1) / st) * batch *
-                         num_kv_heads;
+  const long long loads = (static_cast<long long>(window) * a.G + 255) / 256;
+  const long long most =
+      ((static_cast<long long>(max_pages) * page_tokens + st - 1) / st * loads + kLead) * batch *
+      num_kv_heads;
   VOOM_REQUIRE(most < (1LL << 31), "%s: %d pages of %d tokens for %d sequences are too many", who,
                max_pages, page_tokens, batch);
   a.W = static_cast<int>(most < device_cu_count() ? most : device_cu_count());  // all run at once
