@@ -135,6 +135,31 @@ def test_a_speculative_step_on_a_bounded_cache(page, spilled):
     assert kv.next_position == 0
 
 
+def test_keeping_drafts_leaves_spilled_pages_alone():
+    """Pages before the drafts stay where they are; those with drafts come back."""
+    print("[speculative] keep_drafts with spilled pages", flush=True)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    S, T, page, path = 150, 9, 32, [1, 4, 7]  # the drafts close page 4
+    kv = PagedKVCache(LAYERS, 1 << 40, page_positions=page, resident_pages=1)
+    full = []
+    for layer in range(LAYERS):
+        k, v = (torch.randn((B, NKV, S + T + 2, D), generator=g, device="cuda").bfloat16()
+                for _ in range(2))
+        kv.append(layer, k[:, :, :S + T].contiguous(), v[:, :, :S + T].contiguous())
+        full.append((k, v))
+    # one page behind the context closed too: 161 tokens, the drafts are the last 11
+    for layer, (k, v) in enumerate(full):
+        kv.append(layer, k[:, :, S + T:].contiguous(), v[:, :, S + T:].contiguous())
+    kv.spill([(layer, i) for layer in range(LAYERS) for i in (0, 2, 4)])
+    kv.keep_drafts(T + 2, path)
+    for layer, (k, v) in enumerate(full):
+        assert [p.resident for p in kv._pages[layer]] == [False, True, False, True]
+        at = list(range(S)) + [S + i for i in path]
+        got_k, got_v = kv.gather(layer)
+        assert torch.equal(got_k, k[:, :, at]) and torch.equal(got_v, v[:, :, at])
+    kv.release()
+
+
 def test_refusals_and_small_calls():
     kv = PagedKVCache(1, 1 << 40, page_positions=32)
     with pytest.raises(ValueError, match="kv cache"):

@@ -772,7 +772,8 @@ class PagedKVCache:
 
     @property
     def next_position(self) -> int:
-        """Rotary position of the next token: the offset, and what evict() dropped."""
+        """Rotary position of the next token: the offset, and what evict() dropped (also
+        where a later trim() takes tokens away: heads keep tokens of different positions)."""
         return self._offset + self._dropped
 
     def nbytes(self) -> int:
@@ -2101,9 +2102,11 @@ class PagedKVCache:
         out = out.permute(0, 2, 1, 3)
         return (out, lse) if return_lse else out
 
-    def _resident(self, layer: int):
-        """(pool, block table) of a layer with every page resident."""
-        spilled = [p for p in self._pages[layer] if not p.resident]
+    def _resident(self, layer: int, first: int = 0):
+        """(pool, block table) of a layer with the pages of its tokens from ``first`` on
+        resident."""
+        spilled = [p for p in self._pages[layer][first // self.page_positions:]
+                   if not p.resident]
         if spilled:
             self.reload(spilled)
         return self._pool(layer), self._tables[layer]
@@ -2133,7 +2136,7 @@ class PagedKVCache:
             counts = torch.full((B,), n, dtype=torch.int32, device=self.device)
             for layer in range(self.num_layers):
                 first = self._len[layer] - drafts
-                pool, table = self._resident(layer)
+                pool, table = self._resident(layer, first)
                 ops.compact_kv(pool.k, pool.v, table, (path + first)[:, None].contiguous(), counts,
                                start=self._positions(first), scores=self._weights[layer])
         self._trim_to([length - drafts + n for length in self._len])
