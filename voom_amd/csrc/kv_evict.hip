@@ -19,10 +19,11 @@ namespace {
 // workgroup per (sequence, head).  Up to 32,768 candidates stay in registers, all loads
 // in flight at once (a loop that loaded them for every pass: 43 us for 16 x 8 heads of
 // up to 32,768 tokens, where this takes 20); of longer ones every pass loads 32,768 at a
-// time (64 heads of 131,072: 65 us; with 49,152 at a time, some of them spilled, 76).  Each histogram of a long row
-// has eight copies, by lane: scores share their leading bits, and atomics of one wavefront
-// on one address take turns.  The second and third pass look only at the keys that share
-// the first digit, from a list in LDS where it holds them.
+// time (64 heads of 131,072: 65 us; with 49,152 at a time, some of them spilled, 76).
+// Each histogram of a long row has eight copies, by lane: scores share their leading
+// bits, and atomics of one wavefront on one address take turns.  The second and third
+// pass look only at the keys that share the first digit, from a list in LDS where it
+// holds them.
 
 constexpr int kBins = 2048;
 constexpr int kList = 16384;  // candidates that share their first digit with the n-th largest
