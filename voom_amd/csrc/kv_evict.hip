@@ -212,12 +212,14 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
   if (tid == 0) listed = 0;
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = digit_shift(pass), bins = digit_bins(pass);
-    for (int i = tid; i < kBins * COPIES; i += kSelThreads) (&hist[0][0])[i] = 0;
+    int* const flat = &hist[0][0];  // one copy serves a short list
+    const int cells = short_list ? bins : kBins * COPIES;
+    for (int i = tid; i < cells / 4; i += kSelThreads)
+      reinterpret_cast<u32x4*>(flat)[i] = u32x4{0u, 0u, 0u, 0u};
     __syncthreads();
     if (short_list) {
       for (int i = tid; i < listed; i += kSelThreads)
-        if ((list[i] & mask) == prefix)
-          atomicAdd(&hist[(list[i] >> shift) & (bins - 1)][lane % COPIES], 1);
+        if ((list[i] & mask) == prefix) atomicAdd(&flat[(list[i] >> shift) & (bins - 1)], 1);
     } else {
       for (int c = 0; c < rounds; ++c) {
         if (rounds > 1 && (pass > 0 || c > 0)) load(c);
@@ -235,10 +237,14 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
     int mine[kPer] = {};
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
+      const int bin = bins - 1 - (tid * per + j);
       if (j < per) {
-        const int* h = hist[bins - 1 - (tid * per + j)];
+        if (short_list) {
+          mine[j] = flat[bin];
+        } else {
 #pragma unroll
-        for (int k = 0; k < COPIES; ++k) mine[j] += h[k];
+          for (int k = 0; k < COPIES; ++k) mine[j] += hist[bin][k];
+        }
       }
     }
     find_digit<kSelThreads>(mine, bins, need, part, found);
@@ -249,10 +255,18 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
       short_list = true;
       for (int c = 0; c < rounds; ++c) {
         if (rounds > 1) load(c);
+        // (one atomic a wavefront: each waits for its answer)
+        int mine_here = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          if (first_of(c) + e * kWave < count && (key[e] & mask) == prefix)
-            list[atomicAdd(&listed, 1)] = key[e];
+          mine_here += first_of(c) + e * kWave < count && (key[e] & mask) == prefix ? 1 : 0;
+        const int x = wave_inclusive_scan(mine_here, lane);
+        int at = 0;
+        if (lane == kWave - 1) at = atomicAdd(&listed, x);
+        at = __builtin_amdgcn_readlane(at, kWave - 1) + x - mine_here;
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (first_of(c) + e * kWave < count && (key[e] & mask) == prefix) list[at++] = key[e];
       }
     }
   }

@@ -2096,8 +2096,9 @@ class PagedKVCache:
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()  # the kernel loads 16 bytes per lane
-        got = ops.paged_gqa_tree(q, pool.k, pool.v, table, self._positions(S), mask=mask,
-                                 scale=scale, return_lse=return_lse)
+        got = ops.paged_gqa_tree(q, pool.k, pool.v, table, self._positions(S),
+                                 mask=None if mask is None else mask.contiguous(), scale=scale,
+                                 return_lse=return_lse)
         out, lse = got if return_lse else (got, None)
         out = out.permute(0, 2, 1, 3)
         return (out, lse) if return_lse else out
