@@ -18,8 +18,9 @@ namespace {
 // What bounds it: the scores once, 4 bytes per token and head, and the latency of one
 // workgroup per (sequence, head).  Up to 32,768 candidates stay in registers, all loads
 // in flight at once (a loop that loaded them for every pass: 43 us for 16 x 8 heads of
-// up to 32,768 tokens, where this takes 20); of longer ones every pass loads 32,768 at a
-// time (64 heads of 131,072: 65 us; with 49,152 at a time, some of them spilled, 76).
+// up to 32,768 tokens, where this takes 17); of longer ones every pass loads 32,768 at a
+// time (64 heads of 131,072: 58 us; 65 before the lists had one atomic a wavefront, and with
+// 49,152 at a time, some of them spilled, 76).
 // Each histogram of a long row has eight copies, by lane: scores share their leading
 // bits, and atomics of one wavefront on one address take turns.  The second and third
 // pass look only at the keys that share the first digit, from a list in LDS where it
@@ -283,9 +284,9 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(
 // Few rows of more than kRowMost scores: a workgroup takes a piece of kPiece candidates,
 // and the row goes through four launches.  Pass 0, 1 and 2 count a digit of the piece's
 // keys, and pass 1, 2 and 3 find the one before from all pieces' counts; pass 3 writes,
-// behind what the pieces before it keep.  8 rows of 131,072: 28 us, 64 for one workgroup per
-// row; 64 rows: 54 and 65; 128 rows of 65,536, which fill the card by themselves, 46 and 38;
-// 8 rows of 36,000: 22 and 34.
+// behind what the pieces before it keep.  8 rows of 131,072: 28 us, 57 for one workgroup per
+// row; 64 rows: 54 and 58; 128 rows of 65,536, which fill the card by themselves, 46 and 33;
+// 8 rows of 36,000: 22 and 31.
 constexpr int kSplitThreads = 1024;
 constexpr int kSplitE = 16;
 constexpr int kPiece = kSplitThreads * kSplitE;
