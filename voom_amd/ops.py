@@ -14,6 +14,7 @@ Pool layouts (per layer):
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -318,13 +319,26 @@ def paged_gqa_prefill(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tenso
     return out
 
 
-def _require_here(*tensors: torch.Tensor | None) -> None:
-    """Contiguous tensors on the current device, to whose stream the launch goes."""
+def _require_here(*tensors: torch.Tensor | None) -> int:
+    """Contiguous tensors on the current device, to whose stream the launch goes; its index.
+    (The calls from here on are those of a decode step, where microseconds of the host count:
+    messages are put together only where a check fails.)"""
     here = _CUR_DEVICE() if _CUR_DEVICE is not None else torch.cuda.current_device()
     for t in tensors:
         if t is not None and (t.get_device() != here or not t.is_contiguous()):
             dev = _require_device(*tensors)
             raise ValueError(f"tensors are on {dev}, but cuda:{here} is the current device")
+    return here
+
+
+def _stream_of(device: int) -> int:
+    """The current stream of the current device."""
+    return _RAW_STREAM(device) if _RAW_STREAM is not None else _stream(None)
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_workspace(device: int, *sizes: int) -> int:
+    return _lib.lib().voom_paged_gqa_tree_workspace_bytes(*sizes)
 
 
 def _is_i32(t: torch.Tensor, *shape: int) -> bool:
@@ -338,14 +352,14 @@ def _is_scores(t: torch.Tensor, batch: int, num_kv_heads: int) -> bool:
 
 def _new_tokens_geometry(q, k_pool, v_pool, block_table, ctx_lens):
     """Checks what the calls over a window of new tokens share; their sizes (v_pool None:
-    keys alone).  (The messages are put together only where a check fails: calls of a
-    decode step count microseconds.)"""
-    if q.dim() != 4:
+    keys alone)."""
+    q_shape, k_shape, table_shape = q.shape, k_pool.shape, block_table.shape
+    if len(q_shape) != 4:
         raise ValueError("q must be [B, NQ, T, D]")
-    if k_pool.dim() != 4:
+    if len(k_shape) != 4:
         raise ValueError("k_pool must be [slots, NKV, PT, D]")
-    B, NQ, T, D = q.shape
-    slots, NKV, PT, Dk = k_pool.shape
+    B, NQ, T, D = q_shape
+    slots, NKV, PT, Dk = k_shape
     if Dk != D:
         raise ValueError(f"k_pool head_dim {Dk} != q head_dim {D}")
     if v_pool is not None:
@@ -355,14 +369,13 @@ def _new_tokens_geometry(q, k_pool, v_pool, block_table, ctx_lens):
             raise ValueError("q and pools must be bfloat16")
     if q.dtype is not torch.bfloat16 or k_pool.dtype is not torch.bfloat16:
         raise ValueError("q and pools must be bfloat16")
-    if (block_table.dtype is not torch.int32 or block_table.dim() != 2
-            or block_table.shape[0] != B):
+    if block_table.dtype is not torch.int32 or len(table_shape) != 2 or table_shape[0] != B:
         raise ValueError(f"block_table must be int32 [{B}, max_pages]")
     if not _is_i32(ctx_lens, B):
         raise ValueError(f"ctx_lens must be int32 [{B}]")
     if NKV == 0 or NQ % NKV:
         raise ValueError("num_q_heads must be a multiple of num_kv_heads")
-    return B, NQ, T, D, slots, NKV, PT, block_table.shape[1]
+    return B, NQ, T, D, slots, NKV, PT, table_shape[1]
 
 
 def paged_gqa_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -381,31 +394,33 @@ def paged_gqa_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     Returns out [B, T, NQ, D] (and the fp32 natural-log LSE [B, T, NQ] when
     ``return_lse``); rows that see nothing, and rows past draft_lens, hold 0 and -inf.
     """
-    _require_here(q, k_pool, v_pool, block_table, ctx_lens, mask, draft_lens)
+    here = _require_here(q, k_pool, v_pool, block_table, ctx_lens, mask, draft_lens)
     B, NQ, T, D, slots, NKV, PT, pages = _new_tokens_geometry(q, k_pool, v_pool, block_table,
                                                               ctx_lens)
     if draft_lens is not None and not _is_i32(draft_lens, B):
         raise ValueError(f"draft_lens must be int32 [{B}]")
     masks = 1
     if mask is not None:
-        if mask.dtype is not torch.bool or mask.shape not in ((T, T), (B, T, T)):
+        mask_shape = mask.shape
+        if mask.dtype is not torch.bool or mask_shape not in ((T, T), (B, T, T)):
             raise ValueError(f"mask must be bool [{T}, {T}] or [{B}, {T}, {T}]")
-        masks = B if mask.dim() == 3 else 1
+        masks = B if len(mask_shape) == 3 else 1
     out = q.new_empty((B, T, NQ, D))
     lse = q.new_empty((B, T, NQ), dtype=torch.float32) if return_lse else None
     if B and T and NQ:
         if _BOUNDS_CHECKS:
             check_block_table(block_table, ctx_lens, slots, PT)
-        lib = _lib.lib()
         # allocated per call, so that calls on several streams or threads and captured
         # graphs never share it
-        need = lib.voom_paged_gqa_tree_workspace_bytes(B, NQ, NKV, D, T, PT, pages)
+        need = _tree_workspace(here, B, NQ, NKV, D, T, PT, pages)
         ws = q.new_empty(need, dtype=torch.uint8) if need else None
-        rc = lib.voom_paged_gqa_tree(
+        rc = _lib.lib().voom_paged_gqa_tree(
             q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
-            ctx_lens.data_ptr(), _ptr(draft_lens), _ptr(mask), masks, out.data_ptr(), _ptr(lse),
-            _ptr(ws), need, B, NQ, NKV, D, PT, pages, slots, T,
-            D ** -0.5 if scale is None else float(scale), _stream(None))
+            ctx_lens.data_ptr(), None if draft_lens is None else draft_lens.data_ptr(),
+            None if mask is None else mask.data_ptr(), masks, out.data_ptr(),
+            None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), need,
+            B, NQ, NKV, D, PT, pages, slots, T, D ** -0.5 if scale is None else float(scale),
+            _stream_of(here))
         if rc:
             _lib.check(rc, "voom_paged_gqa_tree")
     return (out, lse) if return_lse else out
@@ -428,7 +443,7 @@ def paged_gqa_observe(q: torch.Tensor, lse: torch.Tensor, k_pool: torch.Tensor,
     """
     if q.dim() == 4 and lse.dim() == 2 and q.shape[2] == 1:
         lse = lse[:, None]
-    _require_here(q, lse, k_pool, block_table, ctx_lens, scores, window_lens, out)
+    here = _require_here(q, lse, k_pool, block_table, ctx_lens, scores, window_lens, out)
     B, NQ, L, D, slots, NKV, PT, pages = _new_tokens_geometry(q, k_pool, None, block_table,
                                                               ctx_lens)
     if lse.dtype is not torch.float32 or lse.shape != (B, L, NQ):
@@ -449,9 +464,9 @@ def paged_gqa_observe(q: torch.Tensor, lse: torch.Tensor, k_pool: torch.Tensor,
         q, lse, L = q.new_zeros((B, NQ, 1, D)), lse.new_full((B, 1, NQ), -float("inf")), 1
     rc = _lib.lib().voom_paged_gqa_observe(
         q.data_ptr(), lse.data_ptr(), k_pool.data_ptr(), block_table.data_ptr(),
-        ctx_lens.data_ptr(), _ptr(window_lens), scores.data_ptr(), out.data_ptr(), B, NQ, NKV, D,
-        PT, pages, slots, L, scores.shape[2], D ** -0.5 if scale is None else float(scale),
-        _stream(None))
+        ctx_lens.data_ptr(), None if window_lens is None else window_lens.data_ptr(),
+        scores.data_ptr(), out.data_ptr(), B, NQ, NKV, D, PT, pages, slots, L, scores.shape[2],
+        D ** -0.5 if scale is None else float(scale), _stream_of(here))
     if rc:
         _lib.check(rc, "voom_paged_gqa_observe")
     return out
@@ -467,11 +482,11 @@ def evict_select(scores: torch.Tensor, ctx_lens: torch.Tensor, budget: int, *, s
     and of those between the ones of largest score, equal scores lowest position first
     (a NaN counts below every number).
     """
-    _require_here(scores, ctx_lens)
-    B = scores.shape[0] if scores.dim() == 3 else 0
-    if scores.dim() != 3 or not _is_scores(scores, B, scores.shape[1]):
+    here = _require_here(scores, ctx_lens)
+    shape = scores.shape
+    if scores.dtype is not torch.float32 or len(shape) != 3 or shape[2] == 0:
         raise ValueError("scores must be float32 [B, NKV, tokens]")
-    NKV, cap = scores.shape[1:]
+    B, NKV, cap = shape
     if not _is_i32(ctx_lens, B):
         raise ValueError(f"ctx_lens must be int32 [{B}]")
     budget, sink, recent = int(budget), int(sink), int(recent)
@@ -485,7 +500,7 @@ def evict_select(scores: torch.Tensor, ctx_lens: torch.Tensor, budget: int, *, s
         ws = scores.new_empty(need, dtype=torch.uint8) if need else None
         rc = lib.voom_evict_select_split(
             scores.data_ptr(), ctx_lens.data_ptr(), keep.data_ptr(), keep_lens.data_ptr(), _ptr(ws),
-            need, B, NKV, cap, budget, sink, recent, _stream(None))
+            need, B, NKV, cap, budget, sink, recent, _stream_of(here))
         if rc:
             _lib.check(rc, "voom_evict_select")
     return keep, keep_lens
@@ -556,20 +571,21 @@ def compact_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Te
     ``scores`` [B, NKV, tokens] fp32 moves along into ``scores_out`` (default: in place);
     behind the last row kept it becomes 0.
     """
-    _require_here(k_pool, v_pool, block_table, keep, keep_lens, start, dst_table, scores,
-                  scores_out)
-    if k_pool.dim() != 4:
+    here = _require_here(k_pool, v_pool, block_table, keep, keep_lens, start, dst_table, scores,
+                         scores_out)
+    k_shape, table_shape, keep_shape = k_pool.shape, block_table.shape, keep.shape
+    if len(k_shape) != 4:
         raise ValueError("k_pool must be [slots, NKV, PT, D]")
-    slots, NKV, PT, D = k_pool.shape
+    slots, NKV, PT, D = k_shape
     if v_pool.shape != (slots,) + v_slot_shape(NKV, D, PT):
         _check_v_pool(v_pool, slots, NKV, D, PT)
     if k_pool.dtype is not torch.bfloat16 or v_pool.dtype is not torch.bfloat16:
         raise ValueError("pools must be bfloat16")
-    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
+    if block_table.dtype is not torch.int32 or len(table_shape) != 2:
         raise ValueError("block_table must be int32 [B, max_pages]")
-    B = block_table.shape[0]
-    if (keep.dtype is not torch.int32 or keep.dim() != 3 or keep.shape[0] != B
-            or keep.shape[1] not in (1, NKV)):
+    B, pages = table_shape
+    if (keep.dtype is not torch.int32 or len(keep_shape) != 3 or keep_shape[0] != B
+            or keep_shape[1] not in (1, NKV)):
         raise ValueError(f"keep must be int32 [{B}, {NKV}, n] or [{B}, 1, n]")
     if not _is_i32(keep_lens, B):
         raise ValueError(f"keep_lens must be int32 [{B}]")
@@ -590,20 +606,23 @@ def compact_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Te
         scores_out = scores
     elif scores_out.dtype is not torch.float32 or scores_out.shape != scores.shape:
         raise ValueError("scores_out must be like scores")
-    n = keep.shape[2]
+    heads, n = keep_shape[1:]
     if B == 0 or (n == 0 and scores is None):
         return
     if _BOUNDS_CHECKS:
-        check_keep(keep, keep_lens, block_table.shape[1] * PT, start, in_place)
+        check_keep(keep, keep_lens, pages * PT, start, in_place)
         if not in_place:
             check_destination(block_table, dst_table, keep, keep_lens, start, PT)
     if n == 0:  # only scores to clear
-        keep, keep_lens, n = keep.new_zeros((B, 1, 1)), torch.zeros_like(keep_lens), 1
+        keep, keep_lens = keep.new_zeros((B, 1, 1)), torch.zeros_like(keep_lens)
+        heads = n = 1
     rc = _lib.lib().voom_compact_kv(
         k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(), dst_table.data_ptr(),
-        keep.data_ptr(), keep_lens.data_ptr(), _ptr(start), _ptr(scores), _ptr(scores_out), B, NKV,
-        D, PT, block_table.shape[1], dst_table.shape[1], slots, keep.shape[1], n,
-        0 if scores is None else scores.shape[2], _stream(None))
+        keep.data_ptr(), keep_lens.data_ptr(), None if start is None else start.data_ptr(),
+        None if scores is None else scores.data_ptr(),
+        None if scores is None else scores_out.data_ptr(), B, NKV, D, PT, pages,
+        pages if in_place else dst_table.shape[1], slots, heads, n,
+        0 if scores is None else scores.shape[2], _stream_of(here))
     if rc:
         _lib.check(rc, "voom_compact_kv")
 
@@ -625,29 +644,30 @@ def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
     [B, nq, L, hd]; K and V of token t land at cache position start[b] + t (start [B]
     int32) for t < new_lens[b] (None: all).  One rounding to bf16 at the end.
     """
-    _require_here(qkv, cos, sin, positions, k_pool, v_pool, block_table, start, q_weight, k_weight,
-                  new_lens)
+    here = _require_here(qkv, cos, sin, positions, k_pool, v_pool, block_table, start, q_weight,
+                         k_weight, new_lens)
     nq, nkv = int(num_q_heads), int(num_kv_heads)
-    if k_pool.dim() != 4:
+    shape, k_shape, cos_shape, table_shape = (qkv.shape, k_pool.shape, cos.shape,
+                                              block_table.shape)
+    if len(k_shape) != 4:
         raise ValueError("k_pool must be [slots, NKV, PT, D]")
-    slots, NKVp, PT, hd = k_pool.shape
+    slots, NKVp, PT, hd = k_shape
     if nq <= 0 or NKVp != nkv:
         raise ValueError("pool geometry does not match the heads")
     if v_pool.shape != (slots,) + v_slot_shape(nkv, hd, PT):
         _check_v_pool(v_pool, slots, nkv, hd, PT)
-    if qkv.dim() != 3 or qkv.shape[2] != (nq + 2 * nkv) * hd:
+    if len(shape) != 3 or shape[2] != (nq + 2 * nkv) * hd:
         raise ValueError(f"qkv must be [B, L, {(nq + 2 * nkv) * hd}]")
-    B, L, _ = qkv.shape
+    B, L, _ = shape
     if (qkv.dtype is not torch.bfloat16 or k_pool.dtype is not torch.bfloat16
             or v_pool.dtype is not torch.bfloat16):
         raise ValueError("qkv and pools must be bfloat16")
-    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.dim() != 2
-            or cos.shape != sin.shape or cos.shape[0] == 0):
+    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or len(cos_shape) != 2
+            or sin.shape != cos_shape or cos_shape[0] == 0):
         raise ValueError("cos and sin must be float32 [positions, rotary / 2]")
     if not _is_i32(positions, B, L):
         raise ValueError(f"positions must be int32 [{B}, {L}]")
-    if (block_table.dtype is not torch.int32 or block_table.dim() != 2
-            or block_table.shape[0] != B):
+    if block_table.dtype is not torch.int32 or len(table_shape) != 2 or table_shape[0] != B:
         raise ValueError(f"block_table must be int32 [{B}, max_pages]")
     if not _is_i32(start, B):
         raise ValueError(f"start must be int32 [{B}]")
@@ -660,11 +680,13 @@ def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
     q = qkv.new_empty((B, nq, L, hd))
     if B and L:
         rc = _lib.lib().voom_qk_norm_rope_append(
-            qkv.data_ptr(), _ptr(q_weight), _ptr(k_weight), float(eps), cos.data_ptr(),
-            sin.data_ptr(), cos.shape[0], 2 * cos.shape[1], 1 if interleaved else 0,
+            qkv.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
+            None if k_weight is None else k_weight.data_ptr(), float(eps), cos.data_ptr(),
+            sin.data_ptr(), cos_shape[0], 2 * cos_shape[1], 1 if interleaved else 0,
             positions.data_ptr(), q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(),
-            block_table.data_ptr(), start.data_ptr(), _ptr(new_lens), B, L, nq, nkv, hd, PT,
-            block_table.shape[1], slots, _stream(None))
+            block_table.data_ptr(), start.data_ptr(),
+            None if new_lens is None else new_lens.data_ptr(), B, L, nq, nkv, hd, PT,
+            table_shape[1], slots, _stream_of(here))
         if rc:
             _lib.check(rc, "voom_qk_norm_rope_append")
     return q
