@@ -568,3 +568,24 @@ def test_abi_refusals_of_workspaces_of_long_rows():
         assert "workspace" in _lib.last_error()
     assert lib.voom_evict_select_split(p, p, p, p, p, need, 2, 8, 100000, 4, 4, 4,
                                        None) == _lib.VOOM_EINVAL
+
+
+def test_destinations_that_a_move_reads_are_refused():
+    def i32(x):
+        return torch.tensor(x, dtype=torch.int32)
+
+    table = i32([[3, 5], [4, 1]])
+    lists, lens = i32([[[2, 7, 9]], [[0, 1, 12]]]), i32([3, 2])  # pages of 8 tokens
+    for match, dst, start in (("read elsewhere", [[5, 0], [6, 7]], None),
+                              ("read elsewhere", [[4, 0], [6, 7]], None),
+                              ("twice", [[6, 0], [6, 7]], None),
+                              ("twice", [[6, 6], [7, 2]], [6, 0]),
+                              ("own pages", [[3, 0], [6, 7]], [3, 0])):
+        with pytest.raises(ValueError, match=match):
+            ops.check_destination(table, i32(dst), lists, lens, None if start is None else
+                                  i32(start), 8)
+    for dst, start in (([[0, 2], [6, 7]], None), ([[3, 2], [1, 7]], None),  # 1 is not read
+                       ([[0], [6]], [6, 0]), ([[3, 3], [4, 4]], None)):
+        ops.check_destination(table, i32(dst), lists, lens, None if start is None else
+                              i32(start), 8)
+    ops.check_destination(table, table, lists, i32([0, 0]), None, 8)
