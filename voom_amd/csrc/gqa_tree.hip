@@ -683,15 +683,12 @@ __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(T
   constexpr int kTogether = kWave / kLanes;
   constexpr int kAhead = 8;  // loads in flight
   const int lane = threadIdx.x & (kWave - 1);
-  const long long task =
-      static_cast<long long>(blockIdx.x) * kReduceWaves + uniform(threadIdx.x / kWave);
-  if (task >= static_cast<long long>(a.B) * a.NKV * a.R) return;
-  const int seg = static_cast<int>(task / a.R);
-  const int rr = static_cast<int>(task - static_cast<long long>(seg) * a.R);
-  const int b = seg / a.NKV;
-  const int kvh = seg - b * a.NKV;
-  const int tile = rr / a.rows;
-  const int r = rr - tile * a.rows;
+  const int b = static_cast<int>(blockIdx.z);
+  const int kvh = static_cast<int>(blockIdx.y);
+  const int rr = static_cast<int>(blockIdx.x) * kReduceWaves + uniform(threadIdx.x / kWave);
+  if (rr >= a.R) return;
+  const int tile = a.rows == 128 ? rr >> 7 : rr >> 6;
+  const int r = rr & (a.rows - 1);
   // units before sequence b, and of all; chunks and row tiles of b
   int before = 0, chunks = 0, tiles = 1, U = 0;
   for (int base = 0; base < a.B; base += kWave) {
@@ -807,7 +804,8 @@ TreePlan plan_tree(int B, int NKV, int D, int G, int T, int max_pages, int page_
 
 bool tree_shape_ok(int batch, int num_q_heads, int num_kv_heads, int head_dim, int drafts,
                    int page_tokens, int max_pages) {
-  return batch > 0 && batch <= kMaxBatch && num_kv_heads > 0 && num_q_heads > 0 &&
+  return batch > 0 && batch <= kMaxBatch && num_kv_heads > 0 && num_kv_heads <= 65535 &&
+         num_q_heads > 0 &&
          num_q_heads % num_kv_heads == 0 && num_q_heads / num_kv_heads <= 16 &&
          (head_dim == 64 || head_dim == 128) && drafts > 0 && drafts <= kMaxDrafts &&
          is_pow2(page_tokens) && page_tokens >= 32 && page_tokens <= 4096 && max_pages > 0 &&
@@ -917,8 +915,8 @@ extern "C" int voom_paged_gqa_tree(const void* q, const void* k_pool, const void
   else launch_tree<64>(a, p, grid, stream);
   const int rc = VOOM_LAUNCH_CHECK("paged_gqa_tree: kernel launch");
   if (rc || p.W == 0) return rc;
-  const long long rows = static_cast<long long>(batch) * num_kv_heads * a.R;
-  const dim3 rgrid(static_cast<unsigned>((rows + kReduceWaves - 1) / kReduceWaves));
+  const dim3 rgrid(static_cast<unsigned>((a.R + kReduceWaves - 1) / kReduceWaves),
+                   static_cast<unsigned>(num_kv_heads), static_cast<unsigned>(batch));
   if (head_dim == 128)
     hipLaunchKernelGGL(gqa_tree_reduce_kernel<128>, rgrid, dim3(kReduceWaves * kWave), 0, stream,
                        a);
