@@ -156,6 +156,30 @@ def test_keys_that_score_minus_infinity_weigh_nothing(page, first, count):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("NQ,NKV,D", [(9, 3, 64), (8, 2, 128)])
+@pytest.mark.parametrize("ctx", [700, 1480, 2500])
+def test_an_infinite_value_stays_infinite_however_a_context_is_cut(NQ, NKV, D, ctx):
+    """Infinities of both signs in V of the newest draft, in the last of any number of pieces:
+    its own row holds them, all else is as without them."""
+    T = 4
+    print(f"[tree] infinite V at the end, D={D} ctx={ctx}", flush=True)
+    q, k, v = inputs(1, NQ, NKV, D, ctx, T, seed=11)
+    plain = v.clone()
+    v[:, :, ctx - 1, 3], v[:, :, ctx - 1, D - 2] = INF, -INF
+    got = []
+    for values in (plain, v):
+        for spare in (0, 60):  # a wider table: the same context in other pieces
+            k_pool, v_pool, table = cache(k, values, 64, spare=spare)
+            got.append(ops.paged_gqa_tree(q, k_pool, v_pool, table, lens_tensor([ctx]),
+                                          return_lse=True))
+    torch.cuda.synchronize()
+    for (finite, lse), (out, lse_inf) in zip(got[:2], got[2:]):
+        want = finite.clone()
+        want[:, T - 1, :, 3], want[:, T - 1, :, D - 2] = INF, -INF
+        assert torch.equal(out, want) and torch.equal(lse, lse_inf)
+
+
+@pytest.mark.gpu
 def test_rows_without_a_key_and_lengths_out_of_range():
     print("[tree] empty mask rows, clamped lengths", flush=True)
     T, D, page = 6, 64, 32

@@ -750,7 +750,7 @@ __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_tree_reduce_kernel(T
       for (int u = 0; u < kAhead; ++u) {
         const int k = k0 + u * kTogether + sub;
         const float ws = __shfl(wt, k & (kWave - 1));
-        acc += v[u] * (k < n ? ws : 0.f);
+        if (k < n) acc += v[u] * ws;  // (0 times the infinity of a piece read again is NaN)
       }
     }
   }
