@@ -267,7 +267,8 @@ int voom_paged_gqa_tree(const void* q, const void* k_pool, const void* v_pool,
  *              sequence's own page at the same index, in a list that may move in place, or
  *              one that no list reads.  No page for two sequences
  *   scores     [batch, num_kv_heads, score_tokens] or NULL: moved the same way into
- *              scores_out (the same array or another one), zero behind the last row
+ *              scores_out (the same array or another one, whichever way a list moves its
+ *              rows), zero behind the last row
  * Rows whose position or slot id lies outside the tables and the pool are left out.
  * ------------------------------------------------------------------------- */
 int voom_paged_gqa_observe(const void* q, const float* lse, const void* k_pool,

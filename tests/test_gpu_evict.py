@@ -322,6 +322,48 @@ def test_move_is_exact(where, B, NKV, D, PT, ctx, n, per_head, start):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,start,lowest", [
+    (4096, 5000, 0), (4097, 5000, 0),   # both sides of what is read at once
+    (10000, 5000, 0),                   # all of them move back
+    (10000, 2500, 1000),                # the first ones back, the others forward
+    (9000, 300, 500),                   # all forward
+    (8193, 0, 0),
+])
+@pytest.mark.parametrize("own_array", [True, False])
+def test_scores_of_long_lists_that_go_to_other_pages(n, start, lowest, own_array):
+    """K and V may go to any place of other pages, and the scores go along, in their own
+    array too."""
+    print(f"[compact] scores n={n} start={start} lowest={lowest} own_array={own_array}", flush=True)
+    NKV, D, PT, ctx = 2, 32, 64, 15100
+    rng = np.random.default_rng(n + start)
+    _, k, v = inputs(1, NKV, NKV, D, ctx, 1)
+    pages = -(-ctx // PT)
+    k_pool, v_pool, both = cache(k, v, PT, spare=pages)
+    table, other = both[:, :pages].contiguous(), both[:, pages:].contiguous()
+    keep = np.stack([np.arange(lowest, lowest + n), np.arange(lowest, lowest + n)])
+    if lowest != 0:  # a gap in the second head's list, further on in the first's
+        keep[0, n // 2:] += 3000
+        keep[1] = np.sort(rng.choice(np.arange(lowest, ctx), n, False))
+    behind = keep >= start + np.arange(n)
+    assert {(5000, 0): not behind.any(), (2500, 1000): behind.any() and not behind.all(),
+            (300, 500): behind.all(), (0, 0): behind.all()}[start, lowest]
+    at = torch.from_numpy(keep).cuda()
+    scores = torch.rand((1, NKV, ctx + 7), device="cuda")
+    want = torch.zeros_like(scores)
+    want[:, :, :start] = scores[:, :, :start]
+    want[0, :, start:start + n] = scores[0].gather(1, at)
+    out = scores if own_array else torch.empty_like(scores)
+    ops.compact_kv(k_pool, v_pool, table, at[None].int(), lens_tensor([n]),
+                   start=lens_tensor([start]), dst_table=other, scores=scores, scores_out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    got_k, got_v = ops.gather_kv(k_pool, v_pool, other, start + n)
+    rows = at[..., None].expand(-1, -1, D)
+    assert torch.equal(got_k[0, :, start:], k[0].gather(1, rows))
+    assert torch.equal(got_v[0, :, start:], v[0].gather(1, rows))
+
+
+@pytest.mark.gpu
 def test_rows_outside_the_tables_are_left_out():
     print("[compact] bad positions, slots and counts", flush=True)
     _, k, v = inputs(2, 2, 2, 64, 128, 1, seed=9)

@@ -537,6 +537,11 @@ __device__ __forceinline__ size_t v_element(uint32_t row, int d, int vb, int D) 
 }
 
 // One workgroup: the scores of one (sequence, kv head), and zeros behind them.
+//
+// In one array a round of kRound rows may only write what no later round reads.  Since the
+// list ascends, keep[i] - i never falls: a first part of the rows, which may be empty, moves
+// back (keep[i] < start + i) and goes from its end, the others from their front.  Where one
+// round holds the list it is read as a whole.
 template <int THREADS>
 __device__ __forceinline__ void move_scores(const CompactArgs& a, const int32_t* keep, int b,
                                             int kvh, int n, int start) {
@@ -548,13 +553,25 @@ __device__ __forceinline__ void move_scores(const CompactArgs& a, const int32_t*
   if (s != o)
     for (int i = tid; i < first; i += THREADS) o[i] = s[i];
   constexpr int kLoads = 8;
-  for (int i0 = 0; i0 < n; i0 += kLoads * THREADS) {
+  constexpr int kRound = kLoads * THREADS;
+  auto moves_back = [&](int i) { return keep[i] < start + static_cast<long long>(i); };
+  int back = 0;  // rows that move back
+  if (s == o && n > kRound && moves_back(0)) {
+    int not_back = n;
+    while (back < not_back) {
+      const int i = back + (not_back - back) / 2;
+      if (moves_back(i)) back = i + 1;
+      else not_back = i;
+    }
+    back = uniform(back);
+  }
+  auto round = [&](int i0, int end) {
     int from[kLoads];
     float v[kLoads];
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int i = i0 + j * THREADS + tid;
-      from[j] = i < n ? keep[i] : -1;
+      from[j] = i < end ? keep[i] : -1;
     }
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) v[j] = from[j] >= 0 && from[j] < a.cap ? s[from[j]] : 0.f;
@@ -564,9 +581,11 @@ __device__ __forceinline__ void move_scores(const CompactArgs& a, const int32_t*
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
       const int i = i0 + j * THREADS + tid;
-      if (i < n && start + static_cast<long long>(i) < a.cap) o[start + i] = v[j];
+      if (i < end && start + static_cast<long long>(i) < a.cap) o[start + i] = v[j];
     }
-  }
+  };
+  for (int i1 = back; i1 > 0; i1 -= kRound) round(i1 > kRound ? i1 - kRound : 0, i1);
+  for (int i0 = back; i0 < n; i0 += kRound) round(i0, n);
   for (long long i = static_cast<long long>(first) + n + tid; i < a.cap; i += THREADS)
     o[i] = 0.f;
 }
