@@ -216,3 +216,74 @@ def test_a_decoder_goes_on_after_an_eviction_at_the_next_position():
     model._rope_tables = lambda positions: seen.append(positions.tolist()) or tables(positions)
     logits = model.forward(prompt[:, :1], kv)
     assert torch.isfinite(logits).all() and seen == [[90]] and kv.offset == 51
+
+
+def filled(layers, tokens, page, max_bytes, seed):
+    """A cache of random K/V, with sums that ask for other tokens in every head; and the K/V."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    kv = PagedKVCache(layers, max_bytes, page_positions=page, resident_pages=1)
+    full = []
+    for layer in range(layers):
+        k, v = (torch.randn((B, NKV, tokens, D), generator=g, device="cuda").bfloat16()
+                for _ in range(2))
+        kv.append(layer, k, v)
+        full.append((k, v))
+    kv._weights = [torch.rand((B, NKV, tokens), generator=g, device="cuda")
+                   for _ in range(layers)]
+    return kv, full
+
+
+def rows_kept(sums, tokens, budget):
+    """[B, NKV, budget] positions of the largest sums, ascending."""
+    best = torch.sort(sums[:, :, :tokens], dim=-1, descending=True, stable=True).indices
+    return best[..., :budget].sort(-1).values
+
+
+@pytest.mark.parametrize("page,budget", [(32, 96), (32, 100), (64, 7)])
+def test_an_eviction_gives_its_pages_back_and_stays_within_the_bytes_allowed(page, budget):
+    print(f"[speculative] evicted pages page={page} budget={budget}", flush=True)
+    layers, tokens = 4, 20 * page + 3
+    page_bytes = B * NKV * page * D * 4
+    allowed = 2 * 20 * page_bytes  # two of the four layers
+    kv, full = filled(layers, tokens, page, allowed, seed=page + budget)
+    sums = [w.clone() for w in kv._weights]
+    open_bytes = layers * 3 * page_bytes // page
+    assert kv.nbytes() <= allowed + open_bytes and kv.stats.spills >= 2 * 20
+    held = []
+    moved = ops.compact_kv
+
+    def compact(*args, **kw):
+        held.append(sum(pool.live_slots * pool.slot_bytes for pool in kv._pools))
+        return moved(*args, **kw)
+
+    ops.compact_kv = compact
+    try:
+        assert kv.evict(budget) == tokens - budget
+    finally:
+        ops.compact_kv = moved
+    # what the cache may hold, an open page per layer, and the layer that is being cut
+    assert len(held) == layers and max(held) <= allowed + (layers + 21) * page_bytes
+    pages = -(-budget // page)
+    resident = sum(p.resident for lp in kv._pages for p in lp) + sum(map(len, kv._open_slots))
+    assert resident <= layers * pages
+    assert sum(pool.live_slots for pool in kv._pools) == B * resident
+    assert sum(pool.live_slots * pool.slot_bytes for pool in kv._pools) <= (
+        kv.nbytes() + layers * page_bytes)
+    for layer, (k, v) in enumerate(full):
+        at = rows_kept(sums[layer], tokens, budget)[..., None].expand(-1, -1, -1, D)
+        got_k, got_v = kv.gather(layer)
+        assert torch.equal(got_k, k.gather(2, at)) and torch.equal(got_v, v.gather(2, at))
+    # the slots are used again: no pool grows while the cache fills up and is cut again
+    capacity = [pool.capacity for pool in kv._pools]
+    for _ in range(3):
+        before = [kv.gather(layer) for layer in range(layers)]
+        for layer, (k, v) in enumerate(full):
+            kv.append(layer, k[:, :, :5 * page], v[:, :, :5 * page])
+        for layer, (k, v) in enumerate(full):
+            got_k, got_v = kv.gather(layer)
+            assert torch.equal(got_k, torch.cat((before[layer][0], k[:, :, :5 * page]), 2))
+            assert torch.equal(got_v, torch.cat((before[layer][1], v[:, :, :5 * page]), 2))
+        assert kv.evict(budget) == 5 * page and kv.offset == budget
+    assert [pool.capacity for pool in kv._pools] == capacity
+    assert kv.next_position == tokens + 15 * page
+    kv.release()

@@ -1023,29 +1023,9 @@ class PagedKVCache:
         tokens is reloaded first if it was spilled, and any other spilled
         page past the cut drops its host copy and page file.
         """
-        PT = self.page_positions
         self._drop_prefetch()
         for layer, n in enumerate(targets):
-            if n >= self._len[layer]:
-                continue
-            pages = self._pages[layer]
-            keep = n // PT  # pages wholly below the cut stay closed
-            partial = keep if n % PT else None  # page that holds the last tokens
-            cut = pages[keep:]
-            again = [p for p in cut if p.index == partial and not p.resident]
-            if again:
-                self.reload(again)
-            del pages[keep:]
-            for p in cut:
-                if p.resident:
-                    self._open_slots[layer][p.index] = p.slots
-                    p.slots = None
-                    self._resident_closed -= 1
-                else:
-                    self._drop_host(p)
-            self._len[layer] = n
-            if self._weights[layer] is not None:
-                self._weights[layer][:, :, n:] = 0
+            self._cut_layer(layer, n)
         self._offset = targets[0] if targets else 0
         if not any(self._len):
             self._dropped = 0
@@ -1053,6 +1033,36 @@ class PagedKVCache:
             B = self._batch
             self._counters_dev.copy_(torch.tensor(
                 [[self._offset] * B, [self._offset + 1] * B], dtype=torch.int32))
+
+    def _cut_layer(self, layer: int, n: int, free: bool = False) -> None:
+        """Cut one layer to n tokens.  ``free``: pages that hold none of them go back to the
+        pool, those opened ahead included."""
+        if n >= self._len[layer]:
+            return
+        PT = self.page_positions
+        pages = self._pages[layer]
+        keep = n // PT  # pages wholly below the cut stay closed
+        partial = keep if n % PT else None  # page that holds the last tokens
+        cut = pages[keep:]
+        again = [p for p in cut if p.index == partial and not p.resident]
+        if again:
+            self.reload(again)
+        del pages[keep:]
+        slots = self._open_slots[layer]
+        for p in cut:
+            if p.resident:
+                slots[p.index] = p.slots
+                p.slots = None
+                self._resident_closed -= 1
+            else:
+                self._drop_host(p)
+        self._len[layer] = n
+        if self._weights[layer] is not None:
+            self._weights[layer][:, :, n:] = 0
+        behind = [i for i in slots if i * PT >= n] if free else []
+        if behind:
+            self._pool(layer).release([s for i in behind for s in slots.pop(i)])
+            self._set_table_cols(layer, dict.fromkeys(behind))
 
     def update(self, layer: int, k: torch.Tensor, v: torch.Tensor):
         """Append, then return the layer's full K/V [B, NKV, S, D] (kv_paged.py:143-181).
@@ -2171,7 +2181,9 @@ class PagedKVCache:
         """Cut every layer to ``budget`` tokens: of each head stay the first ``sink``, the
         newest ``recent``, and of the others those that received most attention weight
         (``observe``).  Keys keep the rotation of their position; the next token's is
-        ``next_position``.  Returns how many tokens were dropped."""
+        ``next_position``.  Layers are cut one after another: one at a time has its spilled
+        pages made resident, its emptied pages go back to the pool, and ``max_bytes`` is
+        enforced before the next.  Returns how many tokens were dropped."""
         self._require_kind(0, "kv")
         budget = int(budget)
         if len(set(self._len)) != 1:
@@ -2187,6 +2199,7 @@ class PagedKVCache:
         if any(w is None for w in self._weights):
             raise ValueError("evict() needs the weights that observe() sums up in every layer")
         ctx = self._positions(S)
+        self._drop_prefetch()
         for layer in range(self.num_layers):
             sums = self._weights[layer]
             if sums.shape[2] < S:  # tokens behind them were not observed yet
@@ -2195,7 +2208,9 @@ class PagedKVCache:
             pool, table = self._resident(layer)
             keep, counts = ops.evict_select(sums, ctx, budget, sink=sink, recent=recent)
             ops.compact_kv(pool.k, pool.v, table, keep, counts, scores=sums)
-        self._trim_to([budget] * self.num_layers)
+            self._cut_layer(layer, budget, free=True)
+            self._enforce_budget()
+        self._offset = budget
         self._dropped += S - budget
         return S - budget
 
