@@ -287,3 +287,76 @@ def test_an_eviction_gives_its_pages_back_and_stays_within_the_bytes_allowed(pag
     assert [pool.capacity for pool in kv._pools] == capacity
     assert kv.next_position == tokens + 15 * page
     kv.release()
+
+
+@pytest.mark.parametrize("fails_in", [0, 1, 2])
+def test_an_eviction_whose_spilled_pages_do_not_come_back(fails_in):
+    """Before the first move the cache is as it was; after it no call takes the layers, of
+    which some are cut, for one cache."""
+    print(f"[speculative] eviction fails in layer {fails_in}", flush=True)
+    layers, tokens, page, budget = 3, 100, 32, 40
+    kv, full = filled(layers, tokens, page, 1 << 40, seed=fails_in)
+    sums = [w.clone() for w in kv._weights]
+    kv.spill([(layer, 1) for layer in range(layers)])
+    reload = kv.reload
+
+    def broken(pages=None, stream=None):
+        if any(p.layer == fails_in for p in pages):
+            raise OSError("a page file is gone")
+        return reload(pages, stream)
+
+    kv.reload = broken
+    with pytest.raises(OSError, match="gone"):
+        kv.evict(budget)
+    kv.reload = reload
+    if fails_in == 0:
+        for layer, (k, v) in enumerate(full):
+            got_k, got_v = kv.gather(layer)
+            assert torch.equal(got_k, k) and torch.equal(got_v, v)
+        assert kv.offset == tokens == kv.next_position
+        assert kv.evict(budget) == tokens - budget
+        for layer, (k, _) in enumerate(full):
+            at = rows_kept(sums[layer], tokens, budget)[..., None].expand(-1, -1, -1, D)
+            assert torch.equal(kv.gather(layer)[0], k.gather(2, at))
+        return
+    k, v = (x[:, :, :1].contiguous() for x in full[0])
+    q = torch.zeros((B, NQ, 1, D), dtype=torch.bfloat16, device="cuda")
+    for call in (lambda: kv.append(0, k, v), lambda: kv.attend(0, q), lambda: kv.gather(2),
+                 lambda: kv.attend_tree(0, q), lambda: kv.evict(budget), lambda: kv.trim(10),
+                 lambda: kv.keep_drafts(2, [1]), lambda: kv.reserve(200),
+                 lambda: kv.observe(0, q, torch.zeros((B, 1, NQ), device="cuda"))):
+        with pytest.raises(RuntimeError, match=r"evict\(\) failed"):
+            call()
+    if fails_in == 1:
+        kv.trim(0)
+    else:
+        kv.release()
+    for layer, (k, v) in enumerate(full):
+        kv.append(layer, k, v)
+    assert kv.offset == tokens == kv.next_position
+    for layer, (k, v) in enumerate(full):
+        got_k, got_v = kv.gather(layer)
+        assert torch.equal(got_k, k) and torch.equal(got_v, v)
+
+
+def test_an_eviction_that_cannot_choose_moves_nothing():
+    print("[speculative] selection fails", flush=True)
+    kv, full = filled(2, 100, 32, 1 << 40, seed=9)
+    select, calls = ops.evict_select, []
+
+    def fails(*args, **kw):
+        calls.append(0)
+        if len(calls) == 2:
+            raise MemoryError("no room for the lists")
+        return select(*args, **kw)
+
+    ops.evict_select = fails
+    try:
+        with pytest.raises(MemoryError):
+            kv.evict(40)
+    finally:
+        ops.evict_select = select
+    for layer, (k, v) in enumerate(full):
+        got_k, got_v = kv.gather(layer)
+        assert torch.equal(got_k, k) and torch.equal(got_v, v)
+    assert kv.evict(40) == 60

@@ -615,6 +615,8 @@ class PagedKVCache:
         self._weights: list[torch.Tensor | None] = [None] * L
         self._dropped = 0
         self._has_reserved = False  # captured steps may exist (until release())
+        # why the layers no longer belong together, where moving rows failed on the way
+        self._torn: str | None = None
 
     @property
     def stats(self) -> KVStats:
@@ -864,6 +866,7 @@ class PagedKVCache:
         return torch.full((self._batch,), start, dtype=torch.int32, device=self.device)
 
     def _append(self, layer: int, L: int, write) -> None:
+        self._require_whole()
         B = self._batch
         pool = self._pool(layer)
         start = self._len[layer]
@@ -905,6 +908,7 @@ class PagedKVCache:
         """
         if self._geom is None:
             raise ValueError("reserve() needs the page geometry: append once first")
+        self._require_whole()
         if self._dropped:
             raise ValueError("reserve(): after evict() a token's place in the cache is not its "
                              "position, which captured steps take it for")
@@ -973,6 +977,7 @@ class PagedKVCache:
     def advance(self, L: int = 1) -> None:
         """Host bookkeeping of ``L`` tokens written by ``append_at`` in every
         layer: lengths, closed pages, the offset."""
+        self._require_whole()
         PT = self.page_positions
         end = self._offset + L
         if end > getattr(self, "_reserved", 0):
@@ -1023,9 +1028,12 @@ class PagedKVCache:
         tokens is reloaded first if it was spilled, and any other spilled
         page past the cut drops its host copy and page file.
         """
+        if any(targets):
+            self._require_whole()
         self._drop_prefetch()
         for layer, n in enumerate(targets):
             self._cut_layer(layer, n)
+        self._torn = None
         self._offset = targets[0] if targets else 0
         if not any(self._len):
             self._dropped = 0
@@ -1109,7 +1117,13 @@ class PagedKVCache:
         self._place_spilled(layer, place)
         return lat_all
 
+    def _require_whole(self) -> None:
+        if self._torn is not None:
+            raise RuntimeError(f"{self._torn} failed after some layers were moved: trim(0) or "
+                               "release() the cache")
+
     def _require_kind(self, layer: int, kind: str) -> None:
+        self._require_whole()
         if self._geom is None or self._geom[0] != kind:
             have = "empty" if self._geom is None else self._geom[0]
             raise ValueError(f"layer {layer}: this call needs a {kind} cache, the cache is {have}")
@@ -2183,7 +2197,9 @@ class PagedKVCache:
         (``observe``).  Keys keep the rotation of their position; the next token's is
         ``next_position``.  Layers are cut one after another: one at a time has its spilled
         pages made resident, its emptied pages go back to the pool, and ``max_bytes`` is
-        enforced before the next.  Returns how many tokens were dropped."""
+        enforced before the next.  What fails before the first layer is moved leaves the
+        cache as it was; after a later failure (a spilled page that does not come back) it
+        refuses every call until it is emptied.  Returns how many tokens were dropped."""
         self._require_kind(0, "kv")
         budget = int(budget)
         if len(set(self._len)) != 1:
@@ -2200,16 +2216,20 @@ class PagedKVCache:
             raise ValueError("evict() needs the weights that observe() sums up in every layer")
         ctx = self._positions(S)
         self._drop_prefetch()
+        chosen = []
         for layer in range(self.num_layers):
             sums = self._weights[layer]
             if sums.shape[2] < S:  # tokens behind them were not observed yet
                 sums = torch.nn.functional.pad(sums, (0, S - sums.shape[2]))
                 self._weights[layer] = sums
+            chosen.append(ops.evict_select(sums, ctx, budget, sink=sink, recent=recent))
+        for layer, (keep, counts) in enumerate(chosen):
             pool, table = self._resident(layer)
-            keep, counts = ops.evict_select(sums, ctx, budget, sink=sink, recent=recent)
-            ops.compact_kv(pool.k, pool.v, table, keep, counts, scores=sums)
+            self._torn = "evict()"  # until every layer is cut
+            ops.compact_kv(pool.k, pool.v, table, keep, counts, scores=self._weights[layer])
             self._cut_layer(layer, budget, free=True)
             self._enforce_budget()
+        self._torn = None
         self._offset = budget
         self._dropped += S - budget
         return S - budget
