@@ -360,3 +360,34 @@ def test_an_eviction_that_cannot_choose_moves_nothing():
         got_k, got_v = kv.gather(layer)
         assert torch.equal(got_k, k) and torch.equal(got_v, v)
     assert kv.evict(40) == 60
+
+
+@pytest.mark.parametrize("fails_in", [0, 2])
+def test_drafts_whose_spilled_pages_do_not_come_back_stay_as_they_are(fails_in):
+    print(f"[speculative] keep_drafts fails in layer {fails_in}", flush=True)
+    layers, tokens = 3, 130
+    kv, full = filled(layers, tokens, 32, 1 << 40, seed=20 + fails_in)
+    sums = [w.clone() for w in kv._weights]
+    kv.spill([(layer, 3) for layer in range(layers)])  # tokens 96 .. 127
+    reload = kv.reload
+
+    def broken(pages=None, stream=None):
+        if any(p.layer == fails_in for p in pages):
+            raise OSError("a page file is gone")
+        return reload(pages, stream)
+
+    kv.reload = broken
+    with pytest.raises(OSError, match="gone"):
+        kv.keep_drafts(9, [1, 4, 8])
+    kv.reload = reload
+    assert kv.layer_lengths() == (tokens,) * layers and kv.offset == tokens
+    for layer, (k, v) in enumerate(full):
+        got_k, got_v = kv.gather(layer)
+        assert torch.equal(got_k, k) and torch.equal(got_v, v)
+        assert torch.equal(kv._weights[layer], sums[layer])
+    kv.keep_drafts(9, [1, 4, 8])
+    stay = list(range(tokens - 9)) + [tokens - 9 + i for i in (1, 4, 8)]
+    for layer, (k, v) in enumerate(full):
+        got_k, got_v = kv.gather(layer)
+        assert torch.equal(got_k, k[:, :, stay]) and torch.equal(got_v, v[:, :, stay])
+        assert torch.equal(kv._weights[layer][:, :, :len(stay)], sums[layer][:, :, stay])

@@ -1004,7 +1004,10 @@ class PagedKVCache:
         left alone, and an attached ``dsa`` state is trimmed with the cache."""
         if isinstance(length, bool) or not isinstance(length, int) or length < 0:
             raise ValueError("trim length must be a non-negative integer")
-        self._trim_to([min(n, length) for n in self._len])
+        targets = [min(n, length) for n in self._len]
+        if any(targets):
+            self._require_whole()
+        self._trim_to(targets)
         dsa = getattr(self, "dsa", None)
         if dsa is not None:
             dsa.trim(length)
@@ -1017,6 +1020,8 @@ class PagedKVCache:
             raise ValueError("invalid per-layer KV rollback lengths")
         if any(t > n for t, n in zip(targets, self._len)):
             raise ValueError("cannot grow KV during rollback")
+        if any(targets):
+            self._require_whole()
         self._trim_to(list(targets))
 
     def _trim_to(self, targets: list[int]) -> None:
@@ -1028,8 +1033,6 @@ class PagedKVCache:
         tokens is reloaded first if it was spilled, and any other spilled
         page past the cut drops its host copy and page file.
         """
-        if any(targets):
-            self._require_whole()
         self._drop_prefetch()
         for layer, n in enumerate(targets):
             self._cut_layer(layer, n)
@@ -2139,7 +2142,8 @@ class PagedKVCache:
     def keep_drafts(self, drafts: int, path) -> None:
         """Of every layer's newest ``drafts`` tokens keep those of ``path`` (ascending draft
         indices, [n] for all sequences or [B, n]) and drop the others: the accepted branch
-        of a tree.  The cache is then ``drafts - n`` tokens shorter."""
+        of a tree.  The cache is then ``drafts - n`` tokens shorter.  Spilled pages that hold
+        drafts are made resident first, of all layers; where that fails no row has moved."""
         self._require_kind(0, "kv")
         drafts = int(drafts)
         B = self._batch
@@ -2159,11 +2163,16 @@ class PagedKVCache:
             raise ValueError(f"{drafts} drafts but a layer holds {min(self._len)} tokens")
         if n and n < drafts:
             counts = torch.full((B,), n, dtype=torch.int32, device=self.device)
-            for layer in range(self.num_layers):
-                first = self._len[layer] - drafts
+            moves = []
+            for layer, length in enumerate(self._len):  # what may fail, before a row is moved
+                first = length - drafts
                 pool, table = self._resident(layer, first)
-                ops.compact_kv(pool.k, pool.v, table, (path + first)[:, None].contiguous(), counts,
-                               start=self._positions(first), scores=self._weights[layer])
+                moves.append((pool, table, (path + first)[:, None].contiguous(),
+                              self._positions(first)))
+            for layer, (pool, table, keep, start) in enumerate(moves):
+                ops.compact_kv(pool.k, pool.v, table, keep, counts, start=start,
+                               scores=self._weights[layer])
+                self._torn = "keep_drafts()"  # until every layer is cut
         self._trim_to([length - drafts + n for length in self._len])
 
     def observe(self, layer: int, q: torch.Tensor, lse: torch.Tensor,
