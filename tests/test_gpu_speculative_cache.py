@@ -391,3 +391,33 @@ def test_drafts_whose_spilled_pages_do_not_come_back_stay_as_they_are(fails_in):
         got_k, got_v = kv.gather(layer)
         assert torch.equal(got_k, k[:, :, stay]) and torch.equal(got_v, v[:, :, stay])
         assert torch.equal(kv._weights[layer][:, :, :len(stay)], sums[layer][:, :, stay])
+
+
+@pytest.mark.parametrize("cut", ["all drafts", "trim", "each layer"])
+def test_a_rollback_whose_spilled_pages_do_not_come_back_cuts_no_layer(cut):
+    print(f"[speculative] rollback fails: {cut}", flush=True)
+    layers, tokens = 3, 130
+    kv, full = filled(layers, tokens, 32, 1 << 40, seed=30)
+    kv.spill([(layer, 3) for layer in range(layers)])  # tokens 96 .. 127
+    reload = kv.reload
+
+    def broken(pages=None, stream=None):
+        if any(p.layer == 2 for p in pages):
+            raise OSError("a page file is gone")
+        return reload(pages, stream)
+
+    call = {"all drafts": lambda: kv.keep_drafts(9, []), "trim": lambda: kv.trim(tokens - 9),
+            "each layer": lambda: kv.trim_layer_lengths([tokens - 9] * layers)}[cut]
+    kv.reload = broken
+    with pytest.raises(OSError, match="gone"):
+        call()
+    kv.reload = reload
+    assert kv.layer_lengths() == (tokens,) * layers and kv.offset == tokens
+    for layer, (k, v) in enumerate(full):
+        got_k, got_v = kv.gather(layer)
+        assert torch.equal(got_k, k) and torch.equal(got_v, v)
+    call()
+    assert kv.layer_lengths() == (tokens - 9,) * layers and kv.offset == tokens - 9
+    for layer, (k, v) in enumerate(full):
+        got_k, got_v = kv.gather(layer)
+        assert torch.equal(got_k, k[:, :, :-9]) and torch.equal(got_v, v[:, :, :-9])

@@ -1029,11 +1029,18 @@ class PagedKVCache:
 
         Closed pages past the cut become open pages again: a resident page
         keeps its slots and table column (so a reserved, captured decode
-        step still finds them), the page that now holds the last partial
-        tokens is reloaded first if it was spilled, and any other spilled
-        page past the cut drops its host copy and page file.
+        step still finds them), the pages that now hold the last partial
+        tokens are reloaded if they were spilled, before any layer is cut, and
+        any other spilled page past the cut drops its host copy and page file.
         """
         self._drop_prefetch()
+        partial = [pages[n // self.page_positions]
+                   for n, length, pages in zip(targets, self._len, self._pages)
+                   if n < length and n % self.page_positions
+                   and n // self.page_positions < len(pages)]
+        again = [p for p in partial if not p.resident]
+        if again:
+            self.reload(again)
         for layer, n in enumerate(targets):
             self._cut_layer(layer, n)
         self._torn = None
@@ -1046,18 +1053,15 @@ class PagedKVCache:
                 [[self._offset] * B, [self._offset + 1] * B], dtype=torch.int32))
 
     def _cut_layer(self, layer: int, n: int, free: bool = False) -> None:
-        """Cut one layer to n tokens.  ``free``: pages that hold none of them go back to the
-        pool, those opened ahead included."""
+        """Cut one layer to n tokens; the page that holds the last of them, if it is not
+        full, is resident.  ``free``: pages that hold none of them go back to the pool, those
+        opened ahead included."""
         if n >= self._len[layer]:
             return
         PT = self.page_positions
         pages = self._pages[layer]
         keep = n // PT  # pages wholly below the cut stay closed
-        partial = keep if n % PT else None  # page that holds the last tokens
         cut = pages[keep:]
-        again = [p for p in cut if p.index == partial and not p.resident]
-        if again:
-            self.reload(again)
         del pages[keep:]
         slots = self._open_slots[layer]
         for p in cut:
