@@ -12,6 +12,7 @@ import torch
 
 from paged_inputs import lens_tensor
 from voom_amd import _lib, ops
+from voom_amd.kv_paged import PagedKVCache
 from voom_amd.page_pool import v_slot_shape
 
 HALF_BF16, FP32 = 2.0 ** -8, 2.0 ** -17
@@ -240,3 +241,61 @@ def test_abi_refusals():
     refused("page_tokens", page=48)
     refused("block table", pages=1 << 25)
     refused("eps", eps=-1.0)
+
+
+def test_checked_places_and_positions():
+    def i32(x):
+        return torch.tensor(x, dtype=torch.int32)
+
+    table = i32([[3, 5], [4, -1]])  # pages of 8 tokens in a pool of 6
+    good = dict(positions=i32([[0, 9, 4], [2, 2, 77]]), rope_rows=10, block_table=table,
+                start=i32([13, 6]), new_lens=i32([3, 2]), num_slots=6, page=8)
+    ops.check_new_tokens(**good)
+    ops.check_new_tokens(**{**good, "new_lens": i32([0, 0]), "start": i32([99, -4])})
+    for match, change in (("positions", dict(rope_rows=9)), ("positions", dict(new_lens=None)),
+                          ("positions", dict(positions=i32([[-1, 0, 0], [0, 0, 0]]))),
+                          ("new_lens", dict(new_lens=i32([4, 0]))),
+                          ("new_lens", dict(new_lens=i32([-1, 0]))),
+                          ("block table", dict(start=i32([14, 6]))),
+                          ("block table", dict(start=i32([-1, 6]))),
+                          ("block table", dict(start=i32([2 ** 31 - 2, 6]))),
+                          ("block table", dict(block_table=table[:, :0])),
+                          ("slot ids", dict(start=i32([13, 7]))),
+                          ("slot ids", dict(num_slots=5))):
+        with pytest.raises(ValueError, match=match):
+            ops.check_new_tokens(**{**good, **change})
+
+
+@pytest.mark.gpu
+def test_checked_calls_raise_and_the_cache_refuses_positions_past_the_tables():
+    print("[qk] checked calls", flush=True)
+    B, L, nq, nkv, hd, PT, ctx = 2, 6, 2, 1, 64, 32, 64
+    st = make(B, L, nq, nkv, hd, 64, PT, ctx)
+    k0 = st["k"].clone()
+
+    def call(positions, start):
+        return ops.qk_norm_rope_append(st["qkv"], st["cos"], st["sin"], positions, st["k"],
+                                       st["v"], st["table"], lens_tensor(start), nq, nkv)
+
+    at = torch.arange(L, dtype=torch.int32, device="cuda").repeat(B, 1)
+    ops.set_bounds_checks(True)
+    try:
+        for match, positions, start in (("positions", at + 64, [0, 0]),
+                                        ("block table", at, [0, 59])):
+            with pytest.raises(ValueError, match=match):
+                call(positions, start)
+        assert torch.equal(st["k"], k0)
+        q = call(at + 63, [0, 58])
+    finally:
+        ops.set_bounds_checks(False)
+    assert torch.equal(q, call(at + 63, [0, 58]))
+
+    kv = PagedKVCache(1, 1 << 40, page_positions=PT)
+    cos, sin = ops.rope_cache(10, hd, 1e4)
+    kv.append_qkv(0, st["qkv"], cos, sin, nq, nkv)
+    with pytest.raises(ValueError, match="6 tokens from position 6 on, but cos and sin hold 10"):
+        kv.append_qkv(0, st["qkv"], cos, sin, nq, nkv)
+    assert kv.offset == L
+    kv.append_qkv(0, st["qkv"][:, :4].contiguous(), cos, sin, nq, nkv)
+    kv.append_qkv(0, st["qkv"][:, :0].contiguous(), cos[:3], sin[:3], nq, nkv)
+    assert kv.offset == 10

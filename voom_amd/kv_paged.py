@@ -837,6 +837,9 @@ class PagedKVCache:
         self._set_geometry(("kv", B, num_kv_heads, W // heads), qkv.dtype)
         if positions is None:
             first = self._len[layer] + self._dropped
+            if L and first + L > cos.shape[0]:
+                raise ValueError(f"{L} tokens from position {first} on, but cos and sin hold "
+                                 f"{cos.shape[0]} positions")
             positions = torch.arange(first, first + L, dtype=torch.int32,
                                      device=self.device).repeat(B, 1)
         q = qkv.new_empty((B, num_q_heads, 0, W // heads))

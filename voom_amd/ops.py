@@ -98,13 +98,15 @@ def workspace(device: torch.device, nbytes: int, tag: int = 0) -> torch.Tensor:
 # Off by default (each check costs a launch and a host synchronisation).  When
 # on, every attention call first counts the slot / page ids and positions its
 # kernel would read out of range and raises ValueError instead of attending:
-# the kernels themselves read slot 0 for a bad id and clamp a bad position.
+# the kernels themselves read slot 0 for a bad id and clamp a bad position.  The
+# calls that move cached rows check their lists and qk_norm_rope_append its places
+# (rows without one are left out) and positions.
 _BOUNDS_CHECKS = os.environ.get("VOOM_BOUNDS_CHECK", "") not in ("", "0")
 
 
 def set_bounds_checks(enabled: bool) -> None:
-    """Turn the debug bounds checks of the attention calls on or off (also
-    VOOM_BOUNDS_CHECK=1 in the environment)."""
+    """Turn the debug bounds checks of the attention calls, compact_kv and
+    qk_norm_rope_append on or off (also VOOM_BOUNDS_CHECK=1 in the environment)."""
     global _BOUNDS_CHECKS
     _BOUNDS_CHECKS = bool(enabled)
 
@@ -627,6 +629,30 @@ def compact_kv(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Te
         _lib.check(rc, "voom_compact_kv")
 
 
+def check_new_tokens(positions: torch.Tensor, rope_rows: int, block_table: torch.Tensor,
+                     start: torch.Tensor, new_lens: torch.Tensor | None, num_slots: int,
+                     page: int) -> None:
+    """Raise ValueError unless every new token t < new_lens[b] has a position in
+    [0, rope_rows) and a page of the pool at its place start[b] + t."""
+    if positions.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("bounds checks synchronise and cannot run under graph capture")
+    B, L = positions.shape
+    max_pages = block_table.shape[1]
+    if new_lens is not None and bool(((new_lens < 0) | (new_lens > L)).any()):
+        raise ValueError(f"new_lens lie outside [0, {L}]")
+    t = torch.arange(L, device=positions.device)
+    used = t < (torch.full_like(start, L) if new_lens is None else new_lens)[:, None]
+    if bool((used & ((positions < 0) | (positions >= rope_rows))).any()):
+        raise ValueError(f"positions lie outside the RoPE tables [0, {rope_rows})")
+    at = start.long()[:, None] + t
+    if bool((used & ((at < 0) | (at >= max_pages * page))).any()):
+        raise ValueError(f"new tokens lie outside the block table [0, {max_pages * page})")
+    if max_pages:
+        slot = block_table.gather(1, (at // page).clamp(0, max_pages - 1))
+        if bool((used & ((slot < 0) | (slot >= num_slots))).any()):
+            raise ValueError(f"new tokens fall on slot ids outside [0, {num_slots})")
+
+
 def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                         positions: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                         block_table: torch.Tensor, start: torch.Tensor, num_q_heads: int,
@@ -642,7 +668,9 @@ def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
     positions[b, t] (int32 [B, L]) of cos / sin [P, rotary / 2] fp32 (rope_cache's), dims
     (i, i + rotary / 2) as a pair, or (2 i, 2 i + 1) with ``interleaved``.  Returns q
     [B, nq, L, hd]; K and V of token t land at cache position start[b] + t (start [B]
-    int32) for t < new_lens[b] (None: all).  One rounding to bf16 at the end.
+    int32) for t < new_lens[b] (None: all).  One rounding to bf16 at the end.  Positions
+    past the tables are clamped and tokens without a page left out; set_bounds_checks
+    refuses both.
     """
     here = _require_here(qkv, cos, sin, positions, k_pool, v_pool, block_table, start, q_weight,
                          k_weight, new_lens)
@@ -679,6 +707,8 @@ def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
         raise ValueError(f"k_weight must be bfloat16 [{hd}]")
     q = qkv.new_empty((B, nq, L, hd))
     if B and L:
+        if _BOUNDS_CHECKS:
+            check_new_tokens(positions, cos_shape[0], block_table, start, new_lens, slots, PT)
         rc = _lib.lib().voom_qk_norm_rope_append(
             qkv.data_ptr(), None if q_weight is None else q_weight.data_ptr(),
             None if k_weight is None else k_weight.data_ptr(), float(eps), cos.data_ptr(),
