@@ -240,7 +240,7 @@ int voom_paged_gqa_tree(const void* q, const void* k_pool, const void* v_pool,
  * for p < ctx; the rest of out stays as it is.
  *   q       [batch, num_q_heads, window, head_dim] bf16, head_dim 64 or 128
  *   lse     [batch, window, num_q_heads] fp32 natural log of those queries' attention
- *           (of -inf: the row adds nothing)
+ *           (of -inf: the row adds nothing; of NaN: what it sees becomes NaN)
  *   scores  [batch, num_kv_heads, score_tokens] fp32; out the same array or another one
  * Contexts are clamped to the block table and to score_tokens.
  *

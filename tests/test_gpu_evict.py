@@ -135,6 +135,27 @@ def test_rows_without_a_sum_and_bad_values_stay_where_they_are():
     assert (same == 3).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [90, 700])
+def test_a_row_whose_lse_is_nan_reaches_what_it_sees_and_nothing_else(S):
+    print(f"[observe] NaN and infinite lse, S={S}", flush=True)
+    B, NQ, NKV, D, L = 1, 4, 2, 128, 5
+    q, k, v = inputs(B, NQ, NKV, D, S, L, seed=14)
+    k_pool, _, table = cache(k, v, 32)
+    lse, _ = window_reference(q, k, [S], [L], D ** -0.5)
+    lse = lse.float().cuda()
+    less = lse.clone()
+    lse[0, 1, 0], less[0, 1, 0] = NAN, -INF     # a head of kv head 0; sees up to S - 4
+    lse[0, 3, 3], less[0, 3, 3] = INF, -INF     # exp(-inf) is 0
+    got, without = (ops.paged_gqa_observe(q, x, k_pool, table, lens_tensor([S]),
+                                          torch.zeros((B, NKV, S), device="cuda"))
+                    for x in (lse, less))
+    torch.cuda.synchronize()
+    assert torch.isnan(got[0, 0, :S - 3]).all()
+    assert torch.equal(got[0, 0, S - 3:], without[0, 0, S - 3:])
+    assert torch.equal(got[0, 1], without[0, 1])
+
+
 # ---- the selection ------------------------------------------------------------------
 
 

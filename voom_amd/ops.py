@@ -441,7 +441,8 @@ def paged_gqa_observe(q: torch.Tensor, lse: torch.Tensor, k_pool: torch.Tensor,
     fp32 [B, NKV, tokens], which takes
         scores[b, h, p] + sum_{t, g} exp(scale q[b, g, t] . k[p] - lse[b, t, g])
     over the window's tokens at or behind p and the q heads of kv head h, for p < ctx;
-    what is behind the context is left as it is.
+    what is behind the context is left as it is.  A row whose lse is -inf adds nothing, one
+    whose lse is NaN makes the sums of the tokens that it sees NaN.
     """
     if q.dim() == 4 and lse.dim() == 2 and q.shape[2] == 1:
         lse = lse[:, None]
