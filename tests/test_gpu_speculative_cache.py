@@ -421,3 +421,22 @@ def test_a_rollback_whose_spilled_pages_do_not_come_back_cuts_no_layer(cut):
     for layer, (k, v) in enumerate(full):
         got_k, got_v = kv.gather(layer)
         assert torch.equal(got_k, k[:, :, :-9]) and torch.equal(got_v, v[:, :, :-9])
+
+
+def test_a_released_cache_forgets_what_was_reserved():
+    """Its counters are of the batch before: a later batch of another size is trimmed, cut to
+    its accepted drafts and evicted as in a new cache."""
+    print("[speculative] released after reserve", flush=True)
+    kv = PagedKVCache(1, 1 << 40, page_positions=32)
+    k = torch.randn((3, NKV, 60, D), device="cuda").to(torch.bfloat16)
+    kv.append(0, k[:1, :, :20].contiguous(), k[:1, :, :20].contiguous())
+    kv.reserve(64)
+    kv.release()
+    kv.append(0, k, k)
+    with pytest.raises(ValueError, match="reserved 0"):
+        kv.advance()
+    kv.keep_drafts(4, [1, 3])
+    assert torch.equal(kv.gather(0)[0], k[:, :, list(range(56)) + [57, 59]])
+    kv.trim(50)
+    kv._weights[0] = torch.rand((3, NKV, 64), device="cuda")
+    assert kv.evict(30) == 20 and kv.offset == 30 and kv.next_position == 50

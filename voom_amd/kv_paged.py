@@ -615,6 +615,8 @@ class PagedKVCache:
         self._weights: list[torch.Tensor | None] = [None] * L
         self._dropped = 0
         self._has_reserved = False  # captured steps may exist (until release())
+        self._reserved = 0  # tokens, by reserve(); and its position counters on the device
+        self._counters_dev: torch.Tensor | None = None
         # why the layers no longer belong together, where moving rows failed on the way
         self._torn: str | None = None
 
@@ -983,8 +985,8 @@ class PagedKVCache:
         self._require_whole()
         PT = self.page_positions
         end = self._offset + L
-        if end > getattr(self, "_reserved", 0):
-            raise ValueError(f"advance past the reserved {getattr(self, '_reserved', 0)} tokens")
+        if end > self._reserved:
+            raise ValueError(f"advance past the reserved {self._reserved} tokens")
         for layer in range(self.num_layers):
             self._len[layer] = end
             pages = self._pages[layer]
@@ -1050,7 +1052,7 @@ class PagedKVCache:
         self._offset = targets[0] if targets else 0
         if not any(self._len):
             self._dropped = 0
-        if getattr(self, "_counters_dev", None) is not None:
+        if self._counters_dev is not None:
             B = self._batch
             self._counters_dev.copy_(torch.tensor(
                 [[self._offset] * B, [self._offset + 1] * B], dtype=torch.int32))
