@@ -172,3 +172,37 @@ def test_captured_step_survives_a_grown_workspace():
         kv_g.advance(1)
         out.append(int(nxt[0]))
     assert out == eager
+
+
+def test_logits_after_an_eviction_match_hf_llama_without_the_dropped_tokens():
+    """The prompt sees all of itself; of the tokens behind the eviction each sees the kept ones
+    alone, at its true position.  Bars as of the teacher-forced logits (the dropped tokens
+    would move these logits by 35 %, positions without them by 12 %)."""
+    print("[decoder] logits after an eviction vs HF LlamaForCausalLM (4 layers)", flush=True)
+    cfg = DecoderConfig(num_hidden_layers=4)
+    weights = random_weights(cfg, seed=0)
+    P, budget, more = 90, 50, 3
+    ids = torch.randint(0, cfg.vocab_size, (1, P + more),
+                        generator=torch.Generator().manual_seed(8))
+    dec = PagedDecoder(cfg, weights)
+    kv = dec.new_cache(page_positions=32)
+    dec.forward(ids[:, :P].cuda(), kv, last_only=True)
+    sums = torch.rand(P, generator=torch.Generator().manual_seed(9))
+    kv._weights = [sums.cuda().expand(1, cfg.num_key_value_heads, P).contiguous()
+                   for _ in range(cfg.num_hidden_layers)]  # one choice for all heads and layers
+    assert kv.evict(budget, sink=2, recent=8) == P - budget
+    sums[:2] = sums[P - 8:] = 2.0
+    dropped = sums.sort(descending=True).indices[budget:]
+    sees = torch.ones((P + more, P + more), dtype=torch.bool).tril()
+    sees[P:, dropped] = False
+    mask = torch.zeros(sees.shape).masked_fill(~sees, torch.finfo(torch.float32).min)[None, None]
+    with torch.no_grad():
+        ref = hf_model(cfg, weights)(ids, attention_mask=mask).logits[0, P:].numpy()
+    got = [dec.forward(ids[:, t:t + 1].cuda(), kv)[0] for t in range(P, P + more)]
+    got = torch.cat(got, 0).cpu().numpy()
+    assert kv.offset == budget + more and kv.next_position == P + more
+    rel = np.linalg.norm(got - ref, axis=-1) / np.linalg.norm(ref, axis=-1)
+    print(f"[decoder] rel L2 max {rel.max():.4f}, abs max {np.abs(got - ref).max():.4f}",
+          flush=True)
+    assert rel.max() <= 3e-2
+    assert np.abs(got - ref).max() <= 8e-2
