@@ -15,10 +15,10 @@
 // tokens, 256 at D = 64) of all (sequence, kv head) segments lie end to end, as often as
 // the window's rows go through the keys and after kLead that stand for what a segment costs
 // besides, and are dealt out evenly (32 sequences of up to 4,000 tokens, 32/8 heads: 32 us,
-// without kLead 62).  K goes straight into LDS (1 KiB loads) through a ring of four 32 KiB
+// without kLead 61).  K goes straight into LDS (1 KiB loads) through a ring of four 32 KiB
 // stages, three of them under way; loaded into operand registers instead, 64 bytes of
 // a row at a time, the same keys took 147 us with no work on them, where 16 sequences of
-// 1k-32k tokens, 32/8 heads, took 136 with all of it (128 since kLead).
+// 1k-32k tokens, 32/8 heads, took 136 with all of it (118-129 since kLead).
 //
 // Eight wavefronts compute, RW of them on other rows (16 NT each, queries in registers)
 // and 8 / RW on other keys of the stage:
