@@ -13,7 +13,7 @@ import torch
 from paged_inputs import trees
 from voom_amd import ops
 from voom_amd.decoder import DecoderConfig, PagedDecoder, random_weights
-from voom_amd.kv_paged import PagedKVCache
+from voom_amd.kv_paged import KVIntegrityError, PagedKVCache
 
 pytestmark = pytest.mark.gpu
 
@@ -440,3 +440,28 @@ def test_a_released_cache_forgets_what_was_reserved():
     kv.trim(50)
     kv._weights[0] = torch.rand((3, NKV, 64), device="cuda")
     assert kv.evict(30) == 20 and kv.offset == 30 and kv.next_position == 50
+
+
+def test_an_eviction_reports_earlier_damage_before_it_moves_a_row():
+    """Damage that attention met in the second layer's spilled pages is raised by the next
+    call, which must not be in the middle of an eviction."""
+    print("[speculative] pending integrity error", flush=True)
+    kv, full = filled(2, 100, 32, 1 << 40, seed=40)
+    sums = [w.clone() for w in kv._weights]
+    kv.spill([(1, 1)])
+    torch.cuda.synchronize()
+    page = kv._pages[1][1]
+    byte = page.host.part(1, page.host_j)
+    byte[100] ^= 0x10
+    kv.attend(1, torch.zeros((B, NQ, 1, D), dtype=torch.bfloat16, device="cuda"))
+    torch.cuda.synchronize()
+    byte[100] ^= 0x10
+    with pytest.raises(KVIntegrityError):
+        kv.evict(40)
+    for layer, (k, v) in enumerate(full):
+        got_k, got_v = kv.gather(layer)
+        assert torch.equal(got_k, k) and torch.equal(got_v, v)
+    assert kv.evict(40) == 60
+    for layer, (k, _) in enumerate(full):
+        at = rows_kept(sums[layer], 100, 40)[..., None].expand(-1, -1, -1, D)
+        assert torch.equal(kv.gather(layer)[0], k.gather(2, at))

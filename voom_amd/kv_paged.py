@@ -2232,6 +2232,7 @@ class PagedKVCache:
             return 0
         if any(w is None for w in self._weights):
             raise ValueError("evict() needs the weights that observe() sums up in every layer")
+        self.check_integrity()  # what an earlier call left to report
         ctx = self._positions(S)
         self._drop_prefetch()
         chosen = []
