@@ -652,3 +652,13 @@ def test_destinations_that_a_move_reads_are_refused():
         ops.check_destination(table, i32(dst), lists, lens, None if start is None else
                               i32(start), 8)
     ops.check_destination(table, table, lists, i32([0, 0]), None, 8)
+
+
+@pytest.mark.gpu
+def test_a_selection_without_heads_is_refused():
+    """(its lengths would not be written)"""
+    for shape in ((2, 0, 10), (2, 3, 0)):
+        with pytest.raises(ValueError, match="scores"):
+            ops.evict_select(torch.zeros(shape, device="cuda"), lens_tensor([4, 4]), 5)
+    keep, lens = ops.evict_select(torch.zeros((0, 3, 10), device="cuda"), lens_tensor([]), 5)
+    assert keep.shape == (0, 3, 5) and lens.shape == (0,)

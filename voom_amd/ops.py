@@ -487,7 +487,7 @@ def evict_select(scores: torch.Tensor, ctx_lens: torch.Tensor, budget: int, *, s
     """
     here = _require_here(scores, ctx_lens)
     shape = scores.shape
-    if scores.dtype is not torch.float32 or len(shape) != 3 or shape[2] == 0:
+    if scores.dtype is not torch.float32 or len(shape) != 3 or 0 in shape[1:]:
         raise ValueError("scores must be float32 [B, NKV, tokens]")
     B, NKV, cap = shape
     if not _is_i32(ctx_lens, B):
@@ -497,7 +497,7 @@ def evict_select(scores: torch.Tensor, ctx_lens: torch.Tensor, budget: int, *, s
         raise ValueError(f"sink {sink} and recent {recent} must fit the budget {budget}")
     keep = ctx_lens.new_empty((B, NKV, budget))
     keep_lens = ctx_lens.new_empty((B,))
-    if B and NKV:
+    if B:
         lib = _lib.lib()
         need = lib.voom_evict_select_workspace_bytes(B, NKV, cap) if cap > 32768 else 0
         ws = scores.new_empty(need, dtype=torch.uint8) if need else None
