@@ -293,6 +293,85 @@ int voom_compact_kv(void* k_pool, void* v_pool, const int32_t* block_table,
                     hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Attention of ragged chunks over paged K/V: the newest tokens of each sequence, one of a
+ * running request or a part of a prompt, with the scores and masks of models that cap them,
+ * lower them with the distance or look back a limited way (the reference: plain causal
+ * windows of one length, runtime/layer_runner.py:166-180).
+ *
+ * Sequence b holds ctx_lens[b] tokens, the newest of them with queries.  The token at
+ * position i scores the one at j
+ *   s = scale q.k,  s = softcap * tanh(s / softcap) (softcap > 0),
+ *   s -= slopes[head] * |i - j| (slopes not NULL)
+ * and sees it where j <= i and (window > 0) i - j < window, or where j < prefix_lens[b].
+ *   q       packed [rows, num_q_heads, head_dim] bf16 with starts [batch + 1] int32,
+ *           ascending: sequence b has rows starts[b] .. starts[b + 1] - 1; or (starts NULL,
+ *           rows 0) [batch, num_q_heads, tokens, head_dim], new_lens [batch] int32 (NULL:
+ *           `tokens` each) of which are new tokens
+ *   out     packed [rows, num_q_heads, head_dim], else [batch, tokens, num_q_heads,
+ *           head_dim] bf16
+ *   lse     the same without head_dim, fp32 natural log, or NULL
+ *   slopes  [num_q_heads] fp32 or NULL;  prefix_lens [batch] int32 or NULL
+ * Rows that see nothing, and those behind a padded sequence's new tokens, give 0 and -inf;
+ * packed rows of no sequence are left as they are.  Where more tokens are new than cached,
+ * the first of them lie before the cache.  Pools, heads, head_dim, page_tokens and bad slot
+ * ids as for voom_paged_gqa_tree; at most 1024 sequences.  The workspace needs no
+ * initialisation; calls that overlap need one each.
+ * ------------------------------------------------------------------------- */
+size_t voom_paged_gqa_chunk_workspace_bytes(int batch, int rows, int tokens, int num_q_heads,
+                                            int num_kv_heads, int head_dim, int page_tokens,
+                                            int max_pages, int window);
+int voom_paged_gqa_chunk(const void* q, const void* k_pool, const void* v_pool,
+                         const int32_t* block_table, const int32_t* ctx_lens,
+                         const int32_t* starts, const int32_t* new_lens, const float* slopes,
+                         const int32_t* prefix_lens, void* out, float* lse, void* workspace,
+                         size_t ws_bytes, int batch, int rows, int tokens, int num_q_heads,
+                         int num_kv_heads, int head_dim, int page_tokens, int max_pages,
+                         int num_slots, int window, float scale, float softcap,
+                         hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Beam search.  No reference counterpart (its decode loop is greedy or samples one
+ * continuation, runtime/engine.py:8459-8503).
+ *
+ * voom_beam_select: of all continuations of a request's beams,
+ *   c(j, v) = scores[j] + logits[j][v] - log sum_u exp logits[j][u],
+ * the `beams` largest, equal ones the lowest (j, v) first.  A beam whose last token is
+ * end_token (last not NULL) has one continuation, that token at scores[j].  One that is NaN,
+ * or of a beam whose score or sum of exponentials is not finite, counts as -inf.  The best
+ * continuation of a beam stays in the beam's row, the others, best first, take the rows of
+ * beams that nothing goes on from, lowest first.
+ *   logits   [batch, beams, vocab] VOOM_DTYPE_BF16 or _F32
+ *   scores   [batch, beams] fp32;  last [batch, beams] int64 or NULL
+ *   scores_out fp32, tokens int64, parents int32  [batch, beams], by row
+ *   shared   [batch, beams, beams] int32 or NULL: leading tokens that rows have in common.
+ *            Then first [batch, beams] takes how many a row already has of its new parent's
+ *            ctx_lens[b] tokens, and shared_out (another array) what rows have in common
+ *            once they are copied
+ * 1 to 32 beams, up to 2^24 tokens.  The workspace (voom_beam_select_workspace_bytes, 8-byte
+ * aligned) needs no initialisation; calls that overlap need one each.
+ *
+ * voom_fork_kv: in every layer, row j of request b takes the K and V of tokens first[b][j]
+ * (NULL: 0) .. ctx_lens[b] - 1 of row parents[b][j], bit for bit; a row that is its own
+ * parent is left alone, and so is every other token.  A row that others go on from must be
+ * its own parent.
+ *   k_pools, v_pools, block_tables, max_pages, num_slots  host arrays [num_layers]; block
+ *            tables int32 [batch * beams, max_pages], pools as for voom_append_kv
+ *   ctx_lens [batch], parents and first [batch, beams] int32
+ * head_dim a multiple of 8 up to 1024, page_tokens a power of two in [8, 4096].  Rows past
+ * the tables and slot ids outside the pools are left out.  One launch for up to 64 layers.
+ * ------------------------------------------------------------------------- */
+size_t voom_beam_select_workspace_bytes(int batch, int beams, int vocab);
+int voom_beam_select(const void* logits, int dtype, const float* scores, const int64_t* last,
+                     int64_t end_token, const int32_t* shared, const int32_t* ctx_lens,
+                     float* scores_out, int64_t* tokens, int32_t* parents, int32_t* first,
+                     int32_t* shared_out, void* workspace, size_t ws_bytes, int batch, int beams,
+                     int vocab, hipStream_t stream);
+int voom_fork_kv(void* const* k_pools, void* const* v_pools, const int32_t* const* block_tables,
+                 const int* max_pages, const int* num_slots, int num_layers,
+                 const int32_t* ctx_lens, const int32_t* parents, const int32_t* first, int batch,
+                 int beams, int num_kv_heads, int head_dim, int page_tokens, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
  * RMS norm of every query and key head, rotary positions, and the page write of
  * new tokens in one launch (the RoPE and cache write of
  * runtime/layer_runner.py:98-109,158, with per-head norms and positions that
@@ -504,6 +583,18 @@ int voom_rope_split(const void* qkv, const float* cos_table, const float* sin_ta
                     int head_dim, hipStream_t stream);
 int voom_silu_mul(const void* gate_up, void* out, int rows, int intermediate,
                   hipStream_t stream);
+
+/* voom_add_post_norm: the norm behind a block, the residual add and the norm before the
+ * next block, for models that norm on both sides (no reference counterpart):
+ *   y = x + scale * gate * post_weight * delta / sqrt(mean delta^2 + eps)
+ *   x_out = bf16(y), out = bf16(weight * y / sqrt(mean y^2 + eps))
+ * in fp32, out of the unrounded y.  x, delta, x_out (may be x), out [rows, hidden] bf16,
+ * post_weight, weight [hidden]; gate [rows / gate_rows, hidden] bf16, one for every
+ * gate_rows consecutive rows, or NULL.  hidden a multiple of 8 up to 8192. */
+int voom_add_post_norm(const void* x, const void* delta, const void* post_weight,
+                       const void* weight, const void* gate, int gate_rows, void* x_out,
+                       void* out, int rows, int hidden, float eps, float scale,
+                       hipStream_t stream);
 
 /* voom_gemv_bf16: one-token projection y [n] = bf16(weight [n, k] . x [k]),
  * fp32 sums -- the _linear calls of a decode step (runtime/layer_runner.py:73,

@@ -50,6 +50,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "voom_evict_select_workspace_bytes": (c_size_t, [c_int] * 3),
     "voom_evict_select_split": (c_int, [_P] * 5 + [c_size_t] + [c_int] * 6 + [_P]),
     "voom_compact_kv": (c_int, [_P] * 9 + [c_int] * 10 + [_P]),
+    "voom_paged_gqa_chunk_workspace_bytes": (c_size_t, [c_int] * 9),
+    "voom_paged_gqa_chunk": (c_int, [_P] * 12 + [c_size_t] + [c_int] * 10
+                             + [c_float, c_float, _P]),
+    "voom_beam_select_workspace_bytes": (c_size_t, [c_int] * 3),
+    "voom_beam_select": (c_int, [_P, c_int, _P, _P, c_longlong] + [_P] * 8
+                         + [c_size_t, c_int, c_int, c_int, _P]),
+    "voom_fork_kv": (c_int, [_P] * 5 + [c_int] + [_P] * 3 + [c_int] * 5 + [_P]),
+    "voom_add_post_norm": (c_int, [_P] * 5 + [c_int, _P, _P, c_int, c_int, c_float, c_float,
+                                              _P]),
     "voom_qk_norm_rope_append": (c_int, [_P, _P, _P, c_float, _P, _P, c_int, c_int, c_int]
                                  + [_P] * 7 + [c_int] * 8 + [_P]),
     "voom_merge_attn_states": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, _P]),

@@ -1,0 +1,109 @@
+// What the kernels of attention over ragged chunks share (gqa_chunk.hip): the call's
+// arguments, which cached tokens a new one sees, and the score of a pair.
+#pragma once
+
+#include "common.h"
+
+namespace voom {
+
+struct ChunkArgs {
+  const uint16_t* q;       // packed [N, NQ, D], or [B, NQ, T, D]
+  const uint16_t* k_pool;
+  const uint16_t* v_pool;
+  const int32_t* table;    // [B, max_pages]
+  const int32_t* ctx;      // [B]
+  const int32_t* starts;   // [B + 1] first rows of the sequences, packed; or null
+  const int32_t* lens;     // [B] new tokens, not packed; or null: T each
+  const float* slopes;     // [NQ], or null
+  const int32_t* prefix;   // [B], or null
+  uint16_t* out;           // [N, NQ, D], or [B, T, NQ, D]
+  float* lse;              // the same without D, or null
+  float* part_o;           // [pieces, rows, D]
+  float* part_ml;          // [pieces, rows, 2]
+  int B, NQ, NKV, G, T, N, max_pages, pt_shift, num_slots;
+  int window;    // tokens, INT_MAX: no window
+  float scale;   // softmax scale in log2 units
+  float cap;     // score cap in log2 units, 0: none
+  float cap_k;   // softmax scale / score cap
+  int tiles;     // row tiles of a sequence, an upper bound of all of them where packed
+  int W;         // workgroups of the split, 0: one per segment
+  int per_xcd;   // workgroups per XCD
+};
+
+__device__ __forceinline__ int context_of(const ChunkArgs& a, int b) {
+  const int cap = a.max_pages << a.pt_shift;
+  const int c = a.ctx[b];
+  return c < 0 ? 0 : (c > cap ? cap : c);
+}
+
+// The new tokens of sequence b and its first row among the packed ones, both kept inside
+// the arrays whatever starts holds.
+__device__ __forceinline__ int new_of(const ChunkArgs& a, int b, int& base) {
+  if (a.starts == nullptr) {
+    base = 0;
+    const int n = a.lens != nullptr ? a.lens[b] : a.T;
+    return n < 0 ? 0 : (n > a.T ? a.T : n);
+  }
+  const int s = a.starts[b], e = a.starts[b + 1];
+  base = s < 0 ? 0 : (s > a.N ? a.N : s);
+  const int end = e > a.N ? a.N : e;
+  return end > base ? end - base : 0;
+}
+
+__device__ __forceinline__ int prefix_of(const ChunkArgs& a, int b, int ctx) {
+  const int p = a.prefix != nullptr ? a.prefix[b] : 0;
+  return p < 0 ? 0 : (p > ctx ? ctx : p);
+}
+
+// Elements from one sequence's queries to the next token's and the next head's, and the
+// row of out and lse of a (sequence, token, head).
+__device__ __forceinline__ size_t query_at(const ChunkArgs& a, int b, int base, int t, int head) {
+  return a.starts != nullptr ? static_cast<size_t>(base + t) * a.NQ + head
+                             : (static_cast<size_t>(b) * a.NQ + head) * a.T + t;
+}
+__device__ __forceinline__ size_t out_at(const ChunkArgs& a, int b, int base, int t, int head) {
+  return (a.starts != nullptr ? static_cast<size_t>(base + t) : static_cast<size_t>(b) * a.T + t) *
+             a.NQ + head;
+}
+
+// The tokens [lo, hi) that token t of the newest n sees, and with them [0, pre) where that
+// does not reach lo (else it is one range).  Both ends rise with t.
+struct Sight {
+  int at, lo, hi;
+  __device__ __forceinline__ Sight(const ChunkArgs& a, int ctx, int n, int pre, int t) {
+    at = ctx - n + t;  // (before the cache where there are more new tokens than cached ones)
+    hi = at + 1 > 0 ? at + 1 : 0;
+    lo = at < a.window ? 0 : at + 1 - a.window;
+    if (pre > 0 && lo <= pre) {
+      lo = 0;
+      hi = hi > pre ? hi : pre;
+    }
+  }
+};
+
+// Bits of 8 consecutive tokens from pos on that lie in [lo, hi).
+__device__ __forceinline__ uint32_t bits_in(int pos, int lo, int hi) {
+  const int a = lo - pos, b = hi - pos;
+  const uint32_t below = b >= 8 ? 0xffu : (b > 0 ? (1u << b) - 1 : 0u);
+  const uint32_t before = a >= 8 ? 0xffu : (a > 0 ? (1u << a) - 1 : 0u);
+  return below & ~before;
+}
+
+// tanh(x) / x for |x| <= kNear as a polynomial of x^2, off by 1.3e-8 at most (found by
+// Remez's exchange of the extrema of the relative error).
+constexpr float kNear = 0.5f;
+__device__ __forceinline__ float tanh_ratio(float x2) {
+  float p = 0.017135007306933403f;
+  p = __builtin_fmaf(p, x2, -0.05298607423901558f);
+  p = __builtin_fmaf(p, x2, 0.13324779272079468f);
+  p = __builtin_fmaf(p, x2, -0.3333306908607483f);
+  return __builtin_fmaf(p, x2, 1.f);
+}
+
+// cap tanh(x) further out, where 1 - 2 / (e^2x + 1) loses nothing to cancellation.
+__device__ __forceinline__ float capped_far(float x, float cap) {
+  const float e = fast_exp2(x * 2.885390081777927f);
+  return __builtin_fmaf(-2.f * cap, __builtin_amdgcn_rcpf(e + 1.f), cap);
+}
+
+}  // namespace voom

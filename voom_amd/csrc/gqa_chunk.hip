@@ -1,0 +1,663 @@
+// Paged GQA attention of ragged chunks for gfx950: the newest tokens of each sequence (one
+// of a running request, a part of a prompt, a whole prompt) over the paged K/V cache.
+//
+// Sequence b holds ctx[b] tokens, the newest n of them with queries.  The token at i scores
+// the one at j
+//   s = scale q.k,  with a cap c:  s = c tanh(s / c),  with slopes:  s -= slope[head] |i - j|
+// and sees it where (j <= i and i - j < window) or j < prefix[b]:
+//   out = sum_j softmax_j(s) v[j],  lse = log sum_j exp s.
+// Rows that see nothing give 0 and -inf.
+//
+// What bounds it: K and V of the tokens seen once (4 D bytes per token and kv head) while
+// few rows share them, then matrix work, 4 NQ D flops per (new token, token seen).
+//
+// gqa_chunk_rows_kernel, for single tokens and short chunks, is built as gqa_tree_kernel is
+// (paged_rows.h): a workgroup takes 64 rows (new token, head of the group) of a
+// (sequence, kv head); the stages of 64 tokens (128 at D = 64) that a sequence's rows see,
+// those behind the prefix and before the window left out, are the units of its segments,
+// which lie end to end and are dealt out evenly; gqa_chunk_reduce_kernel merges cut ones.
+// Stages run through one ring in order; a stage that every row of the tile sees whole skips
+// the masks.
+#include "chunk_rows.h"
+#include "paged_rows.h"
+
+#include <climits>
+
+namespace voom {
+namespace {
+
+constexpr int kRows = 16 * kRowWaves;  // of a tile
+constexpr int kLead = 8;               // units that a segment costs besides its stages
+constexpr int kMaxBatch = 1024;
+
+// Units of a sequence: for every kv head and row tile the stages that its rows see, after
+// kLead units that stand for what a segment costs besides.  Stages from `pre` on lie `gap`
+// further on in the context.
+template <int D>
+struct Units {
+  int chunks, tiles, pre, gap;
+  __device__ __forceinline__ int all(const ChunkArgs& a) const {
+    if (a.W == 0) return tiles * a.NKV;
+    return chunks == 0 ? 0 : (chunks + kLead) * tiles * a.NKV;
+  }
+  __device__ __forceinline__ Units(const ChunkArgs& a, int b) {
+    constexpr int kTok = stage_tokens(D);
+    int base;
+    const int ctx = context_of(a, b), n = new_of(a, b, base), p = prefix_of(a, b, ctx);
+    const Sight first(a, ctx, n, p, 0);
+    pre = (p + kTok - 1) / kTok;
+    gap = first.lo / kTok - pre;
+    gap = gap < 0 ? 0 : gap;
+    chunks = n == 0 ? 0 : (ctx + kTok - 1) / kTok - gap;
+    // (rows behind a padded sequence's are written by its segments where none is cut)
+    tiles = ((a.W == 0 && a.starts == nullptr ? a.T : n) * a.G + kRows - 1) / kRows;
+  }
+};
+
+// The units of up to 64 sequences from `base` on, one per lane, and their inclusive sum.
+template <int D>
+__device__ __forceinline__ Units<D> scan_units(const ChunkArgs& a, int base, int lane, int& x) {
+  const bool in = base + lane < a.B;
+  const Units<D> u(a, in ? base + lane : 0);
+  x = wave_inclusive_scan(in ? u.all(a) : 0, lane);
+  return u;
+}
+
+// What the row of this lane's column sees, and its score's slope.
+struct View {
+  int ctx, pre, at, lo, hi;
+  float slope;  // log2 units
+  bool biased;
+  // Bit e: it sees token pos + e, e < 8.
+  __device__ __forceinline__ uint32_t seen(int pos) const {
+    return hi > 0 ? bits_in(pos, lo, hi) | bits_in(pos, 0, pre) : 0u;
+  }
+};
+
+// Scores in log2 units, of this lane's 8 tokens from pos on.
+__device__ __forceinline__ void score(f32x4 (&sc)[1][2], const ChunkArgs& a, const View& view,
+                                      int pos) {
+  if (a.cap != 0.f) {
+    float x[8];
+    bool far = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = sc[0][e >> 2][e & 3] * a.cap_k;
+      far |= fabsf(x[e]) > kNear;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sc[0][e >> 2][e & 3] = a.cap * x[e] * tanh_ratio(x[e] * x[e]);
+    if (__builtin_amdgcn_ballot_w64(far) != 0) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = capped_far(x[e], a.cap);
+        sc[0][e >> 2][e & 3] = fabsf(x[e]) > kNear ? y : sc[0][e >> 2][e & 3];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sc[0][e >> 2][e & 3] *= a.scale;
+  }
+  if (view.biased) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int d = view.at - (pos + e);
+      sc[0][e >> 2][e & 3] -= view.slope * static_cast<float>(d < 0 ? -d : d);
+    }
+  }
+}
+
+// Forms P of a block's scores.
+template <int D>
+__device__ __forceinline__ void weights_of(const f32x4 (&sc)[1][2], State<D, 1>& st,
+                                           u32x4 (&p)[1]) {
+  float mx[1] = {fmaxf(sc[0][0][0], sc[0][1][0])};
+#pragma unroll
+  for (int e = 1; e < 4; ++e) mx[0] = fmaxf(fmaxf(mx[0], sc[0][0][e]), sc[0][1][e]);
+  if (__builtin_amdgcn_ballot_w64(mx[0] > st.m[0] + kSlack) != 0) raise_maxima<D, 1>(mx, st);
+  float w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = fast_exp2(sc[0][e >> 2][e & 3] - st.m[0]);
+  st.l[0] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+#pragma unroll
+  for (int e = 0; e < 4; ++e) p[0][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
+}
+
+// A block that some row of the tile does not see whole.
+template <int D>
+__device__ __forceinline__ void edge_block(const uint16_t* tile, const u32x4 (&qop)[1][D / 32],
+                                           const ChunkArgs& a, State<D, 1>& st, const View& view,
+                                           int bi, int lane) {
+  const int pos = bi * kBlk + 8 * (lane >> 4);
+  f32x4 sc[1][2];
+  u32x4 p[1];
+  {
+    Operands<D> o;
+    read_keys<D>(o, tile, lane);
+    scores_of<D, 1>(o, qop, sc);
+  }
+  score(sc, a, view, pos);
+  const uint32_t seen = view.seen(pos);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    sc[0][e >> 2][e & 3] = (seen >> e & 1) != 0 ? sc[0][e >> 2][e & 3] : -INFINITY;
+  weights_of<D>(sc, st, p);
+  masked_products<D, 1>(tile, p, st, view.ctx - pos, lane, [&](int) { return seen; });
+}
+
+template <int D, int AUX>
+__global__ __launch_bounds__(kThreads, 2) void gqa_chunk_rows_kernel(ChunkArgs a) {
+  constexpr int kBlocks = stage_blocks(D);
+  constexpr int kTok = stage_tokens(D);
+  constexpr int kLoads = 2 * kBlocks * (kBlk * D / 512) / kWaves;  // a wavefront's, of a stage
+  constexpr int kPad = D + 4;  // floats of a row in LDS: 16 rows start in 16 bank groups
+  // The ring.  Distinct objects, so that reads of one provably miss the pending
+  // direct-to-LDS loads of the others; the merge uses them when the loop is done.
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_0[kStageElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_1[kStageElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_2[kStageElems];
+  __shared__ __attribute__((aligned(1024))) uint16_t stage_3[kStageElems];
+  static_assert(kLoads == 4, "the waits below count the loads of a stage");
+  static_assert(sizeof(float) * 16 * kPad <= sizeof(stage_0), "a merge buffer fits a stage");
+
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wv = uniform(threadIdx.x / kWave) & (kWaves - 1);
+  const int kw = wv % kKeyWaves;
+  const int rw = wv / kKeyWaves;
+  const int i16 = lane & 15;
+  const int g = lane >> 4;
+  // Consecutive workgroups of one XCD take consecutive units, so that the row tiles
+  // that read the same keys share an L2.
+  const int bid = static_cast<int>(blockIdx.x);
+  const int w = (bid & 7) * a.per_xcd + (bid >> 3);
+
+  int b = 0, kvh, tile, c0, c1, chunks = 0, tiles = 1, pre = 0, gap = 0;
+  int u0 = w, u1 = w + 1, begin = 0;  // the workgroup's units, and the segment's first one
+  int x0;  // (every wavefront for itself: no barrier)
+  const Units<D> first = scan_units<D>(a, 0, lane, x0);
+  if (a.W != 0) {
+    int U = __builtin_amdgcn_readlane(x0, kWave - 1);
+    for (int base = kWave; base < a.B; base += kWave) {
+      int x;
+      scan_units<D>(a, base, lane, x);
+      U += __builtin_amdgcn_readlane(x, kWave - 1);
+    }
+    const Split split(U, a.W);
+    if (w >= split.We || U == 0) return;
+    u0 = split.begin(w);
+    u1 = split.begin(w + 1);
+  }
+  for (int base = 0;; base += kWave) {  // the sequence that holds unit u0
+    if (base >= a.B) return;
+    int x = x0;
+    Units<D> units = first;
+    if (base != 0) units = scan_units<D>(a, base, lane, x);
+    const int here = __builtin_amdgcn_readlane(x, kWave - 1);
+    if (u0 < begin + here) {
+      const int k = __popcll(__builtin_amdgcn_ballot_w64(begin + x <= u0));
+      b = base + k;
+      chunks = __builtin_amdgcn_readlane(units.chunks, k);
+      tiles = __builtin_amdgcn_readlane(units.tiles, k);
+      pre = __builtin_amdgcn_readlane(units.pre, k);
+      gap = __builtin_amdgcn_readlane(units.gap, k);
+      begin += __builtin_amdgcn_readlane(x, k) - __builtin_amdgcn_readlane(units.all(a), k);
+      break;
+    }
+    begin += here;
+  }
+  {
+    const int each = a.W != 0 ? chunks + kLead : 1;
+    const int s = (u0 - begin) / each;
+    kvh = s / tiles;
+    tile = s - kvh * tiles;
+    begin += s * each;
+  }
+  while (true) {
+    if (a.W == 0) {
+      c0 = 0;
+      c1 = chunks;  // (0 below for a tile behind a padded sequence's new tokens)
+    } else {
+      const int at = begin + kLead;  // the segment's first stage
+      if (u1 <= at) return;
+      c0 = u0 > at ? u0 - at : 0;
+      c1 = (u1 < at + chunks ? u1 : at + chunks) - at;
+    }
+    const int ctx = uniform(context_of(a, b));
+    int base;
+    const int n = uniform(new_of(a, b, base));
+    const int prefix = uniform(prefix_of(a, b, ctx));
+    if (tile * kRows >= n * a.G) c1 = c0;
+    // the row of this lane's column, and what the tile's rows all see
+    const int row = tile * kRows + rw * 16 + i16;
+    const int t_row = row / a.G;
+    const bool live = t_row < n;
+    const int head = kvh * a.G + (row - t_row * a.G);
+    View view;
+    {
+      const Sight sight(a, ctx, n, prefix, t_row);
+      view.ctx = ctx;
+      view.pre = live ? prefix : 0;
+      view.at = sight.at;
+      view.lo = sight.lo;
+      view.hi = live ? sight.hi : 0;
+      view.biased = a.slopes != nullptr;
+      view.slope = view.biased ? a.slopes[head] * 1.4426950408889634f : 0.f;
+    }
+    const int t_lo = tile * kRows / a.G;
+    int t_hi = (tile * kRows + kRows - 1) / a.G;
+    t_hi = t_hi < n ? t_hi : n - 1;
+    const int hi_min = Sight(a, ctx, n, prefix, t_lo).hi;
+    const int lo_max = Sight(a, ctx, n, prefix, t_hi).lo;
+    // Q^T operands of this wavefront's rows
+    u32x4 qop[1][D / 32];
+    {
+      const uint16_t* qr = a.q + (live ? query_at(a, b, base, t_row, head) * D : 0) + 8 * g;
+#pragma unroll
+      for (int s = 0; s < D / 32; ++s) qop[0][s] = *reinterpret_cast<const u32x4*>(qr + 32 * s);
+    }
+    State<D, 1> st;
+    // never -inf: keys of score -inf then weigh 0 also where nothing came before
+    st.m[0] = -FLT_MAX;
+    st.l[0] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) st.acc[0][i] = f32x4{};
+
+    const int last_blk = (ctx - 1) / kBlk;
+    Pages pg(a.table + static_cast<size_t>(b) * a.max_pages, a.max_pages, a.num_slots, a.NKV, kvh,
+             a.pt_shift - 5, last_blk);
+    // (else this wavefront only loads)
+    const bool rows_here = tile * kRows + rw * 16 < n * a.G;
+    int t = c0;
+    auto stage_of = [&](int c) { return c < pre ? c : c + gap; };
+    auto load = [&](int c, uint16_t* stage) {
+      load_stage<D, AUX>(stage, a.k_pool, a.v_pool, pg, stage_of(c) * kBlocks, wv, lane);
+    };
+    if (t < c1) load(t, stage_0);
+    if (t + 1 < c1) load(t + 1, stage_1);
+    if (t + 2 < c1) load(t + 2, stage_2);
+    auto step = [&](const uint16_t* cur, uint16_t* free) {
+      // Stage t has landed for every wavefront, and stage t - 1 is no longer read.  gfx9
+      // encoding: vmcnt of the loads of stages t + 1 and t + 2, expcnt 7, lgkmcnt 15.
+      if (t + 2 < c1) __builtin_amdgcn_s_waitcnt(0x0F78);
+      else if (t + 1 < c1) __builtin_amdgcn_s_waitcnt(0x0F74);
+      else __builtin_amdgcn_s_waitcnt(0x0F70);
+      lds_barrier();
+      const int at = stage_of(t) * kTok;
+      if ((at >= lo_max && at + kTok <= hi_min) || at + kTok <= prefix) {
+        Operands<D> o;  // (the next loads are prepared while the first operands come)
+        read_block<D>(o, cur + kw * block_elems(D), lane);
+        if (t + 3 < c1) load(t + 3, free);
+#pragma unroll
+        for (int j = 0; j < kBlocks / kKeyWaves && rows_here; ++j) {
+          if (j != 0) read_block<D>(o, cur + (kKeyWaves * j + kw) * block_elems(D), lane);
+          f32x4 sc[1][2];
+          u32x4 p[1];
+          scores_of<D, 1>(o, qop, sc);
+          score(sc, a, view, at + (kKeyWaves * j + kw) * kBlk + 8 * g);
+          weights_of<D>(sc, st, p);
+          products<D, 1>(o, p, st);
+        }
+      } else {
+        if (t + 3 < c1) load(t + 3, free);
+        if (rows_here) {
+#pragma unroll 1
+          for (int j = kw; j < kBlocks && at / kBlk + j <= last_blk; j += kKeyWaves)
+            edge_block<D>(cur + j * block_elems(D), qop, a, st, view, at / kBlk + j, lane);
+        }
+      }
+      return ++t < c1;
+    };
+    if (t < c1) {
+      while (step(stage_0, stage_3) && step(stage_1, stage_0) && step(stage_2, stage_1) &&
+             step(stage_3, stage_2)) {
+      }
+    }
+    wait_vmem_all();
+    lds_barrier();  // the ring is no longer read or written
+
+    // Merge the two wavefronts of each group of rows: one leaves its state in LDS, the
+    // other adds its own and writes.
+    const bool all = a.W == 0 || (c0 == 0 && c1 == chunks);
+    const size_t slot = 2 * static_cast<size_t>(w) + (c0 == 0 ? 1 : 0);
+    float* const buf = reinterpret_cast<float*>(rw < 2 ? (rw == 0 ? stage_0 : stage_1)
+                                                       : (rw == 2 ? stage_2 : stage_3)) +
+                       i16 * kPad;
+    const float lt = wave_sum_across_groups(st.l[0]);
+    if (kw == 1) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+        *reinterpret_cast<f32x4*>(buf + 16 * i + 4 * g) = st.acc[0][i];
+      if (g == 0) {
+        buf[D] = st.m[0];
+        buf[D + 1] = lt;
+      }
+    }
+    __syncthreads();
+    if (kw == 0) {
+      const float m1 = buf[D];
+      const float M = fmaxf(st.m[0], m1);
+      const float f0 = fast_exp2(st.m[0] - M), f1 = fast_exp2(m1 - M);
+      const float L = lt * f0 + buf[D + 1] * f1;
+      const bool empty = !live || L == 0.f;
+      const float inv = 1.f / L;
+      const int r = rw * 16 + i16;
+      // (rows behind the last one are in the workspace, but not in out)
+      const bool mine = a.starts != nullptr ? live : t_row < a.T;
+      const size_t at = out_at(a, b, base, t_row, head);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const f32x4 o =
+            st.acc[0][i] * f0 + *reinterpret_cast<const f32x4*>(buf + 16 * i + 4 * g) * f1;
+        if (!all) {
+          *reinterpret_cast<f32x4*>(a.part_o + (slot * kRows + r) * D + 16 * i + 4 * g) = o;
+        } else if (mine) {
+          *reinterpret_cast<u32x2*>(a.out + at * D + 16 * i + 4 * g) =
+              empty ? u32x2{0u, 0u}
+                    : u32x2{pack_bf16x2(o[0] * inv, o[1] * inv),
+                            pack_bf16x2(o[2] * inv, o[3] * inv)};
+        }
+      }
+      if (g == 0 && !all) *reinterpret_cast<float2*>(a.part_ml + (slot * kRows + r) * 2) = {M, L};
+      if (g == 0 && all && mine && a.lse != nullptr)
+        a.lse[at] = empty ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
+    }
+    if (a.W == 0) return;
+    begin += kLead + chunks;
+    u0 = u1 < begin ? u1 : begin;
+    if (u0 >= u1) return;
+    if (++tile == tiles) {
+      tile = 0;
+      if (++kvh == a.NKV) {
+        kvh = 0;
+        do {
+          const Units<D> units(a, ++b);
+          chunks = uniform(units.chunks);
+          tiles = uniform(units.tiles);
+          pre = uniform(units.pre);
+          gap = uniform(units.gap);
+        } while (b < a.B - 1 && chunks == 0);
+      }
+    }
+    __syncthreads();  // the next piece writes the ring
+  }
+}
+
+constexpr int kReduceWaves = 4;
+
+// One wavefront per row: merges the pieces of its segment, where the split cut it, and
+// writes the rows that no segment holds.
+template <int D>
+__global__ __launch_bounds__(kReduceWaves * kWave) void gqa_chunk_reduce_kernel(ChunkArgs a) {
+  // A wavefront holds the row of kTogether pieces at a time, 4 dims per lane.
+  constexpr int kLanes = D / 4;
+  constexpr int kTogether = kWave / kLanes;
+  constexpr int kAhead = 8;  // loads in flight
+  const int lane = threadIdx.x & (kWave - 1);
+  const int kvh = static_cast<int>(blockIdx.y);
+  const int all = static_cast<int>(blockIdx.x) * kReduceWaves + uniform(threadIdx.x / kWave);
+  int b = static_cast<int>(blockIdx.z);
+  int rr = all;  // the row within its sequence
+  if (a.starts != nullptr) {
+    const int token = all / a.G;
+    if (token >= a.N) return;
+    // the last sequence that starts at or before the token (those behind it are empty)
+    b = -1;
+    for (int at = 0; at < a.B; at += kWave) {
+      const bool in = at + lane < a.B && a.starts[at + lane < a.B ? at + lane : 0] <= token;
+      b += __popcll(__builtin_amdgcn_ballot_w64(in));
+    }
+    if (b < 0) return;
+  } else if (all >= a.T * a.G) {
+    return;
+  }
+  int base;
+  const int n = uniform(new_of(a, b, base));
+  if (a.starts != nullptr) rr -= base * a.G;
+  const int t = rr / a.G;
+  if (a.starts != nullptr && (t < 0 || t >= n)) return;  // of no sequence
+  const int tile = rr / kRows;
+  const int r = rr - tile * kRows;
+  const int head = kvh * a.G + (rr - t * a.G);
+  const size_t at = out_at(a, b, base, t, head);
+  const int sub = lane / kLanes;
+  const int dim = lane % kLanes * 4;
+  int first = 0, last = -1;
+  if (t < n) {  // (else 0)
+    // units before sequence b, and of all; stages and row tiles of b
+    int before = 0, chunks = 0, tiles = 1, U = 0;
+    for (int from = 0; from < a.B; from += kWave) {
+      int x;
+      const Units<D> units = scan_units<D>(a, from, lane, x);
+      if (b >= from && b < from + kWave) {
+        chunks = __builtin_amdgcn_readlane(units.chunks, b - from);
+        tiles = __builtin_amdgcn_readlane(units.tiles, b - from);
+        before = U + __builtin_amdgcn_readlane(x, b - from) - (chunks + kLead) * tiles * a.NKV;
+      }
+      U += __builtin_amdgcn_readlane(x, kWave - 1);
+    }
+    if (chunks != 0) {  // (a context of no tokens has no segments)
+      const Split split(U, a.W);
+      const int S = before + (kvh * tiles + tile) * (chunks + kLead) + kLead;
+      first = split.group(S);
+      last = split.group(S + chunks - 1);
+      if (first == last) return;  // written by its workgroup
+    }
+  }
+  // Up to 64 pieces at a time, one per lane for their maxima and sums.  A workgroup leaves
+  // the piece that starts a segment, its last one, in its second slot.
+  float M = -FLT_MAX, L = 0.f;
+  f32x4 acc = {};
+  for (int w0 = first; w0 <= last; w0 += kWave) {
+    const int m = last - w0 + 1 < kWave ? last - w0 + 1 : kWave;
+    const size_t p0 = 2 * static_cast<size_t>(w0) * kRows + r;
+    const int odd = w0 == first ? kRows : 0;  // of the first one
+    auto row_at = [&](int k) {
+      k = k < m ? k : m - 1;
+      return p0 + 2 * static_cast<size_t>(k) * kRows + (k == 0 ? odd : 0);
+    };
+    f32x4 v[kAhead];
+    auto read = [&](int k0) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        v[u] = *reinterpret_cast<const f32x4*>(a.part_o + row_at(k0 + u * kTogether + sub) * D +
+                                               dim);
+    };
+    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + row_at(lane) * 2);
+    read(0);  // (under way while the weights are formed)
+    const float mn = fmaxf(M, wave_max_uniform(lane < m ? ml.x : -FLT_MAX));
+    const float wt = lane < m ? fast_exp2(ml.x - mn) : 0.f;
+    const float f = fast_exp2(M - mn);
+    M = mn;
+    L = L * f + wave_sum_uniform(lane < m ? ml.y * wt : 0.f);
+    acc *= f;
+    for (int k0 = 0; k0 < m; k0 += kAhead * kTogether) {
+      if (k0 != 0) read(k0);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int k = k0 + u * kTogether + sub;
+        const float ws = __shfl(wt, k & (kWave - 1));
+        if (k < m) acc += v[u] * ws;  // (0 times the infinity of a piece read again is NaN)
+      }
+    }
+  }
+#pragma unroll
+  for (int k = kLanes; k < kWave; k <<= 1) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], k);
+  }
+  const bool empty = L == 0.f;
+  const float inv = 1.f / L;
+  if (sub == 0)
+    *reinterpret_cast<u32x2*>(a.out + at * D + dim) =
+        empty ? u32x2{0u, 0u}
+              : u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv),
+                      pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+  if (a.lse != nullptr && lane == 0)
+    a.lse[at] = empty ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
+}
+
+// How a call is cut.
+struct ChunkPlan {
+  int tiles;         // row tiles of a sequence; of all of them at most, where packed
+  long long segs;    // (sequence, kv head, row tile) segments at most
+  int W;             // workgroups of the split; 0: one per segment, no reduce launch
+};
+
+constexpr int kShort = 8, kLong = 64;  // stages of a segment that is not cut
+
+ChunkPlan plan_chunk(int B, int NKV, int D, int G, int N, int T, int max_pages, int page_tokens,
+                     int window) {
+  ChunkPlan p;
+  const long long tok = stage_tokens(D);
+  if (N > 0) {
+    p.tiles = static_cast<int>(static_cast<long long>(N) * G / kRows + (B < N ? B : N));
+    p.segs = static_cast<long long>(p.tiles) * NKV;
+  } else {
+    p.tiles = (T * G + kRows - 1) / kRows;
+    p.segs = static_cast<long long>(B) * NKV * p.tiles;
+  }
+  long long stages = (static_cast<long long>(max_pages) * page_tokens + tok - 1) / tok;
+  const long long seen = (static_cast<long long>(window) + kRows / G) / tok + 2;
+  if (seen < stages) stages = seen;
+  // All workgroups of a split run at once.  Without one a workgroup walks a segment, which
+  // saves the merges and the reduce launch, where the segments are short, the longer the
+  // better they fill the card.
+  const int cus = device_cu_count();
+  const long long full = (p.segs + cus - 1) / cus * cus;
+  const int most = 16 * p.segs >= 15 * full ? kLong : (2 * p.segs >= full ? 2 * kShort : kShort);
+  p.W = stages <= most ? 0 : cus;
+  return p;
+}
+
+bool chunk_shape_ok(int batch, int rows, int tokens, int num_q_heads, int num_kv_heads,
+                    int head_dim, int page_tokens, int max_pages) {
+  const long long all = rows > 0 ? rows : static_cast<long long>(batch) * tokens;
+  return batch > 0 && batch <= kMaxBatch && (rows > 0) != (tokens > 0) && rows >= 0 &&
+         tokens >= 0 && num_kv_heads > 0 && num_kv_heads <= 65535 && num_q_heads > 0 &&
+         num_q_heads % num_kv_heads == 0 && num_q_heads / num_kv_heads <= 16 &&
+         (head_dim == 64 || head_dim == 128) && is_pow2(page_tokens) && page_tokens >= 32 &&
+         page_tokens <= 4096 && max_pages > 0 &&
+         static_cast<long long>(max_pages) * page_tokens < (1LL << 30) &&
+         all * num_q_heads < (1LL << 28);
+}
+
+size_t part_o_bytes(const ChunkPlan& p, int D) {
+  return static_cast<size_t>(2) * p.W * kRows * D * sizeof(float);
+}
+
+}  // namespace
+}  // namespace voom
+
+using namespace voom;
+
+extern "C" size_t voom_paged_gqa_chunk_workspace_bytes(int batch, int rows, int tokens,
+                                                       int num_q_heads, int num_kv_heads,
+                                                       int head_dim, int page_tokens,
+                                                       int max_pages, int window) {
+  if (!chunk_shape_ok(batch, rows, tokens, num_q_heads, num_kv_heads, head_dim, page_tokens,
+                      max_pages) || window < 0)
+    return 0;
+  const ChunkPlan p = plan_chunk(batch, num_kv_heads, head_dim, num_q_heads / num_kv_heads, rows,
+                                 tokens, max_pages, page_tokens, window == 0 ? INT_MAX : window);
+  return part_o_bytes(p, head_dim) + static_cast<size_t>(2) * p.W * kRows * 2 * sizeof(float);
+}
+
+extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const void* v_pool,
+                                    const int32_t* block_table, const int32_t* ctx_lens,
+                                    const int32_t* starts, const int32_t* new_lens,
+                                    const float* slopes, const int32_t* prefix_lens, void* out,
+                                    float* lse, void* workspace, size_t ws_bytes, int batch,
+                                    int rows, int tokens, int num_q_heads, int num_kv_heads,
+                                    int head_dim, int page_tokens, int max_pages, int num_slots,
+                                    int window, float scale, float softcap, hipStream_t stream) {
+  const char* who = "paged_gqa_chunk";
+  VOOM_REQUIRE(q && k_pool && v_pool && block_table && ctx_lens && out,
+               "%s: null pointer argument", who);
+  VOOM_REQUIRE(num_slots > 0, "%s: empty page pool", who);
+  VOOM_REQUIRE(chunk_shape_ok(batch, rows, tokens, num_q_heads, num_kv_heads, head_dim,
+                              page_tokens, max_pages),
+               "%s: unsupported geometry (batch %d, %d rows, %d tokens, heads %d/%d, head_dim %d, "
+               "%d pages of %d)",
+               who, batch, rows, tokens, num_q_heads, num_kv_heads, head_dim, max_pages,
+               page_tokens);
+  VOOM_REQUIRE((starts != nullptr) == (rows > 0) && (starts == nullptr || new_lens == nullptr),
+               "%s: packed rows come with starts, padded ones with new_lens", who);
+  VOOM_REQUIRE(window >= 0, "%s: window %d must not be negative", who, window);
+  VOOM_REQUIRE(std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0.f,
+               "%s: the scale must be finite, the cap finite and not negative", who);
+  VOOM_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(k_pool) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(v_pool) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(out) % 8 == 0,
+               "%s: q and pools must be 16-byte aligned", who);
+  const int G = num_q_heads / num_kv_heads;
+  const int win = window == 0 ? INT_MAX : window;
+  const ChunkPlan p = plan_chunk(batch, num_kv_heads, head_dim, G, rows, tokens, max_pages,
+                                 page_tokens, win);
+  const long long stages = (static_cast<long long>(max_pages) * page_tokens + 63) / 64;
+  VOOM_REQUIRE((stages + kLead) * p.segs < (1LL << 31),
+               "%s: %d pages of %d tokens for %d sequences are too many", who, max_pages,
+               page_tokens, batch);
+  const size_t need = voom_paged_gqa_chunk_workspace_bytes(batch, rows, tokens, num_q_heads,
+                                                           num_kv_heads, head_dim, page_tokens,
+                                                           max_pages, window);
+  VOOM_REQUIRE(need == 0 || (workspace != nullptr && ws_bytes >= need &&
+                             reinterpret_cast<uintptr_t>(workspace) % 16 == 0),
+               "%s: workspace %zu bytes < required %zu (16-byte aligned)", who, ws_bytes, need);
+  ChunkArgs a;
+  a.q = static_cast<const uint16_t*>(q);
+  a.k_pool = static_cast<const uint16_t*>(k_pool);
+  a.v_pool = static_cast<const uint16_t*>(v_pool);
+  a.table = block_table;
+  a.ctx = ctx_lens;
+  a.starts = starts;
+  a.lens = new_lens;
+  a.slopes = slopes;
+  a.prefix = prefix_lens;
+  a.out = static_cast<uint16_t*>(out);
+  a.lse = lse;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                              part_o_bytes(p, head_dim))
+                   : nullptr;
+  a.B = batch;
+  a.NQ = num_q_heads;
+  a.NKV = num_kv_heads;
+  a.G = G;
+  a.T = tokens;
+  a.N = rows;
+  a.max_pages = max_pages;
+  a.pt_shift = ilog2(page_tokens);
+  a.num_slots = num_slots;
+  a.window = win;
+  a.scale = scale * 1.4426950408889634f;
+  a.cap = softcap * 1.4426950408889634f;
+  a.cap_k = softcap > 0.f ? scale / softcap : 0.f;
+  a.tiles = p.tiles;
+  a.W = p.W;
+  const long long groups = p.W != 0 ? p.W : p.segs;
+  a.per_xcd = static_cast<int>((groups + 7) / 8);
+  const dim3 grid(static_cast<unsigned>(8 * a.per_xcd));
+  // (a byte of K/V that one row tile alone reads is streamed past the caches)
+  const bool once = rows > 0 ? rows <= batch : p.tiles == 1;
+  if (head_dim == 128) {
+    if (once) hipLaunchKernelGGL((gqa_chunk_rows_kernel<128, 2>), grid, dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((gqa_chunk_rows_kernel<128, 0>), grid, dim3(kThreads), 0, stream, a);
+  } else {
+    if (once) hipLaunchKernelGGL((gqa_chunk_rows_kernel<64, 2>), grid, dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((gqa_chunk_rows_kernel<64, 0>), grid, dim3(kThreads), 0, stream, a);
+  }
+  const int rc = VOOM_LAUNCH_CHECK("paged_gqa_chunk: kernel launch");
+  if (rc || p.W == 0) return rc;
+  const long long row_groups =
+      ((rows > 0 ? rows : static_cast<long long>(tokens)) * G + kReduceWaves - 1) / kReduceWaves;
+  const dim3 rgrid(static_cast<unsigned>(row_groups), static_cast<unsigned>(num_kv_heads),
+                   static_cast<unsigned>(rows > 0 ? 1 : batch));
+  if (head_dim == 128)
+    hipLaunchKernelGGL(gqa_chunk_reduce_kernel<128>, rgrid, dim3(kReduceWaves * kWave), 0, stream,
+                       a);
+  else
+    hipLaunchKernelGGL(gqa_chunk_reduce_kernel<64>, rgrid, dim3(kReduceWaves * kWave), 0, stream,
+                       a);
+  return VOOM_LAUNCH_CHECK("paged_gqa_chunk: reduce launch");
+}

@@ -352,15 +352,19 @@ def _is_scores(t: torch.Tensor, batch: int, num_kv_heads: int) -> bool:
             and t.shape[0] == batch and t.shape[1] == num_kv_heads)
 
 
-def _new_tokens_geometry(q, k_pool, v_pool, block_table, ctx_lens):
+def _new_tokens_geometry(q, k_pool, v_pool, block_table, ctx_lens, packed=False):
     """Checks what the calls over a window of new tokens share; their sizes (v_pool None:
-    keys alone)."""
+    keys alone; packed: q [N, NQ, D], and T is N)."""
     q_shape, k_shape, table_shape = q.shape, k_pool.shape, block_table.shape
-    if len(q_shape) != 4:
-        raise ValueError("q must be [B, NQ, T, D]")
+    if len(q_shape) != (3 if packed else 4):
+        raise ValueError("q must be [N, NQ, D]" if packed else "q must be [B, NQ, T, D]")
     if len(k_shape) != 4:
         raise ValueError("k_pool must be [slots, NKV, PT, D]")
-    B, NQ, T, D = q_shape
+    if packed:
+        T, NQ, D = q_shape
+        B = table_shape[0] if table_shape else 0
+    else:
+        B, NQ, T, D = q_shape
     slots, NKV, PT, Dk = k_shape
     if Dk != D:
         raise ValueError(f"k_pool head_dim {Dk} != q head_dim {D}")
@@ -426,6 +430,213 @@ def paged_gqa_tree(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         if rc:
             _lib.check(rc, "voom_paged_gqa_tree")
     return (out, lse) if return_lse else out
+
+
+def check_chunk_rows(starts: torch.Tensor | None, new_lens: torch.Tensor | None, rows: int,
+                     tokens: int) -> None:
+    """Raise ValueError unless ``starts`` ascends within [0, rows] and ``new_lens`` lie in
+    [0, tokens]."""
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("bounds checks synchronise and cannot run under graph capture")
+    if starts is not None and (bool(((starts < 0) | (starts > rows)).any())
+                               or bool((starts[1:] < starts[:-1]).any())):
+        raise ValueError(f"starts must ascend within [0, {rows}]")
+    if new_lens is not None and bool(((new_lens < 0) | (new_lens > tokens)).any()):
+        raise ValueError(f"new_lens lie outside [0, {tokens}]")
+
+
+@functools.lru_cache(maxsize=256)
+def _chunk_workspace(device: int, *sizes: int) -> int:
+    return _lib.lib().voom_paged_gqa_chunk_workspace_bytes(*sizes)
+
+
+def paged_gqa_chunk(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                    block_table: torch.Tensor, ctx_lens: torch.Tensor, *,
+                    starts: torch.Tensor | None = None, new_lens: torch.Tensor | None = None,
+                    scale: float | None = None, softcap: float | None = None,
+                    slopes: torch.Tensor | None = None, window: int | None = None,
+                    prefix_lens: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                    return_lse: bool = False):
+    """Attention of each sequence's newest tokens over paged K/V: single tokens, parts of
+    prompts and whole ones in one call.
+
+    q is packed [N, NQ, D] bf16 with ``starts`` [B + 1] int32 ascending (sequence b has rows
+    starts[b] to starts[b + 1] - 1), or padded [B, NQ, T, D], ``new_lens`` [B] int32 of which
+    are new tokens (None: all T).  They are the newest of the ctx_lens [B] int32 cached ones.
+    The token at position i scores the one at j with s = scale q.k, capped to softcap *
+    tanh(s / softcap) where ``softcap`` is given, less slopes[head] * |i - j| with ``slopes``
+    [NQ] fp32; it sees j <= i, with a ``window`` only where i - j < window, and always the
+    first ``prefix_lens`` [B] int32 tokens of its sequence (in both directions).  A cap or a
+    window of 0 is none.
+
+    Returns out [N, NQ, D] or [B, T, NQ, D] (``out`` where it is given; and the fp32
+    natural-log LSE without the last dim when ``return_lse``).  Rows that see nothing, and
+    those behind new_lens, hold 0 and -inf; packed rows of no sequence are not written.
+    """
+    here = _require_here(q, k_pool, v_pool, block_table, ctx_lens, starts, new_lens, slopes,
+                         prefix_lens, out)
+    packed = starts is not None
+    B, NQ, T, D, slots, NKV, PT, pages = _new_tokens_geometry(q, k_pool, v_pool, block_table,
+                                                              ctx_lens, packed)
+    if packed:
+        if new_lens is not None or not _is_i32(starts, B + 1):
+            raise ValueError(f"packed q takes starts int32 [{B + 1}] and no new_lens")
+        rows = (T, NQ)
+    else:
+        if new_lens is not None and not _is_i32(new_lens, B):
+            raise ValueError(f"new_lens must be int32 [{B}]")
+        rows = (B, T, NQ)
+    if slopes is not None and (slopes.dtype is not torch.float32 or slopes.shape != (NQ,)):
+        raise ValueError(f"slopes must be float32 [{NQ}]")
+    if prefix_lens is not None and not _is_i32(prefix_lens, B):
+        raise ValueError(f"prefix_lens must be int32 [{B}]")
+    window = 0 if window is None else int(window)
+    softcap = 0.0 if softcap is None else float(softcap)
+    if window < 0 or not 0.0 <= softcap < float("inf"):
+        raise ValueError(f"window {window} and softcap {softcap} must not be negative")
+    if out is None:
+        out = q.new_empty((*rows, D))
+    elif out.dtype is not torch.bfloat16 or out.shape != (*rows, D):
+        raise ValueError(f"out must be bfloat16 {[*rows, D]}")
+    lse = q.new_empty(rows, dtype=torch.float32) if return_lse else None
+    if B and T and NQ:
+        if _BOUNDS_CHECKS:
+            check_block_table(block_table, ctx_lens, slots, PT)
+            check_chunk_rows(starts, new_lens, T, T)
+        window = min(window, (1 << 31) - 1)
+        N, T = (T, 0) if packed else (0, T)
+        # allocated per call, so that calls on several streams or threads and captured
+        # graphs never share it
+        need = _chunk_workspace(here, B, N, T, NQ, NKV, D, PT, pages, window)
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        rc = _lib.lib().voom_paged_gqa_chunk(
+            q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), block_table.data_ptr(),
+            ctx_lens.data_ptr(), _ptr(starts), _ptr(new_lens), _ptr(slopes), _ptr(prefix_lens),
+            out.data_ptr(), _ptr(lse), _ptr(ws), need, B, N, T, NQ, NKV, D, PT, pages, slots,
+            window, D ** -0.5 if scale is None else float(scale), softcap, _stream_of(here))
+        if rc:
+            _lib.check(rc, "voom_paged_gqa_chunk")
+    return (out, lse) if return_lse else out
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, last: torch.Tensor | None = None,
+                end_token: int | None = None, shared: torch.Tensor | None = None,
+                ctx_lens: torch.Tensor | None = None):
+    """One step of a beam search: the K best continuations of each request's K beams.
+
+    logits [B, K, V] bf16 or fp32, scores [B, K] fp32 (sums of log-probabilities, -inf for a
+    beam that does not count).  A continuation of beam j by token v is worth scores[j] +
+    log softmax(logits[j])[v]; a beam whose ``last`` [B, K] int64 token is ``end_token`` has
+    one continuation, that token again at its score.  Of equal ones the lowest (j, v) wins,
+    NaN and beams of infinite score or sum count as -inf.
+
+    Returns (scores fp32, tokens int64, parents int32) [B, K] by row: the best continuation of
+    a beam stays in its row (parents[b, j] == j), the others take, best first, the rows of
+    beams that nothing goes on from.  With ``shared`` [B, K, K] int32, the leading tokens that
+    rows have in common, and ``ctx_lens`` [B] int32, the tokens that each holds, two more:
+    first [B, K] int32, how many a row already has in common with its parent (fork_kv's), and
+    the next step's shared, before the tokens chosen here are appended.
+    """
+    here = _require_here(logits, scores, last, shared, ctx_lens)
+    if logits.dim() != 3 or logits.dtype not in _BEAM_DTYPES:
+        raise ValueError("logits must be bfloat16 or float32 [B, K, V]")
+    B, K, V = logits.shape
+    if scores.dtype is not torch.float32 or scores.shape != (B, K):
+        raise ValueError(f"scores must be float32 [{B}, {K}]")
+    if (last is None) != (end_token is None):
+        raise ValueError("last and end_token come together")
+    if last is not None and (last.dtype is not torch.int64 or last.shape != (B, K)):
+        raise ValueError(f"last must be int64 [{B}, {K}]")
+    if (shared is None) != (ctx_lens is None):
+        raise ValueError("shared and ctx_lens come together")
+    if shared is not None and not (_is_i32(shared, B, K, K) and _is_i32(ctx_lens, B)):
+        raise ValueError(f"shared must be int32 [{B}, {K}, {K}], ctx_lens int32 [{B}]")
+    out = scores.new_empty((B, K))
+    tokens = scores.new_empty((B, K), dtype=torch.int64)
+    parents = scores.new_empty((B, K), dtype=torch.int32)
+    first = next_shared = None
+    if shared is not None:
+        first, next_shared = torch.empty_like(parents), torch.empty_like(shared)
+    if B:
+        dtype = _BEAM_DTYPES[logits.dtype]
+        lib = _lib.lib()
+        need = lib.voom_beam_select_workspace_bytes(B, K, V)
+        ws = scores.new_empty(max(need, 1), dtype=torch.uint8)
+        rc = lib.voom_beam_select(
+            logits.data_ptr(), dtype, scores.data_ptr(), _ptr(last),
+            -1 if end_token is None else int(end_token), _ptr(shared), _ptr(ctx_lens),
+            out.data_ptr(), tokens.data_ptr(), parents.data_ptr(), _ptr(first),
+            _ptr(next_shared), ws.data_ptr(), need, B, K, V, _stream_of(here))
+        if rc:
+            _lib.check(rc, "voom_beam_select")
+    return (out, tokens, parents) if shared is None else (out, tokens, parents, first, next_shared)
+
+
+_BEAM_DTYPES = {torch.bfloat16: 0, torch.float32: 2}
+
+
+def check_parents(parents: torch.Tensor) -> None:
+    """Raise ValueError unless every row's parent [B, K] is one of the K and its own parent."""
+    if parents.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("bounds checks synchronise and cannot run under graph capture")
+    K = parents.shape[1]
+    if bool(((parents < 0) | (parents >= K)).any()):
+        raise ValueError(f"parents lie outside [0, {K})")
+    if bool((parents.gather(1, parents.long()) != parents).any()):
+        raise ValueError("a row that others go on from must be its own parent")
+
+
+def fork_kv(k_pools, v_pools, block_tables, ctx_lens: torch.Tensor, parents: torch.Tensor,
+            first: torch.Tensor | None = None) -> None:
+    """Cached tokens of beams that go on from another one, copied bit for bit in all layers.
+
+    k_pools, v_pools and block_tables are lists, one entry a layer (pools as in the module
+    docstring, tables int32 [B * K, max_pages], row b * K + j for beam j of request b).  Row j
+    takes the K and V of tokens first[b, j] (``first`` int32 [B, K], None: 0) to ctx_lens[b]
+    (int32 [B]) of row parents[b, j] (int32 [B, K]); a row that is its own parent is left
+    alone, as beam_select gives them.  A row that others go on from must be its own parent,
+    and a page that is written must not be another row's (set_bounds_checks refuses parents
+    that are not).
+    """
+    layers = len(k_pools)
+    if layers == 0 or len(v_pools) != layers or len(block_tables) != layers:
+        raise ValueError("k_pools, v_pools and block_tables must hold one entry a layer")
+    here = _require_here(*k_pools, *v_pools, *block_tables, ctx_lens, parents, first)
+    if parents.dtype is not torch.int32 or parents.dim() != 2:
+        raise ValueError("parents must be int32 [B, K]")
+    B, K = parents.shape
+    if not _is_i32(ctx_lens, B):
+        raise ValueError(f"ctx_lens must be int32 [{B}]")
+    if first is not None and not _is_i32(first, B, K):
+        raise ValueError(f"first must be int32 [{B}, {K}]")
+    if k_pools[0].dim() != 4:
+        raise ValueError("k_pool must be [slots, NKV, PT, D]")
+    _, NKV, PT, D = k_pools[0].shape
+    pages, slots = (ctypes.c_int * layers)(), (ctypes.c_int * layers)()
+    for i, (k, v, table) in enumerate(zip(k_pools, v_pools, block_tables)):
+        if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16:
+            raise ValueError("pools must be bfloat16")
+        n = slots[i] = k.shape[0]
+        if k.shape != (n, NKV, PT, D):
+            raise ValueError(f"layer {i}: k_pool must be [slots, {NKV}, {PT}, {D}]")
+        _check_v_pool(v, n, NKV, D, PT)
+        if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != B * K:
+            raise ValueError(f"layer {i}: block_table must be int32 [{B * K}, max_pages]")
+        pages[i] = table.shape[1]
+    if B * K == 0:
+        return
+    if _BOUNDS_CHECKS:
+        check_parents(parents)
+        rows = ctx_lens.repeat_interleave(K)
+        for k, table in zip(k_pools, block_tables):
+            check_block_table(table, rows, k.shape[0], PT)
+    pointers = ctypes.c_void_p * layers
+    rc = _lib.lib().voom_fork_kv(
+        pointers(*(t.data_ptr() for t in k_pools)), pointers(*(t.data_ptr() for t in v_pools)),
+        pointers(*(t.data_ptr() for t in block_tables)), pages, slots, layers,
+        ctx_lens.data_ptr(), parents.data_ptr(), _ptr(first), B, K, NKV, D, PT, _stream_of(here))
+    if rc:
+        _lib.check(rc, "voom_fork_kv")
 
 
 def paged_gqa_observe(q: torch.Tensor, lse: torch.Tensor, k_pool: torch.Tensor,
@@ -1125,6 +1336,50 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float,
         out = torch.empty_like(x)
     _lib.call("voom_add_rms_norm", _ptr(x), _ptr(delta), _ptr(weight), _ptr(out),
               x.numel() // H, H, float(eps), _stream(stream))
+    return out
+
+
+def add_post_norm(x: torch.Tensor, delta: torch.Tensor, post_weight: torch.Tensor,
+                  weight: torch.Tensor, eps: float, *, gate: torch.Tensor | None = None,
+                  scale: float = 1.0, x_out: torch.Tensor | None = None) -> torch.Tensor:
+    """The norm behind a block, the residual add and the norm before the next block:
+    y = x + scale * gate * post_weight * delta / rms(delta) is stored to ``x_out`` (None: x
+    itself), weight * y / rms(y) returned, rms(v) = sqrt(mean v^2 + eps) over the last dim.
+
+    x and delta [..., hidden] bf16, weights [hidden]; ``gate`` [hidden], or [G, hidden] with
+    one for every rows / G consecutive rows (G a divisor of the rows).  Everything in fp32,
+    y and the result rounded to bf16 once each, the result of the unrounded y.
+    """
+    here = _require_here(x, delta, post_weight, weight, gate, x_out)
+    shape = x.shape
+    if not shape or x.dtype is not torch.bfloat16:
+        raise ValueError("x must be bfloat16 [..., hidden]")
+    H = shape[-1]
+    if delta.shape != shape or delta.dtype is not torch.bfloat16:
+        raise ValueError("delta must be like x")
+    if (post_weight.shape != (H,) or weight.shape != (H,)
+            or post_weight.dtype is not torch.bfloat16 or weight.dtype is not torch.bfloat16):
+        raise ValueError(f"weights must be bfloat16 [{H}]")
+    if x_out is None:
+        x_out = x
+    elif x_out.shape != shape or x_out.dtype is not torch.bfloat16:
+        raise ValueError("x_out must be like x")
+    rows = x.numel() // H if H else 0
+    per_gate = 0
+    if gate is not None:
+        groups = gate.shape[0] if gate.dim() == 2 else 1
+        if (gate.dtype is not torch.bfloat16 or gate.dim() not in (1, 2) or gate.shape[-1] != H
+                or groups == 0 or rows % groups):
+            raise ValueError(f"gate must be bfloat16 [{H}] or [G, {H}], G a divisor of {rows}")
+        per_gate = rows // groups
+    out = torch.empty_like(x)
+    if rows:
+        rc = _lib.lib().voom_add_post_norm(
+            x.data_ptr(), delta.data_ptr(), post_weight.data_ptr(), weight.data_ptr(), _ptr(gate),
+            per_gate, x_out.data_ptr(), out.data_ptr(), rows, H, float(eps), float(scale),
+            _stream_of(here))
+        if rc:
+            _lib.check(rc, "voom_add_post_norm")
     return out
 
 
