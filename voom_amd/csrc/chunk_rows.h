@@ -1,10 +1,13 @@
-// What the kernels of attention over ragged chunks share (gqa_chunk.hip): the call's
+// What the kernels of attention over ragged chunks share (gqa_chunk.hip,
+// gqa_chunk_wide.hip): the call's
 // arguments, which cached tokens a new one sees, and the score of a pair.
 #pragma once
 
 #include "common.h"
 
 namespace voom {
+
+constexpr int kMaxChunkBatch = 1024;  // sequences of a call
 
 struct ChunkArgs {
   const uint16_t* q;       // packed [N, NQ, D], or [B, NQ, T, D]
@@ -25,7 +28,6 @@ struct ChunkArgs {
   float scale;   // softmax scale in log2 units
   float cap;     // score cap in log2 units, 0: none
   float cap_k;   // softmax scale / score cap
-  int tiles;     // row tiles of a sequence, an upper bound of all of them where packed
   int W;         // workgroups of the split, 0: one per segment
   int per_xcd;   // workgroups per XCD
 };
@@ -89,15 +91,15 @@ __device__ __forceinline__ uint32_t bits_in(int pos, int lo, int hi) {
   return below & ~before;
 }
 
-// tanh(x) / x for |x| <= kNear as a polynomial of x^2, off by 1.3e-8 at most (found by
-// Remez's exchange of the extrema of the relative error).
-constexpr float kNear = 0.5f;
+// tanh(x) / x for |x| <= kNear as a polynomial of x^2, off by 3.5e-8 at most (found by
+// Remez's exchange of the extrema of the relative error); a term more would hold to 0.5.
+constexpr float kNear = 0.35f;
+constexpr float kTanh[4] = {1.f, -0.33332422375679016f, 0.13295799493789673f,
+                            -0.04895823076367378f};
 __device__ __forceinline__ float tanh_ratio(float x2) {
-  float p = 0.017135007306933403f;
-  p = __builtin_fmaf(p, x2, -0.05298607423901558f);
-  p = __builtin_fmaf(p, x2, 0.13324779272079468f);
-  p = __builtin_fmaf(p, x2, -0.3333306908607483f);
-  return __builtin_fmaf(p, x2, 1.f);
+  float p = __builtin_fmaf(kTanh[3], x2, kTanh[2]);
+  p = __builtin_fmaf(p, x2, kTanh[1]);
+  return __builtin_fmaf(p, x2, kTanh[0]);
 }
 
 // cap tanh(x) further out, where 1 - 2 / (e^2x + 1) loses nothing to cancellation.
@@ -105,5 +107,20 @@ __device__ __forceinline__ float capped_far(float x, float cap) {
   const float e = fast_exp2(x * 2.885390081777927f);
   return __builtin_fmaf(-2.f * cap, __builtin_amdgcn_rcpf(e + 1.f), cap);
 }
+
+// ---- the kernel of long chunks (gqa_chunk_wide.hip) ------------------------------
+
+// Its workspace, sized for any lengths that the call's rows allow.
+struct WidePlan {
+  int entries;     // (sequence, row tile) pairs at most
+  int pieces;      // of a kv head at most, row tiles cut over keys
+  int cuts;        // row tiles of a kv head that are cut, at most
+  int slots;       // pieces of those
+  int workers;     // workgroups that run at once
+  size_t bytes;
+};
+WidePlan plan_wide(int B, int NKV, int D, int G, int N, int T);
+int launch_wide(const ChunkArgs& a, const WidePlan& p, int D, void* workspace,
+                hipStream_t stream);
 
 }  // namespace voom

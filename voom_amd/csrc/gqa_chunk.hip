@@ -11,13 +11,13 @@
 // What bounds it: K and V of the tokens seen once (4 D bytes per token and kv head) while
 // few rows share them, then matrix work, 4 NQ D flops per (new token, token seen).
 //
-// gqa_chunk_rows_kernel, for single tokens and short chunks, is built as gqa_tree_kernel is
-// (paged_rows.h): a workgroup takes 64 rows (new token, head of the group) of a
-// (sequence, kv head); the stages of 64 tokens (128 at D = 64) that a sequence's rows see,
-// those behind the prefix and before the window left out, are the units of its segments,
-// which lie end to end and are dealt out evenly; gqa_chunk_reduce_kernel merges cut ones.
-// Stages run through one ring in order; a stage that every row of the tile sees whole skips
-// the masks.
+// gqa_chunk_rows_kernel, for single tokens and short chunks (long ones: gqa_chunk_wide.hip),
+// is built as gqa_tree_kernel is (paged_rows.h): a workgroup takes 64 rows (new token, head
+// of the group) of a (sequence, kv head); the stages of 64 tokens (128 at D = 64) that a
+// sequence's rows see, those behind the prefix and before the window left out, are the units
+// of its segments, which lie end to end and are dealt out evenly; gqa_chunk_reduce_kernel
+// merges cut ones.  Stages run through one ring in order; a stage that every row of the tile
+// sees whole skips the masks.
 #include "chunk_rows.h"
 #include "paged_rows.h"
 
@@ -28,7 +28,6 @@ namespace {
 
 constexpr int kRows = 16 * kRowWaves;  // of a tile
 constexpr int kLead = 8;               // units that a segment costs besides its stages
-constexpr int kMaxBatch = 1024;
 
 // Units of a sequence: for every kv head and row tile the stages that its rows see, after
 // kLead units that stand for what a segment costs besides.  Stages from `pre` on lie `gap`
@@ -532,13 +531,20 @@ ChunkPlan plan_chunk(int B, int NKV, int D, int G, int N, int T, int max_pages, 
 bool chunk_shape_ok(int batch, int rows, int tokens, int num_q_heads, int num_kv_heads,
                     int head_dim, int page_tokens, int max_pages) {
   const long long all = rows > 0 ? rows : static_cast<long long>(batch) * tokens;
-  return batch > 0 && batch <= kMaxBatch && (rows > 0) != (tokens > 0) && rows >= 0 &&
+  return batch > 0 && batch <= kMaxChunkBatch && (rows > 0) != (tokens > 0) && rows >= 0 &&
          tokens >= 0 && num_kv_heads > 0 && num_kv_heads <= 65535 && num_q_heads > 0 &&
          num_q_heads % num_kv_heads == 0 && num_q_heads / num_kv_heads <= 16 &&
          (head_dim == 64 || head_dim == 128) && is_pow2(page_tokens) && page_tokens >= 32 &&
          page_tokens <= 4096 && max_pages > 0 &&
          static_cast<long long>(max_pages) * page_tokens < (1LL << 30) &&
          all * num_q_heads < (1LL << 28);
+}
+
+// Calls with more rows a sequence than one row tile takes, on the average, go to the kernel of
+// long chunks (gqa_chunk_wide.hip).
+bool is_wide(int batch, int rows, int tokens, int G) {
+  return rows > 0 ? static_cast<long long>(rows) * G > static_cast<long long>(kRows) * batch
+                  : static_cast<long long>(tokens) * G > kRows;
 }
 
 size_t part_o_bytes(const ChunkPlan& p, int D) {
@@ -557,8 +563,11 @@ extern "C" size_t voom_paged_gqa_chunk_workspace_bytes(int batch, int rows, int 
   if (!chunk_shape_ok(batch, rows, tokens, num_q_heads, num_kv_heads, head_dim, page_tokens,
                       max_pages) || window < 0)
     return 0;
-  const ChunkPlan p = plan_chunk(batch, num_kv_heads, head_dim, num_q_heads / num_kv_heads, rows,
-                                 tokens, max_pages, page_tokens, window == 0 ? INT_MAX : window);
+  const int G = num_q_heads / num_kv_heads;
+  if (is_wide(batch, rows, tokens, G))
+    return plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens).bytes;
+  const ChunkPlan p = plan_chunk(batch, num_kv_heads, head_dim, G, rows, tokens, max_pages,
+                                 page_tokens, window == 0 ? INT_MAX : window);
   return part_o_bytes(p, head_dim) + static_cast<size_t>(2) * p.W * kRows * 2 * sizeof(float);
 }
 
@@ -616,10 +625,6 @@ extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const voi
   a.prefix = prefix_lens;
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) +
-                                              part_o_bytes(p, head_dim))
-                   : nullptr;
   a.B = batch;
   a.NQ = num_q_heads;
   a.NKV = num_kv_heads;
@@ -633,7 +638,15 @@ extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const voi
   a.scale = scale * 1.4426950408889634f;
   a.cap = softcap * 1.4426950408889634f;
   a.cap_k = softcap > 0.f ? scale / softcap : 0.f;
-  a.tiles = p.tiles;
+  a.part_o = a.part_ml = nullptr;
+  a.W = a.per_xcd = 0;
+  if (is_wide(batch, rows, tokens, G))
+    return launch_wide(a, plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens), head_dim,
+                       workspace, stream);
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) +
+                                              part_o_bytes(p, head_dim))
+                   : nullptr;
   a.W = p.W;
   const long long groups = p.W != 0 ? p.W : p.segs;
   a.per_xcd = static_cast<int>((groups + 7) / 8);
