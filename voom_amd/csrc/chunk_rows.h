@@ -119,7 +119,7 @@ struct WidePlan {
   int workers;     // workgroups that run at once
   size_t bytes;
 };
-WidePlan plan_wide(int B, int NKV, int D, int G, int N, int T);
+WidePlan plan_wide(int B, int NKV, int D, int G, int N, int T, long long tokens);
 int launch_wide(const ChunkArgs& a, const WidePlan& p, int D, void* workspace,
                 hipStream_t stream);
 

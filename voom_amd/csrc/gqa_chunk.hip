@@ -565,7 +565,9 @@ extern "C" size_t voom_paged_gqa_chunk_workspace_bytes(int batch, int rows, int 
     return 0;
   const int G = num_q_heads / num_kv_heads;
   if (is_wide(batch, rows, tokens, G))
-    return plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens).bytes;
+    return plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens,
+                     static_cast<long long>(max_pages) * page_tokens)
+        .bytes;
   const ChunkPlan p = plan_chunk(batch, num_kv_heads, head_dim, G, rows, tokens, max_pages,
                                  page_tokens, window == 0 ? INT_MAX : window);
   return part_o_bytes(p, head_dim) + static_cast<size_t>(2) * p.W * kRows * 2 * sizeof(float);
@@ -641,8 +643,10 @@ extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const voi
   a.part_o = a.part_ml = nullptr;
   a.W = a.per_xcd = 0;
   if (is_wide(batch, rows, tokens, G))
-    return launch_wide(a, plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens), head_dim,
-                       workspace, stream);
+    return launch_wide(a,
+                       plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens,
+                                 static_cast<long long>(max_pages) * page_tokens),
+                       head_dim, workspace, stream);
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                               part_o_bytes(p, head_dim))

@@ -16,10 +16,8 @@
 // loop, those at the window's edge and the diagonal one with masks, two at a time.
 //
 // gqa_chunk_plan_kernel lists the row tiles of all sequences, from their lengths on the
-// device, the longest of a sequence first, and cuts those over keys that are longer than a
-// workgroup's share of all tiles; the pieces leave (m, l, o) in fp32 and
-// gqa_chunk_join_kernel merges them.  Workgroups are dealt pieces in runs of 32 an XCD, which
-// share K and V in its L2.
+// device, and cuts long ones over keys, so that the workgroups are done at about the same time;
+// the pieces leave (m, l, o) in fp32 and gqa_chunk_join_kernel merges them.
 #include "chunk_rows.h"
 
 #include <cfloat>
@@ -35,7 +33,6 @@ constexpr int kRows = 32;       // rows of a wavefront
 constexpr int NW = 4;           // wavefronts of a workgroup
 constexpr int kTileRows = NW * kRows;
 constexpr int kAhead = 4;       // operand reads ahead of the MFMAs
-constexpr int kRun = 32;        // pieces that an XCD takes at a time
 constexpr int kMinPiece = 8;    // tiles of a piece at least
 constexpr float kSlack = 8.f;   // the reference maxima stay that far behind, in log2 units
 
@@ -77,47 +74,63 @@ struct KeyTiles {
   __device__ __forceinline__ int tile(int c) const { return c < pre ? c : c + gap; }
 };
 
-// Inclusive sum over the workgroup's 1,024 threads; `total` that of all of them.
-__device__ __forceinline__ int group_scan(int x, int* shared, int& total) {
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wv = threadIdx.x / kWave;
-  x = wave_inclusive_scan(x, lane);
-  __syncthreads();
-  if (lane == kWave - 1) shared[wv] = x;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int v = shared[i];
-    before += i < wv ? v : 0;
-    total += v;
-  }
-  return before + x;
-}
+// Cuts the row tiles of all sequences into pieces.  A piece has at most `most` key tiles; of
+// some candidates the one is taken with which the workers are done first: `rounds` of pieces
+// of the average length (where one round holds them all, a CU's two workers are a long and a
+// short one), each with what it costs besides (kLead key tiles, kCutLead where it also
+// leaves its state to be merged).  Pieces are listed in falling length.
+constexpr int kPlanThreads = 256;
+constexpr int kHeld = 2048;      // row tiles whose lengths are held in LDS
+constexpr int kClasses = 64;     // of lengths
+constexpr int kTries = 8;
+constexpr float kLead = 3.f, kCutLead = 9.f;
+constexpr float kCaps[kTries] = {0.f, 2.f, 1.5f, 1.2f, 1.f, 0.8f, 0.6f, 0.4f};  // of a share
 
-__global__ __launch_bounds__(1024) void gqa_chunk_plan_kernel(WideArgs w) {
+__global__ __launch_bounds__(kPlanThreads) void gqa_chunk_plan_kernel(WideArgs w) {
+  constexpr int kPlanWaves = kPlanThreads / kWave;
   const ChunkArgs& a = w.c;
   __shared__ int first[kMaxChunkBatch + 1];  // row tiles before each sequence
-  __shared__ int sums[16];
+  __shared__ int4 seqs[kMaxChunkBatch];      // context, new tokens, prefix
+  __shared__ int held[kHeld];
+  __shared__ int sums[kPlanWaves];
   __shared__ unsigned long long all;
+  __shared__ int longest, tried[kTries], classes[kClasses], slots, cuts;
   const int tid = static_cast<int>(threadIdx.x);
-  if (tid == 0) all = 0;
-  {
-    int tiles = 0, total, base;
-    if (tid < a.B) {
-      const int rows = (a.starts != nullptr ? new_of(a, tid, base) : a.T) * a.G;
-      tiles = (rows + kTileRows - 1) / kTileRows;
-    }
-    const int x = group_scan(tiles, sums, total);
-    if (tid < a.B) first[tid + 1] = x;
-    if (tid == 0) first[0] = 0;
+  const int lane = tid & (kWave - 1);
+  const int wv = uniform(tid / kWave);
+  if (tid < kClasses) classes[tid] = 0;
+  if (tid < kTries) tried[tid] = 0;
+  if (tid == 0) {
+    all = 0;
+    longest = slots = cuts = 0;
+    first[0] = 0;
   }
-  __syncthreads();
-  int entries = first[a.B];
-  entries = entries < w.p.entries ? entries : w.p.entries;  // (starts that overlap)
-  // entry e: its sequence, row tile (the last, which sees most, first) and key tiles
-  auto entry = [&](int e, int& b, int& rt) {
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kPlanThreads) {
+    const int b = b0 + tid;
+    int tiles = 0;
+    if (b < a.B) {
+      int base;
+      const int ctx = context_of(a, b), n = new_of(a, b, base);
+      seqs[b] = {ctx, n, prefix_of(a, b, ctx), 0};
+      tiles = ((a.starts != nullptr ? n : a.T) * a.G + kTileRows - 1) / kTileRows;
+    }
+    const int x = wave_inclusive_scan(tiles, lane);
+    if (lane == kWave - 1) sums[wv] = x;
+    __syncthreads();
+    int here = 0, total = 0;
+#pragma unroll
+    for (int i = 0; i < kPlanWaves; ++i) {
+      here += i < wv ? sums[i] : 0;
+      total += sums[i];
+    }
+    if (b < a.B) first[b + 1] = before + here + x;
+    before += total;
+    __syncthreads();
+  }
+  const int entries = before < w.p.entries ? before : w.p.entries;  // (starts that overlap)
+  // row tile e: its sequence, its place there (the last, which sees most, first), key tiles
+  auto place = [&](int e, int& b, int& rt) {
     int lo = 0, hi = a.B;
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -126,43 +139,103 @@ __global__ __launch_bounds__(1024) void gqa_chunk_plan_kernel(WideArgs w) {
     }
     b = lo;
     rt = first[lo + 1] - 1 - e;
-    int base;
-    const int ctx = context_of(a, b), n = new_of(a, b, base);
-    return KeyTiles(a, ctx, n, prefix_of(a, b, ctx), rt).count;
+  };
+  auto length = [&](int e) {
+    int b, rt;
+    place(e, b, rt);
+    return KeyTiles(a, seqs[b].x, seqs[b].y, seqs[b].z, rt).count;
   };
   unsigned long long mine = 0;
-  for (int e = tid; e < entries; e += 1024) {
-    int b, rt;
-    mine += entry(e, b, rt);
+  int top = 0;
+  for (int e = tid; e < entries; e += kPlanThreads) {
+    const int n = length(e);
+    if (e < kHeld) held[e] = n;
+    mine += n;
+    top = n > top ? n : top;
   }
-  atomicAdd(&all, mine);
+#pragma unroll
+  for (int k = 1; k < kWave; k <<= 1) {
+    mine += __shfl_xor(mine, k);
+    const int o = __shfl_xor(top, k);
+    top = o > top ? o : top;
+  }
+  if (lane == 0) {
+    atomicAdd(&all, mine);
+    atomicMax(&longest, top);
+  }
   __syncthreads();
-  const unsigned long long share = (all * a.NKV + w.p.workers - 1) / w.p.workers;
-  const int most = share < kMinPiece ? kMinPiece : (share < INT_MAX ? static_cast<int>(share)
-                                                                    : INT_MAX);
-  int pieces = 0, slots = 0, cuts = 0;
-  for (int e0 = 0; e0 < entries; e0 += 1024) {
-    const int e = e0 + tid;
-    int b = 0, rt = 0, count = 0, parts = 0, total;
-    if (e < entries) {
-      count = entry(e, b, rt);
-      parts = count > most ? (count + most - 1) / most : 1;
+  const float share = static_cast<float>(all) * a.NKV / w.p.workers;  // of a worker
+  // (no piece so short that there are more of them than the workspace holds)
+  auto limit = [&](int i) {
+    const float part = share * (i == 0 ? 1e9f : kCaps[i]);
+    const int least = static_cast<int>(share * kCaps[kTries - 1]) + 1;
+    const int n = part < static_cast<float>(longest) ? static_cast<int>(part) + 1 : longest;
+    const int floor = least > kMinPiece ? least : kMinPiece;
+    return n > floor ? n : floor;
+  };
+  {
+    int parts[kTries] = {};
+    for (int e = tid; e < entries; e += kPlanThreads) {
+      const int n = e < kHeld ? held[e] : length(e);
+#pragma unroll
+      for (int i = 0; i < kTries; ++i) parts[i] += n > limit(i) ? (n + limit(i) - 1) / limit(i) : 1;
     }
-    int p = pieces + group_scan(parts, sums, total) - parts;
-    pieces += total;
-    const bool cut = parts > 1;
-    int s = slots + group_scan(cut ? parts : 0, sums, total) - (cut ? parts : 0);
-    slots += total;
-    const int k = cuts + group_scan(cut ? 1 : 0, sums, total) - (cut ? 1 : 0);
-    cuts += total;
-    if (cut && k < w.p.cuts) w.cuts[k] = {b, rt, parts, s};
-    for (int i = 0; i < parts && p < w.p.pieces; ++i, ++p) {
-      w.pieces[p] = {b, rt, static_cast<int>(static_cast<long long>(count) * i / parts),
-                     static_cast<int>(static_cast<long long>(count) * (i + 1) / parts)};
-      w.slots[p] = cut && s + i < w.p.slots ? s + i : -1;
+#pragma unroll
+    for (int i = 0; i < kTries; ++i) {
+      const int n = __builtin_amdgcn_readlane(wave_inclusive_scan(parts[i], lane), kWave - 1);
+      if (lane == 0) atomicAdd(&tried[i], n);
     }
   }
+  __syncthreads();
+  int most = 0;
+  float best = FLT_MAX;
+#pragma unroll
+  for (int i = 0; i < kTries; ++i) {
+    const float pieces = static_cast<float>(tried[i]) * a.NKV;
+    const float rounds = ceilf(pieces / w.p.workers);
+    const float cut = tried[i] > entries ? kCutLead : kLead;
+    const float part = static_cast<float>(longest < limit(i) ? longest : limit(i));
+    const float mean = rounds * (static_cast<float>(all) * a.NKV / pieces + cut);
+    const float cost = rounds <= 1.f ? 0.5f * (part + share) + cut : fmaxf(mean, part + cut);
+    if (cost < best) {
+      best = cost;
+      most = limit(i);
+    }
+  }
+  auto parts_of = [&](int n) { return n > most ? (n + most - 1) / most : 1; };
+  const float step = (kClasses - 1) / static_cast<float>(longest < most ? longest + 1 : most + 1);
+  auto class_of = [&](int n) { return kClasses - 1 - static_cast<int>(n * step); };
+  for (int e = tid; e < entries; e += kPlanThreads) {
+    const int n = e < kHeld ? held[e] : length(e);
+    const int parts = parts_of(n);
+    atomicAdd(&classes[class_of(n / parts)], parts);
+  }
+  __syncthreads();
+  if (wv == 0) {
+    const int n = classes[lane];
+    classes[lane] = wave_inclusive_scan(n, lane) - n;
+  }
+  __syncthreads();
+  for (int e = tid; e < entries; e += kPlanThreads) {
+    const int n = e < kHeld ? held[e] : length(e);
+    const int parts = parts_of(n);
+    int b, rt, s = -1;
+    place(e, b, rt);
+    if (parts > 1) {
+      s = atomicAdd(&slots, parts);
+      const int k = atomicAdd(&cuts, 1);
+      if (k < w.p.cuts) w.cuts[k] = {b, rt, parts, s};
+    }
+    int p = atomicAdd(&classes[class_of(n / parts)], parts);
+    for (int i = 0; i < parts && p < w.p.pieces; ++i, ++p) {
+      w.pieces[p] = {b, rt, static_cast<int>(static_cast<long long>(n) * i / parts),
+                     static_cast<int>(static_cast<long long>(n) * (i + 1) / parts)};
+      w.slots[p] = s < 0 || s + i >= w.p.slots ? -1 : s + i;
+    }
+  }
+  __syncthreads();
   if (tid == 0) {
+    const int pieces = classes[kClasses - 1];  // (past the last class: all of them)
     w.head[0] = pieces < w.p.pieces ? pieces : w.p.pieces;
     w.head[1] = cuts < w.p.cuts ? cuts : w.p.cuts;
   }
@@ -204,19 +277,20 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
   __shared__ __attribute__((aligned(1024))) uint16_t tile_b[4 * kBlkElems];
   const ChunkArgs& a = wa.c;
 
-  // Runs of consecutive pieces to the XCDs in turn, shorter ones where there are few.
-  const int per_head = wa.head[0];
-  const int total = per_head * a.NKV;
-  int run = (total + 7) / 8;
-  run = run < kRun ? run : kRun;
-  const int bid = static_cast<int>(blockIdx.x);
-  const int in_xcd = bid >> 3;
-  if (total == 0) return;
-  const int wk = ((in_xcd / run) * 8 + (bid & 7)) * run + in_xcd % run;
-  if (wk >= total) return;
-  const int kvh = wk / per_head;
-  const int4 piece = wa.pieces[wk - kvh * per_head];
-  const int slot = wa.slots[wk - kvh * per_head];
+  // A piece for all kv heads in turn, the longest first: an XCD takes every eighth, so that
+  // the heads of its pieces, and with them K and V in its L2, are few.  Where one round holds
+  // all of them the second half is dealt the other way round: a CU then has a long one and a
+  // short one.
+  const int total = wa.head[0] * a.NKV;
+  int wk = static_cast<int>(blockIdx.x);
+  if (total <= wa.p.workers && wk >= wa.p.workers / 2)
+    wk = 8 * ((total + 7) / 8 - 1 - (wk - wa.p.workers / 2) / 8) + (wk & 7);
+  if (wk >= total || (wk < wa.p.workers / 2) != (static_cast<int>(blockIdx.x) < wa.p.workers / 2))
+    return;
+  const int in_head = wk / a.NKV;
+  const int kvh = wk - in_head * a.NKV;
+  const int4 piece = wa.pieces[in_head];
+  const int slot = uniform(wa.slots[in_head]);
   const int b = uniform(piece.x);
   const int rt = uniform(piece.y);
   const int c_lo = uniform(piece.z);
@@ -712,6 +786,7 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
       a.lse[at] = empty ? -INFINITY : (m + __log2f(lt)) * 0.6931471805599453f;
     return;
   }
+  if (row >= R) return;  // (not merged)
   const size_t p = (static_cast<size_t>(kvh) * wa.p.slots + slot) * kTileRows + w * kRows + l32;
   float* o = a.part_o + p * D + 4 * lh;
 #pragma unroll
@@ -726,35 +801,36 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
 }
 
 // Merges the pieces of cut row tiles, a row at a time to a wavefront.
-constexpr int kJoinWaves = 4;
-constexpr int kJoinRows = 16;  // rows of a workgroup
+constexpr int kJoinWaves = 16;
+constexpr int kJoinGroups = 512;
 
 template <int D>
 __global__ __launch_bounds__(kJoinWaves * kWave) void gqa_chunk_join_kernel(WideArgs wa) {
   constexpr int DPL = D / kWave;
   constexpr int kTogether = 8;  // rows in flight
   const ChunkArgs& a = wa.c;
-  if (static_cast<int>(blockIdx.x) >= wa.head[1]) return;
-  const int4 cut = wa.cuts[blockIdx.x];
-  const int kvh = static_cast<int>(blockIdx.y);
   const int lane = threadIdx.x & (kWave - 1);
-  const int b = uniform(cut.x), rt = uniform(cut.y), parts = uniform(cut.z);
-  int base;
-  const int n = uniform(new_of(a, b, base));
-  for (int i = uniform(threadIdx.x / kWave); i < kJoinRows; i += kJoinWaves) {
-    const int r = static_cast<int>(blockIdx.z) * kJoinRows + i;
+  const long long rows = static_cast<long long>(wa.head[1]) * a.NKV * kTileRows;
+  for (long long at_row = static_cast<long long>(blockIdx.x) * kJoinWaves +
+                          uniform(threadIdx.x / kWave);
+       at_row < rows; at_row += kJoinGroups * kJoinWaves) {
+    const int r = static_cast<int>(at_row) & (kTileRows - 1);
+    const int head_cut = static_cast<int>(at_row / kTileRows);
+    const int kvh = head_cut % a.NKV;
+    const int4 cut = wa.cuts[head_cut / a.NKV];
+    const int b = uniform(cut.x), rt = uniform(cut.y), parts = uniform(cut.z);
+    int base;
+    const int n = uniform(new_of(a, b, base));
     const int row = rt * kTileRows + r;
     const int tok = row / a.G;
-    if (tok >= n) {
-      if (a.starts != nullptr || tok >= a.T) return;
-    }
+    if (tok >= n && (a.starts != nullptr || tok >= a.T)) continue;
     const int head = kvh * a.G + (row - tok * a.G);
     const size_t p0 = (static_cast<size_t>(kvh) * wa.p.slots + cut.w) * kTileRows + r;
     const float2* ml2 = reinterpret_cast<const float2*>(a.part_ml);
     // up to 64 pieces at a time, one per lane for their maxima and sums
     float M = -FLT_MAX, L = 0.f;
     float acc[DPL] = {};
-    for (int s0 = 0; s0 < parts; s0 += kWave) {
+    for (int s0 = 0; s0 < parts && tok < n; s0 += kWave) {
       const int m = parts - s0 < kWave ? parts - s0 : kWave;
       const float2 ml = ml2[p0 + static_cast<size_t>(s0 + (lane < m ? lane : 0)) * kTileRows];
       const float mn = fmaxf(M, wave_max_uniform(lane < m ? ml.x : -FLT_MAX));
@@ -809,19 +885,23 @@ void launch_tiles(const WideArgs& w, bool bias, dim3 grid, hipStream_t stream) {
 
 }  // namespace
 
-// A row tile is cut where it is longer than a worker's share of all key tiles, so a kv head
-// has at most `workers / NKV` pieces more than row tiles, as many cut ones, and twice as
-// many pieces of those.
-WidePlan plan_wide(int B, int NKV, int D, int G, int N, int T) {
+// A piece of a cut row tile has more than half of the shortest candidate's key tiles, of which
+// all workers' shares hold workers / kCaps[last]: at most twice as many pieces, all heads
+// together, and half as many cut row tiles.
+WidePlan plan_wide(int B, int NKV, int D, int G, int N, int T, long long tokens) {
   WidePlan p;
   p.workers = 2 * device_cu_count();
   const long long entries =
       N > 0 ? static_cast<long long>(N) * G / kTileRows + (B < N ? B : N)
             : static_cast<long long>(B) * ((static_cast<long long>(T) * G + kTileRows - 1) / kTileRows);
   p.entries = static_cast<int>(entries);
-  p.cuts = p.workers / NKV + 1;
-  p.pieces = p.entries + p.cuts;
-  p.slots = 2 * p.cuts;
+  p.cuts = static_cast<int>(p.workers / kCaps[kTries - 1] / NKV) + 1;
+  // (nor more than pieces of kMinPiece key tiles or a little under)
+  const long long parts = (tokens / kKeys + 1) / (kMinPiece / 2) + 1;
+  if (p.cuts > entries) p.cuts = p.entries;
+  p.slots = static_cast<int>(2LL * (p.workers / kCaps[kTries - 1] / NKV + 1));
+  if (p.slots > parts * entries) p.slots = static_cast<int>(parts * entries);
+  p.pieces = p.entries + p.slots;
   const size_t rows = static_cast<size_t>(p.slots) * NKV * kTileRows;
   p.bytes = up(rows * D * sizeof(float)) + up(rows * sizeof(float2)) +
             up(p.pieces * sizeof(int4)) + up(p.pieces * sizeof(int32_t)) +
@@ -847,12 +927,11 @@ int launch_wide(const ChunkArgs& a, const WidePlan& p, int D, void* workspace,
   w.cuts = reinterpret_cast<int4*>(at);
   at += up(p.cuts * sizeof(int4));
   w.head = reinterpret_cast<int32_t*>(at);
-  hipLaunchKernelGGL(gqa_chunk_plan_kernel, dim3(1), dim3(1024), 0, stream, w);
+  hipLaunchKernelGGL(gqa_chunk_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, w);
   int rc = VOOM_LAUNCH_CHECK("paged_gqa_chunk: plan launch");
   if (rc) return rc;
-  // (the last run of each XCD may be a part of one)
-  const long long in_xcd = (static_cast<long long>(p.pieces) * a.NKV + 7) / 8 + 2 * kRun;
-  const dim3 grid(static_cast<unsigned>(8 * in_xcd));
+  const long long most = static_cast<long long>(p.pieces) * a.NKV;
+  const dim3 grid(static_cast<unsigned>(most > p.workers ? most : p.workers));
   const bool bias = a.slopes != nullptr || (a.cap == 0.f && !(a.scale > 0.f));
   if (D == 128) {
     if (a.cap != 0.f) launch_tiles<128, true>(w, bias, grid, stream);
@@ -863,8 +942,7 @@ int launch_wide(const ChunkArgs& a, const WidePlan& p, int D, void* workspace,
   }
   rc = VOOM_LAUNCH_CHECK("paged_gqa_chunk: tiles launch");
   if (rc) return rc;
-  const dim3 jgrid(static_cast<unsigned>(p.cuts < p.entries ? p.cuts : p.entries),
-                   static_cast<unsigned>(a.NKV), kTileRows / kJoinRows);
+  const dim3 jgrid(kJoinGroups);
   if (D == 128)
     hipLaunchKernelGGL(gqa_chunk_join_kernel<128>, jgrid, dim3(kJoinWaves * kWave), 0, stream, w);
   else
