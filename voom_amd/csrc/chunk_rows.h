@@ -108,6 +108,17 @@ __device__ __forceinline__ float capped_far(float x, float cap) {
   return __builtin_fmaf(-2.f * cap, __builtin_amdgcn_rcpf(e + 1.f), cap);
 }
 
+// ---- the kernels of single tokens (gqa_chunk_token.hip) and short chunks ------------
+
+// How a call with few rows is cut.
+struct FewPlan {
+  int rows;        // of a row tile
+  long long segs;  // (sequence, kv head, row tile) segments at most
+  int W;           // workers of the split; 0: one per segment, no reduce launch
+};
+FewPlan plan_token(int B, int NKV, int G, int N, int T, long long tokens, int window);
+int launch_token(const ChunkArgs& a, const FewPlan& p, int D, hipStream_t stream);
+
 // ---- the kernel of long chunks (gqa_chunk_wide.hip) ------------------------------
 
 // Its workspace, sized for any lengths that the call's rows allow.

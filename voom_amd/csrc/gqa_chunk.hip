@@ -18,8 +18,7 @@
 // of its segments, which lie end to end and are dealt out evenly; gqa_chunk_reduce_kernel
 // merges cut ones.  Stages run through one ring in order; a stage that every row of the tile
 // sees whole skips the masks.
-#include "chunk_rows.h"
-#include "paged_rows.h"
+#include "chunk_few.h"
 
 #include <climits>
 
@@ -27,100 +26,8 @@ namespace voom {
 namespace {
 
 constexpr int kRows = 16 * kRowWaves;  // of a tile
-constexpr int kLead = 8;               // units that a segment costs besides its stages
-
-// Units of a sequence: for every kv head and row tile the stages that its rows see, after
-// kLead units that stand for what a segment costs besides.  Stages from `pre` on lie `gap`
-// further on in the context.
 template <int D>
-struct Units {
-  int chunks, tiles, pre, gap;
-  __device__ __forceinline__ int all(const ChunkArgs& a) const {
-    if (a.W == 0) return tiles * a.NKV;
-    return chunks == 0 ? 0 : (chunks + kLead) * tiles * a.NKV;
-  }
-  __device__ __forceinline__ Units(const ChunkArgs& a, int b) {
-    constexpr int kTok = stage_tokens(D);
-    int base;
-    const int ctx = context_of(a, b), n = new_of(a, b, base), p = prefix_of(a, b, ctx);
-    const Sight first(a, ctx, n, p, 0);
-    pre = (p + kTok - 1) / kTok;
-    gap = first.lo / kTok - pre;
-    gap = gap < 0 ? 0 : gap;
-    chunks = n == 0 ? 0 : (ctx + kTok - 1) / kTok - gap;
-    // (rows behind a padded sequence's are written by its segments where none is cut)
-    tiles = ((a.W == 0 && a.starts == nullptr ? a.T : n) * a.G + kRows - 1) / kRows;
-  }
-};
-
-// The units of up to 64 sequences from `base` on, one per lane, and their inclusive sum.
-template <int D>
-__device__ __forceinline__ Units<D> scan_units(const ChunkArgs& a, int base, int lane, int& x) {
-  const bool in = base + lane < a.B;
-  const Units<D> u(a, in ? base + lane : 0);
-  x = wave_inclusive_scan(in ? u.all(a) : 0, lane);
-  return u;
-}
-
-// What the row of this lane's column sees, and its score's slope.
-struct View {
-  int ctx, pre, at, lo, hi;
-  float slope;  // log2 units
-  bool biased;
-  // Bit e: it sees token pos + e, e < 8.
-  __device__ __forceinline__ uint32_t seen(int pos) const {
-    return hi > 0 ? bits_in(pos, lo, hi) | bits_in(pos, 0, pre) : 0u;
-  }
-};
-
-// Scores in log2 units, of this lane's 8 tokens from pos on.
-__device__ __forceinline__ void score(f32x4 (&sc)[1][2], const ChunkArgs& a, const View& view,
-                                      int pos) {
-  if (a.cap != 0.f) {
-    float x[8];
-    bool far = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = sc[0][e >> 2][e & 3] * a.cap_k;
-      far |= fabsf(x[e]) > kNear;
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sc[0][e >> 2][e & 3] = a.cap * x[e] * tanh_ratio(x[e] * x[e]);
-    if (__builtin_amdgcn_ballot_w64(far) != 0) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y = capped_far(x[e], a.cap);
-        sc[0][e >> 2][e & 3] = fabsf(x[e]) > kNear ? y : sc[0][e >> 2][e & 3];
-      }
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sc[0][e >> 2][e & 3] *= a.scale;
-  }
-  if (view.biased) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int d = view.at - (pos + e);
-      sc[0][e >> 2][e & 3] -= view.slope * static_cast<float>(d < 0 ? -d : d);
-    }
-  }
-}
-
-// Forms P of a block's scores.
-template <int D>
-__device__ __forceinline__ void weights_of(const f32x4 (&sc)[1][2], State<D, 1>& st,
-                                           u32x4 (&p)[1]) {
-  float mx[1] = {fmaxf(sc[0][0][0], sc[0][1][0])};
-#pragma unroll
-  for (int e = 1; e < 4; ++e) mx[0] = fmaxf(fmaxf(mx[0], sc[0][0][e]), sc[0][1][e]);
-  if (__builtin_amdgcn_ballot_w64(mx[0] > st.m[0] + kSlack) != 0) raise_maxima<D, 1>(mx, st);
-  float w[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = fast_exp2(sc[0][e >> 2][e & 3] - st.m[0]);
-  st.l[0] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-#pragma unroll
-  for (int e = 0; e < 4; ++e) p[0][e] = pack_bf16x2(w[2 * e], w[2 * e + 1]);
-}
+using Geo = Geometry<kRows, stage_tokens(D), 8>;
 
 // A block that some row of the tile does not see whole.
 template <int D>
@@ -141,13 +48,14 @@ __device__ __forceinline__ void edge_block(const uint16_t* tile, const u32x4 (&q
   for (int e = 0; e < 8; ++e)
     sc[0][e >> 2][e & 3] = (seen >> e & 1) != 0 ? sc[0][e >> 2][e & 3] : -INFINITY;
   weights_of<D>(sc, st, p);
-  masked_products<D, 1>(tile, p, st, view.ctx - pos, lane, [&](int) { return seen; });
+  masked_products<D, 1>([&](int n) { return read_v<D>(tile, n, lane); }, p, st, view.ctx - pos,
+                        [&](int) { return seen; });
 }
 
 template <int D, int AUX>
 __global__ __launch_bounds__(kThreads, 2) void gqa_chunk_rows_kernel(ChunkArgs a) {
   constexpr int kBlocks = stage_blocks(D);
-  constexpr int kTok = stage_tokens(D);
+  constexpr int kTok = stage_tokens(D), kLead = Geo<D>::kLead;
   constexpr int kLoads = 2 * kBlocks * (kBlk * D / 512) / kWaves;  // a wavefront's, of a stage
   constexpr int kPad = D + 4;  // floats of a row in LDS: 16 rows start in 16 bank groups
   // The ring.  Distinct objects, so that reads of one provably miss the pending
@@ -173,12 +81,12 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_chunk_rows_kernel(ChunkArgs a
   int b = 0, kvh, tile, c0, c1, chunks = 0, tiles = 1, pre = 0, gap = 0;
   int u0 = w, u1 = w + 1, begin = 0;  // the workgroup's units, and the segment's first one
   int x0;  // (every wavefront for itself: no barrier)
-  const Units<D> first = scan_units<D>(a, 0, lane, x0);
+  const Units<Geo<D>> first = scan_units<Geo<D>>(a, 0, lane, x0);
   if (a.W != 0) {
     int U = __builtin_amdgcn_readlane(x0, kWave - 1);
     for (int base = kWave; base < a.B; base += kWave) {
       int x;
-      scan_units<D>(a, base, lane, x);
+      scan_units<Geo<D>>(a, base, lane, x);
       U += __builtin_amdgcn_readlane(x, kWave - 1);
     }
     const Split split(U, a.W);
@@ -189,8 +97,8 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_chunk_rows_kernel(ChunkArgs a
   for (int base = 0;; base += kWave) {  // the sequence that holds unit u0
     if (base >= a.B) return;
     int x = x0;
-    Units<D> units = first;
-    if (base != 0) units = scan_units<D>(a, base, lane, x);
+    Units<Geo<D>> units = first;
+    if (base != 0) units = scan_units<Geo<D>>(a, base, lane, x);
     const int here = __builtin_amdgcn_readlane(x, kWave - 1);
     if (u0 < begin + here) {
       const int k = __popcll(__builtin_amdgcn_ballot_w64(begin + x <= u0));
@@ -369,7 +277,7 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_chunk_rows_kernel(ChunkArgs a
       if (++kvh == a.NKV) {
         kvh = 0;
         do {
-          const Units<D> units(a, ++b);
+          const Units<Geo<D>> units(a, ++b);
           chunks = uniform(units.chunks);
           tiles = uniform(units.tiles);
           pre = uniform(units.pre);
@@ -381,141 +289,15 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_chunk_rows_kernel(ChunkArgs a
   }
 }
 
-constexpr int kReduceWaves = 4;
-
-// One wavefront per row: merges the pieces of its segment, where the split cut it, and
-// writes the rows that no segment holds.
-template <int D>
-__global__ __launch_bounds__(kReduceWaves * kWave) void gqa_chunk_reduce_kernel(ChunkArgs a) {
-  // A wavefront holds the row of kTogether pieces at a time, 4 dims per lane.
-  constexpr int kLanes = D / 4;
-  constexpr int kTogether = kWave / kLanes;
-  constexpr int kAhead = 8;  // loads in flight
-  const int lane = threadIdx.x & (kWave - 1);
-  const int kvh = static_cast<int>(blockIdx.y);
-  const int all = static_cast<int>(blockIdx.x) * kReduceWaves + uniform(threadIdx.x / kWave);
-  int b = static_cast<int>(blockIdx.z);
-  int rr = all;  // the row within its sequence
-  if (a.starts != nullptr) {
-    const int token = all / a.G;
-    if (token >= a.N) return;
-    // the last sequence that starts at or before the token (those behind it are empty)
-    b = -1;
-    for (int at = 0; at < a.B; at += kWave) {
-      const bool in = at + lane < a.B && a.starts[at + lane < a.B ? at + lane : 0] <= token;
-      b += __popcll(__builtin_amdgcn_ballot_w64(in));
-    }
-    if (b < 0) return;
-  } else if (all >= a.T * a.G) {
-    return;
-  }
-  int base;
-  const int n = uniform(new_of(a, b, base));
-  if (a.starts != nullptr) rr -= base * a.G;
-  const int t = rr / a.G;
-  if (a.starts != nullptr && (t < 0 || t >= n)) return;  // of no sequence
-  const int tile = rr / kRows;
-  const int r = rr - tile * kRows;
-  const int head = kvh * a.G + (rr - t * a.G);
-  const size_t at = out_at(a, b, base, t, head);
-  const int sub = lane / kLanes;
-  const int dim = lane % kLanes * 4;
-  int first = 0, last = -1;
-  if (t < n) {  // (else 0)
-    // units before sequence b, and of all; stages and row tiles of b
-    int before = 0, chunks = 0, tiles = 1, U = 0;
-    for (int from = 0; from < a.B; from += kWave) {
-      int x;
-      const Units<D> units = scan_units<D>(a, from, lane, x);
-      if (b >= from && b < from + kWave) {
-        chunks = __builtin_amdgcn_readlane(units.chunks, b - from);
-        tiles = __builtin_amdgcn_readlane(units.tiles, b - from);
-        before = U + __builtin_amdgcn_readlane(x, b - from) - (chunks + kLead) * tiles * a.NKV;
-      }
-      U += __builtin_amdgcn_readlane(x, kWave - 1);
-    }
-    if (chunks != 0) {  // (a context of no tokens has no segments)
-      const Split split(U, a.W);
-      const int S = before + (kvh * tiles + tile) * (chunks + kLead) + kLead;
-      first = split.group(S);
-      last = split.group(S + chunks - 1);
-      if (first == last) return;  // written by its workgroup
-    }
-  }
-  // Up to 64 pieces at a time, one per lane for their maxima and sums.  A workgroup leaves
-  // the piece that starts a segment, its last one, in its second slot.
-  float M = -FLT_MAX, L = 0.f;
-  f32x4 acc = {};
-  for (int w0 = first; w0 <= last; w0 += kWave) {
-    const int m = last - w0 + 1 < kWave ? last - w0 + 1 : kWave;
-    const size_t p0 = 2 * static_cast<size_t>(w0) * kRows + r;
-    const int odd = w0 == first ? kRows : 0;  // of the first one
-    auto row_at = [&](int k) {
-      k = k < m ? k : m - 1;
-      return p0 + 2 * static_cast<size_t>(k) * kRows + (k == 0 ? odd : 0);
-    };
-    f32x4 v[kAhead];
-    auto read = [&](int k0) {
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        v[u] = *reinterpret_cast<const f32x4*>(a.part_o + row_at(k0 + u * kTogether + sub) * D +
-                                               dim);
-    };
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + row_at(lane) * 2);
-    read(0);  // (under way while the weights are formed)
-    const float mn = fmaxf(M, wave_max_uniform(lane < m ? ml.x : -FLT_MAX));
-    const float wt = lane < m ? fast_exp2(ml.x - mn) : 0.f;
-    const float f = fast_exp2(M - mn);
-    M = mn;
-    L = L * f + wave_sum_uniform(lane < m ? ml.y * wt : 0.f);
-    acc *= f;
-    for (int k0 = 0; k0 < m; k0 += kAhead * kTogether) {
-      if (k0 != 0) read(k0);
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int k = k0 + u * kTogether + sub;
-        const float ws = __shfl(wt, k & (kWave - 1));
-        if (k < m) acc += v[u] * ws;  // (0 times the infinity of a piece read again is NaN)
-      }
-    }
-  }
-#pragma unroll
-  for (int k = kLanes; k < kWave; k <<= 1) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], k);
-  }
-  const bool empty = L == 0.f;
-  const float inv = 1.f / L;
-  if (sub == 0)
-    *reinterpret_cast<u32x2*>(a.out + at * D + dim) =
-        empty ? u32x2{0u, 0u}
-              : u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv),
-                      pack_bf16x2(acc[2] * inv, acc[3] * inv)};
-  if (a.lse != nullptr && lane == 0)
-    a.lse[at] = empty ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
-}
-
-// How a call is cut.
-struct ChunkPlan {
-  int tiles;         // row tiles of a sequence; of all of them at most, where packed
-  long long segs;    // (sequence, kv head, row tile) segments at most
-  int W;             // workgroups of the split; 0: one per segment, no reduce launch
-};
-
 constexpr int kShort = 8, kLong = 64;  // stages of a segment that is not cut
 
-ChunkPlan plan_chunk(int B, int NKV, int D, int G, int N, int T, int max_pages, int page_tokens,
-                     int window) {
-  ChunkPlan p;
+FewPlan plan_rows(int B, int NKV, int D, int G, int N, int T, long long tokens, int window) {
+  FewPlan p;
   const long long tok = stage_tokens(D);
-  if (N > 0) {
-    p.tiles = static_cast<int>(static_cast<long long>(N) * G / kRows + (B < N ? B : N));
-    p.segs = static_cast<long long>(p.tiles) * NKV;
-  } else {
-    p.tiles = (T * G + kRows - 1) / kRows;
-    p.segs = static_cast<long long>(B) * NKV * p.tiles;
-  }
-  long long stages = (static_cast<long long>(max_pages) * page_tokens + tok - 1) / tok;
+  const long long tiles = N > 0 ? static_cast<long long>(N) * G / kRows + (B < N ? B : N)
+                                : static_cast<long long>(B) * ((T * G + kRows - 1) / kRows);
+  p.segs = tiles * NKV;
+  long long stages = (tokens + tok - 1) / tok;
   const long long seen = (static_cast<long long>(window) + kRows / G) / tok + 2;
   if (seen < stages) stages = seen;
   // All workgroups of a split run at once.  Without one a workgroup walks a segment, which
@@ -525,7 +307,26 @@ ChunkPlan plan_chunk(int B, int NKV, int D, int G, int N, int T, int max_pages, 
   const long long full = (p.segs + cus - 1) / cus * cus;
   const int most = 16 * p.segs >= 15 * full ? kLong : (2 * p.segs >= full ? 2 * kShort : kShort);
   p.W = stages <= most ? 0 : cus;
+  p.rows = kRows;
   return p;
+}
+
+// The kernel that takes a call goes by the rows (new token, head of the group) a kv head of
+// a sequence, on the average: up to 16 that of single tokens, up to 64 the one above, beyond
+// that the one of long chunks.  All three are right for any lengths.
+enum class Kind { kToken, kRows, kWide };
+Kind kind_of(int batch, int rows, int tokens, int G) {
+  const long long all = rows > 0 ? static_cast<long long>(rows) * G
+                                 : static_cast<long long>(tokens) * G * batch;
+  return all <= 16LL * batch ? Kind::kToken
+                             : (all <= static_cast<long long>(kRows) * batch ? Kind::kRows
+                                                                            : Kind::kWide);
+}
+
+FewPlan plan_few(Kind kind, int B, int NKV, int D, int G, int N, int T, long long tokens,
+                 int window) {
+  return kind == Kind::kToken ? plan_token(B, NKV, G, N, T, tokens, window)
+                              : plan_rows(B, NKV, D, G, N, T, tokens, window);
 }
 
 bool chunk_shape_ok(int batch, int rows, int tokens, int num_q_heads, int num_kv_heads,
@@ -540,15 +341,8 @@ bool chunk_shape_ok(int batch, int rows, int tokens, int num_q_heads, int num_kv
          all * num_q_heads < (1LL << 28);
 }
 
-// Calls with more rows a sequence than one row tile takes, on the average, go to the kernel of
-// long chunks (gqa_chunk_wide.hip).
-bool is_wide(int batch, int rows, int tokens, int G) {
-  return rows > 0 ? static_cast<long long>(rows) * G > static_cast<long long>(kRows) * batch
-                  : static_cast<long long>(tokens) * G > kRows;
-}
-
-size_t part_o_bytes(const ChunkPlan& p, int D) {
-  return static_cast<size_t>(2) * p.W * kRows * D * sizeof(float);
+size_t part_o_bytes(const FewPlan& p, int D) {
+  return static_cast<size_t>(2) * p.W * p.rows * D * sizeof(float);
 }
 
 }  // namespace
@@ -564,13 +358,13 @@ extern "C" size_t voom_paged_gqa_chunk_workspace_bytes(int batch, int rows, int 
                       max_pages) || window < 0)
     return 0;
   const int G = num_q_heads / num_kv_heads;
-  if (is_wide(batch, rows, tokens, G))
-    return plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens,
-                     static_cast<long long>(max_pages) * page_tokens)
-        .bytes;
-  const ChunkPlan p = plan_chunk(batch, num_kv_heads, head_dim, G, rows, tokens, max_pages,
-                                 page_tokens, window == 0 ? INT_MAX : window);
-  return part_o_bytes(p, head_dim) + static_cast<size_t>(2) * p.W * kRows * 2 * sizeof(float);
+  const long long cap = static_cast<long long>(max_pages) * page_tokens;
+  const Kind kind = kind_of(batch, rows, tokens, G);
+  if (kind == Kind::kWide)
+    return plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens, cap).bytes;
+  const FewPlan p = plan_few(kind, batch, num_kv_heads, head_dim, G, rows, tokens, cap,
+                             window == 0 ? INT_MAX : window);
+  return part_o_bytes(p, head_dim) + static_cast<size_t>(2) * p.W * p.rows * 2 * sizeof(float);
 }
 
 extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const void* v_pool,
@@ -603,10 +397,10 @@ extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const voi
                "%s: q and pools must be 16-byte aligned", who);
   const int G = num_q_heads / num_kv_heads;
   const int win = window == 0 ? INT_MAX : window;
-  const ChunkPlan p = plan_chunk(batch, num_kv_heads, head_dim, G, rows, tokens, max_pages,
-                                 page_tokens, win);
-  const long long stages = (static_cast<long long>(max_pages) * page_tokens + 63) / 64;
-  VOOM_REQUIRE((stages + kLead) * p.segs < (1LL << 31),
+  const long long cap = static_cast<long long>(max_pages) * page_tokens;
+  const Kind kind = kind_of(batch, rows, tokens, G);
+  const FewPlan p = plan_few(kind, batch, num_kv_heads, head_dim, G, rows, tokens, cap, win);
+  VOOM_REQUIRE(kind == Kind::kWide || (cap / kBlk + 16) * p.segs < (1LL << 31),
                "%s: %d pages of %d tokens for %d sequences are too many", who, max_pages,
                page_tokens, batch);
   const size_t need = voom_paged_gqa_chunk_workspace_bytes(batch, rows, tokens, num_q_heads,
@@ -642,21 +436,20 @@ extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const voi
   a.cap_k = softcap > 0.f ? scale / softcap : 0.f;
   a.part_o = a.part_ml = nullptr;
   a.W = a.per_xcd = 0;
-  if (is_wide(batch, rows, tokens, G))
-    return launch_wide(a,
-                       plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens,
-                                 static_cast<long long>(max_pages) * page_tokens),
+  if (kind == Kind::kWide)
+    return launch_wide(a, plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens, cap),
                        head_dim, workspace, stream);
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = need ? reinterpret_cast<float*>(static_cast<char*>(workspace) +
                                               part_o_bytes(p, head_dim))
                    : nullptr;
   a.W = p.W;
+  if (kind == Kind::kToken) return launch_token(a, p, head_dim, stream);
   const long long groups = p.W != 0 ? p.W : p.segs;
   a.per_xcd = static_cast<int>((groups + 7) / 8);
   const dim3 grid(static_cast<unsigned>(8 * a.per_xcd));
   // (a byte of K/V that one row tile alone reads is streamed past the caches)
-  const bool once = rows > 0 ? rows <= batch : p.tiles == 1;
+  const bool once = rows == 0 && tokens * G <= kRows;
   if (head_dim == 128) {
     if (once) hipLaunchKernelGGL((gqa_chunk_rows_kernel<128, 2>), grid, dim3(kThreads), 0, stream, a);
     else hipLaunchKernelGGL((gqa_chunk_rows_kernel<128, 0>), grid, dim3(kThreads), 0, stream, a);
@@ -666,15 +459,6 @@ extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const voi
   }
   const int rc = VOOM_LAUNCH_CHECK("paged_gqa_chunk: kernel launch");
   if (rc || p.W == 0) return rc;
-  const long long row_groups =
-      ((rows > 0 ? rows : static_cast<long long>(tokens)) * G + kReduceWaves - 1) / kReduceWaves;
-  const dim3 rgrid(static_cast<unsigned>(row_groups), static_cast<unsigned>(num_kv_heads),
-                   static_cast<unsigned>(rows > 0 ? 1 : batch));
-  if (head_dim == 128)
-    hipLaunchKernelGGL(gqa_chunk_reduce_kernel<128>, rgrid, dim3(kReduceWaves * kWave), 0, stream,
-                       a);
-  else
-    hipLaunchKernelGGL(gqa_chunk_reduce_kernel<64>, rgrid, dim3(kReduceWaves * kWave), 0, stream,
-                       a);
-  return VOOM_LAUNCH_CHECK("paged_gqa_chunk: reduce launch");
+  return head_dim == 128 ? launch_reduce<128, Geo<128>>(a, stream)
+                         : launch_reduce<64, Geo<64>>(a, stream);
 }

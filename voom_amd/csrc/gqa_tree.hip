@@ -215,7 +215,8 @@ __device__ __forceinline__ void edge_block(const uint16_t* tile,
     __builtin_amdgcn_sched_barrier(0);
   }
   weights_of<D, NT>(sc, scale, st, p);
-  masked_products<D, NT>(tile, p, st, view.ctx - bi * kBlk - 8 * g, lane,
+  masked_products<D, NT>([&](int n) { return read_v<D>(tile, n, lane); }, p, st,
+                         view.ctx - bi * kBlk - 8 * g,
                          [&](int i) { return view.seen(i, bi * kBlk + 8 * g); });
 }
 

@@ -171,11 +171,10 @@ __device__ __forceinline__ void products(const Operands<D>& o, const u32x4 (&p)[
 // them lie before the context's end.  Tokens past the end are garbage and are cut out of
 // V^T; where only some rows see a token, 0 times a NaN or an infinity is NaN: where V holds
 // one it is taken out, and products of indicators (V is NaN, +inf, -inf; the row sees the
-// token) say which sums it belongs to.
-template <int D, int NT, class Seen>
-__device__ __forceinline__ void masked_products(const uint16_t* tile, const u32x4 (&p)[NT],
-                                                State<D, NT>& st, int valid, int lane,
-                                                Seen seen_of) {
+// token) say which sums it belongs to.  v_of(n) gives the V^T operand of dims 16 n ...
+template <int D, int NT, class Read, class Seen>
+__device__ __forceinline__ void masked_products(Read v_of, const u32x4 (&p)[NT],
+                                                State<D, NT>& st, int valid, Seen seen_of) {
   uint32_t keep[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -183,7 +182,7 @@ __device__ __forceinline__ void masked_products(const uint16_t* tile, const u32x
   uint32_t odd = 0;  // not 0: V holds a NaN or an infinity
 #pragma unroll
   for (int n = 0; n < D / 16; ++n) {
-    u32x4 v = read_v<D>(tile, n, lane);
+    u32x4 v = v_of(n);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t bad = nan_bf16(v[e] & keep[e]);
@@ -208,7 +207,7 @@ __device__ __forceinline__ void masked_products(const uint16_t* tile, const u32x
   }
 #pragma unroll
   for (int n = 0; n < D / 16; ++n) {
-    const u32x4 v = read_v<D>(tile, n, lane);
+    const u32x4 v = v_of(n);
     u32x4 is_nan, is_pos, is_neg;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
