@@ -12,8 +12,8 @@
 //
 // Where segments are long their blocks lie end to end, each segment's after kLead units that
 // stand for what it costs besides, and are dealt out evenly to four wavefronts a CU;
-// gqa_chunk_reduce_kernel merges the cut ones.  Where they are short, or fill the card, a
-// workgroup's eight wavefronts share one and merge it in LDS: one launch.
+// gqa_chunk_reduce_kernel merges the cut ones.  Where they are short a workgroup's wavefronts
+// share one and merge it in LDS: one launch.
 #include "chunk_few.h"
 
 #include <climits>
@@ -25,6 +25,7 @@ constexpr int kTileRows = 16;
 constexpr int kAhead = 2;          // blocks in flight besides the one computed
 constexpr int kSplitWaves = 4;     // wavefronts of a workgroup, split
 constexpr int kSegWaves = 4;       // and of one that walks a whole segment
+constexpr int kShort = 32;         // blocks of a segment that is not cut
 typedef Geometry<kTileRows, kBlk, 4> Geo;
 
 // A wavefront's walk over blocks of one segment.
@@ -339,9 +340,8 @@ FewPlan plan_token(int B, int NKV, int G, int N, int T, long long tokens, int wi
   long long blocks = (tokens + kBlk - 1) / kBlk;
   const long long seen = (static_cast<long long>(window) + kTileRows / G) / kBlk + 2;
   if (seen < blocks) blocks = seen;
-  // One launch where its workgroups are as good as balanced or the contexts short.
-  const int cus = device_cu_count();
-  p.W = blocks <= 4 * kSegWaves ? 0 : kSplitWaves * cus;
+  // One launch where contexts are short.
+  p.W = blocks <= kShort ? 0 : kSplitWaves * device_cu_count();
   p.rows = kTileRows;
   return p;
 }

@@ -49,6 +49,7 @@ struct WideArgs {
   int4* pieces;    // {sequence, row tile, first and last + 1 of its key tiles}
   int32_t* slots;  // where a piece leaves its state, -1: it is the whole row tile
   int4* cuts;      // {sequence, row tile, pieces, first slot}
+  int32_t* lengths;  // key tiles of the row tiles
   WidePlan p;
 };
 
@@ -75,10 +76,11 @@ struct KeyTiles {
 };
 
 // Cuts the row tiles of all sequences into pieces.  A piece has at most `most` key tiles; of
-// some candidates the one is taken with which the workers are done first: `rounds` of pieces
-// of the average length (where one round holds them all, a CU's two workers are a long and a
-// short one), each with what it costs besides (kLead key tiles, kCutLead where it also
-// leaves its state to be merged).  Pieces are listed in falling length.
+// some candidates the one is taken with which the workers are done first.  Each piece costs
+// kLead key tiles besides its own, kCutLead where it also leaves its state to be merged.  Where
+// all pieces run at once, a CU's two workers are a long and a short one; else a worker has its
+// share, and at the end half a piece more or less than others.  Pieces are listed in falling
+// length.
 constexpr int kPlanThreads = 256;
 constexpr int kHeld = 2048;      // row tiles whose lengths are held in LDS
 constexpr int kClasses = 64;     // of lengths
@@ -93,16 +95,15 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_chunk_plan_kernel(WideArgs w
   __shared__ int4 seqs[kMaxChunkBatch];      // context, new tokens, prefix
   __shared__ int held[kHeld];
   __shared__ int sums[kPlanWaves];
-  __shared__ unsigned long long all;
-  __shared__ int longest, tried[kTries], classes[kClasses], slots, cuts;
+  __shared__ float alls[kPlanWaves], tops[kPlanWaves];
+  __shared__ int tried[kTries], classes[kClasses], slots, cuts;
   const int tid = static_cast<int>(threadIdx.x);
   const int lane = tid & (kWave - 1);
   const int wv = uniform(tid / kWave);
   if (tid < kClasses) classes[tid] = 0;
   if (tid < kTries) tried[tid] = 0;
   if (tid == 0) {
-    all = 0;
-    longest = slots = cuts = 0;
+    slots = cuts = 0;
     first[0] = 0;
   }
   int before = 0;
@@ -140,45 +141,45 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_chunk_plan_kernel(WideArgs w
     b = lo;
     rt = first[lo + 1] - 1 - e;
   };
-  auto length = [&](int e) {
+  auto length = [&](int e) -> int& { return e < kHeld ? held[e] : w.lengths[e]; };
+  // (sums in fp32: they weigh candidates, and bound nothing by less than a tile)
+  float mine = 0.f, top = 0.f;
+  for (int e = tid; e < entries; e += kPlanThreads) {
     int b, rt;
     place(e, b, rt);
-    return KeyTiles(a, seqs[b].x, seqs[b].y, seqs[b].z, rt).count;
-  };
-  unsigned long long mine = 0;
-  int top = 0;
-  for (int e = tid; e < entries; e += kPlanThreads) {
-    const int n = length(e);
-    if (e < kHeld) held[e] = n;
-    mine += n;
-    top = n > top ? n : top;
+    const int n = KeyTiles(a, seqs[b].x, seqs[b].y, seqs[b].z, rt).count;
+    length(e) = n;  // (read again by this thread alone)
+    mine += static_cast<float>(n);
+    top = fmaxf(top, static_cast<float>(n));
   }
-#pragma unroll
-  for (int k = 1; k < kWave; k <<= 1) {
-    mine += __shfl_xor(mine, k);
-    const int o = __shfl_xor(top, k);
-    top = o > top ? o : top;
-  }
+  mine = wave_sum_uniform(mine);
+  top = wave_max_uniform(top);
   if (lane == 0) {
-    atomicAdd(&all, mine);
-    atomicMax(&longest, top);
+    alls[wv] = mine;
+    tops[wv] = top;
   }
   __syncthreads();
-  const float share = static_cast<float>(all) * a.NKV / w.p.workers;  // of a worker
-  // (no piece so short that there are more of them than the workspace holds)
-  auto limit = [&](int i) {
-    const float part = share * (i == 0 ? 1e9f : kCaps[i]);
-    const int least = static_cast<int>(share * kCaps[kTries - 1]) + 1;
-    const int n = part < static_cast<float>(longest) ? static_cast<int>(part) + 1 : longest;
-    const int floor = least > kMinPiece ? least : kMinPiece;
-    return n > floor ? n : floor;
+  mine = (alls[0] + alls[1]) + (alls[2] + alls[3]);
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const float share = mine * a.NKV / w.p.workers;  // of a worker
+  // a candidate's key tiles of a piece; no piece so short that the workspace could not hold
+  // all of them
+  auto limit_of = [&](float cap) {
+    const float least = floorf(share * kCaps[kTries - 1]) + 1.f;
+    return fmaxf(fminf(cap == 0.f ? top : floorf(share * cap) + 1.f, top),
+                 fmaxf(least, static_cast<float>(kMinPiece)));
+  };
+  // pieces of n key tiles, `most` in each (in fp32: one more now and then is no matter)
+  auto parts_of = [&](int n, float most) {
+    const float x = static_cast<float>(n);
+    return x > most ? static_cast<int>(ceilf(x * __builtin_amdgcn_rcpf(most))) : 1;
   };
   {
     int parts[kTries] = {};
     for (int e = tid; e < entries; e += kPlanThreads) {
-      const int n = e < kHeld ? held[e] : length(e);
+      const int n = length(e);
 #pragma unroll
-      for (int i = 0; i < kTries; ++i) parts[i] += n > limit(i) ? (n + limit(i) - 1) / limit(i) : 1;
+      for (int i = 0; i < kTries; ++i) parts[i] += n > 0 ? parts_of(n, limit_of(kCaps[i])) : 0;
     }
 #pragma unroll
     for (int i = 0; i < kTries; ++i) {
@@ -187,28 +188,37 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_chunk_plan_kernel(WideArgs w
     }
   }
   __syncthreads();
-  int most = 0;
-  float best = FLT_MAX;
+  float most;
+  {  // a candidate a lane
+    float cap = 0.f;
 #pragma unroll
-  for (int i = 0; i < kTries; ++i) {
-    const float pieces = static_cast<float>(tried[i]) * a.NKV;
-    const float rounds = ceilf(pieces / w.p.workers);
-    const float cut = tried[i] > entries ? kCutLead : kLead;
-    const float part = static_cast<float>(longest < limit(i) ? longest : limit(i));
-    const float mean = rounds * (static_cast<float>(all) * a.NKV / pieces + cut);
-    const float cost = rounds <= 1.f ? 0.5f * (part + share) + cut : fmaxf(mean, part + cut);
-    if (cost < best) {
-      best = cost;
-      most = limit(i);
-    }
+    for (int i = 1; i < kTries; ++i) cap = lane % kTries == i ? kCaps[i] : cap;
+    most = limit_of(cap);
+    const float pieces = static_cast<float>(tried[lane % kTries]) * a.NKV;
+    const float lead = tried[lane % kTries] > tried[0] ? kCutLead : kLead;
+    const float part = fminf(top, most);
+    const float mean = mine * a.NKV / pieces;  // key tiles of a piece
+    const float rounds = pieces / w.p.workers;
+    float cost = rounds <= 1.f ? 0.5f * (part + share) + lead
+                               : fmaxf(part + lead, share + lead * rounds + 0.5f * mean);
+    float best = cost;
+#pragma unroll
+    for (int k = 1; k < kTries; k <<= 1) best = fminf(best, __shfl_xor(best, k));
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(cost == best);
+    most = __builtin_bit_cast(
+        float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, most),
+                                         hit != 0 ? __builtin_ctzll(hit) : 0));
   }
-  auto parts_of = [&](int n) { return n > most ? (n + most - 1) / most : 1; };
-  const float step = (kClasses - 1) / static_cast<float>(longest < most ? longest + 1 : most + 1);
-  auto class_of = [&](int n) { return kClasses - 1 - static_cast<int>(n * step); };
+  const float step = (kClasses - 1) / (fminf(top, most) + 1.f);
+  // the class of a piece's length, the longest first
+  auto class_of = [&](int n, int parts) {
+    const int c = static_cast<int>(n * step / parts);
+    return kClasses - 1 - (c < kClasses ? c : kClasses - 1);
+  };
   for (int e = tid; e < entries; e += kPlanThreads) {
-    const int n = e < kHeld ? held[e] : length(e);
-    const int parts = parts_of(n);
-    atomicAdd(&classes[class_of(n / parts)], parts);
+    const int n = length(e);
+    const int parts = parts_of(n, most);
+    atomicAdd(&classes[class_of(n, parts)], parts);
   }
   __syncthreads();
   if (wv == 0) {
@@ -217,8 +227,8 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_chunk_plan_kernel(WideArgs w
   }
   __syncthreads();
   for (int e = tid; e < entries; e += kPlanThreads) {
-    const int n = e < kHeld ? held[e] : length(e);
-    const int parts = parts_of(n);
+    const int n = length(e);
+    const int parts = parts_of(n, most);
     int b, rt, s = -1;
     place(e, b, rt);
     if (parts > 1) {
@@ -226,11 +236,14 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_chunk_plan_kernel(WideArgs w
       const int k = atomicAdd(&cuts, 1);
       if (k < w.p.cuts) w.cuts[k] = {b, rt, parts, s};
     }
-    int p = atomicAdd(&classes[class_of(n / parts)], parts);
+    int p = atomicAdd(&classes[class_of(n, parts)], parts);
+    const int each = n / parts, more = n - each * parts;  // `more` of them one tile longer
+    int from = 0;
     for (int i = 0; i < parts && p < w.p.pieces; ++i, ++p) {
-      w.pieces[p] = {b, rt, static_cast<int>(static_cast<long long>(n) * i / parts),
-                     static_cast<int>(static_cast<long long>(n) * (i + 1) / parts)};
+      const int to = from + each + (i < more ? 1 : 0);
+      w.pieces[p] = {b, rt, from, to};
       w.slots[p] = s < 0 || s + i >= w.p.slots ? -1 : s + i;
+      from = to;
     }
   }
   __syncthreads();
@@ -278,15 +291,18 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
   const ChunkArgs& a = wa.c;
 
   // A piece for all kv heads in turn, the longest first: an XCD takes every eighth, so that
-  // the heads of its pieces, and with them K and V in its L2, are few.  Where one round holds
-  // all of them the second half is dealt the other way round: a CU then has a long one and a
-  // short one.
+  // the heads of its pieces, and with them K and V in its L2, are few.  Of those that run from
+  // the start, two a CU, the second half is dealt the other way round: a CU then has a long
+  // one and a short one.
   const int total = wa.head[0] * a.NKV;
+  const int half = wa.p.workers / 2;
   int wk = static_cast<int>(blockIdx.x);
-  if (total <= wa.p.workers && wk >= wa.p.workers / 2)
-    wk = 8 * ((total + 7) / 8 - 1 - (wk - wa.p.workers / 2) / 8) + (wk & 7);
-  if (wk >= total || (wk < wa.p.workers / 2) != (static_cast<int>(blockIdx.x) < wa.p.workers / 2))
-    return;
+  if (wk >= half && wk < 2 * half) {
+    const int end = total < 2 * half ? (total + 7) / 8 : half / 4;  // eights of the first round
+    wk = 8 * (end - 1 - (wk - half) / 8) + (wk & 7);
+    if (wk < half) return;
+  }
+  if (wk >= total) return;
   const int in_head = wk / a.NKV;
   const int kvh = wk - in_head * a.NKV;
   const int4 piece = wa.pieces[in_head];
@@ -905,7 +921,7 @@ WidePlan plan_wide(int B, int NKV, int D, int G, int N, int T, long long tokens)
   const size_t rows = static_cast<size_t>(p.slots) * NKV * kTileRows;
   p.bytes = up(rows * D * sizeof(float)) + up(rows * sizeof(float2)) +
             up(p.pieces * sizeof(int4)) + up(p.pieces * sizeof(int32_t)) +
-            up(p.cuts * sizeof(int4)) + 256;
+            up(p.cuts * sizeof(int4)) + 256 + up(p.entries * sizeof(int32_t));
   return p;
 }
 
@@ -927,6 +943,8 @@ int launch_wide(const ChunkArgs& a, const WidePlan& p, int D, void* workspace,
   w.cuts = reinterpret_cast<int4*>(at);
   at += up(p.cuts * sizeof(int4));
   w.head = reinterpret_cast<int32_t*>(at);
+  at += 256;
+  w.lengths = reinterpret_cast<int32_t*>(at);
   hipLaunchKernelGGL(gqa_chunk_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, w);
   int rc = VOOM_LAUNCH_CHECK("paged_gqa_chunk: plan launch");
   if (rc) return rc;

@@ -601,7 +601,16 @@ def fork_kv(k_pools, v_pools, block_tables, ctx_lens: torch.Tensor, parents: tor
     layers = len(k_pools)
     if layers == 0 or len(v_pools) != layers or len(block_tables) != layers:
         raise ValueError("k_pools, v_pools and block_tables must hold one entry a layer")
-    here = _require_here(*k_pools, *v_pools, *block_tables, ctx_lens, parents, first)
+    k_pools, v_pools, block_tables = list(k_pools), list(v_pools), list(block_tables)
+    tensors = [*k_pools, *v_pools, *block_tables, ctx_lens, parents]
+    if first is not None:
+        tensors.append(first)
+    # (one pass over all of them for each property: a hundred tensors and their checks one by
+    # one took the host longer than the copies take the card)
+    here = _CUR_DEVICE() if _CUR_DEVICE is not None else torch.cuda.current_device()
+    if (not all(map(torch.Tensor.is_contiguous, tensors))
+            or set(map(torch.Tensor.get_device, tensors)) != {here}):
+        _require_here(*tensors)
     if parents.dtype is not torch.int32 or parents.dim() != 2:
         raise ValueError("parents must be int32 [B, K]")
     B, K = parents.shape
@@ -609,20 +618,22 @@ def fork_kv(k_pools, v_pools, block_tables, ctx_lens: torch.Tensor, parents: tor
         raise ValueError(f"ctx_lens must be int32 [{B}]")
     if first is not None and not _is_i32(first, B, K):
         raise ValueError(f"first must be int32 [{B}, {K}]")
-    if k_pools[0].dim() != 4:
+    if {t.dtype for t in k_pools} | {t.dtype for t in v_pools} != {torch.bfloat16}:
+        raise ValueError("pools must be bfloat16")
+    if {t.dtype for t in block_tables} != {torch.int32}:
+        raise ValueError(f"block_tables must be int32 [{B * K}, max_pages]")
+    k_sizes, tables = (list(map(torch.Tensor.size, ts)) for ts in (k_pools, block_tables))
+    if len(k_sizes[0]) != 4:
         raise ValueError("k_pool must be [slots, NKV, PT, D]")
-    _, NKV, PT, D = k_pools[0].shape
-    pages, slots = (ctypes.c_int * layers)(), (ctypes.c_int * layers)()
-    for i, (k, v, table) in enumerate(zip(k_pools, v_pools, block_tables)):
-        if k.dtype is not torch.bfloat16 or v.dtype is not torch.bfloat16:
-            raise ValueError("pools must be bfloat16")
-        n = slots[i] = k.shape[0]
-        if k.shape != (n, NKV, PT, D):
-            raise ValueError(f"layer {i}: k_pool must be [slots, {NKV}, {PT}, {D}]")
-        _check_v_pool(v, n, NKV, D, PT)
-        if table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != B * K:
-            raise ValueError(f"layer {i}: block_table must be int32 [{B * K}, max_pages]")
-        pages[i] = table.shape[1]
+    _, NKV, PT, D = k_sizes[0]
+    sizes = {pair: i for i, pair in enumerate(zip(k_sizes, map(torch.Tensor.size, v_pools)))}
+    for (k_size, v_size), layer in sizes.items():
+        if k_size[1:] != (NKV, PT, D) or v_size != (k_size[0], *v_slot_shape(NKV, D, PT)):
+            raise ValueError(f"layer {layer}: k_pool must be [slots, {NKV}, {PT}, {D}] and v_pool "
+                             f"{['slots', *v_slot_shape(NKV, D, PT)]}, not {[*k_size]} and "
+                             f"{[*v_size]}")
+    if any(len(t) != 2 or t[0] != B * K for t in set(tables)):
+        raise ValueError(f"block_tables must be int32 [{B * K}, max_pages]")
     if B * K == 0:
         return
     if _BOUNDS_CHECKS:
@@ -630,10 +641,11 @@ def fork_kv(k_pools, v_pools, block_tables, ctx_lens: torch.Tensor, parents: tor
         rows = ctx_lens.repeat_interleave(K)
         for k, table in zip(k_pools, block_tables):
             check_block_table(table, rows, k.shape[0], PT)
-    pointers = ctypes.c_void_p * layers
+    ints, pointers = ctypes.c_int * layers, ctypes.c_void_p * layers
+    k_ptr, v_ptr, t_ptr = (pointers(*map(torch.Tensor.data_ptr, ts))
+                           for ts in (k_pools, v_pools, block_tables))
     rc = _lib.lib().voom_fork_kv(
-        pointers(*(t.data_ptr() for t in k_pools)), pointers(*(t.data_ptr() for t in v_pools)),
-        pointers(*(t.data_ptr() for t in block_tables)), pages, slots, layers,
+        k_ptr, v_ptr, t_ptr, ints(*(t[1] for t in tables)), ints(*(k[0] for k in k_sizes)), layers,
         ctx_lens.data_ptr(), parents.data_ptr(), _ptr(first), B, K, NKV, D, PT, _stream_of(here))
     if rc:
         _lib.check(rc, "voom_fork_kv")
