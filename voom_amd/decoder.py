@@ -20,8 +20,10 @@ voom_norm_swiglu_rows, voom_linear_rows).  Where the products outweigh the
 launches they are PyTorch-ROCm GEMMs (hipBLASLt) between the separate kernels
 (voom_add_rms_norm, voom_rope_split, voom_silu_mul).  Every attention call is
 the paged HIP kernel.  ``generate_graph`` replays each decode step from one captured HIP
-graph.  Weights use the Hugging Face Llama parameter names so that an
-in-code ``LlamaForCausalLM`` can load them.
+graph, ``generate_beam`` searches with beams whose rows of the cache are copied from one
+another.  Decoders that cap their scores, look back a limited way or norm behind their blocks
+as well (DecoderConfig's last fields) take the separate kernels throughout.  Weights use the
+Hugging Face Llama parameter names so that an in-code ``LlamaForCausalLM`` can load them.
 """
 
 from __future__ import annotations
@@ -49,13 +51,33 @@ class DecoderConfig:
     rms_norm_eps: float = 1e-5
     rope_theta: float = 10000.0
     vocab_size: int = 49152
+    # attention scores capped to attn_softcap * tanh(score / attn_softcap); 0: not
+    attn_softcap: float = 0.0
+    # tokens that a layer looks back (itself included; 0: all of them), but for every
+    # full_attention_every-th layer, which sees all (0: none does)
+    sliding_window: int = 0
+    full_attention_every: int = 0
+    # norms behind the attention and the MLP as well as before them, and what the residual
+    # stream takes of a block
+    post_norms: bool = False
+    residual_scale: float = 1.0
+
+    def window_of(self, layer: int) -> int:
+        """Tokens that a layer looks back, 0: all."""
+        every = self.full_attention_every
+        return 0 if every and (layer + 1) % every == 0 else self.sliding_window
+
+    @property
+    def plain(self) -> bool:
+        """A Llama block: plain softmax scores over all tokens, norms before the blocks."""
+        return not (self.attn_softcap or self.sliding_window or self.post_norms)
 
     @property
     def param_count(self) -> int:
         h, i = self.hidden_size, self.intermediate_size
         qkv = h * (self.num_attention_heads + 2 * self.num_key_value_heads) * self.head_dim
         o = self.num_attention_heads * self.head_dim * h
-        per_layer = qkv + o + 3 * h * i + 2 * h
+        per_layer = qkv + o + 3 * h * i + (4 if self.post_norms else 2) * h
         return self.vocab_size * h + self.num_hidden_layers * per_layer + h
 
 
@@ -83,6 +105,9 @@ def random_weights(cfg: DecoderConfig, seed: int = 0, device=None,
         w[f"{p}.mlp.down_proj.weight"] = mat(h, i)
         w[f"{p}.input_layernorm.weight"] = torch.ones(h, dtype=dtype)
         w[f"{p}.post_attention_layernorm.weight"] = torch.ones(h, dtype=dtype)
+        if cfg.post_norms:
+            w[f"{p}.pre_feedforward_layernorm.weight"] = torch.ones(h, dtype=dtype)
+            w[f"{p}.post_feedforward_layernorm.weight"] = torch.ones(h, dtype=dtype)
     w["model.norm.weight"] = torch.ones(h, dtype=dtype)
     if device is not None:
         w = {k: v.to(device) for k, v in w.items()}
@@ -103,6 +128,8 @@ class PagedDecoder:
     """Greedy decoder over a PagedKVCache (one GEMM per fused projection)."""
 
     def __init__(self, cfg: DecoderConfig, weights: dict[str, torch.Tensor], device=None):
+        if cfg.residual_scale != 1.0 and not cfg.post_norms:
+            raise ValueError("residual_scale belongs to post_norms")
         self.cfg = cfg
         self.device = torch.device(device) if device is not None else torch.device("cuda")
         dev = self.device
@@ -122,17 +149,28 @@ class PagedDecoder:
                 "down": w[f"{p}.mlp.down_proj.weight"],
                 "ln1": w[f"{p}.input_layernorm.weight"],
                 "ln2": w[f"{p}.post_attention_layernorm.weight"],
+                "post1": None,
+                "post2": None,
             })
+            if cfg.post_norms:
+                self.layers[-1].update(
+                    post1=w[f"{p}.post_attention_layernorm.weight"],
+                    ln2=w[f"{p}.pre_feedforward_layernorm.weight"],
+                    post2=w[f"{p}.post_feedforward_layernorm.weight"])
         half = cfg.head_dim // 2
         self.inv_freq = 1.0 / (cfg.rope_theta ** (
             torch.arange(half, dtype=torch.float32, device=dev) / half))
 
     # ---- pieces -------------------------------------------------------------
 
-    def _norm(self, x: torch.Tensor, weight: torch.Tensor,
-              delta: torch.Tensor | None = None) -> torch.Tensor:
+    def _norm(self, x: torch.Tensor, weight: torch.Tensor, delta: torch.Tensor | None = None,
+              post: torch.Tensor | None = None) -> torch.Tensor:
         """x += delta (in place, when given), then RMSNorm: fp32 statistics,
-        result cast to bf16 before the weight (HF LlamaRMSNorm)."""
+        result cast to bf16 before the weight (HF LlamaRMSNorm).  ``post``: the weight of
+        the norm behind the block that delta comes from."""
+        if delta is not None and post is not None:
+            return ops.add_post_norm(x, delta, post, weight, self.cfg.rms_norm_eps,
+                                     scale=self.cfg.residual_scale)
         return ops.add_rms_norm(x, weight, self.cfg.rms_norm_eps, delta=delta)
 
     @staticmethod
@@ -191,7 +229,7 @@ class PagedDecoder:
         H, inter = cfg.hidden_size, cfg.intermediate_size
         qd, kvd = cfg.num_attention_heads * cfg.head_dim, cfg.num_key_value_heads * cfg.head_dim
         rows = x.shape[0] * x.shape[1]
-        return (rows > 1 and rows * H * (2 * qd + 2 * kvd + 3 * inter) <= FUSED_MAX_WORK
+        return (cfg.plain and rows > 1 and rows * H * (2 * qd + 2 * kvd + 3 * inter) <= FUSED_MAX_WORK
                 and cfg.head_dim % 32 == 0 and H % 32 == 0 and inter % 32 == 0
                 and max(H, inter, qd) <= ops.GEMV_MAX_K)
 
@@ -225,18 +263,25 @@ class PagedDecoder:
         lw = self.layers[layer]
         B, L, _ = x.shape
         nq, nkv, hd = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
-        h = self._norm(x, lw["ln1"], delta)
+        scale = hd ** -0.5
+        h = self._norm(x, lw["ln1"], delta, self.layers[layer - 1]["post2"])
+        q, k, v = ops.rope_split(self._linear(h, lw["qkv"]), cos, sin, nq, nkv, hd)
+        scores = {}
+        if cfg.attn_softcap or cfg.window_of(layer):
+            scores = {"softcap": cfg.attn_softcap, "window": cfg.window_of(layer)}
         if graph:
-            q, k, v = ops.rope_split(self._linear(h, lw["qkv"]), cos, sin, nq, nkv, hd)
             kv.append_at(layer, k, v)
-            attn = kv.attend_at(layer, q, hd ** -0.5)
+            attn = (kv.attend_chunk_at(layer, q, scale, **scores) if scores
+                    else kv.attend_at(layer, q, scale))
         else:
-            q, k, v = ops.rope_split(self._linear(h, lw["qkv"]), cos, sin, nq, nkv, hd)
             kv.append(layer, k, v)
-            attn = (kv.attend(layer, q, scale=hd ** -0.5) if L == 1
-                    else kv.attend_prefill(layer, q, scale=hd ** -0.5))
+            if scores:
+                attn = kv.attend_chunk(layer, q, scale, **scores)
+            else:
+                attn = (kv.attend(layer, q, scale=scale) if L == 1
+                        else kv.attend_prefill(layer, q, scale=scale))
         o = self._linear(attn.transpose(1, 2).reshape(B, L, nq * hd), lw["o"])
-        h = self._norm(x, lw["ln2"], o)
+        h = self._norm(x, lw["ln2"], o, lw["post1"])
         return self._mlp(h, lw)
 
     # ---- model --------------------------------------------------------------
@@ -266,7 +311,7 @@ class PagedDecoder:
         if last_only:  # the rows before the last one end here
             x = x[:, -1:].contiguous()
             delta = None if delta is None else delta[:, -1:].contiguous()
-        x = self._norm(x, self.final_norm, delta)
+        x = self._norm(x, self.final_norm, delta, self.layers[-1]["post2"])
         return self._linear(x, self.embed).float()
 
     # ---- one decode step in a HIP graph ------------------------------------------
@@ -283,7 +328,7 @@ class PagedDecoder:
         x = self.embed[tok]
         delta = None
         cfg = self.cfg
-        if B == 1 and max(cfg.hidden_size, cfg.intermediate_size,
+        if cfg.plain and B == 1 and max(cfg.hidden_size, cfg.intermediate_size,
                           cfg.num_attention_heads * cfg.head_dim) <= ops.GEMV_MAX_K:
             # whole RoPE tables (capture_decode's, one row per reserved
             # position, the same elementwise torch ops as _rope_tables): the
@@ -303,7 +348,7 @@ class PagedDecoder:
         cos, sin = self._rope_tables(kv._pos_dev[:1])
         for layer in range(self.cfg.num_hidden_layers):
             delta = self._block(x, delta, layer, kv, cos, sin, graph=True)
-        x = self._norm(x, self.final_norm, delta)
+        x = self._norm(x, self.final_norm, delta, self.layers[-1]["post2"])
         step_logits = self._linear(x, self.embed).float()
         if logits is not None:
             logits.copy_(step_logits[:, -1])
@@ -392,3 +437,43 @@ class PagedDecoder:
             times.append(time.perf_counter() - t1)
             out.append(nxt)
         return out, prefill_s, times
+
+    @torch.no_grad()
+    def generate_beam(self, prompt: torch.Tensor, beams: int, max_tokens: int, kv: PagedKVCache,
+                      end_token: int | None = None):
+        """Beam search behind each prompt [B, L] (of one length): the ``beams`` continuations
+        of up to ``max_tokens`` tokens with the largest sum of log-probabilities that the
+        search finds, a beam ending at ``end_token``.
+
+        Returns (tokens [B, beams, n] int64, best first and filled up with end_token; their
+        scores [B, beams]).  Afterwards the cache holds B * beams rows, the prompt and all
+        tokens but the last of each, in the order of the search.
+        """
+        if kv.offset:
+            raise ValueError("generate_beam() starts on an empty cache")
+        prompt = prompt.to(self.device)
+        B, L = prompt.shape
+        K = int(beams)
+        logits = self.forward(prompt, kv, last_only=True)
+        kv.expand(K)
+        logits = logits.expand(B, K, -1).contiguous()
+        scores = torch.full((B, K), -float("inf"), device=self.device)
+        scores[:, 0] = 0.0  # the prompt's one continuation so far
+        shared = torch.full((B, K, K), L, dtype=torch.int32, device=self.device)
+        tokens = torch.empty((B, K, 0), dtype=torch.long, device=self.device)
+        last = None
+        for step in range(max_tokens):
+            ctx = torch.full((B,), L + step, dtype=torch.int32, device=self.device)
+            ended = {} if end_token is None or last is None else {"last": last,
+                                                                 "end_token": end_token}
+            scores, last, parents, first, shared = ops.beam_select(
+                logits, scores, shared=shared, ctx_lens=ctx, **ended)
+            past = tokens.gather(1, parents.long()[..., None].expand(-1, -1, step))
+            tokens = torch.cat((past, last[..., None]), -1)
+            over = end_token is not None and bool((last == end_token).all())
+            if over or step + 1 == max_tokens:
+                break
+            kv.fork(parents, first, since=L)
+            logits = self.forward(last.view(B * K, 1), kv).view(B, K, -1)
+        order = torch.argsort(scores, dim=1, descending=True, stable=True)
+        return tokens.gather(1, order[..., None].expand_as(tokens)), scores.gather(1, order)

@@ -17,6 +17,10 @@ introspection its tests use, and adds the explicit verbs of the paged path:
   keep_drafts(n, path)     of the newest n tokens only the accepted branch stays
   observe(layer, q, lse)   the attention weight that cached tokens receive is summed up
   evict(budget)            tokens of least weight leave, head by head
+  attend_chunk(layer, q)   attention of the newest tokens with capped or biased scores, a
+                           sliding window or a prefix that all of them see
+  expand(beams)            every sequence becomes that many rows of the cache
+  fork(parents)            rows take the tokens of the row that they go on from (beam search)
   append_latent / update_latent / attend_mla
                            the absorbed-MLA latent cache (runtime/glm.py:265-330)
   spill(pages)             byte-plane split on the GPU -> D2H into the arena
@@ -973,6 +977,14 @@ class PagedKVCache:
         pool = self._pool(layer)
         return ops.paged_gqa_decode(q, pool.k, pool.v, self._tables[layer], self._ctx_dev,
                                     scale=scale)
+
+    def attend_chunk_at(self, layer: int, q: torch.Tensor, scale: float, **scores) -> torch.Tensor:
+        """``attend_chunk`` of one token's q [B, NQ, 1, D] over the device context counter
+        (all pages resident, as ``reserve`` guarantees)."""
+        pool = self._pool(layer)
+        out = ops.paged_gqa_chunk(q, pool.k, pool.v, self._tables[layer], self._ctx_dev,
+                                  scale=scale, **scores)
+        return out.permute(0, 2, 1, 3)
 
     def step_counters(self) -> None:
         """Advance the device position counters by one token (the end of a
@@ -2139,6 +2151,36 @@ class PagedKVCache:
         out = out.permute(0, 2, 1, 3)
         return (out, lse) if return_lse else out
 
+    def attend_chunk(self, layer: int, q: torch.Tensor, scale: float | None = None, *,
+                     window: int = 0, prefix_lens: torch.Tensor | None = None,
+                     return_lse: bool = False, **scores):
+        """Attention of the layer's newest T tokens, whose queries q [B, NQ, T, D] are, with
+        ``ops.paged_gqa_chunk``'s scores (softcap, slopes) and masks (``window``,
+        ``prefix_lens``).  Returns out [B, NQ, T, D] (and the LSE [B, T, NQ]).  Spilled pages
+        of the layer are made resident first, with a window and no prefix those alone that it
+        reaches."""
+        self._require_kind(layer, "kv")
+        B, NQ, T, D = q.shape
+        S = self._len[layer]
+        if T > S:
+            raise ValueError(f"{T} queries but the layer holds {S} tokens")
+        reach = 0
+        if window and prefix_lens is None and not ops.bounds_checks_enabled():
+            reach = max(0, S - T + 1 - int(window))
+        if T == 0:
+            out = torch.empty_like(q)
+            return (out, q.new_empty((B, 0, NQ), dtype=torch.float32)) if return_lse else out
+        pool, table = self._resident(layer, reach)
+        q = q.contiguous()
+        if q.data_ptr() % 16:
+            q = q.clone()  # the kernels load 16 bytes per lane
+        got = ops.paged_gqa_chunk(q, pool.k, pool.v, table, self._positions(S), scale=scale,
+                                  window=window, prefix_lens=prefix_lens, return_lse=return_lse,
+                                  **scores)
+        out, lse = got if return_lse else (got, None)
+        out = out.permute(0, 2, 1, 3)
+        return (out, lse) if return_lse else out
+
     def _resident(self, layer: int, first: int = 0):
         """(pool, block table) of a layer with the pages of its tokens from ``first`` on
         resident."""
@@ -2183,6 +2225,101 @@ class PagedKVCache:
                                scores=self._weights[layer])
                 self._torn = "keep_drafts()"  # until every layer is cut
         self._trim_to([length - drafts + n for length in self._len])
+
+    def _require_forkable(self, what: str) -> int:
+        """The length of every layer of a K/V cache whose rows may be copied."""
+        self._require_kind(0, "kv")
+        if len(set(self._len)) != 1:
+            raise ValueError(f"{what} needs layers of one length")
+        return self._len[0]
+
+    def expand(self, beams: int) -> None:
+        """Every sequence becomes ``beams`` rows, rows b * beams to (b + 1) * beams - 1 of the
+        batch, all of them with its tokens: the start of a beam search behind one prompt.
+        Spilled pages are made resident first; ``max_bytes`` is enforced afterwards."""
+        beams = int(beams)
+        S = self._require_forkable("expand()")
+        if beams <= 0:
+            raise ValueError(f"{beams} beams")
+        if self._has_reserved:
+            raise ValueError("expand(): captured steps hold the cache's batch")
+        if beams == 1:
+            return
+        self.check_integrity()
+        self._drop_prefetch()
+        for layer in range(self.num_layers):
+            self._resident(layer)
+        kind, B, NKV, D = self._geom
+        rows = B * beams
+        # slots of every layer before anything changes: what may fail, fails here
+        grown = []
+        for layer in range(self.num_layers):
+            pool = self._pool(layer)
+            pages = [(p.index, p.slots) for p in self._pages[layer]]
+            pages += list(self._open_slots[layer].items())
+            new = pool.allocate(len(pages) * (rows - B))
+            each = rows - B
+            cols = {}
+            for i, (index, old) in enumerate(pages):
+                mine = iter(new[i * each:(i + 1) * each])
+                cols[index] = [old[r // beams] if r % beams == 0 else next(mine)
+                               for r in range(rows)]
+            grown.append(cols)
+        self._torn = "expand()"  # until every row holds its tokens
+        self._geom = (kind, rows, NKV, D)
+        for layer, cols in enumerate(grown):
+            for p in self._pages[layer]:
+                p.slots = cols[p.index]
+                p.nbytes = self.page_nbytes
+            self._open_slots[layer] = {i: cols[i] for i in self._open_slots[layer]}
+            self._tables[layer] = self._tables_host[layer] = None
+            if cols:
+                self._set_table_cols(layer, cols)
+            if self._weights[layer] is not None:
+                self._weights[layer] = self._weights[layer].repeat_interleave(beams, 0)
+        if S:
+            first_row = torch.zeros((B, beams), dtype=torch.int32, device=self.device)
+            self._fork(first_row, None, S)
+        self._torn = None
+        self._enforce_budget()
+
+    def fork(self, parents: torch.Tensor, first: torch.Tensor | None = None, *,
+             since: int = 0) -> None:
+        """In every layer row j of request b takes the tokens of row parents[b, j] (int32
+        [requests, beams] on the device; requests x beams is the cache's batch, and a row that
+        others go on from is its own parent: ``ops.beam_select``'s), those before first[b, j]
+        (int32, None: 0) excepted, which the two have in common.  ``since``: no first[b, j] is
+        below it, so that spilled pages before it may stay spilled; of the others all come back
+        before a token is copied."""
+        S = self._require_forkable("fork()")
+        since = int(since)
+        if (parents.dtype is not torch.int32 or parents.dim() != 2
+                or parents.numel() != self._batch):
+            raise ValueError(f"parents must be int32 [requests, beams] of {self._batch} rows")
+        if first is not None and (first.dtype is not torch.int32 or first.shape != parents.shape):
+            raise ValueError("first must be like parents")
+        if not 0 <= since <= S:
+            raise ValueError(f"since {since} lies outside the {S} tokens")
+        if ops.bounds_checks_enabled():
+            since = 0
+        self._drop_prefetch()
+        for layer in range(self.num_layers):
+            self._resident(layer, since)
+        self._torn = "fork()"  # until every layer is copied
+        self._fork(parents, first, S)
+        self._torn = None
+        B, K = parents.shape
+        for layer, sums in enumerate(self._weights):
+            if sums is not None:
+                row = (parents + K * torch.arange(B, device=self.device)[:, None]).reshape(-1)
+                self._weights[layer] = sums.index_select(0, row.long())
+
+    def _fork(self, parents: torch.Tensor, first: torch.Tensor | None, S: int) -> None:
+        if S == 0:
+            return
+        pools = [self._pool(layer) for layer in range(self.num_layers)]
+        ctx = torch.full((parents.shape[0],), S, dtype=torch.int32, device=self.device)
+        ops.fork_kv([p.k for p in pools], [p.v for p in pools], self._tables, ctx, parents, first)
 
     def observe(self, layer: int, q: torch.Tensor, lse: torch.Tensor,
                 scale: float | None = None) -> None:
