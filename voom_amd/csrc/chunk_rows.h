@@ -32,10 +32,12 @@ struct ChunkArgs {
   int per_xcd;   // workgroups per XCD
 };
 
+__device__ __forceinline__ int clamped(int x, int most) {
+  return x < 0 ? 0 : (x > most ? most : x);
+}
+
 __device__ __forceinline__ int context_of(const ChunkArgs& a, int b) {
-  const int cap = a.max_pages << a.pt_shift;
-  const int c = a.ctx[b];
-  return c < 0 ? 0 : (c > cap ? cap : c);
+  return clamped(a.ctx[b], a.max_pages << a.pt_shift);
 }
 
 // The new tokens of sequence b and its first row among the packed ones, both kept inside
@@ -43,18 +45,15 @@ __device__ __forceinline__ int context_of(const ChunkArgs& a, int b) {
 __device__ __forceinline__ int new_of(const ChunkArgs& a, int b, int& base) {
   if (a.starts == nullptr) {
     base = 0;
-    const int n = a.lens != nullptr ? a.lens[b] : a.T;
-    return n < 0 ? 0 : (n > a.T ? a.T : n);
+    return clamped(a.lens != nullptr ? a.lens[b] : a.T, a.T);
   }
-  const int s = a.starts[b], e = a.starts[b + 1];
-  base = s < 0 ? 0 : (s > a.N ? a.N : s);
-  const int end = e > a.N ? a.N : e;
+  base = clamped(a.starts[b], a.N);
+  const int end = clamped(a.starts[b + 1], a.N);
   return end > base ? end - base : 0;
 }
 
 __device__ __forceinline__ int prefix_of(const ChunkArgs& a, int b, int ctx) {
-  const int p = a.prefix != nullptr ? a.prefix[b] : 0;
-  return p < 0 ? 0 : (p > ctx ? ctx : p);
+  return a.prefix != nullptr ? clamped(a.prefix[b], ctx) : 0;
 }
 
 // Elements from one sequence's queries to the next token's and the next head's, and the

@@ -41,13 +41,13 @@ constexpr float kSlack = 8.f;   // the reference maxima stay that far behind, in
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void;
-typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 struct WideArgs {
   ChunkArgs c;
-  int32_t* head;   // pieces of a kv head, row tiles of it that are cut
-  int4* pieces;    // {sequence, row tile, first and last + 1 of its key tiles}
-  int32_t* slots;  // where a piece leaves its state, -1: it is the whole row tile
+  int32_t* head;   // row tiles of a kv head that are cut
+  int4* pieces;    // {sequence, row tile, first and last + 1 of its key tiles}, and its
+                   // sequence's {context, new tokens, prefix} and where the piece leaves its
+                   // state, -1: it is the whole row tile
   int4* cuts;      // {sequence, row tile, pieces, first slot}
   int32_t* lengths;  // key tiles of the row tiles
   WidePlan p;
@@ -223,9 +223,19 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_chunk_plan_kernel(WideArgs w
   __syncthreads();
   if (wv == 0) {
     const int n = classes[lane];
-    classes[lane] = wave_inclusive_scan(n, lane) - n;
+    const int x = wave_inclusive_scan(n, lane);
+    classes[lane] = x - n;
+    if (lane == kWave - 1) sums[0] = x;
   }
   __syncthreads();
+  const int listed = sums[0] < w.p.pieces ? sums[0] : w.p.pieces;
+  // Of the pieces that run from the start, two a CU, the second half is dealt the other way
+  // round: a CU then has a long one and a short one.
+  const int half = w.p.workers / 2 / a.NKV;
+  auto dealt = [&](int p, int n) {
+    const int end = n < 2 * half ? n : 2 * half;
+    return p < half || p >= end ? p : half + end - 1 - p;
+  };
   for (int e = tid; e < entries; e += kPlanThreads) {
     const int n = length(e);
     const int parts = parts_of(n, most);
@@ -239,19 +249,19 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_chunk_plan_kernel(WideArgs w
     int p = atomicAdd(&classes[class_of(n, parts)], parts);
     const int each = n / parts, more = n - each * parts;  // `more` of them one tile longer
     int from = 0;
+    const int4 seq = seqs[b];
     for (int i = 0; i < parts && p < w.p.pieces; ++i, ++p) {
       const int to = from + each + (i < more ? 1 : 0);
-      w.pieces[p] = {b, rt, from, to};
-      w.slots[p] = s < 0 || s + i >= w.p.slots ? -1 : s + i;
+      const int at = dealt(p, listed);
+      w.pieces[2 * at] = {b, rt, from, to};
+      w.pieces[2 * at + 1] = {seq.x, seq.y, seq.z, s < 0 || s + i >= w.p.slots ? -1 : s + i};
       from = to;
     }
   }
+  for (int p = listed + tid; p < w.p.pieces; p += kPlanThreads)
+    w.pieces[2 * p] = {-1, 0, 0, 0};
   __syncthreads();
-  if (tid == 0) {
-    const int pieces = classes[kClasses - 1];  // (past the last class: all of them)
-    w.head[0] = pieces < w.p.pieces ? pieces : w.p.pieces;
-    w.head[1] = cuts < w.p.cuts ? cuts : w.p.cuts;
-  }
+  if (tid == 0) w.head[0] = cuts < w.p.cuts ? cuts : w.p.cuts;
 }
 
 // Key (0..31 of a block) that row r of the score tile holds: lane half h then
@@ -288,33 +298,24 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
   // that reads of one provably miss the other's pending direct-to-LDS loads.
   __shared__ __attribute__((aligned(1024))) uint16_t tile_a[4 * kBlkElems];
   __shared__ __attribute__((aligned(1024))) uint16_t tile_b[4 * kBlkElems];
+  __shared__ int again;
   const ChunkArgs& a = wa.c;
 
-  // A piece for all kv heads in turn, the longest first: an XCD takes every eighth, so that
-  // the heads of its pieces, and with them K and V in its L2, are few.  Of those that run from
-  // the start, two a CU, the second half is dealt the other way round: a CU then has a long
-  // one and a short one.
-  const int total = wa.head[0] * a.NKV;
-  const int half = wa.p.workers / 2;
-  int wk = static_cast<int>(blockIdx.x);
-  if (wk >= half && wk < 2 * half) {
-    const int end = total < 2 * half ? (total + 7) / 8 : half / 4;  // eights of the first round
-    wk = 8 * (end - 1 - (wk - half) / 8) + (wk & 7);
-    if (wk < half) return;
-  }
-  if (wk >= total) return;
-  const int in_head = wk / a.NKV;
-  const int kvh = wk - in_head * a.NKV;
-  const int4 piece = wa.pieces[in_head];
-  const int slot = uniform(wa.slots[in_head]);
+  // A piece for all kv heads in turn: an XCD takes every eighth, so that the heads of its
+  // pieces, and with them K and V in its L2, are few.
+  const int in_head = static_cast<int>(blockIdx.x) / a.NKV;
+  const int kvh = static_cast<int>(blockIdx.x) - in_head * a.NKV;
+  const int4 piece = wa.pieces[2 * in_head], seq = wa.pieces[2 * in_head + 1];
   const int b = uniform(piece.x);
+  if (b < 0) return;
   const int rt = uniform(piece.y);
   const int c_lo = uniform(piece.z);
   const int c_hi = uniform(piece.w);
-  const int ctx = uniform(context_of(a, b));
-  int base;
-  const int n = uniform(new_of(a, b, base));
-  const int prefix = uniform(prefix_of(a, b, ctx));
+  const int ctx = uniform(seq.x);
+  const int n = uniform(seq.y);
+  const int prefix = uniform(seq.z);
+  const int slot = uniform(seq.w);
+  const int base = a.starts != nullptr ? clamped(uniform(a.starts[b]), a.N) : 0;
   const KeyTiles keys(a, ctx, n, prefix, rt);
   const int R = n * a.G;  // rows of the sequence
 
@@ -413,12 +414,13 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
     v_lane[ks] = l32 * (kBlk * 2) + 16 * ((2 * ks + lh) ^ ((l32 >> 2) & 3));
 
   f32x16 acc[DT];
-#pragma unroll
-  for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+  // A piece is walked as if no value that a row does not see were NaN or infinite.  Where its
+  // sums end so, it is walked once more, and tiles with masks key by key.
+  bool careful = false;
   // Reference of the exponentials, log2 units, the same in both halves, 0 until a key of
   // any weight is seen; it is raised where a score is more than `above` ahead of it.
-  float m = 0.f, above = -FLT_MAX;
-  float l = 0.f;        // over this lane's keys
+  float m, above;
+  float l;              // over this lane's keys
 
   // Scores of a tile (accumulator i of block j: key key_of(j, i) + 8 lh): raw, or with kMod
   // as logits in log2 units less m.
@@ -484,6 +486,14 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
           if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
       }
+    }
+    if (t * kKeys >= lo_max && t * kKeys >= prefix) {  // the diagonal alone
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[j][i] = key_of(j, i) < rel_hi ? sc[j][i] : -INFINITY;
+      }
+      return;
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -648,42 +658,30 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
     u32x4 pk[2][2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) form_p(e, sc, pk);
-    // Tokens past the sequence's end are garbage and are cut out of V^T.  Keys
-    // that a row does not see have P = 0 in that row, but 0 times a NaN or an
-    // infinity is NaN: `finite` ends up with a zero half if V holds one.
-    u16x2 finite = {0xffff, 0xffff};
-#pragma unroll
-    for (int jk = 0; jk < 4; ++jk) {
-      uint32_t keep[4];
-      tail_mask(t, jk, keep);
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        const u32x4 vv = read_v(tile, jk * DT + d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          finite = __builtin_elementwise_min(
-              finite, __builtin_bit_cast(u16x2, ~(vv[e] & keep[e]) & 0x7f807f80u));
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    // read V^T again below instead of holding all of it across the branch
-    asm volatile("" ::: "memory");
-    if (__builtin_amdgcn_ballot_w64(finite[0] == 0 || finite[1] == 0) == 0) {
+    // Tokens past the sequence's end are garbage and are cut out of V^T.  Keys that a row does
+    // not see have P = 0 in that row, but 0 times a NaN or an infinity is NaN: see `careful`.
+    auto values = [&](auto masked) VOOM_INLINE {
 #pragma unroll
       for (int jk = 0; jk < 4; ++jk) {
         uint32_t keep[4];
-        tail_mask(t, jk, keep);
+        if constexpr (masked.value) tail_mask(t, jk, keep);
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           u32x4 vv = read_v(tile, jk * DT + d);
+          if constexpr (masked.value) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) vv[e] &= keep[e];
+            for (int e = 0; e < 4; ++e) vv[e] &= keep[e];
+          }
           acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
               __builtin_bit_cast(bf16x8, vv), __builtin_bit_cast(bf16x8, pk[jk >> 1][jk & 1]),
               acc[d], 0, 0, 0);
         }
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (masked.value) __builtin_amdgcn_sched_barrier(0);
       }
+    };
+    if (!careful) {
+      if ((t + 1) * kKeys > ctx) values(std::true_type{});
+      else values(std::false_type{});
     } else {
       // Key by key: V^T with one key's column alone times P^T, added only to
       // the rows that see the key.
@@ -727,27 +725,13 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
     wait_vmem_all();
     lds_barrier();
   };
-  if (c_lo < c_hi) {
-    // K of the first tile, then (in flight while it is scored) the first stage
-    stage_blocks(c_lo - 1);
-#pragma unroll
-    for (int i = 0; i < kLoads / 2; ++i) load_piece(i, tile_b);
-    load_q();
-    load_stage(c_lo, tile_a);
-    static_assert(kLoads == 8 || kLoads == 4, "the wait below counts the first stage's loads");
-    // gfx9 encoding: vmcnt kLoads, expcnt 7, lgkmcnt 15
-    if constexpr (kLoads == 8) __builtin_amdgcn_s_waitcnt(0x0F78);
-    else __builtin_amdgcn_s_waitcnt(0x0F74);
-    lds_barrier();
-    edge_scores(c_lo, tile_b, sc_a);
-  }
   // The stages of tiles that every row of the wavefront sees whole, [whole, whole_end): the
   // first at an even distance from the piece's start (an edge tile may be a whole one).  All
   // wavefronts pass one barrier a stage, whichever loop they are in.
   int whole = (lo_max + kKeys - 1) / kKeys - keys.gap;
   whole = whole > c_lo ? whole + ((whole - c_lo) & 1) : c_lo;
   const int whole_end = hi_min / kKeys - keys.gap;
-  int c = c_lo;
+  int c;
   auto edges = [&](int end) VOOM_INLINE {
     for (; c < end; c += 2) {
       landed();
@@ -764,18 +748,56 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
       if (c + 2 < c_hi) edge_scores(c + 2, tile_b, sc_a);
     }
   };
+  if (threadIdx.x == 0) again = 0;
 #pragma unroll 1
-  for (int phase = 0; phase < 2; ++phase) {
-    edges(phase == 0 && whole + 2 < whole_end && whole + 2 < c_hi ? whole : c_hi);
-    // (pairs, the tile after them included: its scores run ahead)
-    for (; c + 2 < c_hi && c + 3 <= whole_end && c >= whole; c += 2) {
-      landed();
-      stage_blocks(c + 1);
-      whole_tile(keys.tile(c), tile_a, tile_b, sc_a, sc_b);
-      landed();
-      stage_blocks(c + 2);
-      whole_tile(keys.tile(c + 1), tile_b, tile_a, sc_b, sc_a);
+  while (true) {
+#pragma unroll
+    for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
+    m = 0.f;
+    above = -FLT_MAX;
+    l = 0.f;
+    c = c_lo;
+    win = -kWave;
+    // (what the first tile needs is formed for it, not kept in registers for a second walk)
+    asm volatile("" : "+s"(c));
+    if (c < c_hi) {
+      // K of the first tile, then (in flight while it is scored) the first stage
+      stage_blocks(c - 1);
+#pragma unroll
+      for (int i = 0; i < kLoads / 2; ++i) load_piece(i, tile_b);
+      load_q();
+      load_stage(c, tile_a);
+      static_assert(kLoads == 8 || kLoads == 4, "the wait below counts the first stage's loads");
+      // gfx9 encoding: vmcnt kLoads, expcnt 7, lgkmcnt 15
+      if constexpr (kLoads == 8) __builtin_amdgcn_s_waitcnt(0x0F78);
+      else __builtin_amdgcn_s_waitcnt(0x0F74);
+      lds_barrier();
+      edge_scores(c, tile_b, sc_a);
     }
+#pragma unroll 1
+    for (int phase = 0; phase < 2; ++phase) {
+      edges(phase == 0 && whole + 2 < whole_end && whole + 2 < c_hi ? whole : c_hi);
+      // (pairs, the tile after them included: its scores run ahead)
+      for (; c + 2 < c_hi && c + 3 <= whole_end && c >= whole; c += 2) {
+        landed();
+        stage_blocks(c + 1);
+        whole_tile(keys.tile(c), tile_a, tile_b, sc_a, sc_b);
+        landed();
+        stage_blocks(c + 2);
+        whole_tile(keys.tile(c + 1), tile_b, tile_a, sc_b, sc_a);
+      }
+    }
+    if (careful || c_lo >= c_hi) break;
+    float odd = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) odd = __builtin_fmaf(acc[d][i], 0.f, odd);
+    }
+    if (__builtin_amdgcn_ballot_w64(odd != 0.f) != 0) again = 1;
+    lds_barrier();  // (the buffers are no longer read either)
+    if (again == 0) break;
+    careful = true;
   }
 
   const float lt = l + __shfl_xor(l, 32);
@@ -826,7 +848,7 @@ __global__ __launch_bounds__(kJoinWaves * kWave) void gqa_chunk_join_kernel(Wide
   constexpr int kTogether = 8;  // rows in flight
   const ChunkArgs& a = wa.c;
   const int lane = threadIdx.x & (kWave - 1);
-  const long long rows = static_cast<long long>(wa.head[1]) * a.NKV * kTileRows;
+  const long long rows = static_cast<long long>(wa.head[0]) * a.NKV * kTileRows;
   for (long long at_row = static_cast<long long>(blockIdx.x) * kJoinWaves +
                           uniform(threadIdx.x / kWave);
        at_row < rows; at_row += kJoinGroups * kJoinWaves) {
@@ -920,8 +942,7 @@ WidePlan plan_wide(int B, int NKV, int D, int G, int N, int T, long long tokens)
   p.pieces = p.entries + p.slots;
   const size_t rows = static_cast<size_t>(p.slots) * NKV * kTileRows;
   p.bytes = up(rows * D * sizeof(float)) + up(rows * sizeof(float2)) +
-            up(p.pieces * sizeof(int4)) + up(p.pieces * sizeof(int32_t)) +
-            up(p.cuts * sizeof(int4)) + 256 + up(p.entries * sizeof(int32_t));
+            up(2 * p.pieces * sizeof(int4)) + up(p.cuts * sizeof(int4)) + 256 + up(p.entries * sizeof(int32_t));
   return p;
 }
 
@@ -937,9 +958,7 @@ int launch_wide(const ChunkArgs& a, const WidePlan& p, int D, void* workspace,
   w.c.part_ml = reinterpret_cast<float*>(at);
   at += up(rows * sizeof(float2));
   w.pieces = reinterpret_cast<int4*>(at);
-  at += up(p.pieces * sizeof(int4));
-  w.slots = reinterpret_cast<int32_t*>(at);
-  at += up(p.pieces * sizeof(int32_t));
+  at += up(2 * p.pieces * sizeof(int4));
   w.cuts = reinterpret_cast<int4*>(at);
   at += up(p.cuts * sizeof(int4));
   w.head = reinterpret_cast<int32_t*>(at);
@@ -948,8 +967,7 @@ int launch_wide(const ChunkArgs& a, const WidePlan& p, int D, void* workspace,
   hipLaunchKernelGGL(gqa_chunk_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, w);
   int rc = VOOM_LAUNCH_CHECK("paged_gqa_chunk: plan launch");
   if (rc) return rc;
-  const long long most = static_cast<long long>(p.pieces) * a.NKV;
-  const dim3 grid(static_cast<unsigned>(most > p.workers ? most : p.workers));
+  const dim3 grid(static_cast<unsigned>(static_cast<long long>(p.pieces) * a.NKV));
   const bool bias = a.slopes != nullptr || (a.cap == 0.f && !(a.scale > 0.f));
   if (D == 128) {
     if (a.cap != 0.f) launch_tiles<128, true>(w, bias, grid, stream);
