@@ -48,7 +48,7 @@ struct WideArgs {
   int4* pieces;    // {sequence, row tile, first and last + 1 of its key tiles}, and its
                    // sequence's {context, new tokens, prefix} and where the piece leaves its
                    // state, -1: it is the whole row tile
-  int4* cuts;      // {sequence, row tile, pieces, first slot}
+  int4* cuts;      // {sequence, row tile, pieces, first slot}, {new tokens, first row}
   int32_t* lengths;  // key tiles of the row tiles
   WidePlan p;
 };
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_chunk_plan_kernel(WideArgs w
   constexpr int kPlanWaves = kPlanThreads / kWave;
   const ChunkArgs& a = w.c;
   __shared__ int first[kMaxChunkBatch + 1];  // row tiles before each sequence
-  __shared__ int4 seqs[kMaxChunkBatch];      // context, new tokens, prefix
+  __shared__ int4 seqs[kMaxChunkBatch];      // context, new tokens, prefix, first row
   __shared__ int held[kHeld];
   __shared__ int sums[kPlanWaves];
   __shared__ float alls[kPlanWaves], tops[kPlanWaves];
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_chunk_plan_kernel(WideArgs w
     if (b < a.B) {
       int base;
       const int ctx = context_of(a, b), n = new_of(a, b, base);
-      seqs[b] = {ctx, n, prefix_of(a, b, ctx), 0};
+      seqs[b] = {ctx, n, prefix_of(a, b, ctx), base};
       tiles = ((a.starts != nullptr ? n : a.T) * a.G + kTileRows - 1) / kTileRows;
     }
     const int x = wave_inclusive_scan(tiles, lane);
@@ -241,15 +241,18 @@ __global__ __launch_bounds__(kPlanThreads) void gqa_chunk_plan_kernel(WideArgs w
     const int parts = parts_of(n, most);
     int b, rt, s = -1;
     place(e, b, rt);
+    const int4 seq = seqs[b];
     if (parts > 1) {
       s = atomicAdd(&slots, parts);
       const int k = atomicAdd(&cuts, 1);
-      if (k < w.p.cuts) w.cuts[k] = {b, rt, parts, s};
+      if (k < w.p.cuts) {
+        w.cuts[2 * k] = {b, rt, parts, s};
+        w.cuts[2 * k + 1] = {seq.y, seq.w, 0, 0};
+      }
     }
     int p = atomicAdd(&classes[class_of(n, parts)], parts);
     const int each = n / parts, more = n - each * parts;  // `more` of them one tile longer
     int from = 0;
-    const int4 seq = seqs[b];
     for (int i = 0; i < parts && p < w.p.pieces; ++i, ++p) {
       const int to = from + each + (i < more ? 1 : 0);
       const int at = dealt(p, listed);
@@ -332,7 +335,9 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
   const int head = kvh * a.G + (rc - tok * a.G);
   const Sight sight(a, ctx, n, prefix, tok);
   const int lo = sight.lo, hi = sight.hi;
-  const int lo_min = uniform(lo), hi_max = __builtin_amdgcn_readlane(hi, 31);
+  // (a wavefront behind the sequence's last row sees nothing: it only loads)
+  const bool has_rows = rt * kTileRows + w * kRows < R;
+  const int lo_min = uniform(lo), hi_max = has_rows ? __builtin_amdgcn_readlane(hi, 31) : 0;
   const int lo_max = __builtin_amdgcn_readlane(lo, 31);
   // (distances of later tokens, in a prefix, have the other sign: not in the loop without masks)
   const int hi_all = uniform(hi), at_min = uniform(sight.at);
@@ -414,9 +419,6 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
     v_lane[ks] = l32 * (kBlk * 2) + 16 * ((2 * ks + lh) ^ ((l32 >> 2) & 3));
 
   f32x16 acc[DT];
-  // A piece is walked as if no value that a row does not see were NaN or infinite.  Where its
-  // sums end so, it is walked once more, and tiles with masks key by key.
-  bool careful = false;
   // Reference of the exponentials, log2 units, the same in both halves, 0 until a key of
   // any weight is seen; it is raised where a score is more than `above` ahead of it.
   float m, above;
@@ -653,13 +655,13 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
 
   // Any tile t (stage c) that some row of the wavefront sees: its scores are in sc, which
   // then takes those of the next one if a row sees that too.
-  auto edge_tile = [&](int c, const uint16_t* tile, Scores& sc) VOOM_INLINE {
+  auto edge_tile = [&](int c, const uint16_t* tile, Scores& sc, auto careful) VOOM_INLINE {
     const int t = keys.tile(c);
     u32x4 pk[2][2];
 #pragma unroll
     for (int e = 0; e < 16; ++e) form_p(e, sc, pk);
     // Tokens past the sequence's end are garbage and are cut out of V^T.  Keys that a row does
-    // not see have P = 0 in that row, but 0 times a NaN or an infinity is NaN: see `careful`.
+    // not see have P = 0 in that row, but 0 times a NaN or an infinity is NaN: then `careful`.
     auto values = [&](auto masked) VOOM_INLINE {
 #pragma unroll
       for (int jk = 0; jk < 4; ++jk) {
@@ -679,7 +681,7 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
         if constexpr (masked.value) __builtin_amdgcn_sched_barrier(0);
       }
     };
-    if (!careful) {
+    if constexpr (!careful.value) {
       if ((t + 1) * kKeys > ctx) values(std::true_type{});
       else values(std::false_type{});
     } else {
@@ -730,13 +732,13 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
   // wavefronts pass one barrier a stage, whichever loop they are in.
   int whole = (lo_max + kKeys - 1) / kKeys - keys.gap;
   whole = whole > c_lo ? whole + ((whole - c_lo) & 1) : c_lo;
-  const int whole_end = hi_min / kKeys - keys.gap;
+  const int whole_end = has_rows ? hi_min / kKeys - keys.gap : 0;
   int c;
-  auto edges = [&](int end) VOOM_INLINE {
+  auto edges = [&](int end, auto careful) VOOM_INLINE {
     for (; c < end; c += 2) {
       landed();
       if (c + 1 < c_hi) load_stage(c + 1, tile_b);
-      if (any_sees(keys.tile(c))) edge_tile(c, tile_a, sc_a);
+      if (any_sees(keys.tile(c))) edge_tile(c, tile_a, sc_a, careful);
       if (c + 1 >= c_hi) {
         c = c_hi;
         return;
@@ -744,13 +746,11 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
       edge_scores(c + 1, tile_a, sc_a);
       landed();
       if (c + 2 < c_hi) load_stage(c + 2, tile_a);
-      if (any_sees(keys.tile(c + 1))) edge_tile(c + 1, tile_b, sc_a);
+      if (any_sees(keys.tile(c + 1))) edge_tile(c + 1, tile_b, sc_a, careful);
       if (c + 2 < c_hi) edge_scores(c + 2, tile_b, sc_a);
     }
   };
-  if (threadIdx.x == 0) again = 0;
-#pragma unroll 1
-  while (true) {
+  auto start = [&]() VOOM_INLINE {
 #pragma unroll
     for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
     m = 0.f;
@@ -774,20 +774,26 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
       lds_barrier();
       edge_scores(c, tile_b, sc_a);
     }
+  };
+  // A piece is walked as if no value that a row does not see were NaN or infinite.  Where its
+  // sums end so, it is walked once more, every tile key by key.
+  if (threadIdx.x == 0) again = 0;
+  start();
 #pragma unroll 1
-    for (int phase = 0; phase < 2; ++phase) {
-      edges(phase == 0 && whole + 2 < whole_end && whole + 2 < c_hi ? whole : c_hi);
-      // (pairs, the tile after them included: its scores run ahead)
-      for (; c + 2 < c_hi && c + 3 <= whole_end && c >= whole; c += 2) {
-        landed();
-        stage_blocks(c + 1);
-        whole_tile(keys.tile(c), tile_a, tile_b, sc_a, sc_b);
-        landed();
-        stage_blocks(c + 2);
-        whole_tile(keys.tile(c + 1), tile_b, tile_a, sc_b, sc_a);
-      }
+  for (int phase = 0; phase < 2; ++phase) {
+    edges(phase == 0 && whole + 2 < whole_end && whole + 2 < c_hi ? whole : c_hi,
+          std::false_type{});
+    // (pairs, the tile after them included: its scores run ahead)
+    for (; c + 2 < c_hi && c + 3 <= whole_end && c >= whole; c += 2) {
+      landed();
+      stage_blocks(c + 1);
+      whole_tile(keys.tile(c), tile_a, tile_b, sc_a, sc_b);
+      landed();
+      stage_blocks(c + 2);
+      whole_tile(keys.tile(c + 1), tile_b, tile_a, sc_b, sc_a);
     }
-    if (careful || c_lo >= c_hi) break;
+  }
+  if (c_lo < c_hi) {
     float odd = 0.f;
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
@@ -796,8 +802,10 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
     }
     if (__builtin_amdgcn_ballot_w64(odd != 0.f) != 0) again = 1;
     lds_barrier();  // (the buffers are no longer read either)
-    if (again == 0) break;
-    careful = true;
+    if (uniform(again) != 0) {
+      start();
+      edges(c_hi, std::true_type{});
+    }
   }
 
   const float lt = l + __shfl_xor(l, 32);
@@ -838,74 +846,70 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
   if (lh == 0) *reinterpret_cast<float2*>(a.part_ml + p * 2) = {lt == 0.f ? -FLT_MAX : m, lt};
 }
 
-// Merges the pieces of cut row tiles, a row at a time to a wavefront.
-constexpr int kJoinWaves = 16;
-constexpr int kJoinGroups = 512;
+// Merges the pieces of cut row tiles, a row to D / 4 lanes, a few rows of one to a workgroup.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinGroups = 2048;
 
 template <int D>
-__global__ __launch_bounds__(kJoinWaves * kWave) void gqa_chunk_join_kernel(WideArgs wa) {
-  constexpr int DPL = D / kWave;
-  constexpr int kTogether = 8;  // rows in flight
+__global__ __launch_bounds__(kJoinThreads) void gqa_chunk_join_kernel(WideArgs wa) {
+  constexpr int kLanes = D / 4;
+  constexpr int kAtOnce = kJoinThreads / kLanes;  // rows
+  constexpr int kTogether = 8;                    // pieces in flight
+  constexpr int kEach = kTileRows / kAtOnce;      // workgroups' shares of a row tile
   const ChunkArgs& a = wa.c;
-  const int lane = threadIdx.x & (kWave - 1);
-  const long long rows = static_cast<long long>(wa.head[0]) * a.NKV * kTileRows;
-  for (long long at_row = static_cast<long long>(blockIdx.x) * kJoinWaves +
-                          uniform(threadIdx.x / kWave);
-       at_row < rows; at_row += kJoinGroups * kJoinWaves) {
-    const int r = static_cast<int>(at_row) & (kTileRows - 1);
-    const int head_cut = static_cast<int>(at_row / kTileRows);
-    const int kvh = head_cut % a.NKV;
-    const int4 cut = wa.cuts[head_cut / a.NKV];
+  const int dim = static_cast<int>(threadIdx.x) % kLanes * 4;
+  const int all = wa.head[0] * a.NKV * kEach;
+  for (int at = static_cast<int>(blockIdx.x); at < all; at += kJoinGroups) {
+    const int pair = at / kEach;
+    const int k = pair / a.NKV, kvh = pair - k * a.NKV;
+    const int4 cut = wa.cuts[2 * k], seq = wa.cuts[2 * k + 1];
     const int b = uniform(cut.x), rt = uniform(cut.y), parts = uniform(cut.z);
-    int base;
-    const int n = uniform(new_of(a, b, base));
+    const int n = uniform(seq.x), base = uniform(seq.y);
+    const int r = (at - pair * kEach) * kAtOnce + static_cast<int>(threadIdx.x) / kLanes;
     const int row = rt * kTileRows + r;
     const int tok = row / a.G;
     if (tok >= n && (a.starts != nullptr || tok >= a.T)) continue;
-    const int head = kvh * a.G + (row - tok * a.G);
-    const size_t p0 = (static_cast<size_t>(kvh) * wa.p.slots + cut.w) * kTileRows + r;
-    const float2* ml2 = reinterpret_cast<const float2*>(a.part_ml);
-    // up to 64 pieces at a time, one per lane for their maxima and sums
+    const size_t first =
+        (static_cast<size_t>(kvh) * wa.p.slots + uniform(cut.w)) * kTileRows + r;
     float M = -FLT_MAX, L = 0.f;
-    float acc[DPL] = {};
-    for (int s0 = 0; s0 < parts && tok < n; s0 += kWave) {
-      const int m = parts - s0 < kWave ? parts - s0 : kWave;
-      const float2 ml = ml2[p0 + static_cast<size_t>(s0 + (lane < m ? lane : 0)) * kTileRows];
-      const float mn = fmaxf(M, wave_max_uniform(lane < m ? ml.x : -FLT_MAX));
-      const float wt = lane < m ? fast_exp2(ml.x - mn) : 0.f;
+    f32x4 acc = {};
+    for (int s0 = 0; s0 < parts && tok < n; s0 += kTogether) {
+      float2 ml[kTogether];
+      f32x4 v[kTogether];
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        if (u > 0 && s0 + u >= parts) break;
+        const size_t p = first + static_cast<size_t>(s0 + u) * kTileRows;
+        ml[u] = *reinterpret_cast<const float2*>(a.part_ml + p * 2);
+        v[u] = *reinterpret_cast<const f32x4*>(a.part_o + p * D + dim);
+      }
+      float mn = M;
+#pragma unroll
+      for (int u = 0; u < kTogether; ++u) {
+        if (u > 0 && s0 + u >= parts) break;
+        mn = fmaxf(mn, ml[u].x);
+      }
       const float f = fast_exp2(M - mn);
       M = mn;
-      L = L * f + wave_sum_uniform(lane < m ? ml.y * wt : 0.f);
+      L *= f;
+      acc *= f;
 #pragma unroll
-      for (int d = 0; d < DPL; ++d) acc[d] *= f;
-      const float* po = a.part_o + (p0 + static_cast<size_t>(s0) * kTileRows) * D + lane * DPL;
-      for (int s1 = 0; s1 < m; s1 += kTogether) {
-        float v[kTogether][DPL];
-#pragma unroll
-        for (int u = 0; u < kTogether; ++u) {
-          const int s = s1 + u < m ? s1 + u : m - 1;
-#pragma unroll
-          for (int d = 0; d < DPL; ++d) v[u][d] = po[static_cast<size_t>(s) * kTileRows * D + d];
-        }
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int u = 0; u < kTogether; ++u) {
-          if (s1 + u >= m) break;
-          const float ws = __builtin_bit_cast(
-              float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wt), s1 + u));
-#pragma unroll
-          for (int d = 0; d < DPL; ++d) acc[d] += v[u][d] * ws;
-        }
+      for (int u = 0; u < kTogether; ++u) {
+        if (u > 0 && s0 + u >= parts) break;
+        const float ws = fast_exp2(ml[u].x - mn);
+        L += ml[u].y * ws;
+        acc += v[u] * ws;
       }
     }
     const bool empty = tok >= n || L == 0.f;
     const float inv = 1.f / L;
-    const size_t at = out_at(a, b, base, tok, head);
-    uint16_t* o = a.out + at * D + lane * DPL;
-#pragma unroll
-    for (int d = 0; d < DPL; ++d) o[d] = empty ? 0 : f2bf(acc[d] * inv);
-    if (lane == 0 && a.lse != nullptr)
-      a.lse[at] = empty ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
+    const size_t out_row = out_at(a, b, base, tok, kvh * a.G + (row - tok * a.G));
+    *reinterpret_cast<u32x2*>(a.out + out_row * D + dim) =
+        empty ? u32x2{0u, 0u}
+              : u32x2{pack_bf16x2(acc[0] * inv, acc[1] * inv),
+                      pack_bf16x2(acc[2] * inv, acc[3] * inv)};
+    if (dim == 0 && a.lse != nullptr)
+      a.lse[out_row] = empty ? -INFINITY : (M + __log2f(L)) * 0.6931471805599453f;
   }
 }
 
@@ -942,7 +946,7 @@ WidePlan plan_wide(int B, int NKV, int D, int G, int N, int T, long long tokens)
   p.pieces = p.entries + p.slots;
   const size_t rows = static_cast<size_t>(p.slots) * NKV * kTileRows;
   p.bytes = up(rows * D * sizeof(float)) + up(rows * sizeof(float2)) +
-            up(2 * p.pieces * sizeof(int4)) + up(p.cuts * sizeof(int4)) + 256 + up(p.entries * sizeof(int32_t));
+            up(2 * p.pieces * sizeof(int4)) + up(2 * p.cuts * sizeof(int4)) + 256 + up(p.entries * sizeof(int32_t));
   return p;
 }
 
@@ -960,7 +964,7 @@ int launch_wide(const ChunkArgs& a, const WidePlan& p, int D, void* workspace,
   w.pieces = reinterpret_cast<int4*>(at);
   at += up(2 * p.pieces * sizeof(int4));
   w.cuts = reinterpret_cast<int4*>(at);
-  at += up(p.cuts * sizeof(int4));
+  at += up(2 * p.cuts * sizeof(int4));
   w.head = reinterpret_cast<int32_t*>(at);
   at += 256;
   w.lengths = reinterpret_cast<int32_t*>(at);
@@ -980,9 +984,9 @@ int launch_wide(const ChunkArgs& a, const WidePlan& p, int D, void* workspace,
   if (rc) return rc;
   const dim3 jgrid(kJoinGroups);
   if (D == 128)
-    hipLaunchKernelGGL(gqa_chunk_join_kernel<128>, jgrid, dim3(kJoinWaves * kWave), 0, stream, w);
+    hipLaunchKernelGGL(gqa_chunk_join_kernel<128>, jgrid, dim3(kJoinThreads), 0, stream, w);
   else
-    hipLaunchKernelGGL(gqa_chunk_join_kernel<64>, jgrid, dim3(kJoinWaves * kWave), 0, stream, w);
+    hipLaunchKernelGGL(gqa_chunk_join_kernel<64>, jgrid, dim3(kJoinThreads), 0, stream, w);
   return VOOM_LAUNCH_CHECK("paged_gqa_chunk: join launch");
 }
 
