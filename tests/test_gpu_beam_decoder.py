@@ -296,6 +296,11 @@ def test_cache_refusals():
         kv.fork(parents, parents[0])
     with pytest.raises(ValueError, match="since"):
         kv.fork(parents, since=41)
+    with pytest.raises(ValueError, match="device"):
+        kv.fork(parents.cpu())
+    with pytest.raises(ValueError, match="65535"):
+        kv.expand(20000)
+    kv.check_integrity()  # (nothing that was refused has touched it)
     with pytest.raises(ValueError, match="queries"):
         kv.attend_chunk(0, torch.zeros((4, 2, 41, 64), dtype=torch.bfloat16, device="cuda"))
     kv.reserve(60)

@@ -148,6 +148,38 @@ def test_scales_and_caps(scale, softcap):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("softcap", [1e-4, 1e30])
+def test_caps_that_leave_nothing_of_a_score_and_all_of_it(softcap):
+    for T, ctx in ((3, 300), (20, 300), (150, 200)):
+        q, k, v = inputs(1, 9, 3, 64, ctx, T, seed=14)
+        q[:, :, 0] = 0  # scores of 0 are on the polynomial, whatever its coefficients
+        k_pool, v_pool, table = cache(k, v, 32)
+        got = ops.paged_gqa_chunk(q, k_pool, v_pool, table, lens_tensor([ctx]), softcap=softcap,
+                                  return_lse=True)
+        check(got, reference(q, k, v, [ctx], [T], softcap=softcap))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("NQ,NKV,D,ctx,lens", [
+    (4, 2, 64, [9000, 40], [33, 1]),       # a row tile in as many pieces as 64 of its keys allow
+    (8, 1, 128, [5000, 70], [18, 70]),
+    (3, 3, 64, [7001, 7001, 3], [40, 1, 0]),
+])
+def test_row_tiles_in_many_pieces(NQ, NKV, D, ctx, lens):
+    print(f"[chunk] pieces {NQ} {NKV} {D} {ctx} {lens}", flush=True)
+    q, k, v = inputs(len(ctx), NQ, NKV, D, max(ctx), max(lens), seed=23)
+    k_pool, v_pool, table = cache(k, v, 64)
+    want = reference(q, k, v, ctx, lens, softcap=9.0)
+    got = ops.paged_gqa_chunk(q, k_pool, v_pool, table, lens_tensor(ctx),
+                              new_lens=lens_tensor(lens), softcap=9.0, return_lse=True)
+    check(got, want)
+    rows, starts = pack(q, lens)
+    got = ops.paged_gqa_chunk(rows, k_pool, v_pool, table, lens_tensor(ctx), starts=starts,
+                              softcap=9.0, return_lse=True)
+    check(got, tuple(packed_of(x, lens) for x in want))
+
+
+@pytest.mark.gpu
 def test_slopes_of_any_sign_and_size():
     """Slopes so steep that a token's own key alone is left, none, and such as favour far
     tokens."""
@@ -430,5 +462,9 @@ def test_abi_refusals():
     refused("finite", scale=float("inf"))
     refused("finite", cap=-1.0)
     refused("finite", cap=float("nan"))
+    for cap in (1e-9, 1e-30, 3e38):
+        refused("out of proportion", cap=cap)
+    refused("out of proportion", scale=1e30, cap=1e28)
+    refused("out of proportion", scale=1e-42, cap=1.0)
     refused("aligned", q=ctypes.c_void_p(264))
     refused("workspace", pages=100, ws=p, ws_bytes=64)

@@ -390,6 +390,14 @@ extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const voi
   VOOM_REQUIRE(window >= 0, "%s: window %d must not be negative", who, window);
   VOOM_REQUIRE(std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0.f,
                "%s: the scale must be finite, the cap finite and not negative", who);
+  // (the cap's polynomial has coefficients up to scale (scale / softcap)^6)
+  const float cap_k = softcap > 0.f ? scale / softcap : 0.f;
+  const float cap_k2 = cap_k * cap_k;
+  VOOM_REQUIRE(cap_k == 0.f ? softcap == 0.f || scale == 0.f
+                            : std::isnormal(cap_k) && std::isfinite(2.f * softcap) &&
+                                  std::isfinite(2.f * scale * cap_k2 * cap_k2 * cap_k2),
+               "%s: a cap of %g is out of proportion to a scale of %g", who,
+               static_cast<double>(softcap), static_cast<double>(scale));
   VOOM_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(k_pool) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(v_pool) % 16 == 0 &&
@@ -433,7 +441,7 @@ extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const voi
   a.window = win;
   a.scale = scale * 1.4426950408889634f;
   a.cap = softcap * 1.4426950408889634f;
-  a.cap_k = softcap > 0.f ? scale / softcap : 0.f;
+  a.cap_k = cap_k;
   a.part_o = a.part_ml = nullptr;
   a.W = a.per_xcd = 0;
   if (kind == Kind::kWide)

@@ -2233,6 +2233,11 @@ class PagedKVCache:
             raise ValueError(f"{what} needs layers of one length")
         return self._len[0]
 
+    @staticmethod
+    def _require_rows(rows: int) -> None:
+        if rows > 65535:
+            raise ValueError(f"{rows} rows of the cache are more than a copy takes, 65535")
+
     def expand(self, beams: int) -> None:
         """Every sequence becomes ``beams`` rows, rows b * beams to (b + 1) * beams - 1 of the
         batch, all of them with its tokens: the start of a beam search behind one prompt.
@@ -2245,6 +2250,7 @@ class PagedKVCache:
             raise ValueError("expand(): captured steps hold the cache's batch")
         if beams == 1:
             return
+        self._require_rows(self._batch * beams)
         self.check_integrity()
         self._drop_prefetch()
         for layer in range(self.num_layers):
@@ -2298,6 +2304,12 @@ class PagedKVCache:
             raise ValueError(f"parents must be int32 [requests, beams] of {self._batch} rows")
         if first is not None and (first.dtype is not torch.int32 or first.shape != parents.shape):
             raise ValueError("first must be like parents")
+        self._require_rows(parents.numel())
+        for t in (parents, first):
+            if t is not None and not t.is_cuda:
+                raise ValueError("parents and first must be on the cache's device")
+        parents = parents.contiguous()
+        first = None if first is None else first.contiguous()
         if not 0 <= since <= S:
             raise ValueError(f"since {since} lies outside the {S} tokens")
         if ops.bounds_checks_enabled():

@@ -467,7 +467,8 @@ def paged_gqa_chunk(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     tanh(s / softcap) where ``softcap`` is given, less slopes[head] * |i - j| with ``slopes``
     [NQ] fp32; it sees j <= i, with a ``window`` only where i - j < window, and always the
     first ``prefix_lens`` [B] int32 tokens of its sequence (in both directions).  A cap or a
-    window of 0 is none.
+    window of 0 is none.  At most 1024 sequences, heads of 64 or 128 dims, 16 query heads a kv
+    head.
 
     Returns out [N, NQ, D] or [B, T, NQ, D] (``out`` where it is given; and the fp32
     natural-log LSE without the last dim when ``return_lse``).  Rows that see nothing, and
