@@ -15,11 +15,28 @@ import ctypes
 import pytest
 import torch
 
-from paged_inputs import cache, inputs, lens_tensor
+import paged_inputs
+from paged_inputs import inputs, lens_tensor
 from voom_amd import ops
 
 REL, LSE_ABS = 4e-3, 2e-4
 INF, NAN = float("inf"), float("nan")
+ROOM = 0  # tokens that the tables have room for besides
+
+
+@pytest.fixture(params=[0, 1 << 17], ids=["tight", "roomy"])
+def room(request):
+    """Tables of the cached tokens alone, and such as a server reserves: the rows that may see
+    many tokens take another kernel."""
+    global ROOM
+    ROOM = request.param
+    yield
+    ROOM = 0
+
+
+def cache(k, v, page, spare=0):
+    k_pool, v_pool, table = paged_inputs.cache(k, v, page, spare=spare)
+    return k_pool, v_pool, torch.nn.functional.pad(table, (0, ROOM // page))
 
 
 def reference(q, k, v, ctx, lens, *, scale=None, softcap=0.0, slopes=None, window=0, prefix=None):
@@ -112,7 +129,7 @@ SHAPES = [
 @pytest.mark.gpu
 @pytest.mark.parametrize("mode", range(len(MODES)))
 @pytest.mark.parametrize("shape", range(len(SHAPES)))
-def test_chunk_against_fp64(shape, mode):
+def test_chunk_against_fp64(shape, mode, room):
     B, NQ, NKV, D, PT, ctx, lens = SHAPES[shape]
     kw = dict(MODES[mode])
     print(f"[chunk] {SHAPES[shape]} {kw}", flush=True)
@@ -135,9 +152,34 @@ def test_chunk_against_fp64(shape, mode):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mode", [m for m in MODES if "window" in m])
+@pytest.mark.parametrize("NQ,NKV,D,PT,ctx,lens", [
+    (16, 8, 64, 64, [900], [800]), (16, 8, 128, 32, [1000, 500], [500, 90])])
+def test_windows_of_long_chunks(NQ, NKV, D, PT, ctx, lens, mode):
+    print(f"[chunk] {NQ} {NKV} {D} {ctx} {lens} {mode}", flush=True)
+    q, k, v = inputs(len(ctx), NQ, NKV, D, max(ctx), max(lens), seed=31)
+    k_pool, v_pool, table = cache(k, v, PT)
+    kw, call = dict(mode), dict(mode)
+    if "slopes" in kw:
+        kw["slopes"] = call["slopes"] = geometric(NQ)
+    if "prefix" in kw:
+        kw["prefix"] = [kw["prefix"]] * len(ctx)
+        call["prefix_lens"] = lens_tensor(kw["prefix"])
+        del call["prefix"]
+    want = reference(q, k, v, ctx, lens, **kw)
+    got = ops.paged_gqa_chunk(q, k_pool, v_pool, table, lens_tensor(ctx),
+                              new_lens=lens_tensor(lens), return_lse=True, **call)
+    check(got, want)
+    rows, starts = pack(q, lens)
+    got = ops.paged_gqa_chunk(rows, k_pool, v_pool, table, lens_tensor(ctx), starts=starts,
+                              return_lse=True, **call)
+    check(got, tuple(packed_of(x, lens) for x in want))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("scale,softcap", [(-0.2, 0.0), (0.0, 0.0), (0.7, 3.0), (-0.4, 20.0),
                                            (0.3, 1000.0)])
-def test_scales_and_caps(scale, softcap):
+def test_scales_and_caps(scale, softcap, room):
     print(f"[chunk] scale={scale} softcap={softcap}", flush=True)
     for T, ctx in ((3, 300), (150, 200)):
         q, k, v = inputs(1, 9, 3, 64, ctx, T, seed=4)
@@ -149,7 +191,7 @@ def test_scales_and_caps(scale, softcap):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("softcap", [1e-4, 1e30])
-def test_caps_that_leave_nothing_of_a_score_and_all_of_it(softcap):
+def test_caps_that_leave_nothing_of_a_score_and_all_of_it(softcap, room):
     for T, ctx in ((3, 300), (20, 300), (150, 200)):
         q, k, v = inputs(1, 9, 3, 64, ctx, T, seed=14)
         q[:, :, 0] = 0  # scores of 0 are on the polynomial, whatever its coefficients
@@ -165,7 +207,7 @@ def test_caps_that_leave_nothing_of_a_score_and_all_of_it(softcap):
     (8, 1, 128, [5000, 70], [18, 70]),
     (3, 3, 64, [7001, 7001, 3], [40, 1, 0]),
 ])
-def test_row_tiles_in_many_pieces(NQ, NKV, D, ctx, lens):
+def test_row_tiles_in_many_pieces(NQ, NKV, D, ctx, lens, room):
     print(f"[chunk] pieces {NQ} {NKV} {D} {ctx} {lens}", flush=True)
     q, k, v = inputs(len(ctx), NQ, NKV, D, max(ctx), max(lens), seed=23)
     k_pool, v_pool, table = cache(k, v, 64)
@@ -180,7 +222,7 @@ def test_row_tiles_in_many_pieces(NQ, NKV, D, ctx, lens):
 
 
 @pytest.mark.gpu
-def test_slopes_of_any_sign_and_size():
+def test_slopes_of_any_sign_and_size(room):
     """Slopes so steep that a token's own key alone is left, none, and such as favour far
     tokens."""
     q, k, v = inputs(1, 8, 2, 128, 500, 80, seed=5)
@@ -195,8 +237,9 @@ def test_slopes_of_any_sign_and_size():
 @pytest.mark.gpu
 @pytest.mark.parametrize("NQ,NKV,D,ctx,T,window,prefix", [
     (9, 3, 64, 90, 5, 20, 3), (8, 2, 128, 1333, 14, 200, 40), (32, 4, 128, 31, 31, 7, 2),
-    (8, 2, 128, 900, 300, 250, 0), (4, 2, 64, 1000, 333, 0, 70)])
-def test_what_a_row_does_not_see_cannot_reach_it(NQ, NKV, D, ctx, T, window, prefix):
+    (8, 2, 128, 900, 300, 250, 0), (4, 2, 64, 1000, 333, 0, 70), (32, 8, 128, 900, 300, 250, 0),
+    (24, 8, 64, 900, 400, 250, 30)])
+def test_what_a_row_does_not_see_cannot_reach_it(NQ, NKV, D, ctx, T, window, prefix, room):
     """NaN and infinities in K and V of tokens before the window and of later ones, in the
     queries of rows behind the new tokens, and behind the context (the pools are NaN there)."""
     print(f"[chunk] NaN in unseen tokens, D={D} T={T} ctx={ctx} window={window}", flush=True)
@@ -230,7 +273,7 @@ def test_what_a_row_does_not_see_cannot_reach_it(NQ, NKV, D, ctx, T, window, pre
 @pytest.mark.gpu
 @pytest.mark.parametrize("T", [4, 200])
 @pytest.mark.parametrize("page,first,count", [(32, 0, 64), (64, 96, 700), (64, 0, 1500)])
-def test_keys_that_score_minus_infinity_weigh_nothing(page, first, count, T):
+def test_keys_that_score_minus_infinity_weigh_nothing(page, first, count, T, room):
     """Whole blocks and splits of them; a row whose every key scores -inf counts as empty."""
     ctx, D = 1500, 128
     print(f"[chunk] -inf keys {first} + {count}", flush=True)
@@ -251,11 +294,11 @@ def test_keys_that_score_minus_infinity_weigh_nothing(page, first, count, T):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T", [6, 120])
-def test_lengths_out_of_range_and_more_new_tokens_than_cached(T):
+@pytest.mark.parametrize("T,NQ,NKV", [(6, 9, 3), (120, 9, 3), (1400, 16, 8)])
+def test_lengths_out_of_range_and_more_new_tokens_than_cached(T, NQ, NKV):
     print(f"[chunk] clamped lengths, T={T}", flush=True)
     D = 64
-    q, k, v = inputs(3, 9, 3, D, 64, T, seed=8)
+    q, k, v = inputs(3, NQ, NKV, D, 64, T, seed=8)
     k_pool, v_pool, table = cache(k, v, 32)
     got = ops.paged_gqa_chunk(q, k_pool, v_pool, table, lens_tensor([1000, -5, 3]),
                               new_lens=lens_tensor([9999, 4, 5]), return_lse=True,
@@ -273,7 +316,7 @@ def test_lengths_out_of_range_and_more_new_tokens_than_cached(T):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("lens,ctx", [([2, 1, 4], [80, 40, 9]), ([150, 1, 0, 260], [900, 40, 9, 260])])
-def test_packed_rows_of_no_sequence_stay(lens, ctx):
+def test_packed_rows_of_no_sequence_stay(lens, ctx, room):
     """Rows before the first and behind the last sequence, and starts past the rows."""
     print(f"[chunk] rows of no sequence, {lens}", flush=True)
     B = len(lens)
@@ -295,7 +338,7 @@ def test_packed_rows_of_no_sequence_stay(lens, ctx):
 
 
 @pytest.mark.gpu
-def test_plain_scores_are_those_of_the_other_attention_calls():
+def test_plain_scores_are_those_of_the_other_attention_calls(room):
     """Without cap, slopes, window and prefix: the decode, window and tree calls' results."""
     D = 128
     q, k, v = inputs(2, 32, 8, D, 1500, 9, seed=10)

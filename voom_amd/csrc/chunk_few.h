@@ -8,12 +8,20 @@
 
 namespace voom {
 
-// How a kernel takes a call: row tiles of kRows, stages of kTok tokens, and kLead units that
-// stand for what a segment costs besides its stages.
-template <int ROWS, int TOK, int LEAD>
+// How a kernel takes a call: row tiles of kRows, stages of kTok tokens, kLead units that
+// stand for what a segment costs besides its stages, and kLeast units of a worker, since each
+// leaves pieces to be merged.
+template <int ROWS, int TOK, int LEAD, int LEAST>
 struct Geometry {
-  static constexpr int kRows = ROWS, kTok = TOK, kLead = LEAD;
+  static constexpr int kRows = ROWS, kTok = TOK, kLead = LEAD, kLeast = LEAST;
 };
+
+// U units over W workers, or fewer.
+template <class Geo>
+__device__ __forceinline__ Split split_of(int U, int W) {
+  const int most = U / Geo::kLeast;
+  return Split(U, most < W ? (most > 1 ? most : 1) : W);
+}
 
 // Units of a sequence: for every kv head and row tile the stages that its rows see, after
 // kLead units.  Stages from `pre` on lie `gap` further on in the context.
@@ -162,7 +170,7 @@ __global__ __launch_bounds__(kReduceWaves * kWave) void gqa_chunk_reduce_kernel(
       U += __builtin_amdgcn_readlane(x, kWave - 1);
     }
     if (chunks != 0) {  // (a context of no tokens has no segments)
-      const Split split(U, a.W);
+      const Split split = split_of<Geo>(U, a.W);
       const int S = before + (kvh * tiles + tile) * (chunks + kLead) + kLead;
       first = split.group(S);
       last = split.group(S + chunks - 1);

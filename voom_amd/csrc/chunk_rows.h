@@ -115,7 +115,7 @@ struct FewPlan {
   long long segs;  // (sequence, kv head, row tile) segments at most
   int W;           // workers of the split; 0: one per segment, no reduce launch
 };
-FewPlan plan_token(int B, int NKV, int G, int N, int T, long long tokens, int window);
+FewPlan plan_token(int B, int NKV, int D, int G, int N, int T, long long tokens, int window);
 int launch_token(const ChunkArgs& a, const FewPlan& p, int D, hipStream_t stream);
 
 // ---- the kernel of long chunks (gqa_chunk_wide.hip) ------------------------------

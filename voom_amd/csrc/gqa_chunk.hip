@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kRows = 16 * kRowWaves;  // of a tile
 template <int D>
-using Geo = Geometry<kRows, stage_tokens(D), 8>;
+using Geo = Geometry<kRows, stage_tokens(D), 8, 1>;
 
 // A block that some row of the tile does not see whole.
 template <int D>
@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_chunk_rows_kernel(ChunkArgs a
       scan_units<Geo<D>>(a, base, lane, x);
       U += __builtin_amdgcn_readlane(x, kWave - 1);
     }
-    const Split split(U, a.W);
+    const Split split = split_of<Geo<D>>(U, a.W);
     if (w >= split.We || U == 0) return;
     u0 = split.begin(w);
     u1 = split.begin(w + 1);
@@ -302,7 +302,8 @@ FewPlan plan_rows(int B, int NKV, int D, int G, int N, int T, long long tokens, 
   if (seen < stages) stages = seen;
   // All workgroups of a split run at once.  Without one a workgroup walks a segment, which
   // saves the merges and the reduce launch, where the segments are short, the longer the
-  // better they fill the card.
+  // better they fill the card (32 rows, 8 kv heads of 128; without and with the split: 8
+  // segments of 500 tokens 14.6 and 14.5 us, of 1,000 21.9 and 14.3; 256 of 4,000 98 and 104).
   const int cus = device_cu_count();
   const long long full = (p.segs + cus - 1) / cus * cus;
   const int most = 16 * p.segs >= 15 * full ? kLong : (2 * p.segs >= full ? 2 * kShort : kShort);
@@ -313,19 +314,29 @@ FewPlan plan_rows(int B, int NKV, int D, int G, int N, int T, long long tokens, 
 
 // The kernel that takes a call goes by the rows (new token, head of the group) a kv head of
 // a sequence, on the average: up to 16 that of single tokens, up to 64 the one above, beyond
-// that the one of long chunks.  All three are right for any lengths.
+// that the one of long chunks.  All three are right for any lengths.  8 sequences of 16,000
+// tokens, 32/8 heads of 128, in us, the first, the second and the third:
+//   16 rows  90  108  124     20 rows  161  107  123
+//   64 rows  316  131  132    96 rows  468  195  134
+// The third has three launches and longer ones (30 us at least where the second has 15), but
+// reads K and V once for twice the rows: calls too small to gain that much take the second
+// (32/8 heads of 128, 300 rows a kv head of 1,000 to 1,200 tokens: 23 us against 38; of 8,100
+// tokens: 51 against 44).
 enum class Kind { kToken, kRows, kWide };
-Kind kind_of(int batch, int rows, int tokens, int G) {
+constexpr long long kSmall = 1LL << 22;  // rows times the tokens that they may see
+Kind kind_of(int batch, int rows, int tokens, int NKV, int G, long long cap, int window) {
   const long long all = rows > 0 ? static_cast<long long>(rows) * G
                                  : static_cast<long long>(tokens) * G * batch;
-  return all <= 16LL * batch ? Kind::kToken
-                             : (all <= static_cast<long long>(kRows) * batch ? Kind::kRows
-                                                                            : Kind::kWide);
+  if (all <= 16LL * batch) return Kind::kToken;
+  const long long reach = window > 0 ? static_cast<long long>(window) + rows + tokens : cap;
+  const long long seen = reach < cap ? reach : cap;
+  return all <= static_cast<long long>(kRows) * batch || all <= kSmall / (seen * NKV)
+             ? Kind::kRows : Kind::kWide;
 }
 
 FewPlan plan_few(Kind kind, int B, int NKV, int D, int G, int N, int T, long long tokens,
                  int window) {
-  return kind == Kind::kToken ? plan_token(B, NKV, G, N, T, tokens, window)
+  return kind == Kind::kToken ? plan_token(B, NKV, D, G, N, T, tokens, window)
                               : plan_rows(B, NKV, D, G, N, T, tokens, window);
 }
 
@@ -359,7 +370,7 @@ extern "C" size_t voom_paged_gqa_chunk_workspace_bytes(int batch, int rows, int 
     return 0;
   const int G = num_q_heads / num_kv_heads;
   const long long cap = static_cast<long long>(max_pages) * page_tokens;
-  const Kind kind = kind_of(batch, rows, tokens, G);
+  const Kind kind = kind_of(batch, rows, tokens, num_kv_heads, G, cap, window);
   if (kind == Kind::kWide)
     return plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens, cap).bytes;
   const FewPlan p = plan_few(kind, batch, num_kv_heads, head_dim, G, rows, tokens, cap,
@@ -406,7 +417,7 @@ extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const voi
   const int G = num_q_heads / num_kv_heads;
   const int win = window == 0 ? INT_MAX : window;
   const long long cap = static_cast<long long>(max_pages) * page_tokens;
-  const Kind kind = kind_of(batch, rows, tokens, G);
+  const Kind kind = kind_of(batch, rows, tokens, num_kv_heads, G, cap, window);
   const FewPlan p = plan_few(kind, batch, num_kv_heads, head_dim, G, rows, tokens, cap, win);
   VOOM_REQUIRE(kind == Kind::kWide || (cap / kBlk + 16) * p.segs < (1LL << 31),
                "%s: %d pages of %d tokens for %d sequences are too many", who, max_pages,

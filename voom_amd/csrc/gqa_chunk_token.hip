@@ -25,8 +25,9 @@ constexpr int kTileRows = 16;
 constexpr int kAhead = 2;          // blocks in flight besides the one computed
 constexpr int kSplitWaves = 4;     // wavefronts of a workgroup, split
 constexpr int kSegWaves = 4;       // and of one that walks a whole segment
-constexpr int kShort = 32;         // blocks of a segment that is not cut
-typedef Geometry<kTileRows, kBlk, 4> Geo;
+constexpr int kShort = 24;         // blocks of 128 dims of a segment that is not cut
+// (3 units at least: 16,000 tokens of one sequence, 3 kv heads of 64: 15.5 us, with 1 22 us)
+typedef Geometry<kTileRows, kBlk, 4, 3> Geo;
 
 // A wavefront's walk over blocks of one segment.
 template <int D>
@@ -175,7 +176,7 @@ __global__ __launch_bounds__(kSplitWaves * kWave, 1) void gqa_chunk_split_kernel
     scan_units<Geo>(a, base, lane, x);
     U += __builtin_amdgcn_readlane(x, kWave - 1);
   }
-  const Split split(U, a.W);
+  const Split split = split_of<Geo>(U, a.W);
   if (w >= split.We || U == 0) return;
   int u0 = split.begin(w);
   const int u1 = split.begin(w + 1);
@@ -332,7 +333,7 @@ __global__ __launch_bounds__(kSegWaves * kWave) void gqa_chunk_segment_kernel(Ch
 
 }  // namespace
 
-FewPlan plan_token(int B, int NKV, int G, int N, int T, long long tokens, int window) {
+FewPlan plan_token(int B, int NKV, int D, int G, int N, int T, long long tokens, int window) {
   FewPlan p;
   const long long tiles = N > 0 ? static_cast<long long>(N) * G / kTileRows + (B < N ? B : N)
                                 : static_cast<long long>(B) * ((T * G + kTileRows - 1) / kTileRows);
@@ -340,8 +341,14 @@ FewPlan plan_token(int B, int NKV, int G, int N, int T, long long tokens, int wi
   long long blocks = (tokens + kBlk - 1) / kBlk;
   const long long seen = (static_cast<long long>(window) + kTileRows / G) / kBlk + 2;
   if (seen < blocks) blocks = seen;
-  // One launch where contexts are short.
-  p.W = blocks <= kShort ? 0 : kSplitWaves * device_cu_count();
+  // One launch where contexts are short, the longer the better their segments fill the card
+  // (8 kv heads, without and with the split: 8 segments of 128 dims and 500 tokens 12.1 and
+  // 13.7 us, of 1,000 16.6 and 14.0; 256 of them 24 and 27.6, of 2,000 44 and 49; 3 segments
+  // of 64 dims and 1,000 tokens 10.9 and 13.9, of 2,000 17.5 and 14.5).
+  const int cus = device_cu_count();
+  const long long full = (p.segs + cus - 1) / cus * cus;
+  const int most = 16 * p.segs >= 15 * full ? 64 : kShort * (128 / D);
+  p.W = blocks <= most ? 0 : kSplitWaves * cus;
   p.rows = kTileRows;
   return p;
 }
