@@ -11,7 +11,7 @@
 // What bounds it: K and V of the tokens seen once (4 D bytes per token and kv head) while
 // few rows share them, then matrix work, 4 NQ D flops per (new token, token seen).
 //
-// gqa_chunk_rows_kernel, for short chunks and small calls (kind_of; single tokens:
+// gqa_chunk_rows_kernel, for small calls of many rows (kind_of; single tokens:
 // gqa_chunk_token.hip, long ones: gqa_chunk_wide.hip), is built as gqa_tree_kernel is
 // (paged_rows.h): a workgroup takes 64 rows (new token, head of the group) of a (sequence, kv
 // head); the stages of 64 tokens (128 at D = 64) that a sequence's rows see, those behind the
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(kThreads, 2) void gqa_chunk_rows_kernel(ChunkArgs a
   }
 }
 
-constexpr int kShort = 8, kLong = 64;  // stages of a segment that is not cut
+constexpr int kShort = 8;  // stages of a segment that is not cut
 
 FewPlan plan_rows(int B, int NKV, int D, int G, int N, int T, long long tokens, int window) {
   FewPlan p;
@@ -302,37 +302,42 @@ FewPlan plan_rows(int B, int NKV, int D, int G, int N, int T, long long tokens, 
   const long long seen = (static_cast<long long>(window) + kRows / G) / tok + 2;
   if (seen < stages) stages = seen;
   // All workgroups of a split run at once.  Without one a workgroup walks a segment, which
-  // saves the merges and the reduce launch, where the segments are short, the longer the
-  // better they fill the card (32 rows, 8 kv heads of 128; without and with the split: 8
-  // segments of 500 tokens 14.6 and 14.5 us, of 1,000 21.9 and 14.3; 256 of 4,000 98 and 104).
+  // saves the merges and the reduce launch, where the segments are short, the longer if they
+  // fill half of the card (32 rows, 8 kv heads of 128; without and with the split: 8 segments of
+  // 500 tokens 14.6 and 14.5 us, of 1,000 21.9 and 14.3; 256 of 1,000 29.6 and 34.9).
   const int cus = device_cu_count();
   const long long full = (p.segs + cus - 1) / cus * cus;
-  const int most = 16 * p.segs >= 15 * full ? kLong : (2 * p.segs >= full ? 2 * kShort : kShort);
+  const int most = 2 * p.segs >= full ? 2 * kShort : kShort;
   p.W = stages <= most ? 0 : cus;
   p.rows = kRows;
   return p;
 }
 
-// The kernel that takes a call goes by the rows (new token, head of the group) a kv head of
-// a sequence, on the average: up to 16 that of single tokens, up to 64 the one above, beyond
-// that the one of long chunks.  All three are right for any lengths.  8 sequences of 16,000
-// tokens, 32/8 heads of 128, in us, the first, the second and the third:
-//   16 rows  90  108  124     20 rows  161  107  123
-//   64 rows  316  131  132    96 rows  468  195  134
-// The third has three launches and longer ones (30 us at least where the second has 15), but
-// reads K and V once for twice the rows: calls too small to gain that much take the second
-// (32/8 heads of 128, 300 rows a kv head of 1,000 to 1,200 tokens: 23 us against 38; of 8,100
-// tokens: 51 against 44).
+// The kernel that takes a call goes by its rows (new token, head of the group) a kv head.  All
+// three are right for any lengths.
+//
+// Up to 16 rows a sequence: that of single tokens, since it streams K and V fastest.  It reads
+// them once for every 16 rows, though, so that packed rows, one chunk among many single tokens
+// perhaps, are two a sequence at most on the average.  64 sequences of 500 to 4,000 tokens, 32/8
+// heads of 128, in us, it and the one of long chunks:
+//   2 tokens each  98  132    63 single tokens and a chunk of 64  138  143    of 128  178  142
+//
+// Beyond that the one of long chunks, which cuts and orders its work by lengths (64 such
+// sequences of 8 tokens: 135 us, the one above 201; 16 tokens: 138 and 315).  It has three
+// launches and longer ones, 30 us at least where the one above has 15: small calls take that
+// (32/8 heads, 300 rows a kv head of 1,000 to 1,200 tokens: 23 us against 38; of 8,100 tokens:
+// 51 against 44.  9/3 heads of 64, 16 sequences, 8 tokens each: 18 and 24; one chunk of 256:
+// 29 and 27).
 enum class Kind { kToken, kRows, kWide };
-constexpr long long kSmall = 1LL << 22;  // rows times the tokens that they may see
-Kind kind_of(int batch, int rows, int tokens, int NKV, int G, long long cap, int window) {
+constexpr long long kSmall = 1LL << 22;  // rows times the tokens of 128 dims that they may see
+Kind kind_of(int batch, int rows, int tokens, int NKV, int G, int D, long long cap, int window) {
   const long long all = rows > 0 ? static_cast<long long>(rows) * G
                                  : static_cast<long long>(tokens) * G * batch;
-  if (all <= 16LL * batch) return Kind::kToken;
   const long long reach = window > 0 ? static_cast<long long>(window) + rows + tokens : cap;
   const long long seen = reach < cap ? reach : cap;
-  return all <= static_cast<long long>(kRows) * batch || all <= kSmall / (seen * NKV)
-             ? Kind::kRows : Kind::kWide;
+  const bool small = all <= kSmall * (128 / D) / (seen * NKV);
+  if (all <= 16LL * batch && (rows <= 2 * batch || small)) return Kind::kToken;
+  return small ? Kind::kRows : Kind::kWide;
 }
 
 FewPlan plan_few(Kind kind, int B, int NKV, int D, int G, int N, int T, long long tokens,
@@ -371,7 +376,7 @@ extern "C" size_t voom_paged_gqa_chunk_workspace_bytes(int batch, int rows, int 
     return 0;
   const int G = num_q_heads / num_kv_heads;
   const long long cap = static_cast<long long>(max_pages) * page_tokens;
-  const Kind kind = kind_of(batch, rows, tokens, num_kv_heads, G, cap, window);
+  const Kind kind = kind_of(batch, rows, tokens, num_kv_heads, G, head_dim, cap, window);
   if (kind == Kind::kWide)
     return plan_wide(batch, num_kv_heads, head_dim, G, rows, tokens, cap).bytes;
   const FewPlan p = plan_few(kind, batch, num_kv_heads, head_dim, G, rows, tokens, cap,
@@ -418,7 +423,7 @@ extern "C" int voom_paged_gqa_chunk(const void* q, const void* k_pool, const voi
   const int G = num_q_heads / num_kv_heads;
   const int win = window == 0 ? INT_MAX : window;
   const long long cap = static_cast<long long>(max_pages) * page_tokens;
-  const Kind kind = kind_of(batch, rows, tokens, num_kv_heads, G, cap, window);
+  const Kind kind = kind_of(batch, rows, tokens, num_kv_heads, G, head_dim, cap, window);
   const FewPlan p = plan_few(kind, batch, num_kv_heads, head_dim, G, rows, tokens, cap, win);
   VOOM_REQUIRE(kind == Kind::kWide || (cap / kBlk + 16) * p.segs < (1LL << 31),
                "%s: %d pages of %d tokens for %d sequences are too many", who, max_pages,
