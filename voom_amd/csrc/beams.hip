@@ -153,8 +153,10 @@ __global__ __launch_bounds__(kThreads) void beam_pieces_kernel(BeamArgs a) {
 #pragma unroll
   for (int i = 0; i < kEach; ++i) s += fast_exp2((x[i] - ref) * 1.4426950408889634f);
   const float top = wave_max_uniform(m);
-  const float sum =
-      wave_sum_uniform(s * fast_exp2((ref - (top > -INFINITY ? top : 0.f)) * 1.4426950408889634f));
+  // (a lane of no logits or -inf alone has the sum 0, and no maximum that it could be scaled by:
+  // below -89 the factor of a reference of 0 would be infinite, and their product NaN)
+  const float sum = wave_sum_uniform(
+      m > -INFINITY ? s * fast_exp2((m - top) * 1.4426950408889634f) : s);
   const float mine = lane_bound(m, a.groups);
   if (lane == 0) {
     part[wv] = {top, sum};
