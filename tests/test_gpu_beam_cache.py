@@ -1,0 +1,114 @@
+"""The cache under beams and windows where its calls can go wrong: rows behind the last step
+of a search, searches refused before they begin, expansions and forks that fail, windows and
+distances after an eviction.
+
+Bars.  A search of the test's own over the same decoder: the same tokens, scores within the
+n-fold bar of a selection (1e-5 + 2^-23 |score|, test_gpu_beams.py).  Keys of the first layer
+by batch shape: bf16 projections of equal inputs, summed in another order at most, so a
+relative L2 of 2^-7, two steps of bf16, over a row; rows of other tokens differ by about
+sqrt(2).  Attention: relative L2 4e-3 (test_gpu_chunk.py).  Copied rows: bit for bit.
+"""
+import pytest
+import torch
+
+from test_gpu_beam_decoder import CFG, REL, weights_of
+from voom_amd import ops
+from voom_amd.decoder import DecoderConfig, PagedDecoder, random_weights
+from voom_amd.kv_paged import PagedKVCache
+
+pytestmark = pytest.mark.gpu
+
+
+def rnd(g, *shape):
+    return torch.randn(shape, generator=g, device="cuda").to(torch.bfloat16)
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def steps_alone(dec, prompt, tokens, K):
+    """Logits [B, K, V] behind prompt and tokens [B, K, n], in a cache of its own whose rows
+    never go on from one another."""
+    B = prompt.shape[0]
+    kv = dec.new_cache(page_positions=32)
+    logits = dec.forward(prompt, kv, last_only=True).expand(B, K, -1)
+    kv.expand(K)
+    for t in range(tokens.shape[2]):
+        logits = dec.forward(tokens[:, :, t].reshape(B * K, 1), kv).view(B, K, -1)
+    kv.release()
+    return logits
+
+
+def search_alone(dec, prompt, K, n):
+    """generate_beam's search, every step of it from the prompt on."""
+    B, rows = prompt.shape[0], torch.arange(K, device="cuda")
+    scores = torch.full((B, K), -float("inf"), device="cuda")
+    scores[:, 0] = 0
+    tokens = torch.empty((B, K, 0), dtype=torch.long, device="cuda")
+    for _ in range(n):
+        logp = torch.log_softmax(steps_alone(dec, prompt, tokens, K).double(), -1)
+        V = logp.shape[-1]
+        best = torch.sort((scores.double()[..., None] + logp).flatten(1), dim=1, descending=True,
+                          stable=True)
+        value, at = best.values[:, :K], best.indices[:, :K]
+        past = tokens.gather(1, (at // V)[..., None].expand(-1, -1, tokens.shape[2]))
+        found = torch.cat((past, (at % V)[..., None]), -1)
+        for b in range(B):  # the best continuation of a beam in the beam's row
+            row, parent = [None] * K, (at[b] // V).tolist()
+            for i, p in enumerate(parent):
+                if row[p] is None:
+                    row[p] = i
+            rest = [i for i in range(K) if i not in row]
+            order = [rest.pop(0) if i is None else i for i in row]
+            value[b], found[b] = value[b][order], found[b][order]
+        scores, tokens = value.float(), found
+    order = scores.argsort(dim=1, descending=True, stable=True)
+    return tokens.gather(1, order[..., None].expand_as(tokens)), scores.gather(1, order)
+
+
+@pytest.mark.parametrize("plain", [False, True])
+def test_a_search_is_one_whose_rows_are_never_copied(plain):
+    print(f"[beam cache] search, plain={plain}", flush=True)
+    cfg = DecoderConfig(num_hidden_layers=2, vocab_size=300) if plain else CFG
+    dec = PagedDecoder(cfg, weights_of(cfg, 11))
+    K, n, L = 4, 7, 37
+    prompt = torch.randint(0, cfg.vocab_size, (2, L), generator=torch.Generator().manual_seed(8))
+    prompt = prompt.cuda()
+    tokens, scores = dec.generate_beam(prompt, K, n, dec.new_cache(page_positions=32))
+    want, value = search_alone(dec, prompt, K, n)
+    assert torch.equal(tokens, want)
+    bar = n * (1e-5 + 2.0 ** -23 * value.abs().max().item())
+    assert (scores - value).abs().max().item() <= bar
+
+
+@pytest.mark.parametrize("end", [False, True])
+def test_rows_hold_their_beams_tokens_behind_a_search(end):
+    """All but the last token of each: the first layer's keys go by token and position."""
+    print(f"[beam cache] rows behind a search, end={end}", flush=True)
+    cfg = DecoderConfig(num_hidden_layers=2, vocab_size=200)
+    dec = PagedDecoder(cfg, random_weights(cfg, seed=3, std=0.05))
+    B, K, n, L = 2, 4, 5, 33
+    prompt = torch.randint(0, 200, (B, L), generator=torch.Generator().manual_seed(6))
+    stop = {}
+    if end:  # the end token is one that some of the beams pass through
+        stop = {"end_token": int(dec.generate_beam(prompt, K, n, dec.new_cache())[0][0, 0, 2])}
+    kv = dec.new_cache(page_positions=32)
+    tokens, _ = dec.generate_beam(prompt, K, n, kv, **stop)
+    n = tokens.shape[2]
+    assert kv.offset == L + n - 1
+    keys = kv.gather(0)[0][:, :, L:].transpose(1, 2).flatten(2).view(B, K, n - 1, -1)
+    apart = 0
+    for b in range(B):
+        fresh = dec.new_cache()
+        dec.forward(torch.cat((prompt[b].cuda().expand(K, L), tokens[b]), 1)[:, :-1].contiguous(),
+                    fresh)
+        want = fresh.gather(0)[0][:, :, L:].transpose(1, 2).flatten(2)
+        off = (keys[b][:, None].double() - want[None].double()).norm(dim=-1) / want.double().norm(
+            dim=-1)
+        same = off.amax(-1) <= 2.0 ** -7  # [cache row, beam]
+        past = tokens[b][:, :-1]
+        alike = (past[:, None] == past[None]).all(-1)  # beams that differ in the last token
+        assert torch.equal(same.sum(0), alike.sum(0)) and same.any(1).all()
+        apart += int((~alike).sum())
+    assert apart > 0

@@ -471,10 +471,10 @@ class PagedDecoder:
                 logits, scores, shared=shared, ctx_lens=ctx, **ended)
             past = tokens.gather(1, parents.long()[..., None].expand(-1, -1, step))
             tokens = torch.cat((past, last[..., None]), -1)
+            kv.fork(parents, first, since=L)
             over = end_token is not None and bool((last == end_token).all())
             if over or step + 1 == max_tokens:
                 break
-            kv.fork(parents, first, since=L)
             logits = self.forward(last.view(B * K, 1), kv).view(B, K, -1)
         order = torch.argsort(scores, dim=1, descending=True, stable=True)
         return tokens.gather(1, order[..., None].expand_as(tokens)), scores.gather(1, order)
