@@ -112,3 +112,90 @@ def test_rows_hold_their_beams_tokens_behind_a_search(end):
         assert torch.equal(same.sum(0), alike.sum(0)) and same.any(1).all()
         apart += int((~alike).sum())
     assert apart > 0
+
+
+def test_windows_and_distances_after_an_eviction():
+    """What a window reaches has to lie behind what the eviction left apart; else places in the
+    cache are no positions, and the call is refused."""
+    print("[beam cache] chunks after an eviction", flush=True)
+    NQ, NKV, D, S, budget, recent = 8, 2, 64, 100, 40, 20
+    g = gen(1)
+    kv = PagedKVCache(1, 1 << 40, page_positions=32)
+    k, v = rnd(g, 2, NKV, S + 10, D), rnd(g, 2, NKV, S + 10, D)
+    slopes = torch.rand(NQ, generator=g, device="cuda") * 0.1
+    prefix = torch.full((2,), 2, dtype=torch.int32, device="cuda")
+
+    def append(a, b):
+        kv.append(0, k[:, :, a:b].contiguous(), v[:, :, a:b].contiguous())
+
+    def reference(q, window):
+        T = q.shape[2]
+        at, token = torch.arange(S + 10 - T, S + 10, device="cuda")[:, None], torch.arange(
+            S + 10, device="cuda")
+        s = q.double() @ k.double().repeat_interleave(NQ // NKV, 1).transpose(2, 3).contiguous()
+        s = s * D ** -0.5 - slopes.double()[:, None, None] * (at - token).abs()
+        s = s.masked_fill((token > at) | (at - token >= window), -float("inf"))
+        return torch.softmax(s, -1) @ v.double().repeat_interleave(NQ // NKV, 1)
+
+    append(0, S)
+    kv.observe(0, rnd(g, 2, NQ, 1, D), torch.zeros((2, 1, NQ), device="cuda"))
+    assert kv.evict(budget, sink=2, recent=recent) == S - budget
+    append(S, S + 10)  # 50 tokens, the newest 30 of each head next to each other
+    for T in (1, 4):
+        q = rnd(g, 2, NQ, T, D)
+        reach = recent + 10 - T + 1
+        got = kv.attend_chunk(0, q, window=reach, slopes=slopes)
+        want = reference(q, reach)
+        assert ((got.double() - want).norm() / want.norm()).item() <= REL
+        for scores in (dict(window=reach + 1), dict(window=1000), dict(slopes=slopes),
+                       dict(slopes=slopes, window=reach + 1), dict(prefix_lens=prefix),
+                       dict(prefix_lens=prefix, window=1)):
+            with pytest.raises(ValueError, match="after evict"):
+                kv.attend_chunk(0, q, **scores)
+        # what goes by no position is as it was
+        whole = kv.attend_chunk(0, q, softcap=5.0, window=0)
+        assert torch.equal(whole, kv.attend_chunk(0, q, softcap=5.0))
+    q = rnd(g, 2, NQ, 1, D)
+    kv.trim(15)  # all that is left lies apart, what follows does not
+    append(0, 5)
+    kv.attend_chunk(0, q, window=5)
+    with pytest.raises(ValueError, match="after evict"):
+        kv.attend_chunk(0, q, window=6)
+    kv.observe(0, q, torch.zeros((2, 1, NQ), device="cuda"))
+    kv.evict(18, recent=16)  # 2 are gone, of the newest 5 none
+    kv.attend_chunk(0, q, window=5)
+    with pytest.raises(ValueError, match="after evict"):
+        kv.attend_chunk(0, q, window=6)
+    kv.evict(10, recent=3)
+    kv.attend_chunk(0, q, window=3)
+    with pytest.raises(ValueError, match="after evict"):
+        kv.attend_chunk(0, q, window=4)
+    kv.trim(0)
+    append(0, 30)
+    kv.attend_chunk(0, q, window=25, slopes=slopes, prefix_lens=prefix)
+    kv.release()
+
+
+def test_a_decoder_refuses_windows_after_an_eviction_before_it_appends():
+    print("[beam cache] decoder after an eviction", flush=True)
+    dec = PagedDecoder(CFG, weights_of(CFG, 5))
+    ids = torch.randint(0, CFG.vocab_size, (1, 70), generator=torch.Generator().manual_seed(2))
+    ids = ids.cuda()
+    window = CFG.sliding_window
+
+    def evicted(recent):
+        kv = dec.new_cache(page_positions=32)
+        dec.forward(ids[:, :60], kv)
+        nq, hd = CFG.num_attention_heads, CFG.head_dim
+        for layer in range(CFG.num_hidden_layers):
+            kv.observe(layer, rnd(gen(layer), 1, nq, 1, hd), torch.zeros((1, 1, nq), device="cuda"))
+        kv.evict(40, sink=1, recent=recent)
+        return kv
+
+    kv = evicted(window - 2)
+    with pytest.raises(ValueError, match="after evict"):
+        dec.forward(ids[:, 60:61], kv)
+    assert kv.layer_lengths() == (40,) * CFG.num_hidden_layers and kv.offset == 40
+    kv = evicted(window - 1)
+    dec.forward(ids[:, 60:65], kv)
+    assert kv.offset == 45

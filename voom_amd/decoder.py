@@ -298,6 +298,10 @@ class PagedDecoder:
         """Logits [B, L, vocab] (fp32) for tokens [B, L] appended at kv.next_position."""
         offset = kv.next_position
         L = tokens.shape[1]
+        if self.cfg.sliding_window:  # (refused before a layer takes a token)
+            for layer in range(self.cfg.num_hidden_layers):
+                if self.cfg.window_of(layer):
+                    kv.require_window(self.cfg.window_of(layer), kv.layer_length(layer))
         cos, sin = self._rope_tables(torch.arange(offset, offset + L, device=self.device))
         x = self.embed[tokens]
         delta = None

@@ -618,6 +618,8 @@ class PagedKVCache:
         # 0 behind the layer's length; and the tokens that evict() has dropped
         self._weights: list[torch.Tensor | None] = [None] * L
         self._dropped = 0
+        # the place from which on evict() has left each head's tokens next to each other
+        self._seam = 0
         self._has_reserved = False  # captured steps may exist (until release())
         self._reserved = 0  # tokens, by reserve(); and its position counters on the device
         self._counters_dev: torch.Tensor | None = None
@@ -1062,6 +1064,7 @@ class PagedKVCache:
             self._cut_layer(layer, n)
         self._torn = None
         self._offset = targets[0] if targets else 0
+        self._seam = min(self._seam, max(self._len))  # (new tokens follow one another)
         if not any(self._len):
             self._dropped = 0
         if self._counters_dev is not None:
@@ -2158,12 +2161,19 @@ class PagedKVCache:
         ``ops.paged_gqa_chunk``'s scores (softcap, slopes) and masks (``window``,
         ``prefix_lens``).  Returns out [B, NQ, T, D] (and the LSE [B, T, NQ]).  Spilled pages
         of the layer are made resident first, with a window and no prefix those alone that it
-        reaches."""
+        reaches.  Windows, slopes and prefixes go by places in the cache: after evict() a window
+        or slopes are refused where a token sees past those that still lie side by side, and a
+        prefix always."""
         self._require_kind(layer, "kv")
         B, NQ, T, D = q.shape
         S = self._len[layer]
         if T > S:
             raise ValueError(f"{T} queries but the layer holds {S} tokens")
+        if window or scores.get("slopes") is not None:
+            self.require_window(window, S - T)
+        if prefix_lens is not None and self._dropped:
+            raise ValueError("attend_chunk(): after evict() the first places in the cache are "
+                             "not the sequence's first tokens")
         reach = 0
         if window and prefix_lens is None and not ops.bounds_checks_enabled():
             reach = max(0, S - T + 1 - int(window))
@@ -2180,6 +2190,15 @@ class PagedKVCache:
         out, lse = got if return_lse else (got, None)
         out = out.permute(0, 2, 1, 3)
         return (out, lse) if return_lse else out
+
+    def require_window(self, window: int | None, first: int) -> None:
+        """Raise ValueError unless the tokens that those from place ``first`` on see through a
+        ``window`` (0: all before them) have places as far apart as their positions, which
+        evict() ends."""
+        reach = max(0, first + 1 - int(window)) if window else 0
+        if reach < self._seam:
+            raise ValueError(f"after evict() only the tokens from place {self._seam} on lie as far "
+                             f"apart as their positions: a window from {reach} on is wrong")
 
     def _resident(self, layer: int, first: int = 0):
         """(pool, block table) of a layer with the pages of its tokens from ``first`` on
@@ -2400,6 +2419,8 @@ class PagedKVCache:
         self._torn = None
         self._offset = budget
         self._dropped += S - budget
+        # the newest `recent` tokens keep their neighbours, where an earlier call left them any
+        self._seam = max(budget - recent, self._seam - (S - budget))
         return S - budget
 
     def attend_mla(self, layer: int, q_nope: torch.Tensor, q_rope: torch.Tensor,
