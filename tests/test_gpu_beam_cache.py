@@ -199,3 +199,31 @@ def test_a_decoder_refuses_windows_after_an_eviction_before_it_appends():
     kv = evicted(window - 1)
     dec.forward(ids[:, 60:65], kv)
     assert kv.offset == 45
+
+
+def test_searches_are_refused_before_the_prompt_runs():
+    print("[beam cache] searches refused", flush=True)
+    cfg = DecoderConfig(num_hidden_layers=2, vocab_size=200)
+    dec = PagedDecoder(cfg, random_weights(cfg, seed=3, std=0.05))
+    prompt = torch.randint(0, 200, (2, 9), generator=torch.Generator().manual_seed(6))
+    kv = dec.new_cache()
+
+    def refused(match, *args, prompt=prompt, kv=kv, **kw):
+        with pytest.raises(ValueError, match=match):
+            dec.generate_beam(prompt, *args, kv, **kw)
+        assert kv.offset == 0 and kv.layer_lengths() == (0, 0)
+
+    refused("beams", 0, 4)
+    refused("beams", -1, 4)
+    refused("beams", 33, 4)
+    refused("end token", 2, 4, end_token=200)
+    refused("end token", 2, 4, end_token=-1)
+    refused("prompt", 2, 4, prompt=prompt[:, :0])
+    assert kv._geom is None
+    kept = dec.new_cache()
+    dec.forward(prompt.cuda(), kept)
+    kept.reserve(30)
+    kept.trim(0)
+    refused("captured", 2, 4, kv=kept)
+    tokens, scores = dec.generate_beam(prompt, 2, 4, kv, end_token=199)
+    assert tokens.shape[:2] == (2, 2) and scores.isfinite().all()

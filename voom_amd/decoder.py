@@ -459,6 +459,14 @@ class PagedDecoder:
         prompt = prompt.to(self.device)
         B, L = prompt.shape
         K = int(beams)
+        # (what the search would be refused for, before the cache takes a token)
+        if L == 0:
+            raise ValueError("a prompt of no tokens")
+        if not 0 < K <= ops.BEAM_MAX:
+            raise ValueError(f"{K} beams lie outside [1, {ops.BEAM_MAX}]")
+        if end_token is not None and not 0 <= end_token < self.embed.shape[0]:
+            raise ValueError(f"end token {end_token} lies outside [0, {self.embed.shape[0]})")
+        kv.require_expandable(B, K)
         logits = self.forward(prompt, kv, last_only=True)
         kv.expand(K)
         logits = logits.expand(B, K, -1).contiguous()

@@ -2257,19 +2257,24 @@ class PagedKVCache:
         if rows > 65535:
             raise ValueError(f"{rows} rows of the cache are more than a copy takes, 65535")
 
+    def require_expandable(self, sequences: int, beams: int) -> None:
+        """Raise ValueError where ``expand(beams)`` of that many sequences would be refused,
+        for callers that fill the cache first."""
+        if beams <= 0:
+            raise ValueError(f"{beams} beams")
+        if self._has_reserved:
+            raise ValueError("expand(): captured steps hold the cache's batch")
+        self._require_rows(sequences * beams)
+
     def expand(self, beams: int) -> None:
         """Every sequence becomes ``beams`` rows, rows b * beams to (b + 1) * beams - 1 of the
         batch, all of them with its tokens: the start of a beam search behind one prompt.
         Spilled pages are made resident first; ``max_bytes`` is enforced afterwards."""
         beams = int(beams)
         S = self._require_forkable("expand()")
-        if beams <= 0:
-            raise ValueError(f"{beams} beams")
-        if self._has_reserved:
-            raise ValueError("expand(): captured steps hold the cache's batch")
+        self.require_expandable(self._batch, beams)
         if beams == 1:
             return
-        self._require_rows(self._batch * beams)
         self.check_integrity()
         self._drop_prefetch()
         for layer in range(self.num_layers):

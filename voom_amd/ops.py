@@ -574,6 +574,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, *, last: torch.Tenso
 
 
 _BEAM_DTYPES = {torch.bfloat16: 0, torch.float32: 2}
+BEAM_MAX = 32  # beams of a request
 
 
 def check_parents(parents: torch.Tensor) -> None:
