@@ -227,3 +227,33 @@ def test_searches_are_refused_before_the_prompt_runs():
     refused("captured", 2, 4, kv=kept)
     tokens, scores = dec.generate_beam(prompt, 2, 4, kv, end_token=199)
     assert tokens.shape[:2] == (2, 2) and scores.isfinite().all()
+
+
+@pytest.mark.parametrize("fails_in", [0, 1, 2])
+def test_an_expansion_without_memory_leaves_the_cache_as_it_was(fails_in):
+    print(f"[beam cache] expand fails in layer {fails_in}", flush=True)
+    B, K, S, page, layers = 2, 3, 100, 32, 3
+    g = gen(fails_in)
+    kv = PagedKVCache(layers, 1 << 40, page_positions=page)
+    want = [(rnd(g, B, 2, S, 64), rnd(g, B, 2, S, 64)) for _ in range(layers)]
+    for layer in range(layers):
+        kv.append(layer, *want[layer])
+    pool = kv._pool(fails_in)
+    live = [p.live_slots for p in kv._pools]
+
+    def fails(count):
+        raise torch.cuda.OutOfMemoryError("no memory for the slots")
+
+    pool.allocate = fails
+    with pytest.raises(torch.cuda.OutOfMemoryError):
+        kv.expand(K)
+    del pool.allocate
+    assert [p.live_slots for p in kv._pools] == live and kv._batch == B
+    for layer in range(layers):
+        assert all(torch.equal(a, b) for a, b in zip(kv.gather(layer), want[layer]))
+    kv.expand(K)
+    assert [p.live_slots for p in kv._pools] == [K * n for n in live]
+    for layer in range(layers):
+        assert all(torch.equal(a, b.repeat_interleave(K, 0))
+                   for a, b in zip(kv.gather(layer), want[layer]))
+    kv.release()

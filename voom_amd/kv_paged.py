@@ -2281,14 +2281,21 @@ class PagedKVCache:
             self._resident(layer)
         kind, B, NKV, D = self._geom
         rows = B * beams
-        # slots of every layer before anything changes: what may fail, fails here
-        grown = []
+        # slots of every layer before anything changes; where one's pool cannot grow, those of
+        # the layers before it go back
+        grown, taken = [], []
+        each = rows - B
         for layer in range(self.num_layers):
             pool = self._pool(layer)
             pages = [(p.index, p.slots) for p in self._pages[layer]]
             pages += list(self._open_slots[layer].items())
-            new = pool.allocate(len(pages) * (rows - B))
-            each = rows - B
+            try:
+                new = pool.allocate(len(pages) * each)
+            except BaseException:
+                for before, slots in taken:
+                    before.release(slots)
+                raise
+            taken.append((pool, new))
             cols = {}
             for i, (index, old) in enumerate(pages):
                 mine = iter(new[i * each:(i + 1) * each])
