@@ -257,3 +257,35 @@ def test_an_expansion_without_memory_leaves_the_cache_as_it_was(fails_in):
         assert all(torch.equal(a, b.repeat_interleave(K, 0))
                    for a, b in zip(kv.gather(layer), want[layer]))
     kv.release()
+
+
+def test_a_fork_that_is_refused_leaves_the_cache_in_use():
+    print("[beam cache] forks refused", flush=True)
+    g = gen(4)
+    k, v = rnd(g, 4, 2, 50, 64), rnd(g, 4, 2, 50, 64)
+    kv = PagedKVCache(1, 1 << 40, page_positions=32)
+    kv.append(0, k, v)
+    dev = dict(dtype=torch.int32, device="cuda")
+    ops.set_bounds_checks(True)
+    try:
+        with pytest.raises(ValueError, match="its own parent"):
+            kv.fork(torch.tensor([[1, 2, 2, 3]], **dev))
+        with pytest.raises(ValueError, match="outside"):
+            kv.fork(torch.tensor([[0, 1, 2, 4]], **dev))
+    finally:
+        ops.set_bounds_checks(False)
+    assert all(torch.equal(a, b) for a, b in zip(kv.gather(0), (k, v)))
+    kv.fork(torch.tensor([[0, 0, 2, 2]], **dev))
+    rows = torch.tensor([0, 0, 2, 2], device="cuda")
+    assert all(torch.equal(a, b[rows]) for a, b in zip(kv.gather(0), (k, v)))
+    # pages and heads that the copy does not take
+    for page, D in ((4, 64), (32, 1032)):
+        kv = PagedKVCache(1, 1 << 40, page_positions=page)
+        k, v = rnd(g, 2, 1, 9, D), rnd(g, 2, 1, 9, D)
+        kv.append(0, k, v)
+        for call in (lambda: kv.expand(2), lambda: kv.fork(torch.zeros((1, 2), **dev))):
+            with pytest.raises(ValueError, match="8 tokens"):
+                call()
+        assert kv._batch == 2
+        assert all(torch.equal(a, b) for a, b in zip(kv.gather(0), (k, v)))
+        kv.release()

@@ -2250,6 +2250,11 @@ class PagedKVCache:
         self._require_kind(0, "kv")
         if len(set(self._len)) != 1:
             raise ValueError(f"{what} needs layers of one length")
+        if self.page_positions < 8 or self._geom[3] > 1024:
+            raise ValueError(f"{what} needs pages of 8 tokens or more and heads of 1024 dims or "
+                             "fewer")
+        if self._pool(0).k.get_device() != torch.cuda.current_device():
+            raise ValueError(f"{what} runs on the cache's device, which has to be the current one")
         return self._len[0]
 
     @staticmethod
@@ -2337,7 +2342,7 @@ class PagedKVCache:
             raise ValueError("first must be like parents")
         self._require_rows(parents.numel())
         for t in (parents, first):
-            if t is not None and not t.is_cuda:
+            if t is not None and t.get_device() != self._pool(0).k.get_device():
                 raise ValueError("parents and first must be on the cache's device")
         parents = parents.contiguous()
         first = None if first is None else first.contiguous()
@@ -2345,6 +2350,7 @@ class PagedKVCache:
             raise ValueError(f"since {since} lies outside the {S} tokens")
         if ops.bounds_checks_enabled():
             since = 0
+            ops.check_parents(parents)  # (here: not once the cache counts as half moved)
         self._drop_prefetch()
         for layer in range(self.num_layers):
             self._resident(layer, since)
