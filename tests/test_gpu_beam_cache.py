@@ -289,3 +289,18 @@ def test_a_fork_that_is_refused_leaves_the_cache_in_use():
         assert kv._batch == 2
         assert all(torch.equal(a, b) for a, b in zip(kv.gather(0), (k, v)))
         kv.release()
+
+
+def test_a_fork_of_observed_rows_leaves_out_parents_that_are_none():
+    print("[beam cache] wild parents, observed", flush=True)
+    g = gen(6)
+    k, v = rnd(g, 6, 2, 40, 64), rnd(g, 6, 2, 40, 64)
+    kv = PagedKVCache(1, 1 << 40, page_positions=32)
+    kv.append(0, k, v)
+    kv.observe(0, rnd(g, 6, 4, 1, 64), torch.zeros((6, 1, 4), device="cuda"))
+    sums = kv._weights[0].clone()
+    kv.fork(torch.tensor([[0, -1, 3], [2, 99, 2]], dtype=torch.int32, device="cuda"))
+    rows = torch.tensor([0, 1, 2, 5, 4, 5], device="cuda")
+    assert all(torch.equal(a, b[rows]) for a, b in zip(kv.gather(0), (k, v)))
+    assert torch.equal(kv._weights[0], sums[rows])
+    kv.release()

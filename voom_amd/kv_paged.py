@@ -2357,11 +2357,19 @@ class PagedKVCache:
         self._torn = "fork()"  # until every layer is copied
         self._fork(parents, first, S)
         self._torn = None
+        if any(sums is not None for sums in self._weights):
+            rows = self._rows_of(parents)
+            self._weights = [None if sums is None else sums.index_select(0, rows)
+                             for sums in self._weights]
+
+    @staticmethod
+    def _rows_of(parents: torch.Tensor) -> torch.Tensor:
+        """The cache row that each row goes on from, itself where its parent is none of the
+        request's (as the copy leaves it alone)."""
         B, K = parents.shape
-        for layer, sums in enumerate(self._weights):
-            if sums is not None:
-                row = (parents + K * torch.arange(B, device=self.device)[:, None]).reshape(-1)
-                self._weights[layer] = sums.index_select(0, row.long())
+        own = torch.arange(K, device=parents.device)
+        kept = torch.where((parents >= 0) & (parents < K), parents.long(), own)
+        return (kept + K * torch.arange(B, device=parents.device)[:, None]).reshape(-1)
 
     def _fork(self, parents: torch.Tensor, first: torch.Tensor | None, S: int) -> None:
         if S == 0:
