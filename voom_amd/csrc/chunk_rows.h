@@ -1,6 +1,6 @@
-// What the kernels of attention over ragged chunks share (gqa_chunk.hip,
-// gqa_chunk_wide.hip): the call's
-// arguments, which cached tokens a new one sees, and the score of a pair.
+// What the kernels of attention over ragged chunks share (gqa_chunk.hip, gqa_chunk_token.hip,
+// gqa_chunk_wide.hip): the call's arguments, which cached tokens a new one sees, and the
+// score of a pair.
 #pragma once
 
 #include "common.h"
@@ -90,8 +90,9 @@ __device__ __forceinline__ uint32_t bits_in(int pos, int lo, int hi) {
   return below & ~before;
 }
 
-// tanh(x) / x for |x| <= kNear as a polynomial of x^2, off by 3.5e-8 at most (found by
-// Remez's exchange of the extrema of the relative error); a term more would hold to 0.5.
+// tanh(x) / x for |x| <= kNear as a polynomial of x^2, off by 7.1e-8 at most, relative: found
+// by Remez's exchange of the extrema of the relative error, which holds to 3.5e-8, its first
+// term then rounded to 1, so that no small score is changed.
 constexpr float kNear = 0.35f;
 constexpr float kTanh[4] = {1.f, -0.33332422375679016f, 0.13295799493789673f,
                             -0.04895823076367378f};
