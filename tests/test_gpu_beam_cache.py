@@ -304,3 +304,31 @@ def test_a_fork_of_observed_rows_leaves_out_parents_that_are_none():
     assert all(torch.equal(a, b[rows]) for a, b in zip(kv.gather(0), (k, v)))
     assert torch.equal(kv._weights[0], sums[rows])
     kv.release()
+
+
+@pytest.mark.parametrize("page,spilled", [(32, 7), (64, 2), (32, 9)])
+def test_a_capped_token_streams_what_the_budget_leaves_out(page, spilled):
+    """Spilled pages that do not fit max_bytes stay spilled; those that do come back."""
+    print(f"[beam cache] capped token, page={page} spilled={spilled}", flush=True)
+    B, NQ, NKV, D, S = 2, 8, 2, 64, 300
+    g = gen(page + spilled)
+    kv = PagedKVCache(2, 1 << 40, page_positions=page)
+    k, v, q = rnd(g, B, NKV, S, D), rnd(g, B, NKV, S, D), rnd(g, B, NQ, 1, D)
+    for layer in range(2):
+        kv.append(layer, k, v)
+    whole = kv.attend_chunk(0, q, softcap=3.0)
+    s = q.double() @ k.double().repeat_interleave(NQ // NKV, 1).transpose(2, 3).contiguous()
+    s = 3 * torch.tanh(s * D ** -0.5 / 3)
+    want = torch.softmax(s, -1) @ v.double().repeat_interleave(NQ // NKV, 1)
+    pages = [(0, i) for i in range(spilled)]
+    assert kv.spill(pages) == spilled
+    kv.max_bytes = kv.nbytes() + spilled * kv.page_nbytes - 1
+    for _ in range(3):
+        got = kv.attend_chunk(0, q, softcap=3.0)
+        assert sum(not p.resident for p in kv._pages[0]) == spilled
+        assert got.shape == whole.shape
+        assert ((got.double() - want).norm() / want.norm()).item() <= REL
+    kv.max_bytes += 1
+    assert torch.equal(kv.attend_chunk(0, q, softcap=3.0), whole)
+    assert all(p.resident for p in kv._pages[0])
+    kv.release()

@@ -2161,7 +2161,8 @@ class PagedKVCache:
         ``ops.paged_gqa_chunk``'s scores (softcap, slopes) and masks (``window``,
         ``prefix_lens``).  Returns out [B, NQ, T, D] (and the LSE [B, T, NQ]).  Spilled pages
         of the layer are made resident first, with a window and no prefix those alone that it
-        reaches.  Windows, slopes and prefixes go by places in the cache: after evict() a window
+        reaches; for a single token without window, slopes, prefix and LSE they stream through
+        as in ``attend`` where they do not fit ``max_bytes``.  Windows, slopes and prefixes go by places in the cache: after evict() a window
         or slopes are refused where a token sees past those that still lie side by side, and a
         prefix always."""
         self._require_kind(layer, "kv")
@@ -2180,10 +2181,17 @@ class PagedKVCache:
         if T == 0:
             out = torch.empty_like(q)
             return (out, q.new_empty((B, 0, NQ), dtype=torch.float32)) if return_lse else out
-        pool, table = self._resident(layer, reach)
         q = q.contiguous()
         if q.data_ptr() % 16:
             q = q.clone()  # the kernels load 16 bytes per lane
+        if (T == 1 and not window and prefix_lens is None and not return_lse
+                and scores.get("slopes") is None):  # (goes by no position: in any order)
+            spilled = sum(not p.resident for p in self._pages[layer])
+            if spilled and self.nbytes() + spilled * self.page_nbytes > self.max_bytes:
+                out = self._attend_pages(layer, lambda pool, table, ctx, lse: ops.paged_gqa_chunk(
+                    q, pool.k, pool.v, table, ctx, scale=scale, return_lse=lse, **scores))
+                return out.permute(0, 2, 1, 3)
+        pool, table = self._resident(layer, reach)
         got = ops.paged_gqa_chunk(q, pool.k, pool.v, table, self._positions(S), scale=scale,
                                   window=window, prefix_lens=prefix_lens, return_lse=return_lse,
                                   **scores)
