@@ -19,7 +19,8 @@
 // piece, and the few logits that are not below it (about K log K) are listed in LDS and
 // ranked by counting.  beam_merge_kernel, a workgroup per request, does the same with all
 // pieces' lists, in 64 bits, where values of different beams meet.  16 requests of 8 beams over
-// 128,256 fp32 logits: 14.4 us and 9.6, both 33 with bounds from single lanes.
+// 128,256 fp32 logits: 14.8 us and 10.9 (medians of a trace), 26.5 a call; 33 with bounds from
+// single lanes.
 #include "common.h"
 
 #include <cmath>
@@ -420,8 +421,9 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
 // Row j of a request takes the K and V of tokens [first, ctx) of the row that it goes on
 // from, in every layer; rows that go on from themselves are left alone.  A workgroup copies
 // blocks of (up to) 32 tokens of a kv head, K and V^T one run of memory each.  Bound by the
-// bytes, each read and written once (71 MB in 8 layers: 32 us, 4.4 TB/s of both); a few tokens
-// by the launch and three dependent reads (the parents, the tables, the rows; 6.4 us).
+// bytes, each read and written once (71 MB in 8 layers: 33.9 us, the median of a trace, 4.2 TB/s
+// of both); a few tokens by the launch and three dependent reads (the parents, the tables, the
+// rows; 6.6 us).
 
 constexpr int kForkThreads = 256;
 constexpr int kForkLayers = 64;

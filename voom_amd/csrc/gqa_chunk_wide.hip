@@ -2,7 +2,8 @@
 // the scores): long parts of prompts, alone or beside single tokens.
 //
 // What bounds it: matrix work, 4 NQ D flops per (new token, token seen), beside an
-// exponential per score and, with a cap, a polynomial of it.
+// exponential per score and, with a cap, a polynomial of it.  Neither unit is busy all of the
+// time: tiles wait for their stage, and workers for the longest one.
 //
 // A row tile is 128 rows (new token, head of the group) of a (sequence, kv head): four
 // wavefronts of 32 rows, which share 64-key tiles of K and V^T in LDS, loaded straight into
@@ -19,8 +20,9 @@
 // device, and cuts long ones over keys, so that the workgroups are done at about the same time;
 // the pieces leave (m, l, o) in fp32 and gqa_chunk_join_kernel merges them.
 //
-// The last 2,011 of 6,007 tokens, 32/8 heads of 128, capped: 192 us, 860 TFLOP/s, of which the
-// plan 5.5 and the join 4.7 (row tiles of 64 through the ring of gqa_chunk.hip: 663 us).
+// The last 2,011 of 6,007 tokens, 32/8 heads of 128, capped: 192-196 us a call, one behind
+// another, 850 TFLOP/s, of which the plan 6 and the join 5 (row tiles of 64 through the ring of
+// gqa_chunk.hip: 663 us).  The plan's 504 uncut pieces leave 17 % of the workers' time idle.
 #include "chunk_rows.h"
 
 #include <cfloat>

@@ -2340,7 +2340,7 @@ class PagedKVCache:
         others go on from is its own parent: ``ops.beam_select``'s), those before first[b, j]
         (int32, None: 0) excepted, which the two have in common.  ``since``: no first[b, j] is
         below it, so that spilled pages before it may stay spilled; of the others all come back
-        before a token is copied."""
+        before a token is copied.  (After evict() rows have other tokens: ``first`` is None.)"""
         S = self._require_forkable("fork()")
         since = int(since)
         if (parents.dtype is not torch.int32 or parents.dim() != 2
