@@ -286,6 +286,7 @@ def test_a_fork_that_is_refused_leaves_the_cache_in_use():
         for call in (lambda: kv.expand(2), lambda: kv.fork(torch.zeros((1, 2), **dev))):
             with pytest.raises(ValueError, match="8 tokens"):
                 call()
+        kv.expand(1)  # (nothing to copy)
         assert kv._batch == 2
         assert all(torch.equal(a, b) for a, b in zip(kv.gather(0), (k, v)))
         kv.release()

@@ -2258,12 +2258,15 @@ class PagedKVCache:
         self._require_kind(0, "kv")
         if len(set(self._len)) != 1:
             raise ValueError(f"{what} needs layers of one length")
+        return self._len[0]
+
+    def _require_copies(self, what: str) -> None:
+        """What ``ops.fork_kv`` would refuse, before the cache changes."""
         if self.page_positions < 8 or self._geom[3] > 1024:
             raise ValueError(f"{what} needs pages of 8 tokens or more and heads of 1024 dims or "
                              "fewer")
         if self._pool(0).k.get_device() != torch.cuda.current_device():
             raise ValueError(f"{what} runs on the cache's device, which has to be the current one")
-        return self._len[0]
 
     @staticmethod
     def _require_rows(rows: int) -> None:
@@ -2277,7 +2280,8 @@ class PagedKVCache:
             raise ValueError(f"{beams} beams")
         if self._has_reserved:
             raise ValueError("expand(): captured steps hold the cache's batch")
-        self._require_rows(sequences * beams)
+        if beams > 1:
+            self._require_rows(sequences * beams)
 
     def expand(self, beams: int) -> None:
         """Every sequence becomes ``beams`` rows, rows b * beams to (b + 1) * beams - 1 of the
@@ -2288,6 +2292,8 @@ class PagedKVCache:
         self.require_expandable(self._batch, beams)
         if beams == 1:
             return
+        if S:
+            self._require_copies("expand()")
         self.check_integrity()
         self._drop_prefetch()
         for layer in range(self.num_layers):
@@ -2356,6 +2362,8 @@ class PagedKVCache:
         first = None if first is None else first.contiguous()
         if not 0 <= since <= S:
             raise ValueError(f"since {since} lies outside the {S} tokens")
+        if S:
+            self._require_copies("fork()")
         if ops.bounds_checks_enabled():
             since = 0
             ops.check_parents(parents)  # (here: not once the cache counts as half moved)
