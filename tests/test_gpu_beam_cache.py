@@ -152,6 +152,7 @@ def test_windows_and_distances_after_an_eviction():
                        dict(prefix_lens=prefix, window=1)):
             with pytest.raises(ValueError, match="after evict"):
                 kv.attend_chunk(0, q, **scores)
+        assert kv.attend_chunk(0, q[:, :, :0], window=1000, prefix_lens=prefix).numel() == 0
         # what goes by no position is as it was
         whole = kv.attend_chunk(0, q, softcap=5.0, window=0)
         assert torch.equal(whole, kv.attend_chunk(0, q, softcap=5.0))
@@ -329,6 +330,17 @@ def test_a_capped_token_streams_what_the_budget_leaves_out(page, spilled):
         assert sum(not p.resident for p in kv._pages[0]) == spilled
         assert got.shape == whole.shape
         assert ((got.double() - want).norm() / want.norm()).item() <= REL
+    assert not kv._prefetched
+    # what the call takes besides goes the way of the layer's resident pages
+    out = torch.empty((B, 1, NQ, D), dtype=torch.bfloat16, device="cuda")
+    more = [dict(new_lens=torch.tensor([1, 0], dtype=torch.int32, device="cuda")), dict(out=out),
+            dict(slopes=torch.zeros(NQ, device="cuda"))]
+    for scores in more:
+        got = kv.attend_chunk(0, q, softcap=3.0, **scores)
+        assert torch.equal(got[:1], whole[:1])
+        assert torch.equal(got[1], 0 * whole[1] if "new_lens" in scores else whole[1])
+        assert kv.spill(pages) == spilled
+    assert torch.equal(out.permute(0, 2, 1, 3), whole)
     kv.max_bytes += 1
     assert torch.equal(kv.attend_chunk(0, q, softcap=3.0), whole)
     assert all(p.resident for p in kv._pages[0])

@@ -2161,18 +2161,18 @@ class PagedKVCache:
         ``ops.paged_gqa_chunk``'s scores (softcap, slopes) and masks (``window``,
         ``prefix_lens``).  Returns out [B, NQ, T, D] (and the LSE [B, T, NQ]).  Spilled pages
         of the layer are made resident first, with a window and no prefix those alone that it
-        reaches; for a single token without window, slopes, prefix and LSE they stream through
-        as in ``attend`` where they do not fit ``max_bytes``.  Windows, slopes and prefixes go by places in the cache: after evict() a window
-        or slopes are refused where a token sees past those that still lie side by side, and a
-        prefix always."""
+        reaches; for a single token of capped scores alone they stream through as in ``attend``
+        where they do not fit ``max_bytes``.  Windows, slopes and prefixes go by places in the
+        cache: after evict() a window or slopes are refused where a token sees past those that
+        still lie side by side, and a prefix always."""
         self._require_kind(layer, "kv")
         B, NQ, T, D = q.shape
         S = self._len[layer]
         if T > S:
             raise ValueError(f"{T} queries but the layer holds {S} tokens")
-        if window or scores.get("slopes") is not None:
+        if T and (window or scores.get("slopes") is not None):
             self.require_window(window, S - T)
-        if prefix_lens is not None and self._dropped:
+        if T and prefix_lens is not None and self._dropped:
             raise ValueError("attend_chunk(): after evict() the first places in the cache are "
                              "not the sequence's first tokens")
         reach = 0
@@ -2185,11 +2185,13 @@ class PagedKVCache:
         if q.data_ptr() % 16:
             q = q.clone()  # the kernels load 16 bytes per lane
         if (T == 1 and not window and prefix_lens is None and not return_lse
-                and scores.get("slopes") is None):  # (goes by no position: in any order)
+                and not {k for k in scores if scores[k] is not None} - {"softcap"}):
+            # (goes by no position: its pages in any order)
             spilled = sum(not p.resident for p in self._pages[layer])
             if spilled and self.nbytes() + spilled * self.page_nbytes > self.max_bytes:
                 out = self._attend_pages(layer, lambda pool, table, ctx, lse: ops.paged_gqa_chunk(
-                    q, pool.k, pool.v, table, ctx, scale=scale, return_lse=lse, **scores))
+                    q, pool.k, pool.v, table, ctx, scale=scale, return_lse=lse, **scores),
+                    ahead=False)
                 return out.permute(0, 2, 1, 3)
         pool, table = self._resident(layer, reach)
         got = ops.paged_gqa_chunk(q, pool.k, pool.v, table, self._positions(S), scale=scale,
@@ -2596,11 +2598,12 @@ class PagedKVCache:
         return ops.mla_sparse_decode(q_lat, self._pool(layer).lat, self._tables[layer], sel,
                                      sel_lens, scale=scale)
 
-    def _attend_pages(self, layer: int, run) -> torch.Tensor:
+    def _attend_pages(self, layer: int, run, ahead: bool = True) -> torch.Tensor:
         """Drive ``run(pool, block_table, ctx_lens, return_lse)`` over a layer:
         one call over the block table when every page is resident, else one
         over the resident pages plus one per landed chunk of spilled pages,
-        folded by log-sum-exp merges."""
+        folded by log-sum-exp merges.  ``ahead``: the next layer's first upload
+        starts behind it (not where that layer may leave its pages spilled)."""
         B = self._batch
         S = self._len[layer]
         pool = self._pool(layer)
@@ -2648,5 +2651,6 @@ class PagedKVCache:
             fold(run(stage, t, c, True))
 
         self._stream_in(layer, spilled, stage, attend_chunk, transient=True)
-        self._prefetch((layer + 1) % self.num_layers)
+        if ahead:
+            self._prefetch((layer + 1) % self.num_layers)
         return state[0].to(torch.bfloat16)
