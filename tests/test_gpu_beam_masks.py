@@ -50,3 +50,17 @@ def test_few_tokens_above_minus_infinity(V, B, K, dtype):
     check(ops.beam_select(logits, scores), search(logits, scores))
     logits[..., 3] = torch.finfo(dtype).min
     check(ops.beam_select(logits, scores), search(logits, scores))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B,K,V", [(1, 5, 1), (2, 3, 40), (64, 4, 700), (1, 2, 9001)])
+def test_rows_of_the_largest_floats(B, K, V, dtype):
+    """All tokens of some beams at one value so large that a score beside it is lost: they are
+    worth the score less log V, and tie."""
+    print(f"[beam masks] large, B={B} K={K} V={V} {dtype}", flush=True)
+    for value in (torch.finfo(dtype).min, torch.finfo(dtype).max, -1e30, 1e20):
+        logits, scores = make(B, K, V, dtype, 7)
+        logits[:, ::2] = value
+        whole = logits.double()  # (less its maximum the oracle's sum keeps log V)
+        want = search(whole - whole.amax(-1, keepdim=True), scores)
+        check(ops.beam_select(logits, scores), want)

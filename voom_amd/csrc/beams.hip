@@ -19,7 +19,7 @@
 // piece, and the few logits that are not below it (about K log K) are listed in LDS and
 // ranked by counting.  beam_merge_kernel, a workgroup per request, does the same with all
 // pieces' lists, in 64 bits, where values of different beams meet.  16 requests of 8 beams over
-// 128,256 fp32 logits: 14.8 us and 10.9 (medians of a trace), 26.5 a call; 33 with bounds from
+// 128,256 fp32 logits: 14.8 us and 10.9 (medians of a trace), 26-28 a call; 33 with bounds from
 // single lanes.
 #include "common.h"
 
@@ -241,7 +241,10 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
   constexpr int kHeld = 2;  // continuations that a lane holds in registers
   __shared__ Cand found[kFound];
   __shared__ double bounds[kMergeWaves];
-  __shared__ double norm[kMaxBeams];   // what is added to a beam's logits
+  // A beam's continuations are worth norm + (logit - peak), norm its score less the logarithm of
+  // its sum: a peak of the largest floats would swallow the score, added to it first.
+  __shared__ double norm[kMaxBeams];
+  __shared__ float peak[kMaxBeams];
   __shared__ int kind[kMaxBeams];      // 0: its lists; 1: ended; 2: -inf alone
   __shared__ Cand best[kMaxBeams];
   __shared__ Cand winner[kMergeWaves];
@@ -289,10 +292,11 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
 #pragma unroll
     for (int k = 1; k < kWave; k <<= 1) S += __shfl_xor(S, k);
     if (lane == 0) {
-      const double lse = M + log(S);
+      const double less = log(S);
       const bool whole = isfinite(score);
-      kind[j] = over ? 1 : (isfinite(lse) && whole ? 0 : 2);
-      norm[j] = over ? (whole ? static_cast<double>(score) : -INFINITY) : score - lse;
+      kind[j] = over ? 1 : (isfinite(M) && isfinite(less) && whole ? 0 : 2);
+      norm[j] = over ? (whole ? static_cast<double>(score) : -INFINITY) : score - less;
+      peak[j] = M;
     }
   }
   __syncthreads();
@@ -304,7 +308,8 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a) {
     const int what = kind[beam];
     const int token = what == 0 ? token_of(key) : (what == 1 ? static_cast<int>(a.end_token) : in);
     c.id = static_cast<uint64_t>(beam) << 32 | static_cast<uint32_t>(token);
-    c.value = what == 0 ? norm[beam] + unordered(static_cast<uint32_t>(key >> 32))
+    c.value = what == 0 ? norm[beam] + (static_cast<double>(unordered(
+                                            static_cast<uint32_t>(key >> 32))) - peak[beam])
                         : (what == 1 ? norm[beam] : -INFINITY);
     return what == 0 ? key != 0 : (what == 1 ? in == 0 : in < K && in < a.V);
   };
